@@ -124,6 +124,37 @@ int gemm_launch_ex(const void* A, const void* B, void* C, int64_t M, int64_t N, 
 size_t gemm_workspace_bytes_ex(const void* A, const void* B, int64_t M, int64_t N, int64_t K, int64_t lda,
                                int64_t ldb, int trans_a, int trans_b, int cfg_id);
 
+/* Types of the 16-bit operands of the entry points below (all operands of a
+ * call alike); gemm_launch and gemm_launch_ex take fp16. */
+#define GEMM_DTYPE_F16 0
+#define GEMM_DTYPE_BF16 1
+
+/* Products grouped by expert with ragged sizes:
+ *   C[r, :] = act(A[r, :] * op(B[e]) + bias[e])   for offsets[e] <= r < offsets[e + 1]
+ *  A       = T x K, pitch lda >= K, rows sorted by group;
+ *  B       = E matrices, stride_b elements apart: K x N (ldb >= N) with
+ *            trans_b = 0, or stored N x K (ldb >= K) with trans_b = 1, read
+ *            in place.  The input gradient is the same call with the other
+ *            trans_b: dA = dC * B[e]^T;
+ *  C       = T x N, pitch ldc >= N;
+ *  offsets = E + 1 non-decreasing row numbers in [0, T] on the device, of
+ *            offsets_bits (32 or 64) bits.  They are read by the kernel: the
+ *            call does not synchronise.  Empty groups are fine.  Offsets that
+ *            decrease or leave [0, T] are clamped (no access leaves the
+ *            operands) and reported by gemm_device_error;
+ *  rows outside [offsets[0], offsets[E]) are written as zeros when zero_rest
+ *            != 0 and left as they are otherwise;
+ *  bias    = E x N (contiguous) or NULL; activation = GEMM_ACT_*.
+ * fp32 accumulation, one rounding.  E <= 1024.  K = 0 gives act(bias).
+ * The workspace comes from gemm_grouped_workspace_bytes under the contract of
+ * gemm_launch.  No counterpart in the reference. */
+int gemm_grouped_launch(const void* A, const void* B, void* C, const void* offsets, int offsets_bits, int64_t T,
+                        int64_t N, int64_t K, int64_t E, int64_t lda, int64_t ldb, int64_t stride_b, int64_t ldc,
+                        int trans_b, const void* bias, int activation, int zero_rest, int dtype, void* workspace,
+                        size_t workspace_bytes, void* stream);
+size_t gemm_grouped_workspace_bytes(const void* A, const void* B, int64_t T, int64_t N, int64_t K, int64_t E,
+                                    int64_t lda, int64_t ldb, int64_t stride_b, int trans_b);
+
 /* Fused all-gather for M-row sharding over the GPUs of one node (one
  * process per GPU).  Same as gemm_launch, and each finished tile of C is
  * also stored, over NVLink, at the same offset and pitch ldc into
@@ -175,7 +206,9 @@ int gemm_default_cfg(int64_t M, int64_t N, int64_t K);
 
 /* Reads and clears the device-side error word of `device` (synchronises
  * that device).  *code receives the OR of the kernels' error bits (0 = none).
- * Returns GEMM_OK, or GEMM_ERR_DEVICE_TIMEOUT when *code != 0.
+ * Returns GEMM_OK when it is 0, GEMM_ERR_INVALID_ARG when only index data that
+ * a kernel read on the device was out of range (group offsets, adapter
+ * indices; the kernel clamped them), else GEMM_ERR_DEVICE_TIMEOUT.
  * No counterpart in the reference (C10_CUDA_KERNEL_LAUNCH_CHECK only,
  * src/gemm_ext.cpp:50). */
 int gemm_device_error(int device, int* code);

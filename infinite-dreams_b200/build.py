@@ -46,12 +46,12 @@ def nvcc() -> str:
 
 
 def sources() -> List[Path]:
-    return [CSRC / "gemm_capi.cu", CSRC / "gemm_noalloc.cu"] + sorted(GEN.glob("gemm_bank_*.cu"))
+    return [CSRC / "gemm_capi.cu", CSRC / "gemm_noalloc.cu", CSRC / "gemm_grouped_capi.cu"] + sorted(GEN.glob("gemm_bank_*.cu"))
 
 
 def headers_digest() -> str:
     h = hashlib.sha256()
-    for p in sorted(list(CSRC.glob("*.cuh")) + list(GEN.glob("*.inc")) + list(INCLUDE.glob("*.h"))):
+    for p in sorted(list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + list(GEN.glob("*.inc")) + list(INCLUDE.glob("*.h"))):
         h.update(p.name.encode())
         h.update(p.read_bytes())
     h.update(" ".join(NVCC_FLAGS).encode())

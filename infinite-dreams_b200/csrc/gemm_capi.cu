@@ -19,6 +19,7 @@
 
 #include "../../include/gemm_sm100.h"
 #include "gemm_bank_common.cuh"
+#include "gemm_capi_shared.h"
 #include "gemm_skinny_kernel.cuh"
 #include "generated/gemm_cfg_menu.inc"
 
@@ -391,21 +392,10 @@ int make_plan(const void* A, const void* B, int64_t M, int64_t N, int64_t K, int
 // boxes); false: plain row-major boxes (the skinny kernel's C blocks).
 int encode_2d(CUtensorMap* map, const void* base, int64_t inner, int64_t outer, int64_t pitch_elems, int box_inner,
               int box_outer, const char* what, bool swizzled = true) {
-  EncodeTiledFn fn = encode_fn();
-  if (!fn) return fail(GEMM_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch_elems) * 2};
-  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_inner), static_cast<cuuint32_t>(box_outer)};
-  const cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) {
-    return fail(GEMM_ERR_CUDA, std::string("cuTensorMapEncodeTiled(") + what + ") failed with CUresult " +
-                                   std::to_string(static_cast<int>(r)));
-  }
-  return GEMM_OK;
+  const int64_t extents[2] = {inner, outer};
+  const int64_t strides[1] = {pitch_elems};
+  const int box[2] = {box_inner, box_outer};
+  return capi_encode(map, base, 2, extents, strides, box, swizzled, what);
 }
 
 // Recently encoded tensor maps of the calling thread.  A map depends only on
@@ -696,6 +686,53 @@ int launch_impl(const void* A, const void* B, void* C, int64_t M, int64_t N, int
 }  // namespace
 
 void record_last_error(const std::string& msg) { t_last_error = msg; }
+
+int capi_fail(int status, const std::string& msg) { return fail(status, msg); }
+int capi_fail_cuda(cudaError_t e, const char* what) { return fail_cuda(e, what); }
+void capi_clear_error() { t_last_error.clear(); }
+
+int capi_device(int* sms, int** err_word) {
+  DeviceInfo dinfo;
+  const int st = device_info(&dinfo);
+  if (st != GEMM_OK) return st;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return fail_cuda(e, "cudaGetDevice");
+  std::call_once(g_err_once[dev], [dev] {
+    g_err_status[dev] = cudaGetSymbolAddress(reinterpret_cast<void**>(&g_err_word[dev]), g_device_error);
+  });
+  if (g_err_status[dev] != cudaSuccess) return fail_cuda(g_err_status[dev], "cudaGetSymbolAddress(g_device_error)");
+  *sms = dinfo.sms;
+  *err_word = g_err_word[dev];
+  return GEMM_OK;
+}
+
+int capi_encode(CUtensorMap* map, const void* base, int rank, const int64_t* extents, const int64_t* strides,
+                const int* box, bool swizzled, const char* what) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(GEMM_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t dims[3], bytes[2];
+  cuuint32_t boxes[3];
+  const cuuint32_t estr[3] = {1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    dims[i] = static_cast<cuuint64_t>(extents[i]);
+    boxes[i] = static_cast<cuuint32_t>(box[i]);
+    if (i + 1 < rank) bytes[i] = static_cast<cuuint64_t>(strides[i]) * 2;
+  }
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims,
+                  bytes, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    return fail(GEMM_ERR_CUDA, std::string("cuTensorMapEncodeTiled(") + what + ") failed with CUresult " +
+                                   std::to_string(static_cast<int>(r)));
+  }
+  return GEMM_OK;
+}
+
+int capi_pack(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols, cudaStream_t stream) {
+  return launch_pack(src, lds, dst, ldd, rows, cols, stream);
+}
 
 // Imported peer pointer -> base of the opened allocation (for gemm_ipc_close).
 std::mutex g_ipc_mu;
@@ -991,6 +1028,12 @@ int gemm_device_error(int device, int* code) {
   if (device != prev) cudaSetDevice(prev);
   if (e != cudaSuccess) return fail_cuda(e, "reading the device error word");
   if (code) *code = v;
+  if (v != 0 && (v & ~(kDevErrBadOffsets | kDevErrBadAdapter)) == 0) {
+    return fail(GEMM_ERR_INVALID_ARG, std::string("a kernel was given ") +
+                                          ((v & kDevErrBadOffsets) ? "group offsets that decrease or leave [0, rows]"
+                                                                   : "an adapter index past the last adapter") +
+                                          " (error bits " + std::to_string(v) + ")");
+  }
   if (v != 0) return fail(GEMM_ERR_DEVICE_TIMEOUT, "a kernel gave up on a bounded wait (error bits " +
                                                        std::to_string(v) + ")");
   return GEMM_OK;

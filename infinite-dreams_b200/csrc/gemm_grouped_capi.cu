@@ -1,0 +1,263 @@
+// C ABI of the products whose weight is picked by the row (declared in
+// include/gemm_sm100.h): validation, repacking of operands that TMA cannot
+// address, tensor maps and launches, in the manner of gemm_capi.cu.
+#include <atomic>
+#include <cstring>
+#include <string>
+
+#include "../../include/gemm_sm100.h"
+#include "gemm_capi_shared.h"
+#include "gemm_grouped_kernel.cuh"
+
+namespace idb {
+namespace {
+
+constexpr int64_t kInt32Max = (1ll << 31) - 1;
+
+int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
+size_t align256(size_t x) { return (x + 255) / 256 * 256; }
+
+// One operand: `batch` matrices of rows x cols, pitch ld, `stride` elements
+// from one matrix to the next.
+struct Operand {
+  const void* p = nullptr;
+  int64_t batch = 1, rows = 0, cols = 0, ld = 0, stride = 0;
+  size_t pack_off = 0;
+  bool pack = false;
+
+  Operand(const void* ptr, int64_t b, int64_t r, int64_t c, int64_t l, int64_t s)
+      : p(ptr), batch(b), rows(r), cols(c), ld(l), stride(s) {}
+
+  // Reserves workspace for a copy when TMA cannot address the operand as it
+  // is (16-byte base, row pitch and matrix stride).  The copy's rows are
+  // padded to 64 elements, one 128-byte line per TMA box row, as in gemm_launch.
+  void plan(size_t* off) {
+    const bool ok = reinterpret_cast<uintptr_t>(p) % 16u == 0 && ld % 8 == 0 &&
+                    (batch == 1 || (stride % 8 == 0 && stride > 0));
+    pack = !ok && batch > 0 && rows > 0 && cols > 0;
+    if (!pack) return;
+    pack_off = *off;
+    *off = align256(*off + static_cast<size_t>(batch) * rows * round_up(cols, 64) * 2);
+  }
+
+  int make(uint8_t* ws, cudaStream_t stream) {
+    if (!pack) return GEMM_OK;
+    const int64_t ldp = round_up(cols, 64);
+    uint8_t* dst = ws + pack_off;
+    // matrices that follow one another without a gap are one tall matrix
+    const bool tall = batch == 1 || stride == rows * ld;
+    const int64_t n = tall ? 1 : batch, r = tall ? batch * rows : rows;
+    for (int64_t b = 0; b < n; ++b) {
+      const int st = capi_pack(static_cast<const uint8_t*>(p) + b * stride * 2, ld, dst + b * rows * ldp * 2, ldp, r,
+                               cols, stream);
+      if (st != GEMM_OK) return st;
+    }
+    p = dst;
+    ld = ldp;
+    stride = rows * ldp;
+    return GEMM_OK;
+  }
+
+  int encode2(CUtensorMap* m, int box_cols, int box_rows, bool swizzled, const char* what) const {
+    const int64_t ext[2] = {cols, rows}, str[1] = {ld};
+    const int box[2] = {box_cols, box_rows};
+    return capi_encode(m, p, 2, ext, str, box, swizzled, what);
+  }
+
+  int encode3(CUtensorMap* m, int box_cols, int box_rows, bool swizzled, const char* what) const {
+    // with one matrix the stride is never used, but has to be a legal one
+    const int64_t ext[3] = {cols, rows, batch}, str[2] = {ld, batch == 1 ? round_up(rows * ld, 8) : stride};
+    const int box[3] = {box_cols, box_rows, 1};
+    return capi_encode(m, p, 3, ext, str, box, swizzled, what);
+  }
+};
+
+bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 2u != 0; }
+
+int check_workspace(size_t need, const void* ws, size_t ws_bytes) {
+  if (need == 0) return GEMM_OK;
+  if (ws == nullptr || ws_bytes < need) {
+    return capi_fail(GEMM_ERR_WORKSPACE, "workspace of " + std::to_string(need) + " bytes required, got " +
+                                             std::to_string(ws == nullptr ? 0 : ws_bytes));
+  }
+  if (reinterpret_cast<uintptr_t>(ws) % 256u != 0) {
+    return capi_fail(GEMM_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  }
+  return GEMM_OK;
+}
+
+int check_common(int64_t T, int64_t N, int64_t K, int64_t E, int offsets_bits, int dtype, const char* groups) {
+  if (T < 0 || N < 0 || K < 0) return capi_fail(GEMM_ERR_INVALID_ARG, "T, N, K must be >= 0");
+  if (T > kInt32Max || N > kInt32Max || K > kInt32Max) {
+    return capi_fail(GEMM_ERR_UNSUPPORTED, "T, N, K must each be < 2^31");
+  }
+  if (E < 1) return capi_fail(GEMM_ERR_INVALID_ARG, std::string(groups) + " must be >= 1");
+  if (offsets_bits != 32 && offsets_bits != 64) {
+    return capi_fail(GEMM_ERR_INVALID_ARG, "index width must be 32 or 64 bits");
+  }
+  if (dtype != GEMM_DTYPE_F16 && dtype != GEMM_DTYPE_BF16) {
+    return capi_fail(GEMM_ERR_INVALID_ARG, "dtype must be GEMM_DTYPE_F16 or GEMM_DTYPE_BF16");
+  }
+  return GEMM_OK;
+}
+
+// Dynamic shared memory above 48 KiB is opted into once per kernel and device.
+template <class Kernel>
+cudaError_t opt_in(Kernel kernel, int bytes, std::atomic<unsigned long long>& configured) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (configured.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) configured.fetch_or(bit, std::memory_order_acq_rel);
+  return e;
+}
+
+template <int CG, class Kernel, class... Args>
+cudaError_t launch(Kernel kernel, int bytes, std::atomic<unsigned long long>& configured, int grid,
+                   cudaStream_t stream, const Args&... args) {
+  cudaError_t e = opt_in(kernel, bytes, configured);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+  cfg.blockDim = dim3(kNumThreads, 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(bytes);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CG == 2 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <int CG, int TM, int STAGES>
+int launch_grouped(const Operand& a, const Operand& b, const GroupedParams& gp, int sms, cudaStream_t stream) {
+  using Plan = GroupedPlan<CG, TM, STAGES>;
+  GroupedParams p = gp;
+  p.tiles_n = static_cast<int>((static_cast<int64_t>(p.N) + kGrpCols * CG - 1) / (kGrpCols * CG));
+  const int64_t row_tiles = static_cast<int64_t>(p.T) / TM + p.E;   // at most one cut tile per group
+  if (row_tiles * p.tiles_n > kInt32Max) return capi_fail(GEMM_ERR_UNSUPPORTED, "too many output tiles");
+  CUtensorMap tmA, tmB, tmC;
+  std::memset(&tmA, 0, sizeof(tmA));
+  std::memset(&tmB, 0, sizeof(tmB));
+  std::memset(&tmC, 0, sizeof(tmC));
+  int st;
+  if (p.K > 0) {
+    st = a.encode2(&tmA, kBK, Plan::kBoxRows, true, "A");
+    if (st != GEMM_OK) return st;
+    st = p.b_kmaj ? b.encode3(&tmB, kBK, kGrpCols, true, "B (stored N x K)") : b.encode3(&tmB, 64, kBK, true, "B");
+    if (st != GEMM_OK) return st;
+  }
+  if (p.c_tma) {
+    const int64_t ext[2] = {p.N, p.T}, str[1] = {p.ldc};
+    const int box[2] = {kGrpCols, kGrpChunk};
+    st = capi_encode(&tmC, p.C, 2, ext, str, box, false, "C");
+    if (st != GEMM_OK) return st;
+  }
+  // persistent: one CTA (pair) per SM (pair), fewer when the most tiles that
+  // these sizes can give are fewer
+  const int64_t most = std::min<int64_t>(row_tiles * p.tiles_n, sms / CG);
+  const int grid = static_cast<int>(most < 1 ? 1 : most) * CG;
+  static std::atomic<unsigned long long> configured{0};
+  cudaError_t e = launch<CG>(gemm_grouped_sm100<CG, TM, STAGES>, Plan::kDynamicBytes, configured, grid, stream, tmA,
+                             tmB, tmC, p);
+  return e == cudaSuccess ? GEMM_OK : capi_fail_cuda(e, "grouped gemm kernel launch");
+}
+
+Operand operand_b(const void* B, int64_t E, int64_t N, int64_t K, int64_t ldb, int64_t stride_b, int trans_b) {
+  return Operand(B, E, trans_b ? N : K, trans_b ? K : N, ldb, stride_b);
+}
+
+}  // namespace
+}  // namespace idb
+
+using namespace idb;
+
+extern "C" {
+
+size_t gemm_grouped_workspace_bytes(const void* A, const void* B, int64_t T, int64_t N, int64_t K, int64_t E,
+                                    int64_t lda, int64_t ldb, int64_t stride_b, int trans_b) {
+  if (T <= 0 || N <= 0 || K < 0 || E < 1) return 0;
+  Operand a(A, 1, T, K, lda, 0), b = operand_b(B, E, N, K, ldb, stride_b, trans_b);
+  const size_t head = align256(gemm_workspace_counter_bytes());
+  size_t off = head;
+  a.plan(&off);
+  b.plan(&off);
+  return off == head ? 0 : off;
+}
+
+int gemm_grouped_launch(const void* A, const void* B, void* C, const void* offsets, int offsets_bits, int64_t T,
+                        int64_t N, int64_t K, int64_t E, int64_t lda, int64_t ldb, int64_t stride_b, int64_t ldc,
+                        int trans_b, const void* bias, int activation, int zero_rest, int dtype, void* workspace,
+                        size_t workspace_bytes, void* stream_v) {
+  capi_clear_error();
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  int st = check_common(T, N, K, E, offsets_bits, dtype, "the number of groups");
+  if (st != GEMM_OK) return st;
+  if (E > kMaxGroups) {
+    return capi_fail(GEMM_ERR_UNSUPPORTED, "at most " + std::to_string(kMaxGroups) + " groups");
+  }
+  if (trans_b != 0 && trans_b != 1) return capi_fail(GEMM_ERR_INVALID_ARG, "trans_b must be 0 or 1");
+  if (activation < GEMM_ACT_NONE || activation > GEMM_ACT_GELU) {
+    return capi_fail(GEMM_ERR_INVALID_ARG, "activation must be GEMM_ACT_NONE, GEMM_ACT_RELU or GEMM_ACT_GELU");
+  }
+  if (T == 0 || N == 0) return GEMM_OK;
+  if (!C || !offsets || (K > 0 && (!A || !B))) {
+    return capi_fail(GEMM_ERR_INVALID_ARG, "A, B, C and offsets must be non-null");
+  }
+  const int64_t b_rows = trans_b ? N : K, b_cols = trans_b ? K : N;
+  if (lda < K || ldb < b_cols || ldc < N || (E > 1 && b_rows > 0 && stride_b < (b_rows - 1) * ldb + b_cols)) {
+    return capi_fail(GEMM_ERR_INVALID_ARG, std::string("pitches must satisfy lda >= K, ldb >= ") +
+                                               (trans_b ? "K" : "N") + ", ldc >= N, and stride_b one matrix of B");
+  }
+  if (misaligned(A) || misaligned(B) || misaligned(C) || misaligned(bias)) {
+    return capi_fail(GEMM_ERR_INVALID_ARG, "A, B, C and bias must be 2-byte aligned");
+  }
+  if (reinterpret_cast<uintptr_t>(offsets) % (offsets_bits / 8) != 0) {
+    return capi_fail(GEMM_ERR_INVALID_ARG, "offsets must be aligned to their width");
+  }
+  Operand a(A, 1, T, K, lda, 0), b = operand_b(B, E, N, K, ldb, stride_b, trans_b);
+  const size_t head = align256(gemm_workspace_counter_bytes());
+  size_t off = head;
+  a.plan(&off);
+  b.plan(&off);
+  if (b.pack && E * b.rows > kInt32Max) return capi_fail(GEMM_ERR_UNSUPPORTED, "too many rows of B to repack");
+  st = check_workspace(off == head ? 0 : off, workspace, workspace_bytes);
+  if (st != GEMM_OK) return st;
+
+  GroupedParams p = {};
+  int sms = 0;
+  st = capi_device(&sms, &p.err);
+  if (st != GEMM_OK) return st;
+  st = a.make(static_cast<uint8_t*>(workspace), stream);
+  if (st == GEMM_OK) st = b.make(static_cast<uint8_t*>(workspace), stream);
+  if (st != GEMM_OK) return st;
+  p.offsets = offsets;
+  p.off64 = offsets_bits == 64;
+  p.E = static_cast<int>(E);
+  p.T = static_cast<int>(T);
+  p.N = static_cast<int>(N);
+  p.K = static_cast<int>(K);
+  p.kb_total = static_cast<int>((K + kBK - 1) / kBK);
+  p.b_kmaj = trans_b;
+  p.bf16 = dtype == GEMM_DTYPE_BF16;
+  p.act = activation;
+  p.bias = static_cast<const unsigned short*>(bias);
+  p.C = static_cast<unsigned short*>(C);
+  p.ldc = ldc;
+  p.c_tma = p.c_vec = reinterpret_cast<uintptr_t>(C) % 16u == 0 && ldc % 8 == 0;
+  p.zero_rest = zero_rest != 0;
+  // Few rows per group: the cost is reading the weights, and single CTAs with
+  // a deep ring read them best.  More rows: CTA pairs with tiles of up to 256
+  // rows, which read every weight once per 256 rows.
+  if (T <= 64 * E || N <= kGrpCols) return launch_grouped<1, 64, 8>(a, b, p, sms, stream);
+  return launch_grouped<2, 256, 6>(a, b, p, sms, stream);
+}
+
+}  // extern "C"

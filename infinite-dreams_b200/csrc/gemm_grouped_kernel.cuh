@@ -1,0 +1,521 @@
+// Products whose weight is picked by the row, for sm_100a:
+//
+//   C[r, :] = act(A[r, :] * B[e] + bias[e])   for off[e] <= r < off[e + 1]
+//
+// A is T x K (rows sorted by group), B a stack of E weights K x N (or stored
+// N x K), 16-bit inputs (fp16 or bf16), fp32 accumulation, one rounding to
+// the inputs' type.  The counts of the groups are only known on the device:
+// every CTA reads the offsets, lays the groups' tiles out one after the other
+// (a prefix sum in shared memory) and walks its share, so nothing is
+// synchronised with the host and one launch serves any split of the rows.
+//
+// The weights sit on the 128 TMEM lanes (MMA M) and the rows are the MMA N,
+// i.e. a tile computes C^T = B^T A^T.  Row counts are ragged and the MMA N is
+// a run-time field with steps of 16 (32 for a CTA pair), so a group of 37 rows costs 48
+// rows of MMA work and of A traffic; with the rows on the lanes it would cost
+// 128 (256).  A group's rows are cut into equal tiles of at most TM rows.
+//
+//   CG = 2, TM = 256: a CTA pair owns 256 columns x up to 256 rows; each CTA
+//     loads its 128 columns of B and half of the rows (no multicast).
+//   CG = 1, TM = 64: one CTA owns 128 columns x up to 64 rows; the ring holds
+//     128 KiB of weights in flight, for groups of few rows, whose cost is
+//     reading the weights.
+//
+// Roles as in gemm_sm100_kernel.cuh: warp 0 TMA producer, warp 1 TMEM owner
+// and MMA issuer, warps 2..5 epilogue.  The accumulator holds C transposed:
+// a thread owns one column of C and walks the rows, so bias is one value per
+// thread, and the 32-row chunks go through shared memory to become rows of
+// 256 bytes.  A chunk that lies wholly inside its group is stored by TMA, a
+// cut one row by row: the rows behind it are the next group's.  Rows that the
+// last A box of a group reads past the group's end only reach accumulator
+// columns that are not stored, so nothing in them (inf, NaN) can spread.
+#pragma once
+#include "gemm_sm100_kernel.cuh"
+
+namespace idb {
+
+constexpr int kGrpCols = 128;      // columns of C per CTA: the TMEM lanes
+constexpr int kMaxGroups = 1024;   // bounded by the offset tables in shared memory
+constexpr int kGrpChunk = 32;      // rows of C per epilogue step
+constexpr int kGrpRaster = 8;      // row tiles walked before the next column tile
+
+struct GroupedParams {
+  const void* offsets;  // int32 or int64 [E + 1]; null: one group of all T rows
+  int off64;
+  int E;
+  int T, N, K;
+  int kb_total;      // ceil(K / 64)
+  int tiles_n;       // ceil(N / (128 * CG))
+  int b_kmaj;        // B[e] stored N x K
+  int bf16;
+  int act;
+  const unsigned short* bias;  // [E, N] or null
+  unsigned short* C;
+  long long ldc;
+  int c_tma;         // C is TMA-addressable
+  int c_vec;         // C rows are 16-byte aligned
+  int zero_rest;     // rows outside [off[0], off[E]): 1 written as 0, 0 left as they are
+  int* err;
+};
+
+template <int CG, int TM, int STAGES>
+struct GroupedPlan {
+  static constexpr int kStep = 16 * CG;                  // granularity of a tile's rows (MMA N)
+  static constexpr int kTokRows = TM / CG;               // rows of A held by this CTA
+  static constexpr int kBoxRows = TM >= 256 ? 32 : 16;   // rows per TMA box of A
+  static constexpr int kWBytes = kGrpCols * kBK * 2;     // 16 KiB of B
+  static constexpr int kTBytes = kTokRows * kBK * 2;
+  static constexpr int kStageBytes = kWBytes + kTBytes;
+  static constexpr int kOutBytes = kGrpChunk * kGrpCols * 2;  // staging of one chunk
+  static constexpr int kOffW = 0;
+  static constexpr int kOffT = kOffW + STAGES * kWBytes;
+  static constexpr int kOffOut = kOffT + STAGES * kTBytes;
+  static constexpr int kOffBar = kOffOut + 2 * kOutBytes;
+  static constexpr int kNumBars = 2 * STAGES + 4 + 1;    // full, empty, tmem_full[2], tmem_empty[2], done
+  static constexpr int kOffMisc = kOffBar + kNumBars * 8;
+  static constexpr int kOffScan = kOffMisc + 16;         // 8 warp totals
+  static constexpr int kOffRows = kOffScan + 32;         // group starts [E + 1]
+  static constexpr int kOffTiles = kOffRows + (kMaxGroups + 1) * 4;  // first tile of each group [E + 1]
+  static constexpr int kUsed = kOffTiles + (kMaxGroups + 1) * 4;
+  static constexpr int kDynamicBytes = kUsed + 1024;
+  static constexpr uint32_t kTmemCols = 2 * TM;          // two accumulators
+  static_assert(TM % (32 * CG) == 0 && TM <= 256, "rows of a tile");
+  static_assert(kTBytes % 1024 == 0 && kOffOut % 1024 == 0, "swizzled tiles need 1024-byte alignment");
+  static_assert(kDynamicBytes <= 227 * 1024, "shared memory of one CTA");
+};
+
+// offsets[i], kept inside [0, T].
+__device__ __forceinline__ int group_offset(const void* offsets, int off64, int i, int T, bool& bad) {
+  const long long v = off64 ? static_cast<const long long*>(offsets)[i] : static_cast<const int*>(offsets)[i];
+  bad |= v < 0 || v > T;
+  return static_cast<int>(v < 0 ? 0 : (v > T ? T : v));
+}
+
+// Row tiles of a group of n rows: `count` tiles of `rows` rows each (the last
+// one may be shorter), rows a multiple of STEP and at most TM.  Equal tiles
+// rather than full ones and a rest: the same count with less padding.
+template <int TM, int STEP>
+__device__ __forceinline__ void row_tiles(int n, int& count, int& rows) {
+  count = (n + TM - 1) / TM;
+  rows = count ? ((n + count - 1) / count + STEP - 1) / STEP * STEP : STEP;
+}
+
+// Fills rows[0..E] with the group starts and first[0..E] with an exclusive
+// prefix sum of units(rows of the group); first[E] is the total.  Called by
+// all kNumThreads threads.  Offsets that decrease or leave [0, T] set the
+// error bit and are read as the nearest valid ones (a running maximum), so
+// that no group ever owns another's rows.
+template <class Units>
+__device__ __forceinline__ void scan_groups(const void* offsets, int off64, int E, int T, int* rows, int* first,
+                                            int* scratch, int* err, Units units) {
+  const int tid = static_cast<int>(threadIdx.x);
+  bool bad = false;
+  if (offsets == nullptr) {
+    if (tid == 0) {
+      rows[0] = 0;
+      rows[1] = T;
+    }
+  } else {
+    for (int i = tid; i <= E; i += kNumThreads) rows[i] = group_offset(offsets, off64, i, T, bad);
+  }
+  __syncthreads();
+  for (int i = tid; i < E; i += kNumThreads) bad |= rows[i + 1] < rows[i];
+  if (__syncthreads_or(bad ? 1 : 0)) {
+    if (tid == 0) {
+      for (int i = 0; i < E; ++i) rows[i + 1] = max(rows[i + 1], rows[i]);
+      atomicOr(err, kDevErrBadOffsets);
+    }
+    __syncthreads();
+  }
+  // each thread owns a run of consecutive groups
+  const int per = (E + kNumThreads - 1) / kNumThreads;
+  const int g0 = min(E, tid * per), g1 = min(E, g0 + per);
+  int sum = 0;
+  for (int g = g0; g < g1; ++g) sum += units(rows[g + 1] - rows[g]);
+  int run = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, run, d);
+    if ((tid & 31) >= d) run += up;
+  }
+  if ((tid & 31) == 31) scratch[tid >> 5] = run;
+  __syncthreads();
+  int base = run - sum;
+  for (int w = 0; w < (tid >> 5); ++w) base += scratch[w];
+  for (int g = g0; g < g1; ++g) {
+    first[g] = base;
+    base += units(rows[g + 1] - rows[g]);
+  }
+  if (tid == 0) {
+    int total = 0;
+    for (int w = 0; w < kNumThreads / 32; ++w) total += scratch[w];
+    first[E] = total;
+  }
+  __syncthreads();
+}
+
+// The group whose units hold unit u: the last g with first[g] <= u.
+__device__ __forceinline__ int find_group(const int* first, int E, int u) {
+  int lo = 0, hi = E - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (first[mid] <= u) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+struct GroupedUnit {
+  int e;      // group
+  int tn;     // column tile
+  int row0;   // first row of A and C
+  int rows;   // rows of C to store
+  int nmma;   // MMA N: rows rounded up
+};
+
+template <int CG, int TM>
+__device__ __forceinline__ GroupedUnit grouped_unit(const GroupedParams& p, const int* rows, const int* first, int t) {
+  GroupedUnit u;
+  u.e = find_group(first, p.E, t);
+  int count, tr;
+  row_tiles<TM, 16 * CG>(rows[u.e + 1] - rows[u.e], count, tr);
+  const int local = t - first[u.e];
+  const int per = kGrpRaster * p.tiles_n;
+  const int g = local / per;
+  const int gs = min(count - g * kGrpRaster, kGrpRaster);
+  const int r = local - g * per;
+  u.tn = r / gs;
+  u.row0 = rows[u.e] + (g * kGrpRaster + r % gs) * tr;
+  u.rows = min(tr, rows[u.e + 1] - u.row0);
+  u.nmma = (u.rows + 16 * CG - 1) / (16 * CG) * (16 * CG);
+  return u;
+}
+
+// Rows outside every group, written as zeros by the epilogue warps of the grid.
+__device__ __forceinline__ void zero_rows(const GroupedParams& p, int lo, int hi, int thread, int threads) {
+  const int outside = lo + (p.T - hi);
+  for (int i = static_cast<int>(blockIdx.x); i < outside; i += static_cast<int>(gridDim.x)) {
+    unsigned short* row = p.C + static_cast<long long>(i < lo ? i : hi + (i - lo)) * p.ldc;
+    int c = 0;
+    if (p.c_vec) {
+      for (c = thread * 8; c + 8 <= p.N; c += threads * 8) {
+        *reinterpret_cast<uint4*>(row + c) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      c = p.N / 8 * 8 + thread;
+    } else {
+      c = thread;
+    }
+    for (; c < p.N; c += threads) row[c] = 0;
+  }
+}
+
+template <int CG, int TM, int STAGES>
+__global__ void __launch_bounds__(kNumThreads, 1)
+    gemm_grouped_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                       const __grid_constant__ CUtensorMap tmC, const __grid_constant__ GroupedParams p) {
+  using Plan = GroupedPlan<CG, TM, STAGES>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sW = smem + Plan::kOffW;
+  uint8_t* sT = smem + Plan::kOffT;
+  uint8_t* sOut = smem + Plan::kOffOut;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + Plan::kOffBar);
+  uint64_t* empty_bar = full_bar + STAGES;
+  uint64_t* tfull_bar = empty_bar + STAGES;
+  uint64_t* tempty_bar = tfull_bar + 2;
+  uint64_t* done_bar = tempty_bar + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Plan::kOffMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* scan = reinterpret_cast<int*>(smem + Plan::kOffScan);
+  int* grp_rows = reinterpret_cast<int*>(smem + Plan::kOffRows);
+  int* grp_tiles = reinterpret_cast<int*>(smem + Plan::kOffTiles);
+
+  const int warp = static_cast<int>(threadIdx.x >> 5);
+  const int lane = static_cast<int>(threadIdx.x & 31);
+  const uint32_t rank = (CG == 2) ? cluster_ctarank() : 0u;
+  const bool leader = (rank == 0);
+  const int worker = static_cast<int>(blockIdx.x) / CG;
+  const int workers = static_cast<int>(gridDim.x) / CG;
+
+  if (threadIdx.x == 64) {
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(&tfull_bar[0], 1);
+    mbar_init(&tfull_bar[1], 1);
+    mbar_init(&tempty_bar[0], kEpiWarps * CG);
+    mbar_init(&tempty_bar[1], kEpiWarps * CG);
+    mbar_init(done_bar, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&tmA);
+    prefetch_tmap(&tmB);
+    if (p.c_tma) prefetch_tmap(&tmC);
+  }
+  if (warp == 1) {
+    __syncwarp();
+    tmem_alloc<CG>(tmem_slot, Plan::kTmemCols);
+    tmem_relinquish<CG>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  griddep_wait();
+
+  scan_groups(p.offsets, p.off64, p.E, p.T, grp_rows, grp_tiles, scan, p.err, [&](int n) {
+    int count, tr;
+    row_tiles<TM, Plan::kStep>(n, count, tr);
+    return count * p.tiles_n;
+  });
+  const int num_tiles = grp_tiles[p.E];
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int issued = 0;
+      bool ok = true;
+      for (int t = worker; ok && t < num_tiles; t += workers) {
+        const GroupedUnit u = grouped_unit<CG, TM>(p, grp_rows, grp_tiles, t);
+        const int half = u.nmma / CG;
+        const int arow = u.row0 + static_cast<int>(rank) * half;
+        const int bcol = (u.tn * CG + static_cast<int>(rank)) * kGrpCols;
+        const int boxes = (half + Plan::kBoxRows - 1) / Plan::kBoxRows;
+        const uint32_t bytes = Plan::kWBytes + boxes * Plan::kBoxRows * 128;
+        for (int kb = 0; kb < p.kb_total; ++kb) {
+          if (issued >= STAGES && !mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) {
+            ok = false;
+            break;
+          }
+          uint8_t* w_dst = sW + stage * Plan::kWBytes;
+          uint8_t* t_dst = sT + stage * Plan::kTBytes;
+          const int k0 = kb * kBK;
+          if constexpr (CG == 1) {
+            uint64_t* bar = &full_bar[stage];
+            mbar_arrive_expect_tx(bar, bytes);
+            if (p.b_kmaj) {
+              tma_load_3d(w_dst, &tmB, bar, k0, bcol, u.e);
+            } else {
+              tma_load_3d(w_dst, &tmB, bar, bcol, k0, u.e);
+              tma_load_3d(w_dst + kBK * 128, &tmB, bar, bcol + 64, k0, u.e);
+            }
+            for (int b = 0; b < boxes; ++b) {
+              tma_load_2d(t_dst + b * Plan::kBoxRows * 128, &tmA, bar, k0, arow + b * Plan::kBoxRows);
+            }
+          } else {
+            // both CTAs' bytes complete on the even CTA's barrier
+            if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * bytes);
+            const uint32_t bar = mapa_shared(smem_u32(&full_bar[stage]), 0);
+            if (p.b_kmaj) {
+              tma_load_3d_pair(w_dst, &tmB, bar, k0, bcol, u.e);
+            } else {
+              tma_load_3d_pair(w_dst, &tmB, bar, bcol, k0, u.e);
+              tma_load_3d_pair(w_dst + kBK * 128, &tmB, bar, bcol + 64, k0, u.e);
+            }
+            for (int b = 0; b < boxes; ++b) {
+              tma_load_2d_pair(t_dst + b * Plan::kBoxRows * 128, &tmA, bar, k0, arow + b * Plan::kBoxRows);
+            }
+          }
+          ++issued;
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      griddep_launch_dependents();
+      if (!ok) {
+        *abort_flag = 1;
+        atomicOr(p.err, kDevErrTimeoutProducer);
+      }
+      // every fill must have landed before the CTA exits (the odd CTA of a
+      // pair is covered by the cluster barrier at teardown)
+      if (leader) {
+        const int outstanding = issued < STAGES ? issued : STAGES;
+        for (int i = 0; i < outstanding; ++i) {
+          stage = (stage == 0) ? STAGES - 1 : stage - 1;
+          if (stage == STAGES - 1) phase ^= 1u;
+          const uint64_t t0 = globaltimer_ns();
+          while (!mbar_try_wait(&full_bar[stage], phase)) {
+            if (globaltimer_ns() - t0 > kWaitLimitNs) {
+              atomicOr(p.err, kDevErrTimeoutTeardown);
+              break;
+            }
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0 && leader) {
+      // descriptor strides of the two major orders: see gemm_sm100_kernel.cuh
+      const uint32_t w_lbo = p.b_kmaj ? 16 : kBK * 128, w_kstep = p.b_kmaj ? kUmmaK * 2 : kUmmaK * 128;
+      int stage = 0;
+      uint32_t phase = 0;
+      int acc = 0;
+      uint32_t acc_phase = 0;
+      int count = 0;
+      bool ok = true;
+      for (int t = worker; ok && t < num_tiles; t += workers) {
+        if (p.kb_total == 0) break;   // the epilogue writes act(bias) by itself
+        const GroupedUnit u = grouped_unit<CG, TM>(p, grp_rows, grp_tiles, t);
+        const uint32_t idesc = idesc_16bit(kGrpCols * CG, u.nmma, p.b_kmaj == 0, false, p.bf16 != 0);
+        if (count >= 2 && !mbar_wait(&tempty_bar[acc], acc_phase ^ 1u, abort_flag)) {
+          ok = false;
+          break;
+        }
+        ++count;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * TM);
+        for (int kb = 0; kb < p.kb_total; ++kb) {
+          if (!mbar_wait(&full_bar[stage], phase, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t w0 = smem_u32(sW + stage * Plan::kWBytes);
+          const uint32_t t0 = smem_u32(sT + stage * Plan::kTBytes);
+#pragma unroll
+          for (int j = 0; j < kBK / kUmmaK; ++j) {
+            mma_f16_ss<CG>(d_tmem, smem_desc_sw128(w0 + j * w_kstep, w_lbo, 1024),
+                           smem_desc_sw128(t0 + j * (kUmmaK * 2), 16, 1024), idesc, (kb > 0 || j > 0) ? 1u : 0u);
+          }
+          mma_commit<CG>(&empty_bar[stage]);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        mma_commit<CG>(&tfull_bar[acc]);
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1u;
+      }
+      if (!ok) {
+        *abort_flag = 1;
+        atomicOr(p.err, kDevErrTimeoutMma);
+      }
+      mma_commit<CG>(done_bar);
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(done_bar, 0)) {
+        if (globaltimer_ns() - t0 > kWaitLimitNs) {
+          atomicOr(p.err, kDevErrTimeoutTeardown);
+          break;
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int ew = warp & 3;                 // TMEM lane quarter of this warp
+    const int col = ew * 32 + lane;          // column inside this CTA's 128
+    const int et = static_cast<int>(threadIdx.x) - 64;
+    const bool bf16 = p.bf16 != 0;
+    const uint32_t tempty_remote0 = (CG == 2) ? mapa_shared(smem_u32(&tempty_bar[0]), 0) : 0u;
+    if (p.zero_rest) zero_rows(p, grp_rows[0], grp_rows[p.E], et, 32 * kEpiWarps);
+    int buf_i = 0;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int t = worker; t < num_tiles; t += workers) {
+      const GroupedUnit u = grouped_unit<CG, TM>(p, grp_rows, grp_tiles, t);
+      const int n0 = (u.tn * CG + static_cast<int>(rank)) * kGrpCols;
+      const int n = n0 + col;
+      const float bias =
+          (p.bias != nullptr && n < p.N) ? from_16bit(p.bias[static_cast<long long>(u.e) * p.N + n], bf16) : 0.0f;
+      bool got = true;
+      if (p.kb_total > 0 && lane == 0) got = mbar_wait(&tfull_bar[acc], acc_phase, abort_flag);
+      got = __shfl_sync(0xffffffffu, got ? 1 : 0, 0) != 0;
+      ok = named_bar_and(1, 32 * kEpiWarps, got);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t tbase = tmem_base + (static_cast<uint32_t>(ew * 32) << 16) + static_cast<uint32_t>(acc * TM);
+#pragma unroll 1
+      for (int r0 = 0; r0 < u.rows; r0 += kGrpChunk) {
+        uint32_t v[32];
+        if (p.kb_total > 0) {
+          tmem_ld_32x32b_x32(tbase + r0, v);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0u;
+        }
+        // A TMA store clips its box at the tensor's edge in units larger than
+        // an element (with an odd N it wrote past the end of the rows), so an
+        // edge tile goes by TMA only when the rows end on a 16-byte boundary.
+        const bool whole = p.c_tma && r0 + kGrpChunk <= u.rows &&
+                           (n0 + kGrpCols <= p.N || (n0 < p.N && p.N % 8 == 0));
+        uint8_t* buf = sOut + buf_i * Plan::kOutBytes;
+        buf_i ^= 1;
+        // the store issued from this buffer two chunks ago has read it
+        if (p.c_tma && et == 0) bulk_wait_group_read<1>();
+        named_bar_sync(1, 32 * kEpiWarps);
+        const uint32_t dst = smem_u32(buf) + col * 2;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float x = apply_act(__uint_as_float(v[i]) + bias, p.act);
+          st_shared_u16(dst + i * (kGrpCols * 2), to_16bit(x, bf16));
+        }
+        if (whole) fence_proxy_async_smem();
+        named_bar_sync(1, 32 * kEpiWarps);
+        if (et == 0 && p.c_tma) {
+          if (whole) tma_store_2d(&tmC, buf, n0, u.row0 + r0);
+          bulk_commit_group();   // empty when the chunk is stored below: the count above stays per buffer
+        }
+        if (!whole) {
+          const int valid = min(kGrpChunk, u.rows - r0);
+          unsigned short* crow = p.C + static_cast<long long>(u.row0 + r0) * p.ldc;
+          if (p.c_vec) {
+            const int seg = (et & 15) * 8;
+            for (int r = et >> 4; r < valid; r += 8) {
+              const unsigned short* src = reinterpret_cast<const unsigned short*>(buf + r * (kGrpCols * 2)) + seg;
+              unsigned short* out = crow + r * p.ldc + n0 + seg;
+              if (n0 + seg + 8 <= p.N) {
+                *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(src);
+              } else {
+                for (int c = 0; c < 8 && n0 + seg + c < p.N; ++c) out[c] = src[c];
+              }
+            }
+          } else if (n < p.N) {
+            for (int r = 0; r < valid; ++r) {
+              crow[r * p.ldc + n] = *(reinterpret_cast<const unsigned short*>(buf + r * (kGrpCols * 2)) + col);
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0 && p.kb_total > 0) {
+        if constexpr (CG == 1) {
+          mbar_arrive(&tempty_bar[acc]);
+        } else {
+          mbar_arrive_cluster(tempty_remote0 + static_cast<uint32_t>(acc * 8));
+        }
+      }
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1u;
+    }
+    if (!ok) {
+      *abort_flag = 1;
+      atomicOr(p.err, kDevErrTimeoutEpilogue);
+    }
+    if (p.c_tma && et == 0) bulk_wait_group_read<0>();
+  }
+
+  // ------------------------------------------------------------ teardown
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<CG>(tmem_base, Plan::kTmemCols);
+  }
+}
+
+}  // namespace idb

@@ -6,6 +6,7 @@
 #pragma once
 #include <cstdint>
 #include <cuda.h>
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 namespace idb {
@@ -22,6 +23,8 @@ enum : int {
   kDevErrTimeoutEpilogue = 1 << 2,
   kDevErrTimeoutTeardown = 1 << 3,
   kDevErrTimeoutSelfTest = 1 << 4,   // gemm_selftest_wait_timeout
+  kDevErrBadOffsets = 1 << 5,        // group offsets that decrease or leave [0, rows]
+  kDevErrBadAdapter = 1 << 6,        // an adapter index at or past the number of adapters
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -185,6 +188,31 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
       " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(m)), "r"(bar_cluster_addr), "r"(x), "r"(y)
       : "memory");
+}
+
+// 3-D forms (z = outermost: the expert or adapter of a stacked weight).
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* m, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* m, uint32_t bar_cluster_addr, int x,
+                                                 int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, const void* src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(m)),
+               "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z)
+               : "memory");
 }
 
 // 2-D tiled TMA store from shared memory (bulk-group completion).
@@ -373,6 +401,21 @@ __host__ __device__ constexpr uint32_t idesc_f16_f32(int m, int n, bool a_mn_maj
          | (static_cast<uint32_t>(b_mn_major) << 16)    // B major
          | (static_cast<uint32_t>(n >> 3) << 17)        // N >> 3
          | (static_cast<uint32_t>(m >> 4) << 24);       // M >> 4
+}
+
+// The same for either 16-bit input type (both operands alike), with shapes
+// known at run time.
+__device__ __forceinline__ uint32_t idesc_16bit(int m, int n, bool a_mn_major, bool b_mn_major, bool bf16) {
+  return idesc_f16_f32(m, n, a_mn_major, b_mn_major) | (bf16 ? (1u << 7) | (1u << 10) : 0u);
+}
+
+// fp32 -> the bits of the 16-bit type, rounded to nearest even, and back.
+__device__ __forceinline__ unsigned short to_16bit(float x, bool bf16) {
+  return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(x)) : __half_as_ushort(__float2half_rn(x));
+}
+
+__device__ __forceinline__ float from_16bit(unsigned short h, bool bf16) {
+  return bf16 ? __bfloat162float(__ushort_as_bfloat16(h)) : __half2float(__ushort_as_half(h));
 }
 
 // fp32 pair -> packed fp16x2 (round to nearest even), as __float2half does.

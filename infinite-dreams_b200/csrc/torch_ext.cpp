@@ -8,6 +8,7 @@
 // Exported (all asynchronous on the current stream of A's device):
 //   gemm_forward_cfg(A, B, cfg_id, out=None) -> C             (gemm_ext.cpp:95-106)
 //   gemm_ex(A, B, cfg_id, alpha, beta, C, bias, act, out) -> out
+//   grouped_gemm(A, B, offsets, bias, act, out) -> out
 //   reset_workspaces()
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -135,6 +136,121 @@ at::Tensor gemm_ex(const at::Tensor& A, const at::Tensor& B, int64_t cfg_id, dou
   return C;
 }
 
+// Scratch of one call of the operators below: the cached workspace, or, while
+// the stream is being captured, memory of the graph's own pool with its
+// tickets cleared by the graph.  Two graphs captured on one stream may be
+// replayed on two, so they must not share the cached buffer.
+struct Scratch {
+  at::Tensor owned;
+  void* ptr = nullptr;
+  size_t len = 0;
+};
+
+Scratch scratch(const at::Device& dev, cudaStream_t stream, size_t nbytes) {
+  Scratch s;
+  if (nbytes == 0) return s;
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) {
+    s.ptr = workspace(dev, stream, nbytes, &s.len);
+    return s;
+  }
+  s.owned = at::empty({static_cast<int64_t>(nbytes)}, at::TensorOptions().dtype(at::kByte).device(dev));
+  s.ptr = s.owned.data_ptr();
+  s.len = nbytes;
+  C10_CUDA_CHECK(cudaMemsetAsync(s.ptr, 0, std::min(nbytes, gemm_workspace_counter_bytes()), stream));
+  return s;
+}
+
+bool is_16bit(const at::Tensor& t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }
+
+int dtype_id(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? GEMM_DTYPE_BF16 : GEMM_DTYPE_F16; }
+
+void check_like(const at::Tensor& t, const at::Tensor& A, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == A.device(), name, " must be on A's device");
+  TORCH_CHECK(t.scalar_type() == A.scalar_type(), name, " must have A's dtype");
+}
+
+void check_index(const at::Tensor& t, const at::Tensor& A, int64_t n, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == A.device(), name, " must be on A's device");
+  TORCH_CHECK(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must be int32 or int64");
+  TORCH_CHECK(t.dim() == 1 && t.size(0) == n, name, " must be 1D with ", n, " elements");
+}
+
+void check_no_grad(const char* what, std::initializer_list<at::Tensor> ts) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const at::Tensor& t : ts) {
+    TORCH_CHECK(!t.defined() || !t.requires_grad(), what);
+  }
+}
+
+// A stack of weights [E, R, C] read in place: (tensor, trans, pitch, stride
+// from one matrix to the next); strides that are neither row-major nor
+// transposed, or matrices that overlap (expanded weights), are copied.
+std::tuple<at::Tensor, int, int64_t, int64_t> stacked_operand(const at::Tensor& X) {
+  const int64_t E = X.size(0), R = X.size(1), Cc = X.size(2), se = X.stride(0), s0 = X.stride(1), s1 = X.stride(2);
+  if ((s1 == 1 || Cc <= 1) && s0 >= std::max<int64_t>(Cc, 1) && (E == 1 || se >= (R - 1) * s0 + Cc)) {
+    return {X, 0, s0, se};
+  }
+  if ((s0 == 1 || R <= 1) && s1 >= std::max<int64_t>(R, 1) && (E == 1 || se >= (Cc - 1) * s1 + R)) {
+    return {X, 1, s1, se};
+  }
+  return {X.contiguous(), 0, std::max<int64_t>(Cc, 1), R * std::max<int64_t>(Cc, 1)};
+}
+
+// Rows read as they are when their elements are adjacent, else copied.
+at::Tensor row_operand(const at::Tensor& X) {
+  const bool ok = (X.stride(1) == 1 || X.size(1) <= 1) && (X.size(0) <= 1 || X.stride(0) >= X.size(1));
+  return ok ? X : X.contiguous();
+}
+
+int64_t pitch(const at::Tensor& X) {
+  return X.size(0) <= 1 ? std::max<int64_t>(X.size(1), 1) : std::max<int64_t>(X.stride(0), 1);
+}
+
+at::Tensor rows_out(const c10::optional<at::Tensor>& out, int64_t T, int64_t N, const at::Tensor& A) {
+  if (!out.has_value()) return at::empty({T, N}, A.options().requires_grad(false));
+  const at::Tensor& C = *out;
+  TORCH_CHECK(C.is_cuda() && C.device() == A.device() && C.scalar_type() == A.scalar_type() && C.dim() == 2 &&
+                  C.size(0) == T && C.size(1) == N && (C.stride(1) == 1 || N <= 1) && (T <= 1 || C.stride(0) >= N),
+              "out must be a (T x N) tensor of A's dtype with unit column stride on A's device");
+  return C;
+}
+
+at::Tensor grouped_gemm(const at::Tensor& A, const at::Tensor& B, const at::Tensor& offsets,
+                        c10::optional<at::Tensor> bias, int64_t act, c10::optional<at::Tensor> out) {
+  TORCH_CHECK(A.is_cuda(), "A must be CUDA tensor");
+  TORCH_CHECK(is_16bit(A), "A must be float16 or bfloat16");
+  TORCH_CHECK(A.dim() == 2, "A must be 2D (T x K)");
+  check_like(B, A, "B");
+  TORCH_CHECK(B.dim() == 3, "B must be 3D (E x K x N)");
+  TORCH_CHECK(A.size(1) == B.size(1), "Inner dimensions must match: A is (T x K), B is (E x K x N)");
+  TORCH_CHECK(B.size(0) >= 1, "B must hold at least one group");
+  check_index(offsets, A, B.size(0) + 1, "offsets");
+  const int64_t T = A.size(0), K = A.size(1), E = B.size(0), N = B.size(2);
+  at::Tensor bvec;
+  if (bias.has_value()) {
+    check_like(*bias, A, "bias");
+    TORCH_CHECK(bias->dim() == 2 && bias->size(0) == E && bias->size(1) == N, "bias must be (E x N)");
+    bvec = bias->contiguous();
+  }
+  check_no_grad("grouped_gemm computes no gradients: use grouped.grouped_linear, or call it under torch.no_grad()",
+                {A, B, bvec});
+  const c10::cuda::CUDAGuard guard(A.device());
+  at::Tensor As = row_operand(A), off = offsets.contiguous();
+  auto [Bs, tb, ldb, sb] = stacked_operand(B);
+  at::Tensor C = rows_out(out, T, N, A);
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream(A.device().index()).stream();
+  const int64_t lda = pitch(As);
+  Scratch ws = scratch(A.device(), stream, gemm_grouped_workspace_bytes(As.data_ptr(), Bs.data_ptr(), T, N, K, E, lda,
+                                                                        ldb, sb, tb));
+  check_status(gemm_grouped_launch(As.data_ptr(), Bs.data_ptr(), C.data_ptr(), off.data_ptr(),
+                                   off.scalar_type() == at::kLong ? 64 : 32, T, N, K, E, lda, ldb, sb,
+                                   std::max<int64_t>(pitch(C), N), tb, bvec.defined() ? bvec.data_ptr() : nullptr,
+                                   static_cast<int>(act), out.has_value() ? 0 : 1, dtype_id(A), ws.ptr, ws.len,
+                                   stream),
+               "gemm_grouped_launch");
+  return C;
+}
+
 void reset_workspaces() {
   std::lock_guard<std::mutex> lock(g_ws_mu);
   g_ws->clear();
@@ -149,5 +265,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm_ex", &gemm_ex, "out = act(alpha * A @ B + beta * C + bias)", py::arg("A"), py::arg("B"),
         py::arg("cfg_id"), py::arg("alpha") = 1.0, py::arg("beta") = 0.0, py::arg("C") = py::none(),
         py::arg("bias") = py::none(), py::arg("act") = 0, py::arg("out") = py::none());
+  m.def("grouped_gemm", &grouped_gemm, "out[r] = act(A[r] @ B[group of r] + bias[group of r])", py::arg("A"),
+        py::arg("B"), py::arg("offsets"), py::arg("bias") = py::none(), py::arg("act") = 0,
+        py::arg("out") = py::none());
   m.def("reset_workspaces", &reset_workspaces, "drop the cached split-K / repack workspaces");
 }

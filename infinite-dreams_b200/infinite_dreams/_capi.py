@@ -28,6 +28,9 @@ GEMM_ACT_RELU = 1
 GEMM_ACT_GELU = 2
 ACTIVATIONS = {"none": GEMM_ACT_NONE, "relu": GEMM_ACT_RELU, "gelu": GEMM_ACT_GELU}
 
+GEMM_DTYPE_F16 = 0
+GEMM_DTYPE_BF16 = 1
+
 # (name, restype, argtypes) of every exported entry point.
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
@@ -50,6 +53,10 @@ _SIG = [
       _P, _I64, _P, ctypes.c_int, ctypes.c_int, _P, ctypes.c_size_t, _P]),
     ("gemm_workspace_bytes_ex", ctypes.c_size_t,
      [_P, _P, _I64, _I64, _I64, _I64, _I64, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    ("gemm_grouped_launch", ctypes.c_int,
+     [_P, _P, _P, _P, ctypes.c_int] + [_I64] * 8 + [ctypes.c_int, _P, ctypes.c_int, ctypes.c_int, ctypes.c_int, _P,
+      ctypes.c_size_t, _P]),
+    ("gemm_grouped_workspace_bytes", ctypes.c_size_t, [_P, _P] + [_I64] * 7 + [ctypes.c_int]),
     ("gemm_launch_gather", ctypes.c_int,
      [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, ctypes.POINTER(ctypes.c_void_p), ctypes.c_int, ctypes.c_int,
       _P, ctypes.c_size_t, _P]),

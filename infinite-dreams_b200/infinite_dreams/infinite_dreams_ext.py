@@ -16,7 +16,9 @@ by the sm_100a kernel bank through its C ABI (include/gemm_sm100.h):
   ``[num_cfg, len(CFG_COLUMNS)]`` (src/gemm_ext.cpp:108-120).
 
 ``gemm_ex`` goes beyond the reference: transposed operand views read in
-place and a fused epilogue (alpha, beta * C, bias, ReLU / GELU).
+place and a fused epilogue (alpha, beta * C, bias, ReLU / GELU).  So do the
+products whose weight is picked by the row, in fp16 and bf16:
+``grouped_gemm`` (rows sorted by expert, ragged counts).
 
 Like the reference, inputs are made contiguous, C is allocated from torch's
 caching allocator on A's device, and the launch is asynchronous on the
@@ -239,6 +241,144 @@ def gemm_ex(A: torch.Tensor, B: torch.Tensor, *, alpha: float = 1.0, beta: float
     return out
 
 
+def _scratch(device: torch.device, stream: torch.cuda.Stream, nbytes: int):
+    """(keep-alive, pointer, bytes) of one call's workspace.
+
+    While the stream is captured the memory comes from the graph's own pool,
+    its tickets cleared by the graph: two graphs captured on one stream may be
+    replayed on two, so they must not share the cached buffer.
+    """
+    if nbytes == 0:
+        return None, None, 0
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws[:int(lib.gemm_workspace_counter_bytes())].zero_()
+        return ws, ws.data_ptr(), nbytes
+    ptr, size = _workspace(device, stream, nbytes)
+    return None, ptr, size
+
+
+def _is_16bit(t) -> bool:
+    return t.dtype in (torch.float16, torch.bfloat16)
+
+
+def _dtype_id(t: torch.Tensor) -> int:
+    return _capi.GEMM_DTYPE_BF16 if t.dtype == torch.bfloat16 else _capi.GEMM_DTYPE_F16
+
+
+def _check_like(t, A: torch.Tensor, name: str) -> None:
+    if not isinstance(t, torch.Tensor) or t.device != A.device:
+        raise RuntimeError(f"{name} must be on A's device")
+    if t.dtype != A.dtype:
+        raise RuntimeError(f"{name} must have A's dtype")
+
+
+def _check_index(t, A: torch.Tensor, n: int, name: str) -> None:
+    if not isinstance(t, torch.Tensor) or t.device != A.device:
+        raise RuntimeError(f"{name} must be on A's device")
+    if t.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError(f"{name} must be int32 or int64")
+    if t.dim() != 1 or t.size(0) != n:
+        raise RuntimeError(f"{name} must be 1D with {n} elements")
+
+
+def _check_no_grad(what: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(what)
+
+
+def _stacked_operand(X: torch.Tensor) -> Tuple[torch.Tensor, int, int, int]:
+    """(tensor, trans, pitch, matrix stride) of a stack of weights [E, R, C] read in place.
+
+    Strides that are neither row-major nor transposed, or matrices that
+    overlap (expanded weights), are copied.
+    """
+    E, R, C = X.shape
+    se, s0, s1 = X.stride()
+    if (s1 == 1 or C <= 1) and s0 >= max(C, 1) and (E == 1 or se >= (R - 1) * s0 + C):
+        return X, 0, s0, se
+    if (s0 == 1 or R <= 1) and s1 >= max(R, 1) and (E == 1 or se >= (C - 1) * s1 + R):
+        return X, 1, s1, se
+    return X.contiguous(), 0, max(C, 1), R * max(C, 1)
+
+
+def _row_operand(X: torch.Tensor) -> torch.Tensor:
+    ok = (X.stride(1) == 1 or X.size(1) <= 1) and (X.size(0) <= 1 or X.stride(0) >= X.size(1))
+    return X if ok else X.contiguous()
+
+
+def _pitch(X: torch.Tensor) -> int:
+    return max(X.size(1), 1) if X.size(0) <= 1 else max(X.stride(0), 1)
+
+
+def _rows_out(out: Optional[torch.Tensor], T: int, N: int, A: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty((T, N), dtype=A.dtype, device=A.device)
+    if (out.device != A.device or out.dtype != A.dtype or tuple(out.shape) != (T, N)
+            or (out.stride(1) != 1 and N > 1) or (T > 1 and out.stride(0) < N)):
+        raise RuntimeError("out must be a (T x N) tensor of A's dtype with unit column stride on A's device")
+    return out
+
+
+def grouped_gemm(A: torch.Tensor, B: torch.Tensor, offsets: torch.Tensor, *, bias: Optional[torch.Tensor] = None,
+                 activation: str = "none", out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out[r] = act(A[r] @ B[e] + bias[e]) for the rows offsets[e] <= r < offsets[e + 1] of group e.
+
+    A is [T, K] with its rows sorted by group, B a stack of weights [E, K, N]
+    (row-major, or a transposed view of [E, N, K] storage; both are read in
+    place), bias [E, N]; fp16 or bf16, all alike.  offsets: E + 1
+    non-decreasing int32 or int64 row numbers on the device; the call never
+    synchronises, and offsets that decrease or leave [0, T] are clamped and
+    reported by ``check_device_errors``.  Groups may be empty.  Rows outside
+    [offsets[0], offsets[E]) are zero in a new ``out`` and left as they are
+    in a given one.  The input gradient of a plain product is
+    ``grouped_gemm(dy, B.transpose(1, 2), offsets)``.  At most 1024 groups.
+    """
+    if activation not in _capi.ACTIVATIONS:
+        raise RuntimeError(f"activation must be one of {sorted(_capi.ACTIVATIONS)}")
+    act = _capi.ACTIVATIONS[activation]
+    if _fast is not None:
+        return _fast.grouped_gemm(A, B, offsets, bias, act, out)
+    if not isinstance(A, torch.Tensor) or not A.is_cuda:
+        raise RuntimeError("A must be CUDA tensor")
+    if not _is_16bit(A):
+        raise RuntimeError("A must be float16 or bfloat16")
+    if A.dim() != 2:
+        raise RuntimeError("A must be 2D (T x K)")
+    _check_like(B, A, "B")
+    if B.dim() != 3:
+        raise RuntimeError("B must be 3D (E x K x N)")
+    if A.size(1) != B.size(1):
+        raise RuntimeError("Inner dimensions must match: A is (T x K), B is (E x K x N)")
+    if B.size(0) < 1:
+        raise RuntimeError("B must hold at least one group")
+    E, K, N = B.shape
+    T = A.size(0)
+    _check_index(offsets, A, E + 1, "offsets")
+    if bias is not None:
+        _check_like(bias, A, "bias")
+        if tuple(bias.shape) != (E, N):
+            raise RuntimeError("bias must be (E x N)")
+        bias = bias.contiguous()
+    _check_no_grad("grouped_gemm computes no gradients: use grouped.grouped_linear, or call it under "
+                   "torch.no_grad()", A, B, bias)
+    with torch.cuda.device(A.device):
+        As, off = _row_operand(A), offsets.contiguous()
+        Bs, tb, ldb, sb = _stacked_operand(B)
+        C = _rows_out(out, T, N, A)
+        stream = torch.cuda.current_stream(A.device)
+        lda = _pitch(As)
+        need = lib.gemm_grouped_workspace_bytes(As.data_ptr(), Bs.data_ptr(), T, N, K, E, lda, ldb, sb, tb)
+        keep, ws_ptr, ws_len = _scratch(A.device, stream, need)
+        st = lib.gemm_grouped_launch(As.data_ptr(), Bs.data_ptr(), C.data_ptr(), off.data_ptr(),
+                                     64 if off.dtype == torch.int64 else 32, T, N, K, E, lda, ldb, sb,
+                                     max(_pitch(C), N), tb, bias.data_ptr() if bias is not None else None, act,
+                                     0 if out is not None else 1, _dtype_id(A), ws_ptr, ws_len,
+                                     stream.cuda_stream or None)
+        _capi.check(st, "gemm_grouped_launch")
+    return C
+
+
 def gemm_cfg_table_cpu() -> torch.Tensor:
     """CPU int32 tensor [num_cfg, len(CFG_COLUMNS)], columns CFG_COLUMNS."""
     cols, rows = _capi.menu()
@@ -250,14 +390,17 @@ def default_cfg(M: int, N: int, K: int) -> int:
 
 
 def check_device_errors(device: Optional[int] = None) -> None:
-    """Raises if a kernel on `device` gave up on a bounded wait (synchronises)."""
+    """Raises if a kernel on `device` gave up on a bounded wait, or was given offsets or adapter indices out of
+    range, since the last call (synchronises)."""
     dev = torch.cuda.current_device() if device is None else int(device)
     code = ctypes.c_int(0)
     st = lib.gemm_device_error(dev, ctypes.byref(code))
     if st != _capi.GEMM_OK:
-        reset_workspaces()
-        raise GemmError(st, f"device {dev}: kernel error bits {code.value}")
+        message = lib.gemm_last_error().decode(errors="replace")
+        if st != _capi.GEMM_ERR_INVALID_ARG:   # index data out of range leaves the workspaces clean
+            reset_workspaces()
+        raise GemmError(st, f"device {dev}: kernel error bits {code.value}: {message}")
 
 
-__all__ = ["gemm_forward", "gemm_forward_cfg", "gemm_ex", "gemm_cfg_table_cpu", "CFG_COLUMNS", "NUM_CFG",
+__all__ = ["gemm_forward", "gemm_forward_cfg", "gemm_ex", "grouped_gemm", "gemm_cfg_table_cpu", "CFG_COLUMNS", "NUM_CFG",
            "default_cfg", "check_device_errors", "GemmError", "reset_workspaces"]

@@ -1,0 +1,59 @@
+"""Refusals and workspace sizes of the grouped products: everything the host decides without a GPU."""
+import pytest
+import torch
+
+from infinite_dreams import _capi, infinite_dreams_ext as ext
+
+LIB = _capi.lib
+P = 1 << 20   # an aligned address that is never read
+
+
+def _launch(A=P, B=P, C=P, off=P, bits=32, T=8, N=8, K=8, E=2, lda=8, ldb=8, sb=64, ldc=8, tb=0, bias=None, act=0,
+            dtype=0):
+    return LIB.gemm_grouped_launch(A, B, C, off, bits, T, N, K, E, lda, ldb, sb, ldc, tb, bias, act, 1, dtype, None, 0,
+                                   None)
+
+
+@pytest.mark.parametrize("bad", [dict(T=-1), dict(K=-1), dict(E=0), dict(bits=16), dict(dtype=2), dict(tb=2),
+                                 dict(act=3), dict(A=None), dict(off=None), dict(C=None), dict(lda=7), dict(ldb=7),
+                                 dict(ldc=7), dict(sb=63), dict(A=P + 1), dict(bias=P + 1), dict(off=P + 2),
+                                 dict(off=P + 4, bits=64)], ids=str)
+def test_invalid_arguments(bad):
+    assert _launch(**bad) == _capi.GEMM_ERR_INVALID_ARG
+    assert LIB.gemm_last_error()
+
+
+def test_unsupported_and_missing_workspace():
+    assert _launch(E=1025) == _capi.GEMM_ERR_UNSUPPORTED
+    assert _launch(T=1 << 31) == _capi.GEMM_ERR_UNSUPPORTED
+    assert _launch(T=8, K=7, lda=7) == _capi.GEMM_ERR_WORKSPACE
+    assert _launch(T=0) == _capi.GEMM_OK and _launch(N=0, sb=0) == _capi.GEMM_OK   # nothing to do
+
+
+def test_workspace_sizes():
+    ws = LIB.gemm_grouped_workspace_bytes
+    head = LIB.gemm_workspace_counter_bytes()
+    assert ws(P, P, 8, 64, 64, 2, 64, 64, 64 * 64, 0) == 0
+    # rows of 77 elements are copied to 128: A, then both matrices of B
+    assert ws(P, P, 100, 64, 77, 2, 77, 64, 77 * 64, 0) == head + 100 * 128 * 2
+    assert ws(P, P, 100, 77, 64, 2, 64, 77, 64 * 77, 0) == head + 2 * 64 * 128 * 2
+    assert ws(P + 2, P, 100, 64, 64, 2, 64, 64, 64 * 64, 0) == head + 100 * 64 * 2
+    # a matrix stride that TMA cannot address
+    assert ws(P, P, 100, 64, 64, 2, 64, 64, 64 * 64 + 1, 0) == head + 2 * 64 * 64 * 2
+
+
+def test_torch_surface_refuses_cpu_tensors():
+    A, B = torch.zeros(4, 8, dtype=torch.float16), torch.zeros(2, 8, 8, dtype=torch.float16)
+    off = torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="A must be CUDA tensor"):
+        ext.grouped_gemm(A, B, off)
+    with pytest.raises(RuntimeError, match="activation must be one of"):
+        ext.grouped_gemm(A, B, off, activation="tanh")
+    keep, ext._fast = ext._fast, None
+    try:
+        with pytest.raises(RuntimeError, match="A must be CUDA tensor"):
+            ext.grouped_gemm(A, B, off)
+    finally:
+        ext._fast = keep
+
+
