@@ -155,6 +155,22 @@ int gemm_grouped_launch(const void* A, const void* B, void* C, const void* offse
 size_t gemm_grouped_workspace_bytes(const void* A, const void* B, int64_t T, int64_t N, int64_t K, int64_t E,
                                     int64_t lda, int64_t ldb, int64_t stride_b, int trans_b);
 
+/* Weight gradient of the grouped product:
+ *   D[e] = A_e^T * G_e,   A_e, G_e = rows [offsets[e], offsets[e + 1]) of A and G
+ *  A = T x M (pitch lda), G = T x N (pitch ldg), both read in place;
+ *  D = E matrices M x N (pitch ldd, stride_d elements apart); every element
+ *      is written, with zeros for an empty group.  For a gradient stored
+ *      N x M exchange A and G.
+ * offsets, dtype, limits and workspace as for gemm_grouped_launch; rows
+ * outside every group (inf and NaN included) do not enter.  The sums run in
+ * row order: results do not vary from call to call.  No counterpart in the
+ * reference. */
+int gemm_grouped_wgrad_launch(const void* A, const void* G, void* D, const void* offsets, int offsets_bits, int64_t T,
+                              int64_t M, int64_t N, int64_t E, int64_t lda, int64_t ldg, int64_t ldd, int64_t stride_d,
+                              int dtype, void* workspace, size_t workspace_bytes, void* stream);
+size_t gemm_grouped_wgrad_workspace_bytes(const void* A, const void* G, int64_t T, int64_t M, int64_t N, int64_t lda,
+                                          int64_t ldg);
+
 /* Fused all-gather for M-row sharding over the GPUs of one node (one
  * process per GPU).  Same as gemm_launch, and each finished tile of C is
  * also stored, over NVLink, at the same offset and pitch ldc into

@@ -719,10 +719,22 @@ int capi_encode(CUtensorMap* map, const void* base, int rank, const int64_t* ext
     boxes[i] = static_cast<cuuint32_t>(box[i]);
     if (i + 1 < rank) bytes[i] = static_cast<cuuint64_t>(strides[i]) * 2;
   }
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims,
-                  bytes, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, bytes,
+              boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    // A thread that has made no runtime call yet (an autograd worker) has no
+    // current context for this driver call; setting its device binds one.
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaSetDevice(dev);
+    if (e != cudaSuccess) return fail_cuda(e, "cudaSetDevice");
+    r = encode();
+  }
   if (r != CUDA_SUCCESS) {
     return fail(GEMM_ERR_CUDA, std::string("cuTensorMapEncodeTiled(") + what + ") failed with CUresult " +
                                    std::to_string(static_cast<int>(r)));

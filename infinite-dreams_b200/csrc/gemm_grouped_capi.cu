@@ -115,13 +115,13 @@ cudaError_t opt_in(Kernel kernel, int bytes, std::atomic<unsigned long long>& co
 }
 
 template <int CG, class Kernel, class... Args>
-cudaError_t launch(Kernel kernel, int bytes, std::atomic<unsigned long long>& configured, int grid,
+cudaError_t launch(Kernel kernel, int threads, int bytes, std::atomic<unsigned long long>& configured, int grid,
                    cudaStream_t stream, const Args&... args) {
   cudaError_t e = opt_in(kernel, bytes, configured);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
-  cfg.blockDim = dim3(kNumThreads, 1, 1);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
   cfg.dynamicSmemBytes = static_cast<size_t>(bytes);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -165,9 +165,32 @@ int launch_grouped(const Operand& a, const Operand& b, const GroupedParams& gp, 
   const int64_t most = std::min<int64_t>(row_tiles * p.tiles_n, sms / CG);
   const int grid = static_cast<int>(most < 1 ? 1 : most) * CG;
   static std::atomic<unsigned long long> configured{0};
-  cudaError_t e = launch<CG>(gemm_grouped_sm100<CG, TM, STAGES>, Plan::kDynamicBytes, configured, grid, stream, tmA,
-                             tmB, tmC, p);
+  cudaError_t e = launch<CG>(gemm_grouped_sm100<CG, TM, STAGES>, kNumThreads, Plan::kDynamicBytes, configured, grid,
+                             stream, tmA, tmB, tmC, p);
   return e == cudaSuccess ? GEMM_OK : capi_fail_cuda(e, "grouped gemm kernel launch");
+}
+
+constexpr int kWgradStages = 6;
+
+int launch_wgrad(const Operand& a, const Operand& g, const WgradParams& p, int sms, cudaStream_t stream) {
+  using Plan = WgradPlan<kWgradStages>;
+  CUtensorMap tmA, tmG, tmD;
+  std::memset(&tmD, 0, sizeof(tmD));
+  int st = a.encode2(&tmA, 64, kBK, true, "A");
+  if (st == GEMM_OK) st = g.encode2(&tmG, 64, kBK, true, "G");
+  if (st != GEMM_OK) return st;
+  if (p.d_tma) {
+    const int64_t ext[3] = {p.N, p.M, p.E}, str[2] = {p.ldd, p.E == 1 ? round_up(p.M * p.ldd, 8) : p.stride_d};
+    const int box[3] = {kStoreCols, kStoreRows, 1};
+    st = capi_encode(&tmD, p.D, 3, ext, str, box, true, "D");
+    if (st != GEMM_OK) return st;
+  }
+  const int64_t tiles = static_cast<int64_t>(p.E) * p.tiles_m * p.tiles_n;
+  const int grid = static_cast<int>(std::min<int64_t>(tiles, sms / 2)) * 2;
+  static std::atomic<unsigned long long> configured{0};
+  cudaError_t e = launch<2>(gemm_grouped_wgrad_sm100<kWgradStages>, kWgradThreads, Plan::kDynamicBytes, configured,
+                            grid, stream, tmA, tmG, tmD, p);
+  return e == cudaSuccess ? GEMM_OK : capi_fail_cuda(e, "grouped weight gradient kernel launch");
 }
 
 Operand operand_b(const void* B, int64_t E, int64_t N, int64_t K, int64_t ldb, int64_t stride_b, int trans_b) {
@@ -258,6 +281,81 @@ int gemm_grouped_launch(const void* A, const void* B, void* C, const void* offse
   // rows, which read every weight once per 256 rows.
   if (T <= 64 * E || N <= kGrpCols) return launch_grouped<1, 64, 8>(a, b, p, sms, stream);
   return launch_grouped<2, 256, 6>(a, b, p, sms, stream);
+}
+
+size_t gemm_grouped_wgrad_workspace_bytes(const void* A, const void* G, int64_t T, int64_t M, int64_t N, int64_t lda,
+                                          int64_t ldg) {
+  if (T <= 0 || M <= 0 || N <= 0) return 0;
+  Operand a(A, 1, T, M, lda, 0), g(G, 1, T, N, ldg, 0);
+  const size_t head = align256(gemm_workspace_counter_bytes());
+  size_t off = head;
+  a.plan(&off);
+  g.plan(&off);
+  return off == head ? 0 : off;
+}
+
+int gemm_grouped_wgrad_launch(const void* A, const void* G, void* D, const void* offsets, int offsets_bits, int64_t T,
+                              int64_t M, int64_t N, int64_t E, int64_t lda, int64_t ldg, int64_t ldd, int64_t stride_d,
+                              int dtype, void* workspace, size_t workspace_bytes, void* stream_v) {
+  capi_clear_error();
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  int st = check_common(T, N, M, E, offsets_bits, dtype, "the number of groups");
+  if (st != GEMM_OK) return st;
+  if (E > kMaxGroups) {
+    return capi_fail(GEMM_ERR_UNSUPPORTED, "at most " + std::to_string(kMaxGroups) + " groups");
+  }
+  if (M == 0 || N == 0) return GEMM_OK;
+  if (!D || (T > 0 && (!A || !G || !offsets))) {
+    return capi_fail(GEMM_ERR_INVALID_ARG, "A, G, D and offsets must be non-null");
+  }
+  if ((T > 0 && (lda < M || ldg < N)) || ldd < N || (E > 1 && stride_d < (M - 1) * ldd + N)) {
+    return capi_fail(GEMM_ERR_INVALID_ARG, "pitches must satisfy lda >= M, ldg >= N, ldd >= N, and stride_d one "
+                                           "matrix of D");
+  }
+  if (misaligned(A) || misaligned(G) || misaligned(D)) {
+    return capi_fail(GEMM_ERR_INVALID_ARG, "A, G and D must be 2-byte aligned");
+  }
+  if (reinterpret_cast<uintptr_t>(offsets) % (offsets_bits / 8) != 0) {
+    return capi_fail(GEMM_ERR_INVALID_ARG, "offsets must be aligned to their width");
+  }
+  WgradParams p = {};
+  const int64_t tm = (M + kWgradTile - 1) / kWgradTile, tn = (N + kWgradTile - 1) / kWgradTile;
+  if (tm * tn > kInt32Max / E) return capi_fail(GEMM_ERR_UNSUPPORTED, "too many output tiles");
+  Operand a(A, 1, T, M, lda, 0), g(G, 1, T, N, ldg, 0);
+  const size_t head = align256(gemm_workspace_counter_bytes());
+  size_t off = head;
+  a.plan(&off);
+  g.plan(&off);
+  st = check_workspace(off == head ? 0 : off, workspace, workspace_bytes);
+  if (st != GEMM_OK) return st;
+  int sms = 0;
+  st = capi_device(&sms, &p.err);
+  if (st != GEMM_OK) return st;
+  if (T == 0) {   // no rows: every gradient is zero
+    for (int64_t e = 0; e < E; ++e) {
+      cudaError_t ce = cudaMemset2DAsync(static_cast<uint8_t*>(D) + e * stride_d * 2, static_cast<size_t>(ldd) * 2, 0,
+                                         static_cast<size_t>(N) * 2, static_cast<size_t>(M), stream);
+      if (ce != cudaSuccess) return capi_fail_cuda(ce, "cudaMemset2DAsync");
+    }
+    return GEMM_OK;
+  }
+  st = a.make(static_cast<uint8_t*>(workspace), stream);
+  if (st == GEMM_OK) st = g.make(static_cast<uint8_t*>(workspace), stream);
+  if (st != GEMM_OK) return st;
+  p.offsets = offsets;
+  p.off64 = offsets_bits == 64;
+  p.E = static_cast<int>(E);
+  p.T = static_cast<int>(T);
+  p.M = static_cast<int>(M);
+  p.N = static_cast<int>(N);
+  p.tiles_m = static_cast<int>(tm);
+  p.tiles_n = static_cast<int>(tn);
+  p.bf16 = dtype == GEMM_DTYPE_BF16;
+  p.D = static_cast<unsigned short*>(D);
+  p.ldd = ldd;
+  p.stride_d = E == 1 ? 0 : stride_d;
+  p.d_tma = reinterpret_cast<uintptr_t>(D) % 16u == 0 && ldd % 8 == 0 && (E == 1 || stride_d % 8 == 0);
+  return launch_wgrad(a, g, p, sms, stream);
 }
 
 }  // extern "C"

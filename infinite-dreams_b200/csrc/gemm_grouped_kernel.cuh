@@ -102,10 +102,10 @@ __device__ __forceinline__ void row_tiles(int n, int& count, int& rows) {
 
 // Fills rows[0..E] with the group starts and first[0..E] with an exclusive
 // prefix sum of units(rows of the group); first[E] is the total.  Called by
-// all kNumThreads threads.  Offsets that decrease or leave [0, T] set the
+// all NT threads of the CTA.  Offsets that decrease or leave [0, T] set the
 // error bit and are read as the nearest valid ones (a running maximum), so
 // that no group ever owns another's rows.
-template <class Units>
+template <int NT, class Units>
 __device__ __forceinline__ void scan_groups(const void* offsets, int off64, int E, int T, int* rows, int* first,
                                             int* scratch, int* err, Units units) {
   const int tid = static_cast<int>(threadIdx.x);
@@ -116,10 +116,10 @@ __device__ __forceinline__ void scan_groups(const void* offsets, int off64, int 
       rows[1] = T;
     }
   } else {
-    for (int i = tid; i <= E; i += kNumThreads) rows[i] = group_offset(offsets, off64, i, T, bad);
+    for (int i = tid; i <= E; i += NT) rows[i] = group_offset(offsets, off64, i, T, bad);
   }
   __syncthreads();
-  for (int i = tid; i < E; i += kNumThreads) bad |= rows[i + 1] < rows[i];
+  for (int i = tid; i < E; i += NT) bad |= rows[i + 1] < rows[i];
   if (__syncthreads_or(bad ? 1 : 0)) {
     if (tid == 0) {
       for (int i = 0; i < E; ++i) rows[i + 1] = max(rows[i + 1], rows[i]);
@@ -128,7 +128,7 @@ __device__ __forceinline__ void scan_groups(const void* offsets, int off64, int 
     __syncthreads();
   }
   // each thread owns a run of consecutive groups
-  const int per = (E + kNumThreads - 1) / kNumThreads;
+  const int per = (E + NT - 1) / NT;
   const int g0 = min(E, tid * per), g1 = min(E, g0 + per);
   int sum = 0;
   for (int g = g0; g < g1; ++g) sum += units(rows[g + 1] - rows[g]);
@@ -148,7 +148,7 @@ __device__ __forceinline__ void scan_groups(const void* offsets, int off64, int 
   }
   if (tid == 0) {
     int total = 0;
-    for (int w = 0; w < kNumThreads / 32; ++w) total += scratch[w];
+    for (int w = 0; w < NT / 32; ++w) total += scratch[w];
     first[E] = total;
   }
   __syncthreads();
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(kNumThreads, 1)
   const uint32_t tmem_base = *tmem_slot;
   griddep_wait();
 
-  scan_groups(p.offsets, p.off64, p.E, p.T, grp_rows, grp_tiles, scan, p.err, [&](int n) {
+  scan_groups<kNumThreads>(p.offsets, p.off64, p.E, p.T, grp_rows, grp_tiles, scan, p.err, [&](int n) {
     int count, tr;
     row_tiles<TM, Plan::kStep>(n, count, tr);
     return count * p.tiles_n;
@@ -515,6 +515,423 @@ __global__ void __launch_bounds__(kNumThreads, 1)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc<CG>(tmem_base, Plan::kTmemCols);
+  }
+}
+
+
+// ------------------------------------------------------------------- weight gradient
+//
+//   D[e] = A_e^T G_e,   A_e, G_e = rows off[e] .. off[e + 1] of A [T, M] and G [T, N]
+//
+// A 256 x 256 tile of D[e] per CTA pair; the reduction runs over the group's
+// rows, 64 per pipeline stage.  Both operands are read as they are stored:
+// their rows are the MMA's K and their columns its M and N, i.e. both are
+// MN-major (64-column atoms of 64 rows x 128 bytes).
+//
+// The rows of a group end anywhere, and the stage that holds the last ones
+// also holds the next group's first ones (or inf / NaN behind the last row).
+// Those must be zero in BOTH operands, since 0 * inf is not 0.  So the last
+// stage of a cut group lands on a barrier of its own, a sixth warp zeroes the
+// rows up to the next multiple of 16 in shared memory (a row of an atom is
+// 128 contiguous bytes whatever the swizzle, at most 15 rows x 4 atoms), and
+// the MMA reads only ceil(rows / 16) of the stage's four K steps.  The loads
+// run ahead, so the fix-up is off the critical path.
+//
+// Groups without rows give a zero matrix, written without any MMA.
+constexpr int kWgradThreads = kNumThreads + 32;
+constexpr int kWgradTile = 256;
+
+struct WgradParams {
+  const void* offsets;
+  int off64;
+  int E;
+  int T, M, N;
+  int tiles_m, tiles_n;
+  int bf16;
+  unsigned short* D;       // [E, M, N], pitch ldd, stride_d from one matrix to the next
+  long long ldd, stride_d;
+  int d_tma;               // D is TMA-addressable
+  int* err;
+};
+
+template <int STAGES>
+struct WgradPlan {
+  static constexpr int kOpBytes = kBK * 128 * 2;         // 64 rows x 128 columns of one operand: two atoms
+  static constexpr int kStageBytes = 2 * kOpBytes;
+  static constexpr int kOutBytes = kStoreRows * kStoreCols * 2;
+  static constexpr int kOffA = 0;
+  static constexpr int kOffG = STAGES * kOpBytes;
+  static constexpr int kOffOut = 2 * STAGES * kOpBytes;
+  static constexpr int kOffBar = kOffOut + kEpiWarps * kOutBytes;
+  static constexpr int kNumBars = 4 * STAGES + 4 + 1;    // full, empty, land, fix, tmem_full[2], tmem_empty[2], done
+  static constexpr int kOffMisc = kOffBar + kNumBars * 8;
+  static constexpr int kOffScan = kOffMisc + 16;
+  static constexpr int kOffRows = kOffScan + 32;
+  static constexpr int kOffBlocks = kOffRows + (kMaxGroups + 1) * 4;
+  static constexpr int kUsed = kOffBlocks + (kMaxGroups + 1) * 4;
+  static constexpr int kDynamicBytes = kUsed + 1024;
+  static_assert(kDynamicBytes <= 227 * 1024, "shared memory of one CTA");
+};
+
+struct WgradUnit {
+  int e, tm, tn;
+  int row0, rows;   // the group's rows
+  int blocks;       // ceil(rows / 64)
+  int tail;         // rows of the last block when it is cut, else 0
+};
+
+__device__ __forceinline__ WgradUnit wgrad_unit(const WgradParams& p, const int* rows, int t) {
+  WgradUnit u;
+  const int tpe = p.tiles_m * p.tiles_n;
+  u.e = t / tpe;
+  const int local = t - u.e * tpe;
+  const int per = kGrpRaster * p.tiles_n;
+  const int g = local / per;
+  const int gs = min(p.tiles_m - g * kGrpRaster, kGrpRaster);
+  const int r = local - g * per;
+  u.tm = g * kGrpRaster + r % gs;
+  u.tn = r / gs;
+  u.row0 = rows[u.e];
+  u.rows = rows[u.e + 1] - u.row0;
+  u.blocks = (u.rows + kBK - 1) / kBK;
+  u.tail = u.rows % kBK;
+  return u;
+}
+
+template <int STAGES>
+__global__ void __launch_bounds__(kWgradThreads, 1)
+    gemm_grouped_wgrad_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmG,
+                             const __grid_constant__ CUtensorMap tmD, const __grid_constant__ WgradParams p) {
+  using Plan = WgradPlan<STAGES>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem + Plan::kOffA;
+  uint8_t* sG = smem + Plan::kOffG;
+  uint8_t* sOut = smem + Plan::kOffOut;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + Plan::kOffBar);
+  uint64_t* empty_bar = full_bar + STAGES;
+  uint64_t* land_bar = empty_bar + STAGES;   // a cut stage's bytes, per CTA
+  uint64_t* fix_bar = land_bar + STAGES;     // ... zeroed, on the even CTA
+  uint64_t* tfull_bar = fix_bar + STAGES;
+  uint64_t* tempty_bar = tfull_bar + 2;
+  uint64_t* done_bar = tempty_bar + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Plan::kOffMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* scan = reinterpret_cast<int*>(smem + Plan::kOffScan);
+  int* grp_rows = reinterpret_cast<int*>(smem + Plan::kOffRows);
+  int* grp_blocks = reinterpret_cast<int*>(smem + Plan::kOffBlocks);
+
+  const int warp = static_cast<int>(threadIdx.x >> 5);
+  const int lane = static_cast<int>(threadIdx.x & 31);
+  const int rank = static_cast<int>(cluster_ctarank());
+  const bool leader = (rank == 0);
+  const int worker = static_cast<int>(blockIdx.x) / 2;
+  const int workers = static_cast<int>(gridDim.x) / 2;
+
+  if (threadIdx.x == 64) {
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+      mbar_init(&land_bar[s], 1);
+      mbar_init(&fix_bar[s], 2);
+    }
+    mbar_init(&tfull_bar[0], 1);
+    mbar_init(&tfull_bar[1], 1);
+    mbar_init(&tempty_bar[0], kEpiWarps * 2);
+    mbar_init(&tempty_bar[1], kEpiWarps * 2);
+    mbar_init(done_bar, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&tmA);
+    prefetch_tmap(&tmG);
+    if (p.d_tma) prefetch_tmap(&tmD);
+  }
+  if (warp == 1) {
+    __syncwarp();
+    tmem_alloc<2>(tmem_slot, 512);
+    tmem_relinquish<2>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  griddep_wait();
+  scan_groups<kWgradThreads>(p.offsets, p.off64, p.E, p.T, grp_rows, grp_blocks, scan, p.err,
+                             [](int n) { return (n + kBK - 1) / kBK; });
+  const int num_tiles = p.E * p.tiles_m * p.tiles_n;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int issued = 0;
+      // per stage: parity of its last whole / cut fill, and which came last
+      uint32_t full_par = 0, land_par = 0, was_cut = 0, used = 0;
+      bool ok = true;
+      for (int t = worker; ok && t < num_tiles; t += workers) {
+        const WgradUnit u = wgrad_unit(p, grp_rows, t);
+        const int acol = u.tm * kWgradTile + rank * 128;
+        const int gcol = u.tn * kWgradTile + rank * 128;
+        for (int b = 0; b < u.blocks; ++b) {
+          if (issued >= STAGES && !mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) {
+            ok = false;
+            break;
+          }
+          uint8_t* a_dst = sA + stage * Plan::kOpBytes;
+          uint8_t* g_dst = sG + stage * Plan::kOpBytes;
+          const int row = u.row0 + b * kBK;
+          const uint32_t bit = 1u << stage;
+          used |= bit;
+          if (b == u.blocks - 1 && u.tail) {
+            uint64_t* bar = &land_bar[stage];
+            mbar_arrive_expect_tx(bar, Plan::kStageBytes);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              tma_load_2d(a_dst + j * (kBK * 128), &tmA, bar, acol + j * 64, row);
+              tma_load_2d(g_dst + j * (kBK * 128), &tmG, bar, gcol + j * 64, row);
+            }
+            was_cut |= bit;
+            land_par ^= bit;
+          } else {
+            if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * Plan::kStageBytes);
+            const uint32_t bar = mapa_shared(smem_u32(&full_bar[stage]), 0);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              tma_load_2d_pair(a_dst + j * (kBK * 128), &tmA, bar, acol + j * 64, row);
+              tma_load_2d_pair(g_dst + j * (kBK * 128), &tmG, bar, gcol + j * 64, row);
+            }
+            was_cut &= ~bit;
+            full_par ^= bit;
+          }
+          ++issued;
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      griddep_launch_dependents();
+      if (!ok) {
+        *abort_flag = 1;
+        atomicOr(p.err, kDevErrTimeoutProducer);
+      }
+      // every fill must have landed before the CTA exits (whole fills of the
+      // odd CTA complete on the even one's barriers and are covered by the
+      // cluster barrier at teardown)
+      for (int s = 0; s < STAGES; ++s) {
+        const uint32_t bit = 1u << s;
+        if (!(used & bit) || (!(was_cut & bit) && !leader)) continue;
+        uint64_t* bar = (was_cut & bit) ? &land_bar[s] : &full_bar[s];
+        const uint32_t par = (((was_cut & bit) ? land_par : full_par) & bit) ? 0u : 1u;   // of the last fill
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(bar, par)) {
+          if (globaltimer_ns() - t0 > kWaitLimitNs) {
+            atomicOr(p.err, kDevErrTimeoutTeardown);
+            break;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0 && leader) {
+      const uint32_t idesc = idesc_16bit(256, kWgradTile, true, true, p.bf16 != 0);
+      int stage = 0;
+      uint32_t full_par = 0, fix_par = 0;   // per stage: parity of its next whole / cut fill
+      int acc = 0;
+      uint32_t acc_phase = 0;
+      int count = 0;
+      bool ok = true;
+      for (int t = worker; ok && t < num_tiles; t += workers) {
+        const WgradUnit u = wgrad_unit(p, grp_rows, t);
+        if (u.blocks == 0) continue;
+        if (count >= 2 && !mbar_wait(&tempty_bar[acc], acc_phase ^ 1u, abort_flag)) {
+          ok = false;
+          break;
+        }
+        ++count;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kWgradTile);
+        for (int b = 0; b < u.blocks; ++b) {
+          const uint32_t bit = 1u << stage;
+          const bool cut = b == u.blocks - 1 && u.tail;
+          const bool got = cut ? mbar_wait_cluster(&fix_bar[stage], (fix_par & bit) ? 1u : 0u, abort_flag)
+                               : mbar_wait(&full_bar[stage], (full_par & bit) ? 1u : 0u, abort_flag);
+          if (!got) {
+            ok = false;
+            break;
+          }
+          if (cut) fix_par ^= bit;
+          else full_par ^= bit;
+          tc_fence_after();
+          const int steps = cut ? (u.tail + kUmmaK - 1) / kUmmaK : kBK / kUmmaK;
+          const uint32_t a0 = smem_u32(sA + stage * Plan::kOpBytes);
+          const uint32_t g0 = smem_u32(sG + stage * Plan::kOpBytes);
+          for (int j = 0; j < steps; ++j) {
+            mma_f16_ss<2>(d_tmem, smem_desc_sw128(a0 + j * (kUmmaK * 128), kBK * 128, 1024),
+                          smem_desc_sw128(g0 + j * (kUmmaK * 128), kBK * 128, 1024), idesc, (b > 0 || j > 0) ? 1u : 0u);
+          }
+          mma_commit<2>(&empty_bar[stage]);
+          if (++stage == STAGES) stage = 0;
+        }
+        if (!ok) break;
+        mma_commit<2>(&tfull_bar[acc]);
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1u;
+      }
+      if (!ok) {
+        *abort_flag = 1;
+        atomicOr(p.err, kDevErrTimeoutMma);
+      }
+      mma_commit<2>(done_bar);
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(done_bar, 0)) {
+        if (globaltimer_ns() - t0 > kWaitLimitNs) {
+          atomicOr(p.err, kDevErrTimeoutTeardown);
+          break;
+        }
+      }
+    }
+  } else if (warp == 6) {
+    // ------------------------------------------------------------ cut stages: zero the rows of others
+    int stage = 0;
+    uint32_t land_par = 0;
+    for (int t = worker; t < num_tiles; t += workers) {
+      const WgradUnit u = wgrad_unit(p, grp_rows, t);
+      if (u.blocks == 0) continue;
+      const int last = (stage + u.blocks - 1) % STAGES;
+      stage = (last + 1) % STAGES;
+      if (!u.tail) continue;
+      const uint32_t bit = 1u << last;
+      bool got = true;
+      if (lane == 0) got = mbar_wait(&land_bar[last], (land_par & bit) ? 1u : 0u, abort_flag);
+      got = __shfl_sync(0xffffffffu, got ? 1 : 0, 0) != 0;
+      if (!got) {
+        if (lane == 0) {
+          *abort_flag = 1;
+          atomicOr(p.err, kDevErrTimeoutProducer);
+        }
+        break;
+      }
+      land_par ^= bit;
+      const int bytes = ((u.tail + kUmmaK - 1) / kUmmaK * kUmmaK - u.tail) * 128;   // per atom
+      for (int o = lane * 16; o < bytes; o += 32 * 16) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int at = last * Plan::kOpBytes + j * (kBK * 128) + u.tail * 128 + o;
+          *reinterpret_cast<uint4*>(sA + at) = make_uint4(0u, 0u, 0u, 0u);
+          *reinterpret_cast<uint4*>(sG + at) = make_uint4(0u, 0u, 0u, 0u);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&fix_bar[last]), 0));
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int ew = warp & 3;
+    const bool bf16 = p.bf16 != 0;
+    const uint32_t tempty_remote0 = mapa_shared(smem_u32(&tempty_bar[0]), 0);
+    uint8_t* buf = sOut + ew * Plan::kOutBytes;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int t = worker; t < num_tiles; t += workers) {
+      const WgradUnit u = wgrad_unit(p, grp_rows, t);
+      if (u.blocks > 0) {
+        bool got = true;
+        if (lane == 0) got = mbar_wait(&tfull_bar[acc], acc_phase, abort_flag);
+        got = __shfl_sync(0xffffffffu, got ? 1 : 0, 0) != 0;
+        ok = named_bar_and(1, 32 * kEpiWarps, got);
+        if (!ok) break;
+        tc_fence_after();
+      }
+      const uint32_t tbase =
+          tmem_base + (static_cast<uint32_t>(ew * 32) << 16) + static_cast<uint32_t>(acc * kWgradTile);
+      const int m0 = u.tm * kWgradTile + rank * 128 + ew * 32;
+      unsigned short* out = p.D + static_cast<long long>(u.e) * p.stride_d;
+#pragma unroll 1
+      for (int c0 = 0; c0 < kWgradTile; c0 += kStoreCols) {
+        const int n0 = u.tn * kWgradTile + c0;
+        if (n0 >= p.N || m0 >= p.M) break;
+        float f[64];
+        if (u.blocks > 0) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(tbase + c0 + h * 32, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[h * 32 + i] = __uint_as_float(v[i]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) f[i] = 0.0f;
+        }
+        const bool whole = p.d_tma && (n0 + kStoreCols <= p.N || p.N % 8 == 0);
+        if (p.d_tma) {
+          if (lane == 0) bulk_wait_group_read<0>();
+          __syncwarp();
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            w[i] = to_16bit(f[8 * c + 2 * i], bf16) |
+                   (static_cast<uint32_t>(to_16bit(f[8 * c + 2 * i + 1], bf16)) << 16);
+          }
+          *reinterpret_cast<uint4*>(buf + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        if (whole) fence_proxy_async_smem();
+        __syncwarp();
+        if (whole) {
+          if (lane == 0) {
+            tma_store_3d(&tmD, buf, n0, m0, u.e);
+            bulk_commit_group();
+          }
+        } else {
+          for (int r = 0; r < kStoreRows && m0 + r < p.M; ++r) {
+            unsigned short* drow = out + static_cast<long long>(m0 + r) * p.ldd;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int c = h * 32 + lane;
+              if (n0 + c < p.N) {
+                drow[n0 + c] = *reinterpret_cast<const unsigned short*>(buf + r * 128 + (((c >> 3) ^ (r & 7)) << 4) +
+                                                                        (c & 7) * 2);
+              }
+            }
+          }
+          __syncwarp();
+        }
+      }
+      if (u.blocks > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(tempty_remote0 + static_cast<uint32_t>(acc * 8));
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1u;
+      }
+    }
+    if (!ok) {
+      *abort_flag = 1;
+      atomicOr(p.err, kDevErrTimeoutEpilogue);
+    }
+    if (p.d_tma && lane == 0) bulk_wait_group_read<0>();
+  }
+
+  // ------------------------------------------------------------ teardown
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<2>(tmem_base, 512);
   }
 }
 

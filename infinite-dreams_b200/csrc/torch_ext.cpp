@@ -9,6 +9,7 @@
 //   gemm_forward_cfg(A, B, cfg_id, out=None) -> C             (gemm_ext.cpp:95-106)
 //   gemm_ex(A, B, cfg_id, alpha, beta, C, bias, act, out) -> out
 //   grouped_gemm(A, B, offsets, bias, act, out) -> out
+//   grouped_gemm_wgrad(A, G, offsets, out) -> out
 //   reset_workspaces()
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -251,6 +252,37 @@ at::Tensor grouped_gemm(const at::Tensor& A, const at::Tensor& B, const at::Tens
   return C;
 }
 
+at::Tensor grouped_gemm_wgrad(const at::Tensor& A, const at::Tensor& G, const at::Tensor& offsets,
+                              c10::optional<at::Tensor> out) {
+  TORCH_CHECK(A.is_cuda(), "A must be CUDA tensor");
+  TORCH_CHECK(is_16bit(A), "A must be float16 or bfloat16");
+  TORCH_CHECK(A.dim() == 2, "A must be 2D (T x K)");
+  check_like(G, A, "G");
+  TORCH_CHECK(G.dim() == 2 && G.size(0) == A.size(0), "G must be 2D (T x N) with A's rows");
+  TORCH_CHECK(offsets.dim() == 1 && offsets.size(0) >= 2, "offsets must be 1D with at least 2 elements");
+  check_index(offsets, A, offsets.size(0), "offsets");
+  const int64_t T = A.size(0), K = A.size(1), N = G.size(1), E = offsets.size(0) - 1;
+  check_no_grad("grouped_gemm_wgrad computes no gradients: call it under torch.no_grad()", {A, G});
+  const c10::cuda::CUDAGuard guard(A.device());
+  at::Tensor D = out.has_value() ? *out : at::empty({E, K, N}, A.options().requires_grad(false));
+  TORCH_CHECK(D.is_cuda() && D.device() == A.device() && D.scalar_type() == A.scalar_type() && D.dim() == 3 &&
+                  D.size(0) == E && D.size(1) == K && D.size(2) == N,
+              "out must be an (E x K x N) tensor of A's dtype on A's device");
+  auto [Ds, td, ldd, sd] = stacked_operand(D);
+  TORCH_CHECK(Ds.data_ptr() == D.data_ptr(), "out must be row-major or a transposed view, its matrices apart");
+  at::Tensor As = row_operand(A), Gs = row_operand(G), off = offsets.contiguous();
+  // a gradient stored N x K is the product with the operands exchanged
+  const at::Tensor &L = td ? Gs : As, &R = td ? As : Gs;
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream(A.device().index()).stream();
+  Scratch ws = scratch(A.device(), stream, gemm_grouped_wgrad_workspace_bytes(L.data_ptr(), R.data_ptr(), T, L.size(1),
+                                                                              R.size(1), pitch(L), pitch(R)));
+  check_status(gemm_grouped_wgrad_launch(L.data_ptr(), R.data_ptr(), Ds.data_ptr(), off.data_ptr(),
+                                         off.scalar_type() == at::kLong ? 64 : 32, T, L.size(1), R.size(1), E,
+                                         pitch(L), pitch(R), ldd, sd, dtype_id(A), ws.ptr, ws.len, stream),
+               "gemm_grouped_wgrad_launch");
+  return D;
+}
+
 void reset_workspaces() {
   std::lock_guard<std::mutex> lock(g_ws_mu);
   g_ws->clear();
@@ -268,5 +300,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("grouped_gemm", &grouped_gemm, "out[r] = act(A[r] @ B[group of r] + bias[group of r])", py::arg("A"),
         py::arg("B"), py::arg("offsets"), py::arg("bias") = py::none(), py::arg("act") = 0,
         py::arg("out") = py::none());
+  m.def("grouped_gemm_wgrad", &grouped_gemm_wgrad, "out[e] = A[rows of e].T @ G[rows of e]", py::arg("A"),
+        py::arg("G"), py::arg("offsets"), py::arg("out") = py::none());
   m.def("reset_workspaces", &reset_workspaces, "drop the cached split-K / repack workspaces");
 }

@@ -18,7 +18,9 @@ by the sm_100a kernel bank through its C ABI (include/gemm_sm100.h):
 ``gemm_ex`` goes beyond the reference: transposed operand views read in
 place and a fused epilogue (alpha, beta * C, bias, ReLU / GELU).  So do the
 products whose weight is picked by the row, in fp16 and bf16:
-``grouped_gemm`` (rows sorted by expert, ragged counts).
+``grouped_gemm`` (rows sorted by expert, ragged counts) and its weight
+gradient ``grouped_gemm_wgrad``; ``grouped.grouped_linear`` is the pair as a
+differentiable function.
 
 Like the reference, inputs are made contiguous, C is allocated from torch's
 caching allocator on A's device, and the launch is asynchronous on the
@@ -379,6 +381,52 @@ def grouped_gemm(A: torch.Tensor, B: torch.Tensor, offsets: torch.Tensor, *, bia
     return C
 
 
+def grouped_gemm_wgrad(A: torch.Tensor, G: torch.Tensor, offsets: torch.Tensor, *,
+                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out[e] = A[r].T @ G[r] over the rows r of group e: the weight gradient of ``grouped_gemm``.
+
+    A is [T, K], G [T, N] (fp16 or bf16, alike), offsets as for
+    ``grouped_gemm``; out is [E, K, N], row-major or a transposed view of
+    [E, N, K] storage.  An empty group's matrix is zero; rows outside every
+    group do not enter.
+    """
+    if _fast is not None:
+        return _fast.grouped_gemm_wgrad(A, G, offsets, out)
+    if not isinstance(A, torch.Tensor) or not A.is_cuda:
+        raise RuntimeError("A must be CUDA tensor")
+    if not _is_16bit(A):
+        raise RuntimeError("A must be float16 or bfloat16")
+    if A.dim() != 2:
+        raise RuntimeError("A must be 2D (T x K)")
+    _check_like(G, A, "G")
+    if G.dim() != 2 or G.size(0) != A.size(0):
+        raise RuntimeError("G must be 2D (T x N) with A's rows")
+    if offsets.dim() != 1 or offsets.size(0) < 2:
+        raise RuntimeError("offsets must be 1D with at least 2 elements")
+    _check_index(offsets, A, offsets.size(0), "offsets")
+    (T, K), N, E = A.shape, G.size(1), offsets.size(0) - 1
+    _check_no_grad("grouped_gemm_wgrad computes no gradients: call it under torch.no_grad()", A, G)
+    with torch.cuda.device(A.device):
+        D = torch.empty((E, K, N), dtype=A.dtype, device=A.device) if out is None else out
+        if D.device != A.device or D.dtype != A.dtype or tuple(D.shape) != (E, K, N):
+            raise RuntimeError("out must be an (E x K x N) tensor of A's dtype on A's device")
+        Ds, td, ldd, sd = _stacked_operand(D)
+        if Ds.data_ptr() != D.data_ptr():
+            raise RuntimeError("out must be row-major or a transposed view, its matrices apart")
+        As, Gs, off = _row_operand(A), _row_operand(G), offsets.contiguous()
+        L, R = (Gs, As) if td else (As, Gs)   # a gradient stored N x K: the operands exchanged
+        stream = torch.cuda.current_stream(A.device)
+        need = lib.gemm_grouped_wgrad_workspace_bytes(L.data_ptr(), R.data_ptr(), T, L.size(1), R.size(1), _pitch(L),
+                                                      _pitch(R))
+        keep, ws_ptr, ws_len = _scratch(A.device, stream, need)
+        st = lib.gemm_grouped_wgrad_launch(L.data_ptr(), R.data_ptr(), Ds.data_ptr(), off.data_ptr(),
+                                           64 if off.dtype == torch.int64 else 32, T, L.size(1), R.size(1), E,
+                                           _pitch(L), _pitch(R), ldd, sd, _dtype_id(A), ws_ptr, ws_len,
+                                           stream.cuda_stream or None)
+        _capi.check(st, "gemm_grouped_wgrad_launch")
+    return D
+
+
 def gemm_cfg_table_cpu() -> torch.Tensor:
     """CPU int32 tensor [num_cfg, len(CFG_COLUMNS)], columns CFG_COLUMNS."""
     cols, rows = _capi.menu()
@@ -402,5 +450,6 @@ def check_device_errors(device: Optional[int] = None) -> None:
         raise GemmError(st, f"device {dev}: kernel error bits {code.value}: {message}")
 
 
-__all__ = ["gemm_forward", "gemm_forward_cfg", "gemm_ex", "grouped_gemm", "gemm_cfg_table_cpu", "CFG_COLUMNS", "NUM_CFG",
+__all__ = ["gemm_forward", "gemm_forward_cfg", "gemm_ex", "grouped_gemm", "grouped_gemm_wgrad",
+           "gemm_cfg_table_cpu", "CFG_COLUMNS", "NUM_CFG",
            "default_cfg", "check_device_errors", "GemmError", "reset_workspaces"]

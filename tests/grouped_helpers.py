@@ -88,3 +88,17 @@ def ref_grouped(A, B, offsets, bias=None, act="none"):
         ref[s] = act64(v, act)
         tol[s] = rounded(ref[s], err, A.dtype)
     return ref, tol
+
+
+def ref_wgrad(A, G, offsets):
+    """(reference, bound) of grouped_gemm_wgrad."""
+    off = offsets.tolist()
+    E = len(off) - 1
+    ref = torch.zeros((E, A.shape[1], G.shape[1]), dtype=torch.float64, device=A.device)
+    tol = torch.zeros_like(ref)
+    for e in range(E):
+        a, g = A[off[e]:off[e + 1]].double(), G[off[e]:off[e + 1]].double()
+        ref[e] = a.T @ g
+        if a.shape[0]:
+            tol[e] = rounded(ref[e], sum_error(a.shape[0], a.abs().T @ g.abs()), A.dtype)
+    return ref, tol

@@ -57,3 +57,23 @@ def test_torch_surface_refuses_cpu_tensors():
         ext._fast = keep
 
 
+
+
+def _wgrad(A=P, G=P, D=P, off=P, bits=32, T=8, M=8, N=8, E=2, lda=8, ldg=8, ldd=8, sd=64, dtype=0):
+    return LIB.gemm_grouped_wgrad_launch(A, G, D, off, bits, T, M, N, E, lda, ldg, ldd, sd, dtype, None, 0, None)
+
+
+@pytest.mark.parametrize("bad", [dict(T=-1), dict(E=0), dict(bits=8), dict(dtype=-1), dict(A=None), dict(G=None),
+                                 dict(D=None), dict(off=None), dict(lda=7), dict(ldg=7), dict(ldd=7), dict(sd=63),
+                                 dict(G=P + 1), dict(off=P + 1)], ids=str)
+def test_wgrad_invalid_arguments(bad):
+    assert _wgrad(**bad) == _capi.GEMM_ERR_INVALID_ARG
+
+
+def test_wgrad_limits_and_workspace():
+    head = LIB.gemm_workspace_counter_bytes()
+    assert _wgrad(E=1025) == _capi.GEMM_ERR_UNSUPPORTED
+    assert _wgrad(M=7, lda=7) == _capi.GEMM_ERR_WORKSPACE
+    assert _wgrad(M=0) == _capi.GEMM_OK
+    assert LIB.gemm_grouped_wgrad_workspace_bytes(P, P, 100, 64, 64, 64, 64) == 0
+    assert LIB.gemm_grouped_wgrad_workspace_bytes(P, P, 100, 77, 64, 77, 64) == head + 100 * 128 * 2
