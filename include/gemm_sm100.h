@@ -171,6 +171,34 @@ int gemm_grouped_wgrad_launch(const void* A, const void* G, void* D, const void*
 size_t gemm_grouped_wgrad_workspace_bytes(const void* A, const void* G, int64_t T, int64_t M, int64_t N, int64_t lda,
                                           int64_t ldg);
 
+/* Low-rank adapters of many requests beside a shared projection:
+ *   C[t, :] = act(X[t, :] * op(W) + scale[a] * (X[t, :] * op(down[a])) * op(up[a]) + bias),  a = adapter[t]
+ *  X       = T x K (ldx >= K); W = K x N (ldw >= N), or stored N x K with
+ *            trans_w = 1 (ldw >= K); C = T x N (ldc >= N);
+ *  down    = L matrices K x R, stride_down elements apart, or stored R x K
+ *            with trans_down = 1; up = L matrices R x N or stored N x R.  An
+ *            adapter of a smaller rank is padded with zeros;
+ *  adapter = T numbers on the device (adapter_bits 32 or 64), in any order;
+ *            negative: the row has no adapter.  A number past the last
+ *            adapter is read as none and reported by gemm_device_error;
+ *  scale   = fp32 [L] or NULL (1); bias = [N] or NULL; activation = GEMM_ACT_*.
+ * Every operand is read in place; X, W and up are repacked into the workspace
+ * when TMA cannot address them (16-byte base, pitches and strides multiples
+ * of 8 elements).  x * down is kept in fp32 and enters the second product as
+ * two 16-bit numbers (their sum is exact to 16 or more bits); fp32
+ * accumulation, one rounding.  Two launches.  R <= GEMM_LORA_MAX_RANK.  The
+ * workspace (never 0 bytes) comes from gemm_lora_workspace_bytes under the
+ * contract of gemm_launch.  No counterpart in the reference. */
+#define GEMM_LORA_MAX_RANK 1024
+int gemm_lora_launch(const void* X, const void* W, const void* down, const void* up, void* C, const void* adapter,
+                     int adapter_bits, int64_t T, int64_t N, int64_t K, int64_t L, int64_t R, int64_t ldx, int64_t ldw,
+                     int trans_w, int64_t ld_down, int64_t stride_down, int trans_down, int64_t ld_up,
+                     int64_t stride_up, int trans_up, int64_t ldc, const float* scale, const void* bias, int activation,
+                     int dtype, void* workspace, size_t workspace_bytes, void* stream);
+size_t gemm_lora_workspace_bytes(const void* X, const void* W, const void* up, int64_t T, int64_t N, int64_t K,
+                                 int64_t L, int64_t R, int64_t ldx, int64_t ldw, int trans_w, int64_t ld_up,
+                                 int64_t stride_up, int trans_up);
+
 /* Fused all-gather for M-row sharding over the GPUs of one node (one
  * process per GPU).  Same as gemm_launch, and each finished tile of C is
  * also stored, over NVLink, at the same offset and pitch ldc into

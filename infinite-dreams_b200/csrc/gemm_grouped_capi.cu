@@ -1,6 +1,7 @@
 // C ABI of the products whose weight is picked by the row (declared in
 // include/gemm_sm100.h): validation, repacking of operands that TMA cannot
 // address, tensor maps and launches, in the manner of gemm_capi.cu.
+#include <algorithm>
 #include <atomic>
 #include <cstring>
 #include <string>
@@ -136,22 +137,29 @@ cudaError_t launch(Kernel kernel, int threads, int bytes, std::atomic<unsigned l
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-template <int CG, int TM, int STAGES>
-int launch_grouped(const Operand& a, const Operand& b, const GroupedParams& gp, int sms, cudaStream_t stream) {
-  using Plan = GroupedPlan<CG, TM, STAGES>;
+// `up` is null without adapters.
+template <int CG, int TM, int STAGES, bool LORA>
+int launch_grouped(const Operand& a, const Operand& b, const Operand* up, const GroupedParams& gp, int sms,
+                   cudaStream_t stream) {
+  using Plan = GroupedPlan<CG, TM, STAGES, LORA>;
   GroupedParams p = gp;
   p.tiles_n = static_cast<int>((static_cast<int64_t>(p.N) + kGrpCols * CG - 1) / (kGrpCols * CG));
   const int64_t row_tiles = static_cast<int64_t>(p.T) / TM + p.E;   // at most one cut tile per group
   if (row_tiles * p.tiles_n > kInt32Max) return capi_fail(GEMM_ERR_UNSUPPORTED, "too many output tiles");
-  CUtensorMap tmA, tmB, tmC;
+  CUtensorMap tmA, tmB, tmC, tmU;
   std::memset(&tmA, 0, sizeof(tmA));
   std::memset(&tmB, 0, sizeof(tmB));
   std::memset(&tmC, 0, sizeof(tmC));
+  std::memset(&tmU, 0, sizeof(tmU));
   int st;
   if (p.K > 0) {
     st = a.encode2(&tmA, kBK, Plan::kBoxRows, true, "A");
     if (st != GEMM_OK) return st;
     st = p.b_kmaj ? b.encode3(&tmB, kBK, kGrpCols, true, "B (stored N x K)") : b.encode3(&tmB, 64, kBK, true, "B");
+    if (st != GEMM_OK) return st;
+  }
+  if (LORA) {
+    st = p.up_kmaj ? up->encode3(&tmU, kBK, kGrpCols, true, "up (stored N x R)") : up->encode3(&tmU, 64, kBK, true, "up");
     if (st != GEMM_OK) return st;
   }
   if (p.c_tma) {
@@ -165,10 +173,101 @@ int launch_grouped(const Operand& a, const Operand& b, const GroupedParams& gp, 
   const int64_t most = std::min<int64_t>(row_tiles * p.tiles_n, sms / CG);
   const int grid = static_cast<int>(most < 1 ? 1 : most) * CG;
   static std::atomic<unsigned long long> configured{0};
-  cudaError_t e = launch<CG>(gemm_grouped_sm100<CG, TM, STAGES>, kNumThreads, Plan::kDynamicBytes, configured, grid,
-                             stream, tmA, tmB, tmC, p);
+  cudaError_t e = launch<CG>(gemm_grouped_sm100<CG, TM, STAGES, LORA>, kNumThreads, Plan::kDynamicBytes, configured,
+                             grid, stream, tmA, tmB, tmC, tmU, p);
   return e == cudaSuccess ? GEMM_OK : capi_fail_cuda(e, "grouped gemm kernel launch");
 }
+
+// ------------------------------------------------------------- low-rank adapters
+// The first kernel's variant: ranks per block (16, 32 or 64, R above 64 in
+// several blocks) and rows of one adapter per MMA chunk (8 or 32).
+using ShrinkFn = void (*)(ShrinkParams);
+
+template <int RT, int NT8>
+ShrinkFn shrink_fn(bool kmaj, bool bf16) {
+  if (kmaj) return bf16 ? lora_shrink<RT, NT8, true, true> : lora_shrink<RT, NT8, true, false>;
+  return bf16 ? lora_shrink<RT, NT8, false, true> : lora_shrink<RT, NT8, false, false>;
+}
+
+int shrink_rank_tiles(int64_t R) { return R <= 16 ? 1 : (R <= 32 ? 2 : 4); }
+int64_t shrink_pitch(int64_t R) { return round_up(R, 16 * shrink_rank_tiles(R)); }
+
+int launch_shrink(const ShrinkParams& sp, bool kmaj, bool bf16, cudaStream_t stream) {
+  ShrinkParams p = sp;
+  const int rt = shrink_rank_tiles(p.R);
+  // Rows per tile: few enough that about 256 CTAs share the work (T = 64: 2
+  // rows x 32 clusters of 8), up to the 32 rows of one MMA chunk.
+  int rows = 1;
+  while (rows < kShrinkMaxRows && rows * 32 < p.T) rows *= 2;
+  p.tile_rows = rows;
+  // CTAs along K: no more than give every warp a slice.
+  const int slices = (p.K + kShrinkSlice - 1) / kShrinkSlice;
+  int cluster = 1;
+  while (cluster < 8 && cluster * kShrinkWarps < slices) cluster *= 2;
+  const bool wide = rows > 8;
+  ShrinkFn fn = rt == 1 ? (wide ? shrink_fn<1, 4>(kmaj, bf16) : shrink_fn<1, 1>(kmaj, bf16))
+                : rt == 2 ? (wide ? shrink_fn<2, 4>(kmaj, bf16) : shrink_fn<2, 1>(kmaj, bf16))
+                          : (wide ? shrink_fn<4, 4>(kmaj, bf16) : shrink_fn<4, 1>(kmaj, bf16));
+  const int bytes = kShrinkWarps * rows * 16 * rt * static_cast<int>(sizeof(float));   // at most 64 KiB
+  static std::atomic<unsigned long long> configured[24];
+  const int which = (((rt == 1 ? 0 : rt == 2 ? 1 : 2) * 2 + wide) * 2 + kmaj) * 2 + bf16;
+  cudaError_t e = opt_in(fn, 64 * 1024, configured[which]);
+  if (e != cudaSuccess) return capi_fail_cuda(e, "adapter kernel attribute");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((p.T + rows - 1) / rows * cluster),
+                     static_cast<unsigned>((p.R + 16 * rt - 1) / (16 * rt)), 1);
+  cfg.blockDim = dim3(kShrinkThreads, 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(bytes);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  e = cudaLaunchKernelEx(&cfg, fn, p);
+  return e == cudaSuccess ? GEMM_OK : capi_fail_cuda(e, "adapter kernel launch");
+}
+
+constexpr int64_t kLoraSmallRows = 64;   // rows that go to the single-CTA tiles
+
+// Workspace of a call with adapters: h, the adapter lists, then repacked operands.
+struct LoraPlan {
+  Operand x, w, up;
+  size_t off_h = 0, off_lists = 0, total = 0;
+  int list_tiles = 0, list_rows = 0;
+
+  LoraPlan(const void* X, const void* W, const void* U, int64_t T, int64_t N, int64_t K, int64_t L, int64_t R,
+           int64_t ldx, int64_t ldw, int trans_w, int64_t ld_up, int64_t stride_up, int trans_up)
+      : x(X, 1, T, K, ldx, 0), w(W, 1, trans_w ? N : K, trans_w ? K : N, ldw, 0),
+        up(U, L, trans_up ? N : R, trans_up ? R : N, ld_up, stride_up) {
+    if (T <= kLoraSmallRows) {
+      row_tiles_host<64, 16>(T);
+    } else {
+      row_tiles_host<256, 32>(T);
+    }
+    size_t off = align256(gemm_workspace_counter_bytes());
+    off_h = off;
+    off = align256(off + static_cast<size_t>(T) * shrink_pitch(R) * sizeof(float));
+    off_lists = off;
+    off = align256(off + static_cast<size_t>(list_tiles) * kAdapterListPitch * sizeof(int));
+    x.plan(&off);
+    w.plan(&off);
+    up.plan(&off);
+    total = off;
+  }
+
+  // the kernel's row tiles (row_tiles in gemm_grouped_kernel.cuh)
+  template <int TM, int STEP>
+  void row_tiles_host(int64_t n) {
+    const int64_t count = (n + TM - 1) / TM;
+    list_tiles = static_cast<int>(count);
+    list_rows = static_cast<int>(((n + count - 1) / count + STEP - 1) / STEP * STEP);
+  }
+};
 
 constexpr int kWgradStages = 6;
 
@@ -279,8 +378,8 @@ int gemm_grouped_launch(const void* A, const void* B, void* C, const void* offse
   // Few rows per group: the cost is reading the weights, and single CTAs with
   // a deep ring read them best.  More rows: CTA pairs with tiles of up to 256
   // rows, which read every weight once per 256 rows.
-  if (T <= 64 * E || N <= kGrpCols) return launch_grouped<1, 64, 8>(a, b, p, sms, stream);
-  return launch_grouped<2, 256, 6>(a, b, p, sms, stream);
+  if (T <= 64 * E || N <= kGrpCols) return launch_grouped<1, 64, 8, false>(a, b, nullptr, p, sms, stream);
+  return launch_grouped<2, 256, 6, false>(a, b, nullptr, p, sms, stream);
 }
 
 size_t gemm_grouped_wgrad_workspace_bytes(const void* A, const void* G, int64_t T, int64_t M, int64_t N, int64_t lda,
@@ -356,6 +455,118 @@ int gemm_grouped_wgrad_launch(const void* A, const void* G, void* D, const void*
   p.stride_d = E == 1 ? 0 : stride_d;
   p.d_tma = reinterpret_cast<uintptr_t>(D) % 16u == 0 && ldd % 8 == 0 && (E == 1 || stride_d % 8 == 0);
   return launch_wgrad(a, g, p, sms, stream);
+}
+
+size_t gemm_lora_workspace_bytes(const void* X, const void* W, const void* up, int64_t T, int64_t N, int64_t K,
+                                 int64_t L, int64_t R, int64_t ldx, int64_t ldw, int trans_w, int64_t ld_up,
+                                 int64_t stride_up, int trans_up) {
+  if (T <= 0 || N <= 0 || K <= 0 || L <= 0 || R <= 0) return 0;
+  return LoraPlan(X, W, up, T, N, K, L, R, ldx, ldw, trans_w, ld_up, stride_up, trans_up).total;
+}
+
+int gemm_lora_launch(const void* X, const void* W, const void* down, const void* up, void* C, const void* adapter,
+                     int adapter_bits, int64_t T, int64_t N, int64_t K, int64_t L, int64_t R, int64_t ldx, int64_t ldw,
+                     int trans_w, int64_t ld_down, int64_t stride_down, int trans_down, int64_t ld_up,
+                     int64_t stride_up, int trans_up, int64_t ldc, const float* scale, const void* bias, int activation,
+                     int dtype, void* workspace, size_t workspace_bytes, void* stream_v) {
+  capi_clear_error();
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  int st = check_common(T, N, K, L, adapter_bits, dtype, "the number of adapters");
+  if (st != GEMM_OK) return st;
+  if (K < 1) return capi_fail(GEMM_ERR_INVALID_ARG, "K must be >= 1");
+  if (R < 1 || R > GEMM_LORA_MAX_RANK) {
+    return capi_fail(R < 1 ? GEMM_ERR_INVALID_ARG : GEMM_ERR_UNSUPPORTED,
+                     "the rank must be in [1, " + std::to_string(GEMM_LORA_MAX_RANK) + "]");
+  }
+  if (L > kInt32Max) return capi_fail(GEMM_ERR_UNSUPPORTED, "the number of adapters must be < 2^31");
+  if ((trans_w != 0 && trans_w != 1) || (trans_down != 0 && trans_down != 1) || (trans_up != 0 && trans_up != 1)) {
+    return capi_fail(GEMM_ERR_INVALID_ARG, "trans_w, trans_down and trans_up must be 0 or 1");
+  }
+  if (activation < GEMM_ACT_NONE || activation > GEMM_ACT_GELU) {
+    return capi_fail(GEMM_ERR_INVALID_ARG, "activation must be GEMM_ACT_NONE, GEMM_ACT_RELU or GEMM_ACT_GELU");
+  }
+  if (T == 0 || N == 0) return GEMM_OK;
+  if (!X || !W || !down || !up || !C || !adapter) {
+    return capi_fail(GEMM_ERR_INVALID_ARG, "X, W, down, up, C and adapter must be non-null");
+  }
+  const int64_t down_rows = trans_down ? R : K, down_cols = trans_down ? K : R;
+  const int64_t up_rows = trans_up ? N : R, up_cols = trans_up ? R : N;
+  if (ldx < K || ldw < (trans_w ? K : N) || ldc < N || ld_down < down_cols || ld_up < up_cols ||
+      (L > 1 && (stride_down < (down_rows - 1) * ld_down + down_cols || stride_up < (up_rows - 1) * ld_up + up_cols))) {
+    return capi_fail(GEMM_ERR_INVALID_ARG, "a pitch is shorter than its row, or a stride than its matrix");
+  }
+  if (misaligned(X) || misaligned(W) || misaligned(down) || misaligned(up) || misaligned(C) || misaligned(bias)) {
+    return capi_fail(GEMM_ERR_INVALID_ARG, "X, W, down, up, C and bias must be 2-byte aligned");
+  }
+  if (reinterpret_cast<uintptr_t>(adapter) % (adapter_bits / 8) != 0 || reinterpret_cast<uintptr_t>(scale) % 4u != 0) {
+    return capi_fail(GEMM_ERR_INVALID_ARG, "adapter and scale must be aligned to their width");
+  }
+  LoraPlan pl(X, W, up, T, N, K, L, R, ldx, ldw, trans_w, ld_up, stride_up, trans_up);
+  if (pl.up.pack && L * pl.up.rows > kInt32Max) {
+    return capi_fail(GEMM_ERR_UNSUPPORTED, "too many rows of up to repack");
+  }
+  st = check_workspace(pl.total, workspace, workspace_bytes);
+  if (st != GEMM_OK) return st;
+  GroupedParams p = {};
+  int sms = 0;
+  st = capi_device(&sms, &p.err);
+  if (st != GEMM_OK) return st;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  st = pl.x.make(ws, stream);
+  if (st == GEMM_OK) st = pl.w.make(ws, stream);
+  if (st == GEMM_OK) st = pl.up.make(ws, stream);
+  if (st != GEMM_OK) return st;
+
+  ShrinkParams s = {};
+  s.x = static_cast<const unsigned short*>(pl.x.p);
+  s.ldx = pl.x.ld;
+  s.down = static_cast<const unsigned short*>(down);
+  s.ld_down = ld_down;
+  s.stride_down = L == 1 ? 0 : stride_down;
+  s.adapter = adapter;
+  s.adapter64 = adapter_bits == 64;
+  s.scale = scale;
+  s.h = reinterpret_cast<float*>(ws + pl.off_h);
+  s.h_pitch = static_cast<int>(shrink_pitch(R));
+  s.T = static_cast<int>(T);
+  s.K = static_cast<int>(K);
+  s.L = static_cast<int>(L);
+  s.R = static_cast<int>(R);
+  s.x_vec = 1;   // TMA-addressable, as it came or repacked
+  const int vec = trans_down ? 8 : 2 * shrink_rank_tiles(R);   // elements per load
+  s.down_vec = reinterpret_cast<uintptr_t>(down) % (2 * vec) == 0 && ld_down % vec == 0 && (L == 1 || stride_down % vec == 0);
+  s.lists = reinterpret_cast<int*>(ws + pl.off_lists);
+  s.list_tiles = pl.list_tiles;
+  s.list_rows = pl.list_rows;
+  s.err = p.err;
+  st = launch_shrink(s, trans_down != 0, dtype == GEMM_DTYPE_BF16, stream);
+  if (st != GEMM_OK) return st;
+
+  p.E = 1;
+  p.T = s.T;
+  p.N = static_cast<int>(N);
+  p.K = s.K;
+  p.kb_total = static_cast<int>((K + kBK - 1) / kBK);
+  p.b_kmaj = trans_w;
+  p.bf16 = dtype == GEMM_DTYPE_BF16;
+  p.act = activation;
+  p.bias = static_cast<const unsigned short*>(bias);
+  p.C = static_cast<unsigned short*>(C);
+  p.ldc = ldc;
+  p.c_tma = p.c_vec = reinterpret_cast<uintptr_t>(C) % 16u == 0 && ldc % 8 == 0;
+  p.h = s.h;
+  p.h_pitch = s.h_pitch;
+  p.L = s.L;
+  p.R = s.R;
+  p.adapter = adapter;
+  p.adapter64 = s.adapter64;
+  p.lists = s.lists;
+  p.up_kmaj = trans_up;
+  p.up = static_cast<const unsigned short*>(pl.up.p);
+  p.ld_up = pl.up.ld;
+  p.stride_up = L == 1 ? 0 : pl.up.stride;
+  if (T <= kLoraSmallRows) return launch_grouped<1, 64, 7, true>(pl.x, pl.w, &pl.up, p, sms, stream);
+  return launch_grouped<2, 256, 5, true>(pl.x, pl.w, &pl.up, p, sms, stream);
 }
 
 }  // extern "C"

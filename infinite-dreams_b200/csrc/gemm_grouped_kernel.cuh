@@ -29,7 +29,28 @@
 // cut one row by row: the rows behind it are the next group's.  Rows that the
 // last A box of a group reads past the group's end only reach accumulator
 // columns that are not stored, so nothing in them (inf, NaN) can spread.
+//
+// LORA = true adds low-rank adapters picked by the row to one shared product
+// (E = 1, no offsets):  C[r, :] = act(A[r, :] * B + h[r, :] * up[a_r] + bias).
+// h (fp32, scaled) comes from lora_shrink (gemm_lora_kernel.cuh), which also
+// lists the adapters of each row tile.  After the K blocks of a tile come its
+// adapter blocks, 32 ranks of one adapter each: the weight slot of a stage
+// holds `up` (64 ranks wide as TMA's swizzle wants it, of which 32 are used)
+// and the row operand is built by the epilogue warps in a buffer of its own:
+// row r holds h[r] when the row picked this adapter and zeros when not, so
+// rows with different adapters share a tile.  h is split into two 16-bit
+// numbers, h = hi + lo with |lo| <= half a step of hi, side by side in the 64
+// columns of the buffer, each multiplied with the same `up`: what tensor cores
+// take is 16-bit, and rounding h to one would cost as much accuracy as the
+// result's own rounding does.
+//
+// A row that did not pick the adapter multiplies `up` with zeros, and 0 * inf
+// is not 0.  So where a tile mixes adapters the thread that owns a column
+// looks its ranks over once they have landed, replaces an inf or NaN by 0 in
+// shared memory, and adds what it replaced to the rows of that adapter in the
+// epilogue: one request's weights cannot reach another's rows.
 #pragma once
+#include "gemm_lora_kernel.cuh"
 #include "gemm_sm100_kernel.cuh"
 
 namespace idb {
@@ -56,9 +77,21 @@ struct GroupedParams {
   int c_vec;         // C rows are 16-byte aligned
   int zero_rest;     // rows outside [off[0], off[E]): 1 written as 0, 0 left as they are
   int* err;
+  // LORA
+  const float* h;    // [T, h_pitch]
+  int h_pitch;
+  int L, R;
+  const void* adapter;
+  int adapter64;
+  const int* lists;  // [row tiles, kAdapterListPitch]
+  int up_kmaj;       // up[a] stored N x R
+  const unsigned short* up;
+  long long ld_up, stride_up;
 };
 
-template <int CG, int TM, int STAGES>
+constexpr int kLoraRanks = 32;   // ranks per adapter block
+
+template <int CG, int TM, int STAGES, bool LORA>
 struct GroupedPlan {
   static constexpr int kStep = 16 * CG;                  // granularity of a tile's rows (MMA N)
   static constexpr int kTokRows = TM / CG;               // rows of A held by this CTA
@@ -70,8 +103,10 @@ struct GroupedPlan {
   static constexpr int kOffW = 0;
   static constexpr int kOffT = kOffW + STAGES * kWBytes;
   static constexpr int kOffOut = kOffT + STAGES * kTBytes;
-  static constexpr int kOffBar = kOffOut + 2 * kOutBytes;
-  static constexpr int kNumBars = 2 * STAGES + 4 + 1;    // full, empty, tmem_full[2], tmem_empty[2], done
+  static constexpr int kOffH = kOffOut + 2 * kOutBytes;  // two buffers of adapter rows (hi | lo)
+  static constexpr int kOffBar = kOffH + (LORA ? 2 * kTBytes : 0);
+  // full, empty, land, tmem_full[2], tmem_empty[2], h_full[2], h_empty[2], done
+  static constexpr int kNumBars = 3 * STAGES + 8 + 1;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;
   static constexpr int kOffScan = kOffMisc + 16;         // 8 warp totals
   static constexpr int kOffRows = kOffScan + 32;         // group starts [E + 1]
@@ -167,6 +202,7 @@ __device__ __forceinline__ int find_group(const int* first, int E, int u) {
 
 struct GroupedUnit {
   int e;      // group
+  int rt;     // row tile of the group
   int tn;     // column tile
   int row0;   // first row of A and C
   int rows;   // rows of C to store
@@ -185,7 +221,8 @@ __device__ __forceinline__ GroupedUnit grouped_unit(const GroupedParams& p, cons
   const int gs = min(count - g * kGrpRaster, kGrpRaster);
   const int r = local - g * per;
   u.tn = r / gs;
-  u.row0 = rows[u.e] + (g * kGrpRaster + r % gs) * tr;
+  u.rt = g * kGrpRaster + r % gs;
+  u.row0 = rows[u.e] + u.rt * tr;
   u.rows = min(tr, rows[u.e + 1] - u.row0);
   u.nmma = (u.rows + 16 * CG - 1) / (16 * CG) * (16 * CG);
   return u;
@@ -209,11 +246,96 @@ __device__ __forceinline__ void zero_rows(const GroupedParams& p, int lo, int hi
   }
 }
 
-template <int CG, int TM, int STAGES>
+// The 32 ranks of one row's block as a row of the swizzled adapter buffer:
+// hi in the first four 16-byte chunks, lo in the last four.
+__device__ __forceinline__ void split_ranks(const float* h, int valid, bool bf16, uint4 (&out)[8]) {
+  uint32_t w[32];
+#pragma unroll
+  for (int i = 0; i < kLoraRanks; i += 4) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (i < valid) v = __ldcg(reinterpret_cast<const float4*>(h + i));   // the pitch of h is a multiple of 16 ranks
+    const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+      uint32_t hi = 0, lo = 0;
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        const unsigned short top = to_16bit(f[e + o], bf16);
+        hi |= static_cast<uint32_t>(top) << (16 * o);
+        // an h beyond the type's range is infinite in hi; lo must not undo that
+        const float rest = f[e + o] - from_16bit(top, bf16);
+        lo |= static_cast<uint32_t>(to_16bit(isfinite(rest) ? rest : 0.0f, bf16)) << (16 * o);
+      }
+      w[(i + e) / 2] = hi;
+      w[16 + (i + e) / 2] = lo;
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 8; ++c) out[c] = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+}
+
+__device__ __forceinline__ bool nonfinite16(uint32_t h, bool bf16) {
+  const uint32_t exponent = bf16 ? 0x7F80u : 0x7C00u;
+  return (h & exponent) == exponent;
+}
+
+// Replaces the inf and NaN among the first 32 ranks of column `col` of a
+// landed `up` tile by zeros; says whether there were any.
+__device__ __forceinline__ bool clear_nonfinite(uint8_t* tile, int col, bool kmaj, bool bf16) {
+  bool any = false;
+  if (kmaj) {   // row `col`, ranks in 16-byte chunks swizzled by the row
+#pragma unroll
+    for (int c = 0; c < kLoraRanks / 8; ++c) {
+      uint32_t* at = reinterpret_cast<uint32_t*>(tile + col * 128 + ((c ^ (col & 7)) << 4));
+      const uint4 v = *reinterpret_cast<const uint4*>(at);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool lo = nonfinite16(w[i], bf16), hi = nonfinite16(w[i] >> 16, bf16);
+        if (lo || hi) {
+          at[i] = w[i] & (lo ? 0xFFFF0000u : 0xFFFFFFFFu) & (hi ? 0x0000FFFFu : 0xFFFFFFFFu);
+          any = true;
+        }
+      }
+    }
+  } else {      // atom col / 64, one rank per row
+    uint8_t* atom = tile + (col >> 6) * (kBK * 128);
+    const int c = col & 63;
+#pragma unroll 8
+    for (int r = 0; r < kLoraRanks; ++r) {
+      unsigned short* at = reinterpret_cast<unsigned short*>(atom + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
+      if (nonfinite16(*at, bf16)) {
+        *at = 0;
+        any = true;
+      }
+    }
+  }
+  return any;
+}
+
+// What clear_nonfinite took out of row t's value in column n.
+__device__ __noinline__ float nonfinite_terms(const GroupedParams& p, int t, int n) {
+  bool bad = false;
+  const int a = adapter_of(p.adapter, p.adapter64, t, p.L, bad);
+  float sum = 0.0f;
+  if (a >= 0) {
+    for (int r = 0; r < p.R; ++r) {
+      const unsigned short w =
+          p.up[a * p.stride_up + (p.up_kmaj ? n * p.ld_up + r : r * p.ld_up + n)];
+      if (nonfinite16(w, p.bf16 != 0)) {
+        sum += p.h[static_cast<long long>(t) * p.h_pitch + r] * from_16bit(w, p.bf16 != 0);
+      }
+    }
+  }
+  return sum;
+}
+
+template <int CG, int TM, int STAGES, bool LORA>
 __global__ void __launch_bounds__(kNumThreads, 1)
     gemm_grouped_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                       const __grid_constant__ CUtensorMap tmC, const __grid_constant__ GroupedParams p) {
-  using Plan = GroupedPlan<CG, TM, STAGES>;
+                       const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmU,
+                       const __grid_constant__ GroupedParams p) {
+  using Plan = GroupedPlan<CG, TM, STAGES, LORA>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sW = smem + Plan::kOffW;
@@ -221,9 +343,13 @@ __global__ void __launch_bounds__(kNumThreads, 1)
   uint8_t* sOut = smem + Plan::kOffOut;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + Plan::kOffBar);
   uint64_t* empty_bar = full_bar + STAGES;
-  uint64_t* tfull_bar = empty_bar + STAGES;
+  uint64_t* land_bar = empty_bar + STAGES;   // an adapter's weights, per CTA
+  uint64_t* tfull_bar = land_bar + STAGES;
   uint64_t* tempty_bar = tfull_bar + 2;
-  uint64_t* done_bar = tempty_bar + 2;
+  uint64_t* hfull_bar = tempty_bar + 2;
+  uint64_t* hempty_bar = hfull_bar + 2;
+  uint64_t* done_bar = hempty_bar + 2;
+  uint8_t* sH = smem + Plan::kOffH;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Plan::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* scan = reinterpret_cast<int*>(smem + Plan::kOffScan);
@@ -242,11 +368,16 @@ __global__ void __launch_bounds__(kNumThreads, 1)
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
+      mbar_init(&land_bar[s], 1);
     }
     mbar_init(&tfull_bar[0], 1);
     mbar_init(&tfull_bar[1], 1);
     mbar_init(&tempty_bar[0], kEpiWarps * CG);
     mbar_init(&tempty_bar[1], kEpiWarps * CG);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&hfull_bar[b], kEpiWarps * CG);
+      mbar_init(&hempty_bar[b], 1);
+    }
     mbar_init(done_bar, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -254,6 +385,7 @@ __global__ void __launch_bounds__(kNumThreads, 1)
   if (warp == 0 && lane == 0) {
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
+    if (LORA) prefetch_tmap(&tmU);
     if (p.c_tma) prefetch_tmap(&tmC);
   }
   if (warp == 1) {
@@ -266,7 +398,11 @@ __global__ void __launch_bounds__(kNumThreads, 1)
   if constexpr (CG == 2) cluster_sync();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  griddep_wait();
+  // With LORA the previous grid is lora_shrink, which lets this one start
+  // once everything before it has completed: A and B can be read at once, and
+  // only what touches h, the lists or C waits (each thread for itself, below).
+  if constexpr (!LORA) griddep_wait();
+  const int rank_blocks = LORA ? (p.R + kLoraRanks - 1) / kLoraRanks : 0;
 
   scan_groups<kNumThreads>(p.offsets, p.off64, p.E, p.T, grp_rows, grp_tiles, scan, p.err, [&](int n) {
     int count, tr;
@@ -281,6 +417,8 @@ __global__ void __launch_bounds__(kNumThreads, 1)
       int stage = 0;
       uint32_t phase = 0;
       int issued = 0;
+      // per stage: parity of its last fill on full / land, and which came last
+      uint32_t full_par = 0, land_par = 0, on_land = 0;
       bool ok = true;
       for (int t = worker; ok && t < num_tiles; t += workers) {
         const GroupedUnit u = grouped_unit<CG, TM>(p, grp_rows, grp_tiles, t);
@@ -323,10 +461,41 @@ __global__ void __launch_bounds__(kNumThreads, 1)
               tma_load_2d_pair(t_dst + b * Plan::kBoxRows * 128, &tmA, bar, k0, arow + b * Plan::kBoxRows);
             }
           }
+          full_par ^= 1u << stage;
+          on_land &= ~(1u << stage);
           ++issued;
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1u;
+          }
+        }
+        if constexpr (LORA) {
+          if (t == worker) griddep_wait();   // the lists are lora_shrink's
+          const int* list = p.lists + static_cast<long long>(u.rt) * kAdapterListPitch;
+          const int adapters = ok ? list[0] : 0;
+          for (int b = 0; b < rank_blocks * adapters; ++b) {
+            const int a = list[1 + b % adapters], r0 = b / adapters * kLoraRanks;
+            if (issued >= STAGES && !mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) {
+              ok = false;
+              break;
+            }
+            uint8_t* w_dst = sW + stage * Plan::kWBytes;
+            // on a barrier of this CTA: its epilogue warps look the weights over
+            uint64_t* bar = &land_bar[stage];
+            mbar_arrive_expect_tx(bar, Plan::kWBytes);
+            if (p.up_kmaj) {
+              tma_load_3d(w_dst, &tmU, bar, r0, bcol, a);
+            } else {
+              tma_load_3d(w_dst, &tmU, bar, bcol, r0, a);
+              tma_load_3d(w_dst + kBK * 128, &tmU, bar, bcol + 64, r0, a);
+            }
+            land_par ^= 1u << stage;
+            on_land |= 1u << stage;
+            ++issued;
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
           }
         }
       }
@@ -335,19 +504,19 @@ __global__ void __launch_bounds__(kNumThreads, 1)
         *abort_flag = 1;
         atomicOr(p.err, kDevErrTimeoutProducer);
       }
-      // every fill must have landed before the CTA exits (the odd CTA of a
-      // pair is covered by the cluster barrier at teardown)
-      if (leader) {
-        const int outstanding = issued < STAGES ? issued : STAGES;
-        for (int i = 0; i < outstanding; ++i) {
-          stage = (stage == 0) ? STAGES - 1 : stage - 1;
-          if (stage == STAGES - 1) phase ^= 1u;
-          const uint64_t t0 = globaltimer_ns();
-          while (!mbar_try_wait(&full_bar[stage], phase)) {
-            if (globaltimer_ns() - t0 > kWaitLimitNs) {
-              atomicOr(p.err, kDevErrTimeoutTeardown);
-              break;
-            }
+      // every fill must have landed before the CTA exits (the odd CTA's fills
+      // of the even one's barriers are covered by the cluster barrier at
+      // teardown)
+      for (int s = 0; s < min(issued, STAGES); ++s) {
+        const uint32_t bit = 1u << s;
+        if (!(on_land & bit) && !leader) continue;
+        uint64_t* bar = (on_land & bit) ? &land_bar[s] : &full_bar[s];
+        const uint32_t par = (((on_land & bit) ? land_par : full_par) & bit) ? 0u : 1u;   // of the last fill
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(bar, par)) {
+          if (globaltimer_ns() - t0 > kWaitLimitNs) {
+            atomicOr(p.err, kDevErrTimeoutTeardown);
+            break;
           }
         }
       }
@@ -358,10 +527,12 @@ __global__ void __launch_bounds__(kNumThreads, 1)
       // descriptor strides of the two major orders: see gemm_sm100_kernel.cuh
       const uint32_t w_lbo = p.b_kmaj ? 16 : kBK * 128, w_kstep = p.b_kmaj ? kUmmaK * 2 : kUmmaK * 128;
       int stage = 0;
-      uint32_t phase = 0;
+      uint32_t full_par = 0;   // per stage: parity of its next fill
       int acc = 0;
       uint32_t acc_phase = 0;
       int count = 0;
+      int hb = 0;
+      uint32_t hphase = 0;
       bool ok = true;
       for (int t = worker; ok && t < num_tiles; t += workers) {
         if (p.kb_total == 0) break;   // the epilogue writes act(bias) by itself
@@ -375,10 +546,11 @@ __global__ void __launch_bounds__(kNumThreads, 1)
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * TM);
         for (int kb = 0; kb < p.kb_total; ++kb) {
-          if (!mbar_wait(&full_bar[stage], phase, abort_flag)) {
+          if (!mbar_wait(&full_bar[stage], (full_par >> stage) & 1u, abort_flag)) {
             ok = false;
             break;
           }
+          full_par ^= 1u << stage;
           tc_fence_after();
           const uint32_t w0 = smem_u32(sW + stage * Plan::kWBytes);
           const uint32_t t0 = smem_u32(sT + stage * Plan::kTBytes);
@@ -388,9 +560,34 @@ __global__ void __launch_bounds__(kNumThreads, 1)
                            smem_desc_sw128(t0 + j * (kUmmaK * 2), 16, 1024), idesc, (kb > 0 || j > 0) ? 1u : 0u);
           }
           mma_commit<CG>(&empty_bar[stage]);
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
+          if (++stage == STAGES) stage = 0;
+        }
+        if constexpr (LORA) {
+          if (t == worker) griddep_wait();
+          const uint32_t idesc_up = idesc_16bit(kGrpCols * CG, u.nmma, p.up_kmaj == 0, false, p.bf16 != 0);
+          const uint32_t u_lbo = p.up_kmaj ? 16 : kBK * 128, u_kstep = p.up_kmaj ? kUmmaK * 2 : kUmmaK * 128;
+          const int adapters = ok ? p.lists[static_cast<long long>(u.rt) * kAdapterListPitch] : 0;
+          for (int b = 0; b < rank_blocks * adapters; ++b) {
+            const int steps = min(kLoraRanks, p.R - b / adapters * kLoraRanks) > kUmmaK ? 2 : 1;
+            if (!mbar_wait_cluster(&hfull_bar[hb], hphase, abort_flag)) {   // `up` has landed, h is built
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t w0 = smem_u32(sW + stage * Plan::kWBytes);
+            const uint32_t h0 = smem_u32(sH + hb * Plan::kTBytes);
+            for (int j = 0; j < steps; ++j) {
+              const uint64_t wd = smem_desc_sw128(w0 + j * u_kstep, u_lbo, 1024);
+#pragma unroll
+              for (int part = 0; part < 2; ++part) {   // hi, lo
+                mma_f16_ss<CG>(d_tmem, wd, smem_desc_sw128(h0 + part * 64 + j * (kUmmaK * 2), 16, 1024), idesc_up, 1u);
+              }
+            }
+            mma_commit<CG>(&empty_bar[stage]);
+            mma_commit<CG>(&hempty_bar[hb]);
+            if (++stage == STAGES) stage = 0;
+            hb ^= 1;
+            if (hb == 0) hphase ^= 1u;
           }
         }
         if (!ok) break;
@@ -418,6 +615,10 @@ __global__ void __launch_bounds__(kNumThreads, 1)
     const int et = static_cast<int>(threadIdx.x) - 64;
     const bool bf16 = p.bf16 != 0;
     const uint32_t tempty_remote0 = (CG == 2) ? mapa_shared(smem_u32(&tempty_bar[0]), 0) : 0u;
+    const uint32_t hfull_remote0 = (CG == 2) ? mapa_shared(smem_u32(&hfull_bar[0]), 0) : 0u;
+    int hb = 0, hcount = 0, stage = 0;
+    uint32_t hphase = 0, land_par = 0;
+    if constexpr (LORA) griddep_wait();
     if (p.zero_rest) zero_rows(p, grp_rows[0], grp_rows[p.E], et, 32 * kEpiWarps);
     int buf_i = 0;
     int acc = 0;
@@ -430,7 +631,54 @@ __global__ void __launch_bounds__(kNumThreads, 1)
       const float bias =
           (p.bias != nullptr && n < p.N) ? from_16bit(p.bias[static_cast<long long>(u.e) * p.N + n], bf16) : 0.0f;
       bool got = true;
-      if (p.kb_total > 0 && lane == 0) got = mbar_wait(&tfull_bar[acc], acc_phase, abort_flag);
+      bool odd = false;   // this column held an inf or NaN in some adapter's `up`
+      if constexpr (LORA) {
+        // adapter rows of this CTA's share of the tile: thread et builds row et
+        const int* list = p.lists + static_cast<long long>(u.rt) * kAdapterListPitch;
+        const int adapters = list[0];
+        const bool mixed = adapters > 1 || list[kAdapterListPitch - 1] > 0;
+        const int half = u.nmma / CG;
+        const int tr = static_cast<int>(rank) * half + et;   // row of the tile
+        bool bad = false;
+        const int mine =
+            (et < half && tr < u.rows) ? adapter_of(p.adapter, p.adapter64, u.row0 + tr, p.L, bad) : -1;
+        const float* hrow = p.h + static_cast<long long>(u.row0 + tr) * p.h_pitch;
+        stage = (stage + p.kb_total) % STAGES;
+        for (int rb = 0; rb < rank_blocks && got; ++rb) {
+          uint4 own[8];
+          if (mine >= 0) split_ranks(hrow + rb * kLoraRanks, p.h_pitch - rb * kLoraRanks, bf16, own);
+          for (int ai = 0; ai < adapters; ++ai) {
+            got = (hcount < 2 || mbar_wait(&hempty_bar[hb], hphase ^ 1u, abort_flag)) &&
+                  mbar_wait(&land_bar[stage], (land_par >> stage) & 1u, abort_flag);
+            got = __all_sync(0xffffffffu, got) != 0;
+            if (!got) break;
+            land_par ^= 1u << stage;
+            if (mixed) odd |= clear_nonfinite(sW + stage * Plan::kWBytes, col, p.up_kmaj != 0, bf16);
+            if (et < half) {
+              const bool is = mine >= 0 && list[1 + ai] == mine;
+              uint8_t* dst = sH + hb * Plan::kTBytes + et * 128;
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {
+                *reinterpret_cast<uint4*>(dst + ((c ^ (et & 7)) << 4)) = is ? own[c] : make_uint4(0u, 0u, 0u, 0u);
+              }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (CG == 1) {
+                mbar_arrive(&hfull_bar[hb]);
+              } else {
+                mbar_arrive_cluster(hfull_remote0 + static_cast<uint32_t>(hb * 8));
+              }
+            }
+            if (++stage == STAGES) stage = 0;
+            ++hcount;
+            hb ^= 1;
+            if (hb == 0) hphase ^= 1u;
+          }
+        }
+      }
+      if (got && p.kb_total > 0 && lane == 0) got = mbar_wait(&tfull_bar[acc], acc_phase, abort_flag);
       got = __shfl_sync(0xffffffffu, got ? 1 : 0, 0) != 0;
       ok = named_bar_and(1, 32 * kEpiWarps, got);
       if (!ok) break;
@@ -449,6 +697,14 @@ __global__ void __launch_bounds__(kNumThreads, 1)
         // A TMA store clips its box at the tensor's edge in units larger than
         // an element (with an odd N it wrote past the end of the rows), so an
         // edge tile goes by TMA only when the rows end on a 16-byte boundary.
+        if (LORA && odd && n < p.N) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (r0 + i < u.rows) {
+              v[i] = __float_as_uint(__uint_as_float(v[i]) + nonfinite_terms(p, u.row0 + r0 + i, n));
+            }
+          }
+        }
         const bool whole = p.c_tma && r0 + kGrpChunk <= u.rows &&
                            (n0 + kGrpCols <= p.N || (n0 < p.N && p.N % 8 == 0));
         uint8_t* buf = sOut + buf_i * Plan::kOutBytes;

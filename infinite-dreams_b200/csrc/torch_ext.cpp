@@ -10,6 +10,7 @@
 //   gemm_ex(A, B, cfg_id, alpha, beta, C, bias, act, out) -> out
 //   grouped_gemm(A, B, offsets, bias, act, out) -> out
 //   grouped_gemm_wgrad(A, G, offsets, out) -> out
+//   lora_gemm(x, W, down, up, adapter, scale, bias, act, out) -> out
 //   reset_workspaces()
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -165,13 +166,14 @@ bool is_16bit(const at::Tensor& t) { return t.scalar_type() == at::kHalf || t.sc
 
 int dtype_id(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? GEMM_DTYPE_BF16 : GEMM_DTYPE_F16; }
 
+// A is the operand that holds the rows; every other one goes by it.
 void check_like(const at::Tensor& t, const at::Tensor& A, const char* name) {
-  TORCH_CHECK(t.is_cuda() && t.device() == A.device(), name, " must be on A's device");
-  TORCH_CHECK(t.scalar_type() == A.scalar_type(), name, " must have A's dtype");
+  TORCH_CHECK(t.is_cuda() && t.device() == A.device(), name, " must be on the rows' device");
+  TORCH_CHECK(t.scalar_type() == A.scalar_type(), name, " must have the rows' dtype");
 }
 
 void check_index(const at::Tensor& t, const at::Tensor& A, int64_t n, const char* name) {
-  TORCH_CHECK(t.is_cuda() && t.device() == A.device(), name, " must be on A's device");
+  TORCH_CHECK(t.is_cuda() && t.device() == A.device(), name, " must be on the rows' device");
   TORCH_CHECK(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must be int32 or int64");
   TORCH_CHECK(t.dim() == 1 && t.size(0) == n, name, " must be 1D with ", n, " elements");
 }
@@ -212,7 +214,7 @@ at::Tensor rows_out(const c10::optional<at::Tensor>& out, int64_t T, int64_t N, 
   const at::Tensor& C = *out;
   TORCH_CHECK(C.is_cuda() && C.device() == A.device() && C.scalar_type() == A.scalar_type() && C.dim() == 2 &&
                   C.size(0) == T && C.size(1) == N && (C.stride(1) == 1 || N <= 1) && (T <= 1 || C.stride(0) >= N),
-              "out must be a (T x N) tensor of A's dtype with unit column stride on A's device");
+              "out must be a (T x N) tensor of the rows' dtype with unit column stride on their device");
   return C;
 }
 
@@ -283,6 +285,58 @@ at::Tensor grouped_gemm_wgrad(const at::Tensor& A, const at::Tensor& G, const at
   return D;
 }
 
+at::Tensor lora_gemm(const at::Tensor& x, const at::Tensor& W, const at::Tensor& down, const at::Tensor& up,
+                     const at::Tensor& adapter, c10::optional<at::Tensor> scale, c10::optional<at::Tensor> bias,
+                     int64_t act, c10::optional<at::Tensor> out) {
+  TORCH_CHECK(x.is_cuda(), "x must be CUDA tensor");
+  TORCH_CHECK(is_16bit(x), "x must be float16 or bfloat16");
+  TORCH_CHECK(x.dim() == 2, "x must be 2D (T x K)");
+  check_like(W, x, "W");
+  check_like(down, x, "down");
+  check_like(up, x, "up");
+  TORCH_CHECK(W.dim() == 2 && W.size(0) == x.size(1), "W must be 2D (K x N)");
+  const int64_t T = x.size(0), K = x.size(1), N = W.size(1);
+  TORCH_CHECK(down.dim() == 3 && down.size(1) == K, "down must be 3D (L x K x R)");
+  const int64_t L = down.size(0), R = down.size(2);
+  TORCH_CHECK(up.dim() == 3 && up.size(0) == L && up.size(1) == R && up.size(2) == N, "up must be 3D (L x R x N)");
+  TORCH_CHECK(K >= 1 && L >= 1 && R >= 1, "K, the number of adapters and the rank must be at least 1");
+  check_index(adapter, x, T, "adapter");
+  at::Tensor svec, bvec;
+  if (scale.has_value()) {
+    svec = *scale;
+    TORCH_CHECK(svec.is_cuda() && svec.device() == x.device() && svec.scalar_type() == at::kFloat && svec.dim() == 1 &&
+                    svec.size(0) == L,
+                "scale must be a float32 tensor of L elements on x's device");
+    svec = svec.contiguous();
+  }
+  if (bias.has_value()) {
+    check_like(*bias, x, "bias");
+    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == N, "bias must be (N)");
+    bvec = bias->contiguous();
+  }
+  check_no_grad("lora_gemm is a serving operator and computes no gradients: call it under torch.no_grad()",
+                {x, W, down, up, svec, bvec});
+  const c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor xs = row_operand(x), ids = adapter.contiguous();
+  auto [Ws, tw, ldw] = operand(W);
+  auto [Ds, td, ldd, sd] = stacked_operand(down);
+  auto [Us, tu, ldu, su] = stacked_operand(up);
+  at::Tensor C = rows_out(out, T, N, x);
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream(x.device().index()).stream();
+  const int64_t ldx = pitch(xs);
+  Scratch ws = scratch(x.device(), stream,
+                       gemm_lora_workspace_bytes(xs.data_ptr(), Ws.data_ptr(), Us.data_ptr(), T, N, K, L, R, ldx, ldw,
+                                                 tw, ldu, su, tu));
+  check_status(gemm_lora_launch(xs.data_ptr(), Ws.data_ptr(), Ds.data_ptr(), Us.data_ptr(), C.data_ptr(),
+                                ids.data_ptr(), ids.scalar_type() == at::kLong ? 64 : 32, T, N, K, L, R, ldx, ldw, tw,
+                                ldd, sd, td, ldu, su, tu, std::max<int64_t>(pitch(C), N),
+                                svec.defined() ? svec.data_ptr<float>() : nullptr,
+                                bvec.defined() ? bvec.data_ptr() : nullptr, static_cast<int>(act), dtype_id(x), ws.ptr,
+                                ws.len, stream),
+               "gemm_lora_launch");
+  return C;
+}
+
 void reset_workspaces() {
   std::lock_guard<std::mutex> lock(g_ws_mu);
   g_ws->clear();
@@ -302,5 +356,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("out") = py::none());
   m.def("grouped_gemm_wgrad", &grouped_gemm_wgrad, "out[e] = A[rows of e].T @ G[rows of e]", py::arg("A"),
         py::arg("G"), py::arg("offsets"), py::arg("out") = py::none());
+  m.def("lora_gemm", &lora_gemm, "out[t] = act(x[t] @ W + scale[a] * (x[t] @ down[a]) @ up[a] + bias), a = adapter[t]",
+        py::arg("x"), py::arg("W"), py::arg("down"), py::arg("up"), py::arg("adapter"), py::arg("scale") = py::none(),
+        py::arg("bias") = py::none(), py::arg("act") = 0, py::arg("out") = py::none());
   m.def("reset_workspaces", &reset_workspaces, "drop the cached split-K / repack workspaces");
 }

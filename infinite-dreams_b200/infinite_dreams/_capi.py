@@ -60,6 +60,11 @@ _SIG = [
     ("gemm_grouped_wgrad_launch", ctypes.c_int,
      [_P, _P, _P, _P, ctypes.c_int] + [_I64] * 8 + [ctypes.c_int, _P, ctypes.c_size_t, _P]),
     ("gemm_grouped_wgrad_workspace_bytes", ctypes.c_size_t, [_P, _P] + [_I64] * 5),
+    ("gemm_lora_launch", ctypes.c_int,
+     [_P] * 6 + [ctypes.c_int] + [_I64] * 7 + [ctypes.c_int, _I64, _I64, ctypes.c_int, _I64, _I64, ctypes.c_int, _I64,
+      _P, _P, ctypes.c_int, ctypes.c_int, _P, ctypes.c_size_t, _P]),
+    ("gemm_lora_workspace_bytes", ctypes.c_size_t,
+     [_P, _P, _P] + [_I64] * 7 + [ctypes.c_int, _I64, _I64, ctypes.c_int]),
     ("gemm_launch_gather", ctypes.c_int,
      [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, ctypes.POINTER(ctypes.c_void_p), ctypes.c_int, ctypes.c_int,
       _P, ctypes.c_size_t, _P]),

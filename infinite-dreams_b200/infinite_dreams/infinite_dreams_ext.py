@@ -19,8 +19,9 @@ by the sm_100a kernel bank through its C ABI (include/gemm_sm100.h):
 place and a fused epilogue (alpha, beta * C, bias, ReLU / GELU).  So do the
 products whose weight is picked by the row, in fp16 and bf16:
 ``grouped_gemm`` (rows sorted by expert, ragged counts) and its weight
-gradient ``grouped_gemm_wgrad``; ``grouped.grouped_linear`` is the pair as a
-differentiable function.
+gradient ``grouped_gemm_wgrad`` (``grouped.grouped_linear`` is the pair as a
+differentiable function), and ``lora_gemm`` (a shared projection with the
+low-rank adapter that each row picks).
 
 Like the reference, inputs are made contiguous, C is allocated from torch's
 caching allocator on A's device, and the launch is asynchronous on the
@@ -269,15 +270,16 @@ def _dtype_id(t: torch.Tensor) -> int:
 
 
 def _check_like(t, A: torch.Tensor, name: str) -> None:
+    """A is the operand that holds the rows; every other one goes by it."""
     if not isinstance(t, torch.Tensor) or t.device != A.device:
-        raise RuntimeError(f"{name} must be on A's device")
+        raise RuntimeError(f"{name} must be on the rows' device")
     if t.dtype != A.dtype:
-        raise RuntimeError(f"{name} must have A's dtype")
+        raise RuntimeError(f"{name} must have the rows' dtype")
 
 
 def _check_index(t, A: torch.Tensor, n: int, name: str) -> None:
     if not isinstance(t, torch.Tensor) or t.device != A.device:
-        raise RuntimeError(f"{name} must be on A's device")
+        raise RuntimeError(f"{name} must be on the rows' device")
     if t.dtype not in (torch.int32, torch.int64):
         raise RuntimeError(f"{name} must be int32 or int64")
     if t.dim() != 1 or t.size(0) != n:
@@ -318,7 +320,7 @@ def _rows_out(out: Optional[torch.Tensor], T: int, N: int, A: torch.Tensor) -> t
         return torch.empty((T, N), dtype=A.dtype, device=A.device)
     if (out.device != A.device or out.dtype != A.dtype or tuple(out.shape) != (T, N)
             or (out.stride(1) != 1 and N > 1) or (T > 1 and out.stride(0) < N)):
-        raise RuntimeError("out must be a (T x N) tensor of A's dtype with unit column stride on A's device")
+        raise RuntimeError("out must be a (T x N) tensor of the rows' dtype with unit column stride on their device")
     return out
 
 
@@ -427,6 +429,79 @@ def grouped_gemm_wgrad(A: torch.Tensor, G: torch.Tensor, offsets: torch.Tensor, 
     return D
 
 
+def lora_gemm(x: torch.Tensor, W: torch.Tensor, down: torch.Tensor, up: torch.Tensor, adapter: torch.Tensor, *,
+              scale: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, activation: str = "none",
+              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out[t] = act(x[t] @ W + scale[a] * (x[t] @ down[a]) @ up[a] + bias) with a = adapter[t].
+
+    The shared projection W [K, N] of all rows, beside the low-rank adapter
+    that each row picks: x is [T, K], down [L, K, R], up [L, R, N] (each
+    weight row-major or a transposed view, read in place), fp16 or bf16, all
+    alike.  adapter: T int32 or int64 numbers on the device, in any order;
+    negative means none, a number past the last adapter counts as none and
+    is reported by ``check_device_errors``.  scale is float32 [L], bias [N].
+    Adapters of smaller ranks are padded with zeros; R is at most 1024.  x @
+    down stays in fp32.  One request's inf or NaN does not reach the rows of
+    others.  A serving operator: it computes no gradients and refuses inputs
+    that ask for them.
+    """
+    if activation not in _capi.ACTIVATIONS:
+        raise RuntimeError(f"activation must be one of {sorted(_capi.ACTIVATIONS)}")
+    act = _capi.ACTIVATIONS[activation]
+    if _fast is not None:
+        return _fast.lora_gemm(x, W, down, up, adapter, scale, bias, act, out)
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise RuntimeError("x must be CUDA tensor")
+    if not _is_16bit(x):
+        raise RuntimeError("x must be float16 or bfloat16")
+    if x.dim() != 2:
+        raise RuntimeError("x must be 2D (T x K)")
+    for t, name in ((W, "W"), (down, "down"), (up, "up")):
+        _check_like(t, x, name)
+    T, K = x.shape
+    if W.dim() != 2 or W.size(0) != K:
+        raise RuntimeError("W must be 2D (K x N)")
+    N = W.size(1)
+    if down.dim() != 3 or down.size(1) != K:
+        raise RuntimeError("down must be 3D (L x K x R)")
+    L, R = down.size(0), down.size(2)
+    if tuple(up.shape) != (L, R, N):
+        raise RuntimeError("up must be 3D (L x R x N)")
+    if K < 1 or L < 1 or R < 1:
+        raise RuntimeError("K, the number of adapters and the rank must be at least 1")
+    _check_index(adapter, x, T, "adapter")
+    if scale is not None:
+        if scale.device != x.device or scale.dtype != torch.float32 or tuple(scale.shape) != (L,):
+            raise RuntimeError("scale must be a float32 tensor of L elements on x's device")
+        scale = scale.contiguous()
+    if bias is not None:
+        _check_like(bias, x, "bias")
+        if tuple(bias.shape) != (N,):
+            raise RuntimeError("bias must be (N)")
+        bias = bias.contiguous()
+    _check_no_grad("lora_gemm is a serving operator and computes no gradients: call it under torch.no_grad()",
+                   x, W, down, up, scale, bias)
+    with torch.cuda.device(x.device):
+        xs, ids = _row_operand(x), adapter.contiguous()
+        Ws, tw, ldw = _operand(W)
+        Ds, td, ldd, sd = _stacked_operand(down)
+        Us, tu, ldu, su = _stacked_operand(up)
+        C = _rows_out(out, T, N, x)
+        stream = torch.cuda.current_stream(x.device)
+        ldx = _pitch(xs)
+        need = lib.gemm_lora_workspace_bytes(xs.data_ptr(), Ws.data_ptr(), Us.data_ptr(), T, N, K, L, R, ldx, ldw, tw,
+                                             ldu, su, tu)
+        keep, ws_ptr, ws_len = _scratch(x.device, stream, need)
+        st = lib.gemm_lora_launch(xs.data_ptr(), Ws.data_ptr(), Ds.data_ptr(), Us.data_ptr(), C.data_ptr(),
+                                  ids.data_ptr(), 64 if ids.dtype == torch.int64 else 32, T, N, K, L, R, ldx, ldw, tw,
+                                  ldd, sd, td, ldu, su, tu, max(_pitch(C), N),
+                                  scale.data_ptr() if scale is not None else None,
+                                  bias.data_ptr() if bias is not None else None, act, _dtype_id(x), ws_ptr, ws_len,
+                                  stream.cuda_stream or None)
+        _capi.check(st, "gemm_lora_launch")
+    return C
+
+
 def gemm_cfg_table_cpu() -> torch.Tensor:
     """CPU int32 tensor [num_cfg, len(CFG_COLUMNS)], columns CFG_COLUMNS."""
     cols, rows = _capi.menu()
@@ -450,6 +525,6 @@ def check_device_errors(device: Optional[int] = None) -> None:
         raise GemmError(st, f"device {dev}: kernel error bits {code.value}: {message}")
 
 
-__all__ = ["gemm_forward", "gemm_forward_cfg", "gemm_ex", "grouped_gemm", "grouped_gemm_wgrad",
+__all__ = ["gemm_forward", "gemm_forward_cfg", "gemm_ex", "grouped_gemm", "grouped_gemm_wgrad", "lora_gemm",
            "gemm_cfg_table_cpu", "CFG_COLUMNS", "NUM_CFG",
            "default_cfg", "check_device_errors", "GemmError", "reset_workspaces"]

@@ -102,3 +102,34 @@ def ref_wgrad(A, G, offsets):
         if a.shape[0]:
             tol[e] = rounded(ref[e], sum_error(a.shape[0], a.abs().T @ g.abs()), A.dtype)
     return ref, tol
+
+
+def ref_lora(x, W, down, up, adapter, scale=None, bias=None, act="none"):
+    """(reference, bound) of lora_gemm.
+
+    h is an fp32 sum of K products, scaled (one more rounding of 2^-24); what
+    its two 16-bit parts leave out is a quarter step of a step, at most
+    half_step^2 of |h|, or half a subnormal step of the type.
+    """
+    K, R = x.shape[1], down.shape[2]
+    dt, xd = x.dtype, x.double()
+    v, mag = xd @ W.double(), xd.abs() @ W.double().abs()
+    err = torch.zeros_like(v)
+    ids = adapter.long()
+    for a in ids.unique().tolist():
+        if not 0 <= a < down.shape[0]:
+            continue
+        at = (ids == a).nonzero().flatten()
+        s = 1.0 if scale is None else float(scale[a])
+        d, u = down[a].double(), up[a].double()
+        h, h_mag = s * (xd[at] @ d), abs(s) * (xd[at].abs() @ d.abs())
+        tiny = torch.finfo(dt).smallest_normal * half_step(dt)
+        h_err = sum_error(K, h_mag) + 2.0 ** -24 * h_mag + half_step(dt) ** 2 * h.abs() + tiny
+        v[at] += h @ u
+        mag[at] += h.abs() @ u.abs()
+        err[at] += h_err @ u.abs()
+    if bias is not None:
+        v, mag = v + bias.double(), mag + bias.double().abs()
+    err = act_error(v, err + sum_error(K + 2 * R, mag), act)
+    ref = act64(v, act)
+    return ref, rounded(ref, err, dt)

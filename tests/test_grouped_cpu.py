@@ -77,3 +77,37 @@ def test_wgrad_limits_and_workspace():
     assert _wgrad(M=0) == _capi.GEMM_OK
     assert LIB.gemm_grouped_wgrad_workspace_bytes(P, P, 100, 64, 64, 64, 64) == 0
     assert LIB.gemm_grouped_wgrad_workspace_bytes(P, P, 100, 77, 64, 77, 64) == head + 100 * 128 * 2
+
+
+def _lora(X=P, W=P, down=P, up=P, C=P, ids=P, bits=32, T=8, N=8, K=8, L=2, R=8, ldx=8, ldw=8, tw=0, ldd=8, sd=64, td=0,
+          ldu=8, su=64, tu=0, ldc=8, scale=None, bias=None, act=0, dtype=0):
+    return LIB.gemm_lora_launch(X, W, down, up, C, ids, bits, T, N, K, L, R, ldx, ldw, tw, ldd, sd, td, ldu, su, tu, ldc,
+                                scale, bias, act, dtype, None, 0, None)
+
+
+@pytest.mark.parametrize("bad", [dict(T=-1), dict(K=0), dict(L=0), dict(R=0), dict(bits=1), dict(dtype=5), dict(tw=2),
+                                 dict(td=-1), dict(tu=2), dict(act=-1), dict(X=None), dict(W=None), dict(down=None),
+                                 dict(up=None), dict(ids=None), dict(ldx=7), dict(ldw=7), dict(ldc=7), dict(ldd=7),
+                                 dict(sd=63), dict(ldu=7), dict(su=63), dict(up=P + 1), dict(ids=P + 2),
+                                 dict(scale=P + 2)], ids=str)
+def test_lora_invalid_arguments(bad):
+    assert _lora(**bad) == _capi.GEMM_ERR_INVALID_ARG
+
+
+def test_lora_limits_and_workspace():
+    head = LIB.gemm_workspace_counter_bytes()
+    assert _lora(R=1025, ldd=1025, sd=1 << 20, su=1 << 20) == _capi.GEMM_ERR_UNSUPPORTED
+    assert _lora() == _capi.GEMM_ERR_WORKSPACE
+    assert _lora(T=0) == _capi.GEMM_OK
+    ws = LIB.gemm_lora_workspace_bytes
+    # h of 100 rows x 16 ranks in fp32, one list of 260 numbers
+    assert ws(P, P, P, 100, 64, 64, 2, 8, 64, 64, 0, 64, 512, 0) == head + 100 * 16 * 4 + 1280
+    # up with rows of 6 elements is copied to 64
+    assert (ws(P, P, P, 100, 64, 64, 2, 6, 64, 64, 0, 6, 384, 1) - ws(P, P, P, 100, 64, 64, 2, 6, 64, 64, 0, 64, 384, 0)
+            == 2 * 64 * 128)
+
+
+def test_lora_refuses_cpu_tensors():
+    z = lambda *s: torch.zeros(s, dtype=torch.float16)   # noqa: E731
+    with pytest.raises(RuntimeError, match="x must be CUDA tensor"):
+        ext.lora_gemm(z(4, 8), z(8, 8), z(2, 8, 4), z(2, 4, 8), torch.zeros(4, dtype=torch.int32))
