@@ -711,9 +711,9 @@ int capi_encode(CUtensorMap* map, const void* base, int rank, const int64_t* ext
                 const int* box, bool swizzled, const char* what) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(GEMM_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-  cuuint64_t dims[3], bytes[2];
-  cuuint32_t boxes[3];
-  const cuuint32_t estr[3] = {1, 1, 1};
+  cuuint64_t dims[4], bytes[3];
+  cuuint32_t boxes[4];
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
   for (int i = 0; i < rank; ++i) {
     dims[i] = static_cast<cuuint64_t>(extents[i]);
     boxes[i] = static_cast<cuuint32_t>(box[i]);

@@ -17,7 +17,7 @@ void capi_clear_error();
 // Fails on a device that is not sm_100.
 int capi_device(int* sms, int** err_word);
 
-// Tensor map of a 16-bit tensor: `rank` (2 or 3) extents, innermost first;
+// Tensor map of a 16-bit tensor: `rank` (2 to 4) extents, innermost first;
 // strides[i] is the element stride of dimension i + 1.
 int capi_encode(CUtensorMap* map, const void* base, int rank, const int64_t* extents, const int64_t* strides,
                 const int* box, bool swizzled, const char* what);

@@ -59,17 +59,32 @@ struct Operand {
     return GEMM_OK;
   }
 
-  int encode2(CUtensorMap* m, int box_cols, int box_rows, bool swizzled, const char* what) const {
+  // Boxes of `box_rows` rows x 64 columns.
+  int encode_rows(CUtensorMap* m, int box_rows, const char* what) const {
     const int64_t ext[2] = {cols, rows}, str[1] = {ld};
-    const int box[2] = {box_cols, box_rows};
-    return capi_encode(m, p, 2, ext, str, box, swizzled, what);
+    const int box[2] = {kBK, box_rows};
+    return capi_encode(m, p, 2, ext, str, box, true, what);
   }
 
-  int encode3(CUtensorMap* m, int box_cols, int box_rows, bool swizzled, const char* what) const {
+  // The columns as (64, cols / 64) when that divides, so that one box holds
+  // two 64-column atoms; else boxes of one atom.
+  bool wide() const { return cols % 64 == 0; }
+
+  // 64 rows x 128 columns of one matrix (load_columns).
+  int encode_columns(CUtensorMap* m, const char* what) const {
+    const int64_t ext[3] = {wide() ? 64 : cols, rows, wide() ? cols / 64 : 1}, str[2] = {ld, wide() ? 64 : ld};
+    const int box[3] = {64, kBK, wide() ? 2 : 1};
+    return capi_encode(m, p, 3, ext, str, box, true, what);
+  }
+
+  // A K block of a stacked weight (load_weights); kmaj: stored N x K.
+  int encode_weights(CUtensorMap* m, bool kmaj, const char* what) const {
     // with one matrix the stride is never used, but has to be a legal one
-    const int64_t ext[3] = {cols, rows, batch}, str[2] = {ld, batch == 1 ? round_up(rows * ld, 8) : stride};
-    const int box[3] = {box_cols, box_rows, 1};
-    return capi_encode(m, p, 3, ext, str, box, swizzled, what);
+    const int64_t last = batch == 1 ? round_up(rows * ld, 8) : stride;
+    const bool w = !kmaj && wide();
+    const int64_t ext[4] = {w ? 64 : cols, rows, w ? cols / 64 : 1, batch}, str[3] = {ld, w ? 64 : ld, last};
+    const int box[4] = {64, kmaj ? kGrpCols : kBK, w ? 2 : 1, 1};
+    return capi_encode(m, p, 4, ext, str, box, true, what);
   }
 };
 
@@ -146,35 +161,31 @@ int launch_grouped(const Operand& a, const Operand& b, const Operand* up, const 
   p.tiles_n = static_cast<int>((static_cast<int64_t>(p.N) + kGrpCols * CG - 1) / (kGrpCols * CG));
   const int64_t row_tiles = static_cast<int64_t>(p.T) / TM + p.E;   // at most one cut tile per group
   if (row_tiles * p.tiles_n > kInt32Max) return capi_fail(GEMM_ERR_UNSUPPORTED, "too many output tiles");
-  CUtensorMap tmA, tmB, tmC, tmU;
-  std::memset(&tmA, 0, sizeof(tmA));
-  std::memset(&tmB, 0, sizeof(tmB));
-  std::memset(&tmC, 0, sizeof(tmC));
-  std::memset(&tmU, 0, sizeof(tmU));
-  int st;
+  GroupedMaps maps;
+  std::memset(&maps, 0, sizeof(maps));
+  int st = GEMM_OK;
   if (p.K > 0) {
-    st = a.encode2(&tmA, kBK, Plan::kBoxRows, true, "A");
-    if (st != GEMM_OK) return st;
-    st = p.b_kmaj ? b.encode3(&tmB, kBK, kGrpCols, true, "B (stored N x K)") : b.encode3(&tmB, 64, kBK, true, "B");
-    if (st != GEMM_OK) return st;
+    for (int i = 0; i < 3 && st == GEMM_OK; ++i) st = a.encode_rows(&maps.a[i], Plan::kTokRows >> i, "A");
+    if (st == GEMM_OK) st = b.encode_weights(&maps.b, p.b_kmaj != 0, "B");
+    p.b_wide = b.wide();
   }
-  if (LORA) {
-    st = p.up_kmaj ? up->encode3(&tmU, kBK, kGrpCols, true, "up (stored N x R)") : up->encode3(&tmU, 64, kBK, true, "up");
-    if (st != GEMM_OK) return st;
+  if (LORA && st == GEMM_OK) {
+    st = up->encode_weights(&maps.u, p.up_kmaj != 0, "up");
+    p.up_wide = up->wide();
   }
-  if (p.c_tma) {
+  if (p.c_tma && st == GEMM_OK) {
     const int64_t ext[2] = {p.N, p.T}, str[1] = {p.ldc};
     const int box[2] = {kGrpCols, kGrpChunk};
-    st = capi_encode(&tmC, p.C, 2, ext, str, box, false, "C");
-    if (st != GEMM_OK) return st;
+    st = capi_encode(&maps.c, p.C, 2, ext, str, box, false, "C");
   }
+  if (st != GEMM_OK) return st;
   // persistent: one CTA (pair) per SM (pair), fewer when the most tiles that
   // these sizes can give are fewer
   const int64_t most = std::min<int64_t>(row_tiles * p.tiles_n, sms / CG);
   const int grid = static_cast<int>(most < 1 ? 1 : most) * CG;
   static std::atomic<unsigned long long> configured{0};
   cudaError_t e = launch<CG>(gemm_grouped_sm100<CG, TM, STAGES, LORA>, kNumThreads, Plan::kDynamicBytes, configured,
-                             grid, stream, tmA, tmB, tmC, tmU, p);
+                             grid, stream, maps, p);
   return e == cudaSuccess ? GEMM_OK : capi_fail_cuda(e, "grouped gemm kernel launch");
 }
 
@@ -271,12 +282,15 @@ struct LoraPlan {
 
 constexpr int kWgradStages = 6;
 
-int launch_wgrad(const Operand& a, const Operand& g, const WgradParams& p, int sms, cudaStream_t stream) {
+int launch_wgrad(const Operand& a, const Operand& g, const WgradParams& wp, int sms, cudaStream_t stream) {
   using Plan = WgradPlan<kWgradStages>;
+  WgradParams p = wp;
   CUtensorMap tmA, tmG, tmD;
   std::memset(&tmD, 0, sizeof(tmD));
-  int st = a.encode2(&tmA, 64, kBK, true, "A");
-  if (st == GEMM_OK) st = g.encode2(&tmG, 64, kBK, true, "G");
+  int st = a.encode_columns(&tmA, "A");
+  if (st == GEMM_OK) st = g.encode_columns(&tmG, "G");
+  p.a_wide = a.wide();
+  p.g_wide = g.wide();
   if (st != GEMM_OK) return st;
   if (p.d_tma) {
     const int64_t ext[3] = {p.N, p.M, p.E}, str[2] = {p.ldd, p.E == 1 ? round_up(p.M * p.ldd, 8) : p.stride_d};

@@ -60,6 +60,13 @@ constexpr int kMaxGroups = 1024;   // bounded by the offset tables in shared mem
 constexpr int kGrpChunk = 32;      // rows of C per epilogue step
 constexpr int kGrpRaster = 8;      // row tiles walked before the next column tile
 
+// A's rows come in one box per K block, of TM / CG, half or a quarter as many
+// rows, the smallest that holds a tile's share.
+struct alignas(64) GroupedMaps {
+  CUtensorMap a[3];
+  CUtensorMap b, c, u;
+};
+
 struct GroupedParams {
   const void* offsets;  // int32 or int64 [E + 1]; null: one group of all T rows
   int off64;
@@ -68,6 +75,7 @@ struct GroupedParams {
   int kb_total;      // ceil(K / 64)
   int tiles_n;       // ceil(N / (128 * CG))
   int b_kmaj;        // B[e] stored N x K
+  int b_wide;        // stored K x N with N a multiple of 64: both 64-column atoms in one box
   int bf16;
   int act;
   const unsigned short* bias;  // [E, N] or null
@@ -85,6 +93,7 @@ struct GroupedParams {
   int adapter64;
   const int* lists;  // [row tiles, kAdapterListPitch]
   int up_kmaj;       // up[a] stored N x R
+  int up_wide;
   const unsigned short* up;
   long long ld_up, stride_up;
 };
@@ -95,7 +104,7 @@ template <int CG, int TM, int STAGES, bool LORA>
 struct GroupedPlan {
   static constexpr int kStep = 16 * CG;                  // granularity of a tile's rows (MMA N)
   static constexpr int kTokRows = TM / CG;               // rows of A held by this CTA
-  static constexpr int kBoxRows = TM >= 256 ? 32 : 16;   // rows per TMA box of A
+  static constexpr int kBoxRows = TM >= 256 ? 128 : 16;  // rows per TMA box of A
   static constexpr int kWBytes = kGrpCols * kBK * 2;     // 16 KiB of B
   static constexpr int kTBytes = kTokRows * kBK * 2;
   static constexpr int kStageBytes = kWBytes + kTBytes;
@@ -330,11 +339,36 @@ __device__ __noinline__ float nonfinite_terms(const GroupedParams& p, int t, int
   return sum;
 }
 
+// One K block (64) of 128 columns of a stacked weight.  The number of TMA
+// instructions is what counts here: with six per K block (four boxes of 32
+// rows of A, two atoms of B) the issuing thread took 830 cycles per block of
+// a 256 x 256 pair tile whose MMAs take 512; with two it keeps up
+// (8192 x 4096 x 4096 in one group: 244 -> 193 us, B stored N x K).  So the
+// two 64-column atoms of a row-major weight come in one box of a map that
+// sees the columns as (64, N / 64), where N allows it.
+template <bool PAIR>
+__device__ __forceinline__ void load_weights(uint8_t* dst, const CUtensorMap* m, uint64_t* bar, uint32_t bar_cluster,
+                                             bool kmaj, bool wide, int k0, int col, int e) {
+  auto box = [&](uint8_t* to, int x, int y, int z) {
+    if constexpr (PAIR) {
+      tma_load_4d_pair(to, m, bar_cluster, x, y, z, e);
+    } else {
+      tma_load_4d(to, m, bar, x, y, z, e);
+    }
+  };
+  if (kmaj) {
+    box(dst, k0, col, 0);
+  } else if (wide) {
+    box(dst, 0, k0, col >> 6);
+  } else {
+    box(dst, col, k0, 0);
+    box(dst + kBK * 128, col + 64, k0, 0);
+  }
+}
+
 template <int CG, int TM, int STAGES, bool LORA>
 __global__ void __launch_bounds__(kNumThreads, 1)
-    gemm_grouped_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                       const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmU,
-                       const __grid_constant__ GroupedParams p) {
+    gemm_grouped_sm100(const __grid_constant__ GroupedMaps maps, const __grid_constant__ GroupedParams p) {
   using Plan = GroupedPlan<CG, TM, STAGES, LORA>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -383,10 +417,10 @@ __global__ void __launch_bounds__(kNumThreads, 1)
     fence_mbar_init();
   }
   if (warp == 0 && lane == 0) {
-    prefetch_tmap(&tmA);
-    prefetch_tmap(&tmB);
-    if (LORA) prefetch_tmap(&tmU);
-    if (p.c_tma) prefetch_tmap(&tmC);
+    for (int i = 0; i < 3; ++i) prefetch_tmap(&maps.a[i]);
+    prefetch_tmap(&maps.b);
+    if (LORA) prefetch_tmap(&maps.u);
+    if (p.c_tma) prefetch_tmap(&maps.c);
   }
   if (warp == 1) {
     __syncwarp();
@@ -425,8 +459,10 @@ __global__ void __launch_bounds__(kNumThreads, 1)
         const int half = u.nmma / CG;
         const int arow = u.row0 + static_cast<int>(rank) * half;
         const int bcol = (u.tn * CG + static_cast<int>(rank)) * kGrpCols;
-        const int boxes = (half + Plan::kBoxRows - 1) / Plan::kBoxRows;
-        const uint32_t bytes = Plan::kWBytes + boxes * Plan::kBoxRows * 128;
+        // the smallest box that holds this CTA's rows
+        const int box = half > Plan::kTokRows / 2 ? 0 : (half > Plan::kTokRows / 4 ? 1 : 2);
+        const CUtensorMap* map_a = &maps.a[box];
+        const uint32_t bytes = Plan::kWBytes + static_cast<uint32_t>(Plan::kTokRows >> box) * 128u;
         for (int kb = 0; kb < p.kb_total; ++kb) {
           if (issued >= STAGES && !mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) {
             ok = false;
@@ -434,32 +470,18 @@ __global__ void __launch_bounds__(kNumThreads, 1)
           }
           uint8_t* w_dst = sW + stage * Plan::kWBytes;
           uint8_t* t_dst = sT + stage * Plan::kTBytes;
+          uint64_t* bar = &full_bar[stage];
           const int k0 = kb * kBK;
           if constexpr (CG == 1) {
-            uint64_t* bar = &full_bar[stage];
             mbar_arrive_expect_tx(bar, bytes);
-            if (p.b_kmaj) {
-              tma_load_3d(w_dst, &tmB, bar, k0, bcol, u.e);
-            } else {
-              tma_load_3d(w_dst, &tmB, bar, bcol, k0, u.e);
-              tma_load_3d(w_dst + kBK * 128, &tmB, bar, bcol + 64, k0, u.e);
-            }
-            for (int b = 0; b < boxes; ++b) {
-              tma_load_2d(t_dst + b * Plan::kBoxRows * 128, &tmA, bar, k0, arow + b * Plan::kBoxRows);
-            }
+            load_weights<false>(w_dst, &maps.b, bar, 0, p.b_kmaj != 0, p.b_wide != 0, k0, bcol, u.e);
+            tma_load_2d(t_dst, map_a, bar, k0, arow);
           } else {
             // both CTAs' bytes complete on the even CTA's barrier
-            if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * bytes);
-            const uint32_t bar = mapa_shared(smem_u32(&full_bar[stage]), 0);
-            if (p.b_kmaj) {
-              tma_load_3d_pair(w_dst, &tmB, bar, k0, bcol, u.e);
-            } else {
-              tma_load_3d_pair(w_dst, &tmB, bar, bcol, k0, u.e);
-              tma_load_3d_pair(w_dst + kBK * 128, &tmB, bar, bcol + 64, k0, u.e);
-            }
-            for (int b = 0; b < boxes; ++b) {
-              tma_load_2d_pair(t_dst + b * Plan::kBoxRows * 128, &tmA, bar, k0, arow + b * Plan::kBoxRows);
-            }
+            if (leader) mbar_arrive_expect_tx(bar, 2 * bytes);
+            const uint32_t even = mapa_shared(smem_u32(bar), 0);
+            load_weights<true>(w_dst, &maps.b, bar, even, p.b_kmaj != 0, p.b_wide != 0, k0, bcol, u.e);
+            tma_load_2d_pair(t_dst, map_a, even, k0, arow);
           }
           full_par ^= 1u << stage;
           on_land &= ~(1u << stage);
@@ -483,12 +505,7 @@ __global__ void __launch_bounds__(kNumThreads, 1)
             // on a barrier of this CTA: its epilogue warps look the weights over
             uint64_t* bar = &land_bar[stage];
             mbar_arrive_expect_tx(bar, Plan::kWBytes);
-            if (p.up_kmaj) {
-              tma_load_3d(w_dst, &tmU, bar, r0, bcol, a);
-            } else {
-              tma_load_3d(w_dst, &tmU, bar, bcol, r0, a);
-              tma_load_3d(w_dst + kBK * 128, &tmU, bar, bcol + 64, r0, a);
-            }
+            load_weights<false>(w_dst, &maps.u, bar, 0, p.up_kmaj != 0, p.up_wide != 0, r0, bcol, a);
             land_par ^= 1u << stage;
             on_land |= 1u << stage;
             ++issued;
@@ -721,7 +738,7 @@ __global__ void __launch_bounds__(kNumThreads, 1)
         if (whole) fence_proxy_async_smem();
         named_bar_sync(1, 32 * kEpiWarps);
         if (et == 0 && p.c_tma) {
-          if (whole) tma_store_2d(&tmC, buf, n0, u.row0 + r0);
+          if (whole) tma_store_2d(&maps.c, buf, n0, u.row0 + r0);
           bulk_commit_group();   // empty when the chunk is stored below: the count above stays per buffer
         }
         if (!whole) {
@@ -807,6 +824,7 @@ struct WgradParams {
   unsigned short* D;       // [E, M, N], pitch ldd, stride_d from one matrix to the next
   long long ldd, stride_d;
   int d_tma;               // D is TMA-addressable
+  int a_wide, g_wide;      // columns a multiple of 64: both atoms in one box
   int* err;
 };
 
@@ -852,6 +870,25 @@ __device__ __forceinline__ WgradUnit wgrad_unit(const WgradParams& p, const int*
   u.blocks = (u.rows + kBK - 1) / kBK;
   u.tail = u.rows % kBK;
   return u;
+}
+
+// 64 rows x 128 columns of an operand (see load_weights on the box count).
+template <bool PAIR>
+__device__ __forceinline__ void load_columns(uint8_t* dst, const CUtensorMap* m, uint64_t* bar, uint32_t bar_cluster,
+                                             bool wide, int col, int row) {
+  auto box = [&](uint8_t* to, int x, int z) {
+    if constexpr (PAIR) {
+      tma_load_3d_pair(to, m, bar_cluster, x, row, z);
+    } else {
+      tma_load_3d(to, m, bar, x, row, z);
+    }
+  };
+  if (wide) {
+    box(dst, 0, col >> 6);
+  } else {
+    box(dst, col, 0);
+    box(dst + kBK * 128, col + 64, 0);
+  }
 }
 
 template <int STAGES>
@@ -946,21 +983,15 @@ __global__ void __launch_bounds__(kWgradThreads, 1)
           if (b == u.blocks - 1 && u.tail) {
             uint64_t* bar = &land_bar[stage];
             mbar_arrive_expect_tx(bar, Plan::kStageBytes);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              tma_load_2d(a_dst + j * (kBK * 128), &tmA, bar, acol + j * 64, row);
-              tma_load_2d(g_dst + j * (kBK * 128), &tmG, bar, gcol + j * 64, row);
-            }
+            load_columns<false>(a_dst, &tmA, bar, 0, p.a_wide != 0, acol, row);
+            load_columns<false>(g_dst, &tmG, bar, 0, p.g_wide != 0, gcol, row);
             was_cut |= bit;
             land_par ^= bit;
           } else {
             if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * Plan::kStageBytes);
             const uint32_t bar = mapa_shared(smem_u32(&full_bar[stage]), 0);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              tma_load_2d_pair(a_dst + j * (kBK * 128), &tmA, bar, acol + j * 64, row);
-              tma_load_2d_pair(g_dst + j * (kBK * 128), &tmG, bar, gcol + j * 64, row);
-            }
+            load_columns<true>(a_dst, &tmA, nullptr, bar, p.a_wide != 0, acol, row);
+            load_columns<true>(g_dst, &tmG, nullptr, bar, p.g_wide != 0, gcol, row);
             was_cut &= ~bit;
             full_par ^= bit;
           }
