@@ -130,9 +130,9 @@ cudaError_t opt_in(Kernel kernel, int bytes, std::atomic<unsigned long long>& co
   return e;
 }
 
-template <int CG, class Kernel, class... Args>
+template <class Kernel, class... Args>
 cudaError_t launch(Kernel kernel, int threads, int bytes, std::atomic<unsigned long long>& configured, int grid,
-                   cudaStream_t stream, const Args&... args) {
+                   int cluster, cudaStream_t stream, const Args&... args) {
   cudaError_t e = opt_in(kernel, bytes, configured);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
@@ -144,11 +144,11 @@ cudaError_t launch(Kernel kernel, int threads, int bytes, std::atomic<unsigned l
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = CG == 2 ? 2 : 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
@@ -159,13 +159,15 @@ int launch_grouped(const Operand& a, const Operand& b, const Operand* up, const 
   using Plan = GroupedPlan<CG, TM, STAGES, LORA>;
   GroupedParams p = gp;
   p.tiles_n = static_cast<int>((static_cast<int64_t>(p.N) + kGrpCols * CG - 1) / (kGrpCols * CG));
-  const int64_t row_tiles = static_cast<int64_t>(p.T) / TM + p.E;   // at most one cut tile per group
-  if (row_tiles * p.tiles_n > kInt32Max) return capi_fail(GEMM_ERR_UNSUPPORTED, "too many output tiles");
+  // at most one cut tile per group, and no tile without a row
+  const int64_t row_tiles = std::min<int64_t>(p.T, static_cast<int64_t>(p.T) / TM + p.E);
+  const int64_t tiles = row_tiles * p.tiles_n;
+  if (tiles > kInt32Max) return capi_fail(GEMM_ERR_UNSUPPORTED, "too many output tiles");
   GroupedMaps maps;
   std::memset(&maps, 0, sizeof(maps));
   int st = GEMM_OK;
   if (p.K > 0) {
-    for (int i = 0; i < 3 && st == GEMM_OK; ++i) st = a.encode_rows(&maps.a[i], Plan::kTokRows >> i, "A");
+    for (int i = 0; i < box_count(TM) && st == GEMM_OK; ++i) st = a.encode_rows(&maps.a[i], box_rows(TM, i), "A");
     if (st == GEMM_OK) st = b.encode_weights(&maps.b, p.b_kmaj != 0, "B");
     p.b_wide = b.wide();
   }
@@ -179,13 +181,18 @@ int launch_grouped(const Operand& a, const Operand& b, const Operand* up, const 
     st = capi_encode(&maps.c, p.C, 2, ext, str, box, false, "C");
   }
   if (st != GEMM_OK) return st;
-  // persistent: one CTA (pair) per SM (pair), fewer when the most tiles that
-  // these sizes can give are fewer
-  const int64_t most = std::min<int64_t>(row_tiles * p.tiles_n, sms / CG);
-  const int grid = static_cast<int>(most < 1 ? 1 : most) * CG;
+  // Single CTAs: with fewer tiles than SMs a cluster splits each tile's K, at
+  // least 4 K blocks to a CTA; the counts are upper bounds (only the device
+  // knows the groups).
+  int cluster = CG;
+  if (CG == 1) {
+    while (cluster < 8 && 2 * cluster * tiles <= sms && p.kb_total >= 8 * cluster) cluster *= 2;
+  }
+  // persistent: one cluster per `cluster` SMs, fewer when there are fewer tiles
+  const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(tiles, sms / cluster))) * cluster;
   static std::atomic<unsigned long long> configured{0};
-  cudaError_t e = launch<CG>(gemm_grouped_sm100<CG, TM, STAGES, LORA>, kNumThreads, Plan::kDynamicBytes, configured,
-                             grid, stream, maps, p);
+  cudaError_t e = launch(gemm_grouped_sm100<CG, TM, STAGES, LORA>, kGrpThreads, Plan::kDynamicBytes, configured, grid,
+                         cluster, stream, maps, p);
   return e == cudaSuccess ? GEMM_OK : capi_fail_cuda(e, "grouped gemm kernel launch");
 }
 
@@ -211,10 +218,12 @@ int launch_shrink(const ShrinkParams& sp, bool kmaj, bool bf16, cudaStream_t str
   int rows = 1;
   while (rows < kShrinkMaxRows && rows * 32 < p.T) rows *= 2;
   p.tile_rows = rows;
-  // CTAs along K: no more than give every warp a slice.
+  // CTAs along K: up to about 300 CTAs in all, and no more than give every
+  // warp a slice.
   const int slices = (p.K + kShrinkSlice - 1) / kShrinkSlice;
+  const int tiles = (p.T + rows - 1) / rows;
   int cluster = 1;
-  while (cluster < 8 && cluster * kShrinkWarps < slices) cluster *= 2;
+  while (cluster < 8 && cluster * kShrinkWarps < slices && cluster * tiles <= 150) cluster *= 2;
   const bool wide = rows > 8;
   ShrinkFn fn = rt == 1 ? (wide ? shrink_fn<1, 4>(kmaj, bf16) : shrink_fn<1, 1>(kmaj, bf16))
                 : rt == 2 ? (wide ? shrink_fn<2, 4>(kmaj, bf16) : shrink_fn<2, 1>(kmaj, bf16))
@@ -261,7 +270,7 @@ struct LoraPlan {
       row_tiles_host<256, 32>(T);
     }
     size_t off = align256(gemm_workspace_counter_bytes());
-    off_h = off;
+      off_h = off;
     off = align256(off + static_cast<size_t>(T) * shrink_pitch(R) * sizeof(float));
     off_lists = off;
     off = align256(off + static_cast<size_t>(list_tiles) * kAdapterListPitch * sizeof(int));
@@ -280,7 +289,7 @@ struct LoraPlan {
   }
 };
 
-constexpr int kWgradStages = 6;
+constexpr int kWgradStages = 5;
 
 int launch_wgrad(const Operand& a, const Operand& g, const WgradParams& wp, int sms, cudaStream_t stream) {
   using Plan = WgradPlan<kWgradStages>;
@@ -301,10 +310,15 @@ int launch_wgrad(const Operand& a, const Operand& g, const WgradParams& wp, int 
   const int64_t tiles = static_cast<int64_t>(p.E) * p.tiles_m * p.tiles_n;
   const int grid = static_cast<int>(std::min<int64_t>(tiles, sms / 2)) * 2;
   static std::atomic<unsigned long long> configured{0};
-  cudaError_t e = launch<2>(gemm_grouped_wgrad_sm100<kWgradStages>, kWgradThreads, Plan::kDynamicBytes, configured,
-                            grid, stream, tmA, tmG, tmD, p);
+  cudaError_t e = launch(gemm_grouped_wgrad_sm100<kWgradStages>, kWgradThreads, Plan::kDynamicBytes, configured, grid,
+                         2, stream, tmA, tmG, tmD, p);
   return e == cudaSuccess ? GEMM_OK : capi_fail_cuda(e, "grouped weight gradient kernel launch");
 }
+
+// Few rows per group: the cost is reading the weights, and single CTAs with a
+// deep ring read them best.  More rows: CTA pairs with tiles of up to 256
+// rows, which read every weight once per 256 rows.
+bool small_tiles(int64_t T, int64_t N, int64_t E) { return T <= 64 * E || N <= kGrpCols; }
 
 Operand operand_b(const void* B, int64_t E, int64_t N, int64_t K, int64_t ldb, int64_t stride_b, int trans_b) {
   return Operand(B, E, trans_b ? N : K, trans_b ? K : N, ldb, stride_b);
@@ -389,10 +403,7 @@ int gemm_grouped_launch(const void* A, const void* B, void* C, const void* offse
   p.ldc = ldc;
   p.c_tma = p.c_vec = reinterpret_cast<uintptr_t>(C) % 16u == 0 && ldc % 8 == 0;
   p.zero_rest = zero_rest != 0;
-  // Few rows per group: the cost is reading the weights, and single CTAs with
-  // a deep ring read them best.  More rows: CTA pairs with tiles of up to 256
-  // rows, which read every weight once per 256 rows.
-  if (T <= 64 * E || N <= kGrpCols) return launch_grouped<1, 64, 8, false>(a, b, nullptr, p, sms, stream);
+  if (small_tiles(T, N, E)) return launch_grouped<1, 64, 7, false>(a, b, nullptr, p, sms, stream);
   return launch_grouped<2, 256, 6, false>(a, b, nullptr, p, sms, stream);
 }
 
@@ -579,7 +590,7 @@ int gemm_lora_launch(const void* X, const void* W, const void* down, const void*
   p.up = static_cast<const unsigned short*>(pl.up.p);
   p.ld_up = pl.up.ld;
   p.stride_up = L == 1 ? 0 : pl.up.stride;
-  if (T <= kLoraSmallRows) return launch_grouped<1, 64, 7, true>(pl.x, pl.w, &pl.up, p, sms, stream);
+  if (T <= kLoraSmallRows) return launch_grouped<1, 64, 6, true>(pl.x, pl.w, &pl.up, p, sms, stream);
   return launch_grouped<2, 256, 5, true>(pl.x, pl.w, &pl.up, p, sms, stream);
 }
 

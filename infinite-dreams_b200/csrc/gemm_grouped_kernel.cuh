@@ -17,9 +17,15 @@
 //
 //   CG = 2, TM = 256: a CTA pair owns 256 columns x up to 256 rows; each CTA
 //     loads its 128 columns of B and half of the rows (no multicast).
-//   CG = 1, TM = 64: one CTA owns 128 columns x up to 64 rows; the ring holds
-//     128 KiB of weights in flight, for groups of few rows, whose cost is
-//     reading the weights.
+//   CG = 1, TM = 64: a cluster of 1, 2, 4 or 8 CTAs owns 128 columns x up to 64
+//     rows, each CTA a share of K; the ring holds over 100 KiB of weights in
+//     flight.  For groups of few rows, whose cost is reading the weights
+//     (steady state 7.3 TB/s on weights stored K x N, 6.4 stored N x K), and
+//     for problems too small to fill the machine with pair tiles.  The
+//     partial sums cross through distributed shared memory: CTA r finishes
+//     every cluster's r-th part of the rows, summing in CTA order.  (Pieces
+//     through global memory with a ticket were measured first: joining two
+//     of them cost 3 us, four times the DSMEM path.)
 //
 // Roles as in gemm_sm100_kernel.cuh: warp 0 TMA producer, warp 1 TMEM owner
 // and MMA issuer, warps 2..5 epilogue.  The accumulator holds C transposed:
@@ -60,10 +66,20 @@ constexpr int kMaxGroups = 1024;   // bounded by the offset tables in shared mem
 constexpr int kGrpChunk = 32;      // rows of C per epilogue step
 constexpr int kGrpRaster = 8;      // row tiles walked before the next column tile
 
-// A's rows come in one box per K block, of TM / CG, half or a quarter as many
-// rows, the smallest that holds a tile's share.
+// A's rows come in one box per K block, the smallest that holds a CTA's share
+// of the tile's rows.  A full pair tile draws 64 bytes per clock and SM from
+// L2, which is what the SM's port gives (measured: 60 without the MMAs), so
+// rows that are not needed cost time.
+constexpr int kBoxes = 6;
+__host__ __device__ constexpr int box_rows(int tm, int i) {
+  constexpr int pair[kBoxes] = {128, 112, 96, 80, 64, 32};
+  constexpr int single[kBoxes] = {64, 48, 32, 16, 16, 16};
+  return tm >= 256 ? pair[i] : single[i];
+}
+__host__ __device__ constexpr int box_count(int tm) { return tm >= 256 ? 6 : 4; }
+
 struct alignas(64) GroupedMaps {
-  CUtensorMap a[3];
+  CUtensorMap a[kBoxes];
   CUtensorMap b, c, u;
 };
 
@@ -100,6 +116,11 @@ struct GroupedParams {
 
 constexpr int kLoraRanks = 32;   // ranks per adapter block
 
+// Two groups of four epilogue warps (one warp per TMEM lane quarter each): they
+// take alternate 32-row chunks, and with adapters one builds hi and one lo.
+constexpr int kGrpEpiWarps = 8;
+constexpr int kGrpThreads = 64 + 32 * kGrpEpiWarps;
+
 template <int CG, int TM, int STAGES, bool LORA>
 struct GroupedPlan {
   static constexpr int kStep = 16 * CG;                  // granularity of a tile's rows (MMA N)
@@ -113,12 +134,13 @@ struct GroupedPlan {
   static constexpr int kOffT = kOffW + STAGES * kWBytes;
   static constexpr int kOffOut = kOffT + STAGES * kTBytes;
   static constexpr int kOffH = kOffOut + 2 * kOutBytes;  // two buffers of adapter rows (hi | lo)
-  static constexpr int kOffBar = kOffH + (LORA ? 2 * kTBytes : 0);
-  // full, empty, land, tmem_full[2], tmem_empty[2], h_full[2], h_empty[2], done
-  static constexpr int kNumBars = 3 * STAGES + 8 + 1;
+  static constexpr int kOffRx = kOffH + (LORA ? 2 * kTBytes : 0);   // fp32 sums from the cluster
+  static constexpr int kOffBar = kOffRx + (CG == 1 ? TM * kGrpCols * 4 : 0);
+  // full, empty, land, tmem_full[2], tmem_empty[2], h_full[2], h_empty[2], rx_full, rx_empty, done
+  static constexpr int kNumBars = 3 * STAGES + 10 + 1;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;
-  static constexpr int kOffScan = kOffMisc + 16;         // 8 warp totals
-  static constexpr int kOffRows = kOffScan + 32;         // group starts [E + 1]
+  static constexpr int kOffScan = kOffMisc + 32;         // warp totals
+  static constexpr int kOffRows = kOffScan + 64;         // group starts [E + 1]
   static constexpr int kOffTiles = kOffRows + (kMaxGroups + 1) * 4;  // first tile of each group [E + 1]
   static constexpr int kUsed = kOffTiles + (kMaxGroups + 1) * 4;
   static constexpr int kDynamicBytes = kUsed + 1024;
@@ -141,7 +163,51 @@ __device__ __forceinline__ int group_offset(const void* offsets, int off64, int 
 template <int TM, int STEP>
 __device__ __forceinline__ void row_tiles(int n, int& count, int& rows) {
   count = (n + TM - 1) / TM;
-  rows = count ? ((n + count - 1) / count + STEP - 1) / STEP * STEP : STEP;
+  rows = (count > 1 ? (n + count - 1) / count + STEP - 1 : n + STEP - 1) / STEP * STEP;
+}
+
+// Few groups: every warp makes the same tables for itself (all write the same
+// values), so no warp waits for another.  False if the offsets are bad.
+constexpr int kWarpScanGroups = 256;
+template <class Units>
+__device__ __forceinline__ bool scan_groups_warp(const void* offsets, int off64, int E, int T, int* rows, int* first,
+                                                 Units units) {
+  const int lane = static_cast<int>(threadIdx.x & 31);
+  int v[kWarpScanGroups / 32 + 1];
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j <= kWarpScanGroups / 32; ++j) {   // all loads in flight at once
+    if (j * 32 <= E) v[j] = group_offset(offsets, off64, min(j * 32 + lane, E), T, bad);
+  }
+  int base = 0;
+#pragma unroll
+  for (int j = 0; j < kWarpScanGroups / 32; ++j) {
+    if (j * 32 < E) {
+      const int g = j * 32 + lane;
+      // the next offset: the next lane's, or the first of the next 32
+      int next = __shfl_down_sync(0xffffffffu, v[j], 1);
+      const int wrap = __shfl_sync(0xffffffffu, (j + 1) * 32 <= E ? v[j + 1] : v[j], 0);
+      if (lane == 31) next = wrap;
+      const int n = g < E ? next - v[j] : 0;
+      bad |= n < 0;
+      const int mine = g < E ? units(n) : 0;
+      int run = mine;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, run, d);
+        if (lane >= d) run += up;
+      }
+      if (g < E) {
+        rows[g] = v[j];
+        first[g] = base + run - mine;
+        if (g == E - 1) rows[E] = next;
+      }
+      base += __shfl_sync(0xffffffffu, run, 31);
+    }
+  }
+  if (lane == 0) first[E] = base;
+  __syncwarp();
+  return __all_sync(0xffffffffu, !bad) != 0;
 }
 
 // Fills rows[0..E] with the group starts and first[0..E] with an exclusive
@@ -153,48 +219,54 @@ template <int NT, class Units>
 __device__ __forceinline__ void scan_groups(const void* offsets, int off64, int E, int T, int* rows, int* first,
                                             int* scratch, int* err, Units units) {
   const int tid = static_cast<int>(threadIdx.x);
-  bool bad = false;
-  if (offsets == nullptr) {
+  if (offsets == nullptr) {   // one group
     if (tid == 0) {
       rows[0] = 0;
       rows[1] = T;
+      first[0] = 0;
+      first[1] = units(T);
     }
-  } else {
-    for (int i = tid; i <= E; i += NT) rows[i] = group_offset(offsets, off64, i, T, bad);
+    __syncthreads();
+    return;
   }
+  bool bad = false;
+  for (int i = tid; i <= E; i += NT) rows[i] = group_offset(offsets, off64, i, T, bad);
   __syncthreads();
-  for (int i = tid; i < E; i += NT) bad |= rows[i + 1] < rows[i];
+  // each thread owns a run of consecutive groups
+  const int per = (E + NT - 1) / NT;
+  const int g0 = min(E, tid * per), g1 = min(E, g0 + per);
+  int sum = 0, run = 0;
+  auto scan = [&] {
+    sum = 0;
+    for (int g = g0; g < g1; ++g) {
+      bad |= rows[g + 1] < rows[g];
+      sum += units(rows[g + 1] - rows[g]);
+    }
+    run = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, run, d);
+      if ((tid & 31) >= d) run += up;
+    }
+    if ((tid & 31) == 31) scratch[tid >> 5] = run;
+  };
+  scan();
   if (__syncthreads_or(bad ? 1 : 0)) {
     if (tid == 0) {
       for (int i = 0; i < E; ++i) rows[i + 1] = max(rows[i + 1], rows[i]);
       atomicOr(err, kDevErrBadOffsets);
     }
     __syncthreads();
+    scan();
+    __syncthreads();
   }
-  // each thread owns a run of consecutive groups
-  const int per = (E + NT - 1) / NT;
-  const int g0 = min(E, tid * per), g1 = min(E, g0 + per);
-  int sum = 0;
-  for (int g = g0; g < g1; ++g) sum += units(rows[g + 1] - rows[g]);
-  int run = sum;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int up = __shfl_up_sync(0xffffffffu, run, d);
-    if ((tid & 31) >= d) run += up;
-  }
-  if ((tid & 31) == 31) scratch[tid >> 5] = run;
-  __syncthreads();
   int base = run - sum;
   for (int w = 0; w < (tid >> 5); ++w) base += scratch[w];
   for (int g = g0; g < g1; ++g) {
     first[g] = base;
     base += units(rows[g + 1] - rows[g]);
   }
-  if (tid == 0) {
-    int total = 0;
-    for (int w = 0; w < NT / 32; ++w) total += scratch[w];
-    first[E] = total;
-  }
+  if (tid == NT - 1) first[E] = base;   // the last thread's base ends at the total
   __syncthreads();
 }
 
@@ -225,12 +297,17 @@ __device__ __forceinline__ GroupedUnit grouped_unit(const GroupedParams& p, cons
   int count, tr;
   row_tiles<TM, 16 * CG>(rows[u.e + 1] - rows[u.e], count, tr);
   const int local = t - first[u.e];
-  const int per = kGrpRaster * p.tiles_n;
-  const int g = local / per;
-  const int gs = min(count - g * kGrpRaster, kGrpRaster);
-  const int r = local - g * per;
-  u.tn = r / gs;
-  u.rt = g * kGrpRaster + r % gs;
+  if (count == 1) {   // no divisions on the way to the first load
+    u.tn = local;
+    u.rt = 0;
+  } else {
+    const int per = kGrpRaster * p.tiles_n;
+    const int g = local / per;
+    const int gs = min(count - g * kGrpRaster, kGrpRaster);
+    const int r = local - g * per;
+    u.tn = r / gs;
+    u.rt = g * kGrpRaster + r % gs;
+  }
   u.row0 = rows[u.e] + u.rt * tr;
   u.rows = min(tr, rows[u.e + 1] - u.row0);
   u.nmma = (u.rows + 16 * CG - 1) / (16 * CG) * (16 * CG);
@@ -255,10 +332,10 @@ __device__ __forceinline__ void zero_rows(const GroupedParams& p, int lo, int hi
   }
 }
 
-// The 32 ranks of one row's block as a row of the swizzled adapter buffer:
-// hi in the first four 16-byte chunks, lo in the last four.
-__device__ __forceinline__ void split_ranks(const float* h, int valid, bool bf16, uint4 (&out)[8]) {
-  uint32_t w[32];
+// The 32 ranks of one row's block as half a row of the swizzled adapter
+// buffer: hi (the first four 16-byte chunks) or lo (the last four).
+__device__ __forceinline__ void split_ranks(const float* h, int valid, bool want_lo, bool bf16, uint4 (&out)[4]) {
+  uint32_t w[16];
 #pragma unroll
   for (int i = 0; i < kLoraRanks; i += 4) {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -266,21 +343,22 @@ __device__ __forceinline__ void split_ranks(const float* h, int valid, bool bf16
     const float f[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int e = 0; e < 4; e += 2) {
-      uint32_t hi = 0, lo = 0;
+      uint32_t word = 0;
 #pragma unroll
       for (int o = 0; o < 2; ++o) {
-        const unsigned short top = to_16bit(f[e + o], bf16);
-        hi |= static_cast<uint32_t>(top) << (16 * o);
-        // an h beyond the type's range is infinite in hi; lo must not undo that
-        const float rest = f[e + o] - from_16bit(top, bf16);
-        lo |= static_cast<uint32_t>(to_16bit(isfinite(rest) ? rest : 0.0f, bf16)) << (16 * o);
+        unsigned short bits = to_16bit(f[e + o], bf16);
+        if (want_lo) {
+          // an h beyond the type's range is infinite in hi; lo must not undo that
+          const float rest = f[e + o] - from_16bit(bits, bf16);
+          bits = to_16bit(isfinite(rest) ? rest : 0.0f, bf16);
+        }
+        word |= static_cast<uint32_t>(bits) << (16 * o);
       }
-      w[(i + e) / 2] = hi;
-      w[16 + (i + e) / 2] = lo;
+      w[(i + e) / 2] = word;
     }
   }
 #pragma unroll
-  for (int c = 0; c < 8; ++c) out[c] = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+  for (int c = 0; c < 4; ++c) out[c] = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
 }
 
 __device__ __forceinline__ bool nonfinite16(uint32_t h, bool bf16) {
@@ -288,13 +366,14 @@ __device__ __forceinline__ bool nonfinite16(uint32_t h, bool bf16) {
   return (h & exponent) == exponent;
 }
 
-// Replaces the inf and NaN among the first 32 ranks of column `col` of a
-// landed `up` tile by zeros; says whether there were any.
-__device__ __forceinline__ bool clear_nonfinite(uint8_t* tile, int col, bool kmaj, bool bf16) {
+// Replaces the inf and NaN among ranks [16 half, 16 half + 16) of column `col`
+// of a landed `up` tile by zeros; says whether there were any.
+__device__ __forceinline__ bool clear_nonfinite(uint8_t* tile, int col, int half, bool kmaj, bool bf16) {
   bool any = false;
   if (kmaj) {   // row `col`, ranks in 16-byte chunks swizzled by the row
 #pragma unroll
-    for (int c = 0; c < kLoraRanks / 8; ++c) {
+    for (int i2 = 0; i2 < 2; ++i2) {
+      const int c = 2 * half + i2;
       uint32_t* at = reinterpret_cast<uint32_t*>(tile + col * 128 + ((c ^ (col & 7)) << 4));
       const uint4 v = *reinterpret_cast<const uint4*>(at);
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -310,8 +389,9 @@ __device__ __forceinline__ bool clear_nonfinite(uint8_t* tile, int col, bool kma
   } else {      // atom col / 64, one rank per row
     uint8_t* atom = tile + (col >> 6) * (kBK * 128);
     const int c = col & 63;
-#pragma unroll 8
-    for (int r = 0; r < kLoraRanks; ++r) {
+#pragma unroll
+    for (int i = 0; i < kLoraRanks / 2; ++i) {
+      const int r = half * (kLoraRanks / 2) + i;
       unsigned short* at = reinterpret_cast<unsigned short*>(atom + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
       if (nonfinite16(*at, bf16)) {
         *at = 0;
@@ -322,21 +402,81 @@ __device__ __forceinline__ bool clear_nonfinite(uint8_t* tile, int col, bool kma
   return any;
 }
 
-// What clear_nonfinite took out of row t's value in column n.
-__device__ __noinline__ float nonfinite_terms(const GroupedParams& p, int t, int n) {
+// What clear_nonfinite took out of row t's value in column n in the adapter
+// blocks [b0, b1) of its tile.
+__device__ __noinline__ float nonfinite_terms(const GroupedParams& p, const int* list, int b0, int b1, int t, int n) {
   bool bad = false;
   const int a = adapter_of(p.adapter, p.adapter64, t, p.L, bad);
+  const int adapters = list[0];
+  int ai = 0;
+  while (ai < adapters && list[1 + ai] != a) ++ai;
   float sum = 0.0f;
-  if (a >= 0) {
-    for (int r = 0; r < p.R; ++r) {
-      const unsigned short w =
-          p.up[a * p.stride_up + (p.up_kmaj ? n * p.ld_up + r : r * p.ld_up + n)];
-      if (nonfinite16(w, p.bf16 != 0)) {
-        sum += p.h[static_cast<long long>(t) * p.h_pitch + r] * from_16bit(w, p.bf16 != 0);
-      }
+  if (a < 0 || ai == adapters) return sum;
+  for (int r = 0; r < p.R; ++r) {
+    const int b = r / kLoraRanks * adapters + ai;
+    if (b < b0 || b >= b1) continue;
+    const unsigned short w = p.up[a * p.stride_up + (p.up_kmaj ? n * p.ld_up + r : r * p.ld_up + n)];
+    if (nonfinite16(w, p.bf16 != 0)) {
+      sum += p.h[static_cast<long long>(t) * p.h_pitch + r] * from_16bit(w, p.bf16 != 0);
     }
   }
   return sum;
+}
+
+// x * Phi(x), Phi the normal distribution, without the branches of erff (whose
+// two paths kept the 32 values of a chunk from overlapping: the epilogue of a
+// 256 x 256 tile took 42000 cycles, more than its mainloop at K = 4096).
+//
+// With a = |x| and q(a) = 1 - Phi(a) = erfc(a / sqrt 2) / 2:
+//   x Phi(x) = max(x, 0) - a q(a)        (both signs of x)
+//   q(a) = exp(-a^2 / 2) t Q(t),  t = 1 / (1 + 0.31 a)
+// where Q is the polynomial of degree 7 with the least relative error to
+// exp(a^2 / 2) q(a) / t over 0 <= a <= 20 (an iteratively reweighted
+// least-squares fit to scipy's erfcx), 1.7e-7.  In fp32 the result errs by at most
+// 4 units of 2^-24 |x| and by 1.5e-6 of its value wherever fp16 is normal.
+// (x + |x|) / 2 rather than max(x, 0), so that a NaN stays one.
+__device__ __forceinline__ float gelu(float x) {
+  const float a = fminf(fabsf(x), 20.0f);
+  float t, e;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.31f, a, 1.0f)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(a * a * -0.72134752f));   // -log2(e) / 2
+  float q = 0.035917483f;
+  q = fmaf(q, t, -0.14193712f);
+  q = fmaf(q, t, 0.15567426f);
+  q = fmaf(q, t, -0.015496778f);
+  q = fmaf(q, t, 0.11044533f);
+  q = fmaf(q, t, 0.10766225f);
+  q = fmaf(q, t, 0.12407906f);
+  q = fmaf(q, t, 0.1236556f);
+  return fmaf(-a, q * t * e, 0.5f * (x + fabsf(x)));
+}
+
+// `count` staged rows (128 columns of 16 bits each) to C at row `row`, column
+// n0, by `threads` threads.
+__device__ __forceinline__ void store_rows(const GroupedParams& p, const uint8_t* buf, int row, int count, int n0,
+                                           int thread, int threads) {
+  unsigned short* crow = p.C + static_cast<long long>(row) * p.ldc + n0;
+  if (p.c_vec) {
+    const int seg = (thread & 15) * 8;
+    const int valid = min(8, p.N - n0 - seg);   // columns of this thread's 16 bytes inside C
+#pragma unroll 1
+    for (int r = thread >> 4; r < count; r += threads >> 4) {
+      const unsigned short* src = reinterpret_cast<const unsigned short*>(buf + r * (kGrpCols * 2)) + seg;
+      unsigned short* out = crow + r * p.ldc + seg;
+      if (valid == 8) {
+        *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(src);
+      } else {
+        for (int c = 0; c < valid; ++c) out[c] = src[c];
+      }
+    }
+  } else {
+    const int c = thread & 127;
+    if (n0 + c >= p.N) return;
+#pragma unroll 1
+    for (int r = thread >> 7; r < count; r += threads >> 7) {
+      crow[r * p.ldc + c] = reinterpret_cast<const unsigned short*>(buf + r * (kGrpCols * 2))[c];
+    }
+  }
 }
 
 // One K block (64) of 128 columns of a stacked weight.  The number of TMA
@@ -367,7 +507,7 @@ __device__ __forceinline__ void load_weights(uint8_t* dst, const CUtensorMap* m,
 }
 
 template <int CG, int TM, int STAGES, bool LORA>
-__global__ void __launch_bounds__(kNumThreads, 1)
+__global__ void __launch_bounds__(kGrpThreads, 1)
     gemm_grouped_sm100(const __grid_constant__ GroupedMaps maps, const __grid_constant__ GroupedParams p) {
   using Plan = GroupedPlan<CG, TM, STAGES, LORA>;
   extern __shared__ uint8_t smem_raw[];
@@ -382,20 +522,29 @@ __global__ void __launch_bounds__(kNumThreads, 1)
   uint64_t* tempty_bar = tfull_bar + 2;
   uint64_t* hfull_bar = tempty_bar + 2;
   uint64_t* hempty_bar = hfull_bar + 2;
-  uint64_t* done_bar = hempty_bar + 2;
+  uint64_t* rxfull_bar = hempty_bar + 2;     // the cluster's sums for this CTA have arrived
+  uint64_t* rxempty_bar = rxfull_bar + 1;    // ... have been read, in every CTA of the cluster
+  uint64_t* done_bar = rxempty_bar + 1;
   uint8_t* sH = smem + Plan::kOffH;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Plan::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* odd_flags = reinterpret_cast<volatile int*>(tmem_slot + 2);   // three tiles in turn
   int* scan = reinterpret_cast<int*>(smem + Plan::kOffScan);
   int* grp_rows = reinterpret_cast<int*>(smem + Plan::kOffRows);
   int* grp_tiles = reinterpret_cast<int*>(smem + Plan::kOffTiles);
 
   const int warp = static_cast<int>(threadIdx.x >> 5);
   const int lane = static_cast<int>(threadIdx.x & 31);
-  const uint32_t rank = (CG == 2) ? cluster_ctarank() : 0u;
+  // CG = 2: position in the CTA pair.  CG = 1: the tile's K blocks are split
+  // over the `parts` CTAs of a cluster.
+  const int csize = static_cast<int>(cluster_nctarank());
+  const int crank = static_cast<int>(cluster_ctarank());
+  const int rank = (CG == 2) ? crank : 0;
+  const int parts = (CG == 1) ? csize : 1;
+  const int part = (CG == 1) ? crank : 0;
   const bool leader = (rank == 0);
-  const int worker = static_cast<int>(blockIdx.x) / CG;
-  const int workers = static_cast<int>(gridDim.x) / CG;
+  const int worker = static_cast<int>(blockIdx.x) / csize;
+  const int workers = static_cast<int>(gridDim.x) / csize;
 
   if (threadIdx.x == 64) {
 #pragma unroll
@@ -406,18 +555,21 @@ __global__ void __launch_bounds__(kNumThreads, 1)
     }
     mbar_init(&tfull_bar[0], 1);
     mbar_init(&tfull_bar[1], 1);
-    mbar_init(&tempty_bar[0], kEpiWarps * CG);
-    mbar_init(&tempty_bar[1], kEpiWarps * CG);
+    mbar_init(&tempty_bar[0], kGrpEpiWarps * CG);
+    mbar_init(&tempty_bar[1], kGrpEpiWarps * CG);
     for (int b = 0; b < 2; ++b) {
-      mbar_init(&hfull_bar[b], kEpiWarps * CG);
+      mbar_init(&hfull_bar[b], kGrpEpiWarps * CG);
       mbar_init(&hempty_bar[b], 1);
     }
+    mbar_init(rxfull_bar, kGrpEpiWarps * parts);
+    mbar_init(rxempty_bar, kGrpEpiWarps * parts);
     mbar_init(done_bar, 1);
     *abort_flag = 0;
+    for (int i = 0; i < 3; ++i) odd_flags[i] = 0;
     fence_mbar_init();
   }
   if (warp == 0 && lane == 0) {
-    for (int i = 0; i < 3; ++i) prefetch_tmap(&maps.a[i]);
+    for (int i = 0; i < box_count(TM); ++i) prefetch_tmap(&maps.a[i]);
     prefetch_tmap(&maps.b);
     if (LORA) prefetch_tmap(&maps.u);
     if (p.c_tma) prefetch_tmap(&maps.c);
@@ -429,7 +581,7 @@ __global__ void __launch_bounds__(kNumThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if constexpr (CG == 2) cluster_sync();
+  if (csize > 1) cluster_sync();   // the peers' barriers are initialised before any remote use
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   // With LORA the previous grid is lora_shrink, which lets this one start
@@ -438,12 +590,13 @@ __global__ void __launch_bounds__(kNumThreads, 1)
   if constexpr (!LORA) griddep_wait();
   const int rank_blocks = LORA ? (p.R + kLoraRanks - 1) / kLoraRanks : 0;
 
-  scan_groups<kNumThreads>(p.offsets, p.off64, p.E, p.T, grp_rows, grp_tiles, scan, p.err, [&](int n) {
-    int count, tr;
-    row_tiles<TM, Plan::kStep>(n, count, tr);
-    return count * p.tiles_n;
-  });
+  auto tiles_of = [&](int n) { return (n + TM - 1) / TM * p.tiles_n; };
+  if (p.offsets == nullptr || p.E > kWarpScanGroups ||
+      !scan_groups_warp(p.offsets, p.off64, p.E, p.T, grp_rows, grp_tiles, tiles_of)) {
+    scan_groups<kGrpThreads>(p.offsets, p.off64, p.E, p.T, grp_rows, grp_tiles, scan, p.err, tiles_of);
+  }
   const int num_tiles = grp_tiles[p.E];
+  const int kb0 = p.kb_total * part / parts, kb1 = p.kb_total * (part + 1) / parts;
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
@@ -453,17 +606,18 @@ __global__ void __launch_bounds__(kNumThreads, 1)
       int issued = 0;
       // per stage: parity of its last fill on full / land, and which came last
       uint32_t full_par = 0, land_par = 0, on_land = 0;
-      bool ok = true;
+      bool ok = true, waited = false;
       for (int t = worker; ok && t < num_tiles; t += workers) {
         const GroupedUnit u = grouped_unit<CG, TM>(p, grp_rows, grp_tiles, t);
         const int half = u.nmma / CG;
-        const int arow = u.row0 + static_cast<int>(rank) * half;
-        const int bcol = (u.tn * CG + static_cast<int>(rank)) * kGrpCols;
+        const int arow = u.row0 + rank * half;
+        const int bcol = (u.tn * CG + rank) * kGrpCols;
         // the smallest box that holds this CTA's rows
-        const int box = half > Plan::kTokRows / 2 ? 0 : (half > Plan::kTokRows / 4 ? 1 : 2);
+        int box = 0;
+        while (box + 1 < box_count(TM) && half <= box_rows(TM, box + 1)) ++box;
         const CUtensorMap* map_a = &maps.a[box];
-        const uint32_t bytes = Plan::kWBytes + static_cast<uint32_t>(Plan::kTokRows >> box) * 128u;
-        for (int kb = 0; kb < p.kb_total; ++kb) {
+        const uint32_t bytes = Plan::kWBytes + static_cast<uint32_t>(box_rows(TM, box)) * 128u;
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (issued >= STAGES && !mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) {
             ok = false;
             break;
@@ -492,10 +646,12 @@ __global__ void __launch_bounds__(kNumThreads, 1)
           }
         }
         if constexpr (LORA) {
-          if (t == worker) griddep_wait();   // the lists are lora_shrink's
+          if (!waited) griddep_wait();   // the lists are lora_shrink's
+          waited = true;
           const int* list = p.lists + static_cast<long long>(u.rt) * kAdapterListPitch;
           const int adapters = ok ? list[0] : 0;
-          for (int b = 0; b < rank_blocks * adapters; ++b) {
+          const int blocks = rank_blocks * adapters;
+          for (int b = blocks * part / parts; b < blocks * (part + 1) / parts; ++b) {
             const int a = list[1 + b % adapters], r0 = b / adapters * kLoraRanks;
             if (issued >= STAGES && !mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) {
               ok = false;
@@ -550,7 +706,7 @@ __global__ void __launch_bounds__(kNumThreads, 1)
       int count = 0;
       int hb = 0;
       uint32_t hphase = 0;
-      bool ok = true;
+      bool ok = true, waited = false;
       for (int t = worker; ok && t < num_tiles; t += workers) {
         if (p.kb_total == 0) break;   // the epilogue writes act(bias) by itself
         const GroupedUnit u = grouped_unit<CG, TM>(p, grp_rows, grp_tiles, t);
@@ -562,7 +718,7 @@ __global__ void __launch_bounds__(kNumThreads, 1)
         ++count;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * TM);
-        for (int kb = 0; kb < p.kb_total; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&full_bar[stage], (full_par >> stage) & 1u, abort_flag)) {
             ok = false;
             break;
@@ -574,17 +730,19 @@ __global__ void __launch_bounds__(kNumThreads, 1)
 #pragma unroll
           for (int j = 0; j < kBK / kUmmaK; ++j) {
             mma_f16_ss<CG>(d_tmem, smem_desc_sw128(w0 + j * w_kstep, w_lbo, 1024),
-                           smem_desc_sw128(t0 + j * (kUmmaK * 2), 16, 1024), idesc, (kb > 0 || j > 0) ? 1u : 0u);
+                           smem_desc_sw128(t0 + j * (kUmmaK * 2), 16, 1024), idesc, (kb > kb0 || j > 0) ? 1u : 0u);
           }
           mma_commit<CG>(&empty_bar[stage]);
           if (++stage == STAGES) stage = 0;
         }
         if constexpr (LORA) {
-          if (t == worker) griddep_wait();
+          if (!waited) griddep_wait();
+          waited = true;
           const uint32_t idesc_up = idesc_16bit(kGrpCols * CG, u.nmma, p.up_kmaj == 0, false, p.bf16 != 0);
           const uint32_t u_lbo = p.up_kmaj ? 16 : kBK * 128, u_kstep = p.up_kmaj ? kUmmaK * 2 : kUmmaK * 128;
           const int adapters = ok ? p.lists[static_cast<long long>(u.rt) * kAdapterListPitch] : 0;
-          for (int b = 0; b < rank_blocks * adapters; ++b) {
+          const int blocks = rank_blocks * adapters;
+          for (int b = blocks * part / parts; b < blocks * (part + 1) / parts; ++b) {
             const int steps = min(kLoraRanks, p.R - b / adapters * kLoraRanks) > kUmmaK ? 2 : 1;
             if (!mbar_wait_cluster(&hfull_bar[hb], hphase, abort_flag)) {   // `up` has landed, h is built
               ok = false;
@@ -630,138 +788,20 @@ __global__ void __launch_bounds__(kNumThreads, 1)
     const int ew = warp & 3;                 // TMEM lane quarter of this warp
     const int col = ew * 32 + lane;          // column inside this CTA's 128
     const int et = static_cast<int>(threadIdx.x) - 64;
+    const int eg = et >> 7;                  // epilogue group
+    const int gt = et & 127;                 // thread of the group
+    const uint32_t group_bar = 2u + static_cast<uint32_t>(eg);
     const bool bf16 = p.bf16 != 0;
     const uint32_t tempty_remote0 = (CG == 2) ? mapa_shared(smem_u32(&tempty_bar[0]), 0) : 0u;
     const uint32_t hfull_remote0 = (CG == 2) ? mapa_shared(smem_u32(&hfull_bar[0]), 0) : 0u;
     int hb = 0, hcount = 0, stage = 0;
     uint32_t hphase = 0, land_par = 0;
     if constexpr (LORA) griddep_wait();
-    if (p.zero_rest) zero_rows(p, grp_rows[0], grp_rows[p.E], et, 32 * kEpiWarps);
-    int buf_i = 0;
-    int acc = 0;
+    if (p.zero_rest) zero_rows(p, grp_rows[0], grp_rows[p.E], et, 32 * kGrpEpiWarps);
+    int acc = 0, turn = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
-    for (int t = worker; t < num_tiles; t += workers) {
-      const GroupedUnit u = grouped_unit<CG, TM>(p, grp_rows, grp_tiles, t);
-      const int n0 = (u.tn * CG + static_cast<int>(rank)) * kGrpCols;
-      const int n = n0 + col;
-      const float bias =
-          (p.bias != nullptr && n < p.N) ? from_16bit(p.bias[static_cast<long long>(u.e) * p.N + n], bf16) : 0.0f;
-      bool got = true;
-      bool odd = false;   // this column held an inf or NaN in some adapter's `up`
-      if constexpr (LORA) {
-        // adapter rows of this CTA's share of the tile: thread et builds row et
-        const int* list = p.lists + static_cast<long long>(u.rt) * kAdapterListPitch;
-        const int adapters = list[0];
-        const bool mixed = adapters > 1 || list[kAdapterListPitch - 1] > 0;
-        const int half = u.nmma / CG;
-        const int tr = static_cast<int>(rank) * half + et;   // row of the tile
-        bool bad = false;
-        const int mine =
-            (et < half && tr < u.rows) ? adapter_of(p.adapter, p.adapter64, u.row0 + tr, p.L, bad) : -1;
-        const float* hrow = p.h + static_cast<long long>(u.row0 + tr) * p.h_pitch;
-        stage = (stage + p.kb_total) % STAGES;
-        for (int rb = 0; rb < rank_blocks && got; ++rb) {
-          uint4 own[8];
-          if (mine >= 0) split_ranks(hrow + rb * kLoraRanks, p.h_pitch - rb * kLoraRanks, bf16, own);
-          for (int ai = 0; ai < adapters; ++ai) {
-            got = (hcount < 2 || mbar_wait(&hempty_bar[hb], hphase ^ 1u, abort_flag)) &&
-                  mbar_wait(&land_bar[stage], (land_par >> stage) & 1u, abort_flag);
-            got = __all_sync(0xffffffffu, got) != 0;
-            if (!got) break;
-            land_par ^= 1u << stage;
-            if (mixed) odd |= clear_nonfinite(sW + stage * Plan::kWBytes, col, p.up_kmaj != 0, bf16);
-            if (et < half) {
-              const bool is = mine >= 0 && list[1 + ai] == mine;
-              uint8_t* dst = sH + hb * Plan::kTBytes + et * 128;
-#pragma unroll
-              for (int c = 0; c < 8; ++c) {
-                *reinterpret_cast<uint4*>(dst + ((c ^ (et & 7)) << 4)) = is ? own[c] : make_uint4(0u, 0u, 0u, 0u);
-              }
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              if constexpr (CG == 1) {
-                mbar_arrive(&hfull_bar[hb]);
-              } else {
-                mbar_arrive_cluster(hfull_remote0 + static_cast<uint32_t>(hb * 8));
-              }
-            }
-            if (++stage == STAGES) stage = 0;
-            ++hcount;
-            hb ^= 1;
-            if (hb == 0) hphase ^= 1u;
-          }
-        }
-      }
-      if (got && p.kb_total > 0 && lane == 0) got = mbar_wait(&tfull_bar[acc], acc_phase, abort_flag);
-      got = __shfl_sync(0xffffffffu, got ? 1 : 0, 0) != 0;
-      ok = named_bar_and(1, 32 * kEpiWarps, got);
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t tbase = tmem_base + (static_cast<uint32_t>(ew * 32) << 16) + static_cast<uint32_t>(acc * TM);
-#pragma unroll 1
-      for (int r0 = 0; r0 < u.rows; r0 += kGrpChunk) {
-        uint32_t v[32];
-        if (p.kb_total > 0) {
-          tmem_ld_32x32b_x32(tbase + r0, v);
-          tmem_ld_wait();
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = 0u;
-        }
-        // A TMA store clips its box at the tensor's edge in units larger than
-        // an element (with an odd N it wrote past the end of the rows), so an
-        // edge tile goes by TMA only when the rows end on a 16-byte boundary.
-        if (LORA && odd && n < p.N) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (r0 + i < u.rows) {
-              v[i] = __float_as_uint(__uint_as_float(v[i]) + nonfinite_terms(p, u.row0 + r0 + i, n));
-            }
-          }
-        }
-        const bool whole = p.c_tma && r0 + kGrpChunk <= u.rows &&
-                           (n0 + kGrpCols <= p.N || (n0 < p.N && p.N % 8 == 0));
-        uint8_t* buf = sOut + buf_i * Plan::kOutBytes;
-        buf_i ^= 1;
-        // the store issued from this buffer two chunks ago has read it
-        if (p.c_tma && et == 0) bulk_wait_group_read<1>();
-        named_bar_sync(1, 32 * kEpiWarps);
-        const uint32_t dst = smem_u32(buf) + col * 2;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float x = apply_act(__uint_as_float(v[i]) + bias, p.act);
-          st_shared_u16(dst + i * (kGrpCols * 2), to_16bit(x, bf16));
-        }
-        if (whole) fence_proxy_async_smem();
-        named_bar_sync(1, 32 * kEpiWarps);
-        if (et == 0 && p.c_tma) {
-          if (whole) tma_store_2d(&maps.c, buf, n0, u.row0 + r0);
-          bulk_commit_group();   // empty when the chunk is stored below: the count above stays per buffer
-        }
-        if (!whole) {
-          const int valid = min(kGrpChunk, u.rows - r0);
-          unsigned short* crow = p.C + static_cast<long long>(u.row0 + r0) * p.ldc;
-          if (p.c_vec) {
-            const int seg = (et & 15) * 8;
-            for (int r = et >> 4; r < valid; r += 8) {
-              const unsigned short* src = reinterpret_cast<const unsigned short*>(buf + r * (kGrpCols * 2)) + seg;
-              unsigned short* out = crow + r * p.ldc + n0 + seg;
-              if (n0 + seg + 8 <= p.N) {
-                *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(src);
-              } else {
-                for (int c = 0; c < 8 && n0 + seg + c < p.N; ++c) out[c] = src[c];
-              }
-            }
-          } else if (n < p.N) {
-            for (int r = 0; r < valid; ++r) {
-              crow[r * p.ldc + n] = *(reinterpret_cast<const unsigned short*>(buf + r * (kGrpCols * 2)) + col);
-            }
-          }
-        }
-      }
+    auto release_acc = [&] {
       tc_fence_before();
       __syncwarp();
       if (lane == 0 && p.kb_total > 0) {
@@ -773,18 +813,242 @@ __global__ void __launch_bounds__(kNumThreads, 1)
       }
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1u;
+    };
+    uint32_t rx_phase = 0;
+    for (int t = worker; t < num_tiles; t += workers) {
+      const GroupedUnit u = grouped_unit<CG, TM>(p, grp_rows, grp_tiles, t);
+      const int n0 = (u.tn * CG + rank) * kGrpCols;
+      const int n = n0 + col;
+      const float bias =
+          (p.bias != nullptr && n < p.N) ? from_16bit(p.bias[static_cast<long long>(u.e) * p.N + n], bf16) : 0.0f;
+      bool got = true;
+      const int* list = nullptr;
+      int b0 = 0, b1 = 0;   // this piece's adapter blocks
+      if constexpr (LORA) {
+        // adapter rows of this CTA's share of the tile: thread gt of a group
+        // builds its half (hi or lo) of row gt
+        list = p.lists + static_cast<long long>(u.rt) * kAdapterListPitch;
+        const int adapters = list[0];
+        b0 = rank_blocks * adapters * part / parts;
+        b1 = rank_blocks * adapters * (part + 1) / parts;
+        const bool mixed = adapters > 1 || list[kAdapterListPitch - 1] > 0;
+        const int half = u.nmma / CG;
+        const int tr = rank * half + gt;   // row of the tile
+        bool bad = false;
+        const int mine =
+            (gt < half && tr < u.rows) ? adapter_of(p.adapter, p.adapter64, u.row0 + tr, p.L, bad) : -1;
+        const float* hrow = p.h + static_cast<long long>(u.row0 + tr) * p.h_pitch;
+        stage = (stage + kb1 - kb0) % STAGES;
+        uint4 own[4];
+        int have = -1;   // rank block held in `own`
+        for (int b = b0; b < b1; ++b) {
+          const int rb = b / adapters, ai = b - rb * adapters;
+          if (rb != have) {
+            if (mine >= 0) split_ranks(hrow + rb * kLoraRanks, p.h_pitch - rb * kLoraRanks, eg != 0, bf16, own);
+            have = rb;
+          }
+          got = (hcount < 2 || mbar_wait(&hempty_bar[hb], hphase ^ 1u, abort_flag)) &&
+                mbar_wait(&land_bar[stage], (land_par >> stage) & 1u, abort_flag);
+          got = __all_sync(0xffffffffu, got) != 0;
+          if (!got) break;
+          land_par ^= 1u << stage;
+          if (mixed && clear_nonfinite(sW + stage * Plan::kWBytes, col, eg, p.up_kmaj != 0, bf16)) odd_flags[turn] = 1;
+          if (gt < half) {
+            const bool is = mine >= 0 && list[1 + ai] == mine;
+            uint8_t* dst = sH + hb * Plan::kTBytes + gt * 128;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              *reinterpret_cast<uint4*>(dst + (((4 * eg + c) ^ (gt & 7)) << 4)) =
+                  is ? own[c] : make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (CG == 1) {
+              mbar_arrive(&hfull_bar[hb]);
+            } else {
+              mbar_arrive_cluster(hfull_remote0 + static_cast<uint32_t>(hb * 8));
+            }
+          }
+          if (++stage == STAGES) stage = 0;
+          ++hcount;
+          hb ^= 1;
+          if (hb == 0) hphase ^= 1u;
+        }
+        // the next tile's flag; its last readers passed the barrier before this one
+        if (et == 0) odd_flags[turn == 2 ? 0 : turn + 1] = 0;
+      }
+      // One lane per warp waits for the accumulator; all warps then take the
+      // same decision, so none is left at a later barrier.
+      if (got && p.kb_total > 0 && lane == 0) got = mbar_wait(&tfull_bar[acc], acc_phase, abort_flag);
+      got = __shfl_sync(0xffffffffu, got ? 1 : 0, 0) != 0;
+      ok = named_bar_and(1, 32 * kGrpEpiWarps, got);
+      if (!ok) break;
+      tc_fence_after();
+      const bool odd = LORA && odd_flags[turn] != 0;
+      turn = turn == 2 ? 0 : turn + 1;
+      const uint32_t tbase = tmem_base + (static_cast<uint32_t>(ew * 32) << 16) + static_cast<uint32_t>(acc * TM);
+
+      auto finish = [&](float v) {
+        v += bias;
+        if (p.act == 1) v = v < 0.0f ? 0.0f : v;   // a NaN stays one
+        if (p.act == 2) v = gelu(v);
+        return v;
+      };
+
+      if constexpr (CG == 2) {
+        // chunks of 32 rows, alternating between the epilogue groups
+#pragma unroll 1
+        for (int r0 = eg * kGrpChunk; r0 < u.rows; r0 += 2 * kGrpChunk) {
+          float f[32];
+          if (p.kb_total > 0) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(tbase + r0, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] = 0.0f;
+          }
+          if (LORA && odd && n < p.N) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              if (r0 + i < u.rows) f[i] += nonfinite_terms(p, list, b0, b1, u.row0 + r0 + i, n);
+            }
+          }
+          // the store issued from this buffer a chunk ago has read it
+          uint8_t* buf = sOut + eg * Plan::kOutBytes;
+          if (p.c_tma && gt == 0) bulk_wait_group_read<0>();
+          named_bar_sync(group_bar, 128);
+          const uint32_t dst = smem_u32(buf) + col * 2;
+          if (p.act == 2) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] = gelu(f[i] + bias);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] = finish(f[i]);
+          }
+          if (bf16) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) st_shared_u16(dst + i * (kGrpCols * 2), to_16bit(f[i], true));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) st_shared_u16(dst + i * (kGrpCols * 2), to_16bit(f[i], false));
+          }
+          // A TMA store clips its box at the tensor's edge in units larger than
+          // an element (with an odd N it wrote past the end of the rows), so an
+          // edge tile goes by TMA only when the rows end on a 16-byte boundary.
+          const bool whole = p.c_tma && r0 + kGrpChunk <= u.rows &&
+                             (n0 + kGrpCols <= p.N || (n0 < p.N && p.N % 8 == 0));
+          if (whole) fence_proxy_async_smem();
+          named_bar_sync(group_bar, 128);
+          if (whole) {
+            if (gt == 0) {
+              tma_store_2d(&maps.c, buf, n0, u.row0 + r0);
+              bulk_commit_group();
+            }
+          } else {
+            store_rows(p, buf, u.row0 + r0, min(kGrpChunk, u.rows - r0), n0, gt, 128);
+          }
+        }
+        release_acc();
+      } else {
+        // Few rows: steps of 8, in loops that are not unrolled.  A small call
+        // runs this once, and what it costs then is fetching the instructions
+        // (the 32-row form above took 5000 cycles for the sums of two rows).
+        uint8_t* buf = sOut;   // all rows of the tile
+        auto read8 = [&](int r0, float (&f)[8]) {
+          uint32_t v[8];
+          tmem_ld_32x32b_x8(tbase + r0, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = p.kb_total > 0 ? __uint_as_float(v[i]) : 0.0f;
+          if (LORA && odd && n < p.N) {
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i) {
+              if (r0 + i >= u.rows) break;
+              const float extra = nonfinite_terms(p, list, b0, b1, u.row0 + r0 + i, n);
+#pragma unroll
+              for (int q = 0; q < 8; ++q) f[q] += q == i ? extra : 0.0f;
+            }
+          }
+        };
+        int mine0 = 0, mine1 = u.rows;   // rows that this CTA finishes
+        if (parts == 1) {
+#pragma unroll 1
+          for (int r0 = eg * 8; r0 < u.rows; r0 += 16) {
+            float f[8];
+            read8(r0, f);
+            const uint32_t dst = smem_u32(buf) + static_cast<uint32_t>(r0 * kGrpCols + col) * 2u;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) st_shared_u16(dst + i * (kGrpCols * 2), to_16bit(finish(f[i]), bf16));
+          }
+          release_acc();
+        } else {
+          // every row's partial sums go to the CTA that finishes it
+          const int per = (u.rows + parts - 1) / parts;   // rows per CTA, at most TM / parts
+          bool got_rx = true;
+          if (t != worker && lane == 0) got_rx = mbar_wait_cluster(rxempty_bar, rx_phase ^ 1u, abort_flag);
+          got_rx = __shfl_sync(0xffffffffu, got_rx ? 1 : 0, 0) != 0;
+          const uint32_t rx = smem_u32(smem + Plan::kOffRx);
+          const uint32_t from = rx + static_cast<uint32_t>(part * per * kGrpCols + col) * 4u;
+#pragma unroll 1
+          for (int r0 = eg * 8; r0 < u.rows && got_rx; r0 += 16) {
+            float f[8];
+            read8(r0, f);
+            int owner = r0 / per, at = r0 - owner * per;
+            const int last = min(8, u.rows - r0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if (i < last) {
+                st_dsmem_f32(mapa_shared(from + static_cast<uint32_t>(at * kGrpCols) * 4u, owner), f[i]);
+                if (++at == per) {
+                  at = 0;
+                  ++owner;
+                }
+              }
+            }
+          }
+          release_acc();   // joins the warp: its stores come before the arrivals
+          if (lane < parts) mbar_arrive_cluster(mapa_shared(smem_u32(rxfull_bar), lane));
+          if (lane == 0 && got_rx) got_rx = mbar_wait_cluster(rxfull_bar, rx_phase, abort_flag);
+          got_rx = __shfl_sync(0xffffffffu, got_rx ? 1 : 0, 0) != 0;
+          ok = named_bar_and(1, 32 * kGrpEpiWarps, got_rx);
+          if (!ok) break;
+          mine0 = min(part * per, u.rows);
+          mine1 = min(mine0 + per, u.rows);
+          const float* sums = reinterpret_cast<const float*>(smem + Plan::kOffRx) + col;
+#pragma unroll 1
+          for (int r = eg; r < mine1 - mine0; r += 2) {
+            float v = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {   // in CTA order
+              if (c < parts) v += sums[(c * per + r) * kGrpCols];
+            }
+            st_shared_u16(smem_u32(buf) + static_cast<uint32_t>(r * kGrpCols + col) * 2u, to_16bit(finish(v), bf16));
+          }
+          __syncwarp();
+          if (lane < parts) mbar_arrive_cluster(mapa_shared(smem_u32(rxempty_bar), lane));
+          rx_phase ^= 1u;
+        }
+        // the next tile's staging comes after its accumulator barrier
+        named_bar_sync(1, 32 * kGrpEpiWarps);
+        store_rows(p, buf, u.row0 + mine0, mine1 - mine0, n0, et, 32 * kGrpEpiWarps);
+      }
     }
     if (!ok) {
       *abort_flag = 1;
       atomicOr(p.err, kDevErrTimeoutEpilogue);
     }
-    if (p.c_tma && et == 0) bulk_wait_group_read<0>();
+    if (CG == 2 && p.c_tma && gt == 0) bulk_wait_group_read<0>();
   }
 
   // ------------------------------------------------------------ teardown
   tc_fence_before();
   __syncthreads();
-  if constexpr (CG == 2) cluster_sync();
+  if (csize > 1) cluster_sync();   // no CTA leaves while a peer may still reach its shared memory
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc<CG>(tmem_base, Plan::kTmemCols);
@@ -804,14 +1068,15 @@ __global__ void __launch_bounds__(kNumThreads, 1)
 // The rows of a group end anywhere, and the stage that holds the last ones
 // also holds the next group's first ones (or inf / NaN behind the last row).
 // Those must be zero in BOTH operands, since 0 * inf is not 0.  So the last
-// stage of a cut group lands on a barrier of its own, a sixth warp zeroes the
+// stage of a cut group lands on a barrier of its own, a warp of its own zeroes the
 // rows up to the next multiple of 16 in shared memory (a row of an atom is
 // 128 contiguous bytes whatever the swizzle, at most 15 rows x 4 atoms), and
 // the MMA reads only ceil(rows / 16) of the stage's four K steps.  The loads
 // run ahead, so the fix-up is off the critical path.
 //
 // Groups without rows give a zero matrix, written without any MMA.
-constexpr int kWgradThreads = kNumThreads + 32;
+constexpr int kWgradThreads = kGrpThreads + 32;
+constexpr int kWgradFixWarp = kGrpThreads / 32;
 constexpr int kWgradTile = 256;
 
 struct WgradParams {
@@ -836,11 +1101,11 @@ struct WgradPlan {
   static constexpr int kOffA = 0;
   static constexpr int kOffG = STAGES * kOpBytes;
   static constexpr int kOffOut = 2 * STAGES * kOpBytes;
-  static constexpr int kOffBar = kOffOut + kEpiWarps * kOutBytes;
+  static constexpr int kOffBar = kOffOut + kGrpEpiWarps * kOutBytes;
   static constexpr int kNumBars = 4 * STAGES + 4 + 1;    // full, empty, land, fix, tmem_full[2], tmem_empty[2], done
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;
   static constexpr int kOffScan = kOffMisc + 16;
-  static constexpr int kOffRows = kOffScan + 32;
+  static constexpr int kOffRows = kOffScan + 64;
   static constexpr int kOffBlocks = kOffRows + (kMaxGroups + 1) * 4;
   static constexpr int kUsed = kOffBlocks + (kMaxGroups + 1) * 4;
   static constexpr int kDynamicBytes = kUsed + 1024;
@@ -931,8 +1196,8 @@ __global__ void __launch_bounds__(kWgradThreads, 1)
     }
     mbar_init(&tfull_bar[0], 1);
     mbar_init(&tfull_bar[1], 1);
-    mbar_init(&tempty_bar[0], kEpiWarps * 2);
-    mbar_init(&tempty_bar[1], kEpiWarps * 2);
+    mbar_init(&tempty_bar[0], kGrpEpiWarps * 2);
+    mbar_init(&tempty_bar[1], kGrpEpiWarps * 2);
     mbar_init(done_bar, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -1084,7 +1349,7 @@ __global__ void __launch_bounds__(kWgradThreads, 1)
         }
       }
     }
-  } else if (warp == 6) {
+  } else if (warp == kWgradFixWarp) {
     // ------------------------------------------------------------ cut stages: zero the rows of others
     int stage = 0;
     uint32_t land_par = 0;
@@ -1124,7 +1389,8 @@ __global__ void __launch_bounds__(kWgradThreads, 1)
     const int ew = warp & 3;
     const bool bf16 = p.bf16 != 0;
     const uint32_t tempty_remote0 = mapa_shared(smem_u32(&tempty_bar[0]), 0);
-    uint8_t* buf = sOut + ew * Plan::kOutBytes;
+    const int half = (warp - 2) >> 2;      // column half of this warp: the two warps of a lane quarter share its rows
+    uint8_t* buf = sOut + (warp - 2) * Plan::kOutBytes;
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
@@ -1134,7 +1400,7 @@ __global__ void __launch_bounds__(kWgradThreads, 1)
         bool got = true;
         if (lane == 0) got = mbar_wait(&tfull_bar[acc], acc_phase, abort_flag);
         got = __shfl_sync(0xffffffffu, got ? 1 : 0, 0) != 0;
-        ok = named_bar_and(1, 32 * kEpiWarps, got);
+        ok = named_bar_and(1, 32 * kGrpEpiWarps, got);
         if (!ok) break;
         tc_fence_after();
       }
@@ -1143,19 +1409,17 @@ __global__ void __launch_bounds__(kWgradThreads, 1)
       const int m0 = u.tm * kWgradTile + rank * 128 + ew * 32;
       unsigned short* out = p.D + static_cast<long long>(u.e) * p.stride_d;
 #pragma unroll 1
-      for (int c0 = 0; c0 < kWgradTile; c0 += kStoreCols) {
+      for (int c0 = half * (kWgradTile / 2); c0 < (half + 1) * (kWgradTile / 2); c0 += kStoreCols) {
         const int n0 = u.tn * kWgradTile + c0;
         if (n0 >= p.N || m0 >= p.M) break;
         float f[64];
         if (u.blocks > 0) {
+          uint32_t v[2][32];
+          tmem_ld_32x32b_x32(tbase + c0, v[0]);
+          tmem_ld_32x32b_x32(tbase + c0 + 32, v[1]);
+          tmem_ld_wait();
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t v[32];
-            tmem_ld_32x32b_x32(tbase + c0 + h * 32, v);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) f[h * 32 + i] = __uint_as_float(v[i]);
-          }
+          for (int i = 0; i < 64; ++i) f[i] = __uint_as_float(v[i >> 5][i & 31]);
         } else {
 #pragma unroll
           for (int i = 0; i < 64; ++i) f[i] = 0.0f;
