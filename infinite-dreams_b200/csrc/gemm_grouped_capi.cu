@@ -130,11 +130,38 @@ cudaError_t opt_in(Kernel kernel, int bytes, std::atomic<unsigned long long>& co
   return e;
 }
 
+// How many clusters of `cluster` CTAs of this kernel the device holds at once
+// (GPCs whose SMs do not divide leave some out: a B200 holds 33 of 4 and 15
+// of 8 CTAs that fill their SM).  Asked once per kernel, device and size.
+template <class Kernel>
+int resident_clusters(Kernel kernel, int bytes, int cluster, int* out) {
+  static std::atomic<int> known[64][9];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return capi_fail_cuda(e, "cudaGetDevice");
+  std::atomic<int>& slot = known[dev & 63][cluster];
+  *out = slot.load(std::memory_order_relaxed);
+  if (*out > 0) return GEMM_OK;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(cluster), 1, 1);
+  cfg.blockDim = dim3(kGrpThreads, 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(bytes);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaOccupancyMaxActiveClusters(out, kernel, &cfg);
+  if (e != cudaSuccess) return capi_fail_cuda(e, "cudaOccupancyMaxActiveClusters");
+  slot.store(*out, std::memory_order_relaxed);
+  return GEMM_OK;
+}
+
 template <class Kernel, class... Args>
-cudaError_t launch(Kernel kernel, int threads, int bytes, std::atomic<unsigned long long>& configured, int grid,
-                   int cluster, cudaStream_t stream, const Args&... args) {
-  cudaError_t e = opt_in(kernel, bytes, configured);
-  if (e != cudaSuccess) return e;
+cudaError_t launch(Kernel kernel, int threads, int bytes, int grid, int cluster, cudaStream_t stream,
+                   const Args&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
   cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
@@ -159,8 +186,8 @@ int launch_grouped(const Operand& a, const Operand& b, const Operand* up, const 
   using Plan = GroupedPlan<CG, TM, STAGES, LORA>;
   GroupedParams p = gp;
   p.tiles_n = static_cast<int>((static_cast<int64_t>(p.N) + kGrpCols * CG - 1) / (kGrpCols * CG));
-  // at most one cut tile per group, and no tile without a row
-  const int64_t row_tiles = std::min<int64_t>(p.T, static_cast<int64_t>(p.T) / TM + p.E);
+  // the most row tiles that T rows in E groups can make
+  const int64_t row_tiles = std::min<int64_t>(p.T, (static_cast<int64_t>(p.T) + static_cast<int64_t>(p.E) * (TM - 1)) / TM);
   const int64_t tiles = row_tiles * p.tiles_n;
   if (tiles > kInt32Max) return capi_fail(GEMM_ERR_UNSUPPORTED, "too many output tiles");
   GroupedMaps maps;
@@ -181,18 +208,28 @@ int launch_grouped(const Operand& a, const Operand& b, const Operand* up, const 
     st = capi_encode(&maps.c, p.C, 2, ext, str, box, false, "C");
   }
   if (st != GEMM_OK) return st;
-  // Single CTAs: with fewer tiles than SMs a cluster splits each tile's K, at
-  // least 4 K blocks to a CTA; the counts are upper bounds (only the device
-  // knows the groups).
-  int cluster = CG;
-  if (CG == 1) {
-    while (cluster < 8 && 2 * cluster * tiles <= sms && p.kb_total >= 8 * cluster) cluster *= 2;
-  }
-  // persistent: one cluster per `cluster` SMs, fewer when there are fewer tiles
-  const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(tiles, sms / cluster))) * cluster;
   static std::atomic<unsigned long long> configured{0};
-  cudaError_t e = launch(gemm_grouped_sm100<CG, TM, STAGES, LORA>, kGrpThreads, Plan::kDynamicBytes, configured, grid,
-                         cluster, stream, maps, p);
+  cudaError_t e = opt_in(gemm_grouped_sm100<CG, TM, STAGES, LORA>, Plan::kDynamicBytes, configured);
+  if (e != cudaSuccess) return capi_fail_cuda(e, "grouped gemm kernel attribute");
+  // Single CTAs: a cluster splits each tile's K, at least 8 K blocks to a CTA
+  // (joining costs as much as 5), as long as there is a cluster for every
+  // tile.  The number of tiles is an upper bound: only the device knows the
+  // groups.
+  int cluster = CG, clusters = sms / CG;
+  if (CG == 1) {
+    for (int c = 2; c <= 8 && p.kb_total >= 8 * c; c *= 2) {
+      int fit = 0;
+      st = resident_clusters(gemm_grouped_sm100<CG, TM, STAGES, LORA>, Plan::kDynamicBytes, c, &fit);
+      if (st != GEMM_OK) return st;
+      if (tiles > fit) break;
+      cluster = c;
+      clusters = fit;
+    }
+  }
+  // persistent: at most one CTA per SM, fewer when there are fewer tiles
+  const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(tiles, clusters))) * cluster;
+  e = launch(gemm_grouped_sm100<CG, TM, STAGES, LORA>, kGrpThreads, Plan::kDynamicBytes, grid, cluster,
+             stream, maps, p);
   return e == cudaSuccess ? GEMM_OK : capi_fail_cuda(e, "grouped gemm kernel launch");
 }
 
@@ -252,40 +289,25 @@ int launch_shrink(const ShrinkParams& sp, bool kmaj, bool bf16, cudaStream_t str
   return e == cudaSuccess ? GEMM_OK : capi_fail_cuda(e, "adapter kernel launch");
 }
 
-constexpr int64_t kLoraSmallRows = 64;   // rows that go to the single-CTA tiles
-
 // Workspace of a call with adapters: h, the adapter lists, then repacked operands.
 struct LoraPlan {
   Operand x, w, up;
   size_t off_h = 0, off_lists = 0, total = 0;
-  int list_tiles = 0, list_rows = 0;
 
   LoraPlan(const void* X, const void* W, const void* U, int64_t T, int64_t N, int64_t K, int64_t L, int64_t R,
            int64_t ldx, int64_t ldw, int trans_w, int64_t ld_up, int64_t stride_up, int trans_up)
       : x(X, 1, T, K, ldx, 0), w(W, 1, trans_w ? N : K, trans_w ? K : N, ldw, 0),
         up(U, L, trans_up ? N : R, trans_up ? R : N, ld_up, stride_up) {
-    if (T <= kLoraSmallRows) {
-      row_tiles_host<64, 16>(T);
-    } else {
-      row_tiles_host<256, 32>(T);
-    }
     size_t off = align256(gemm_workspace_counter_bytes());
-      off_h = off;
+    off_h = off;
     off = align256(off + static_cast<size_t>(T) * shrink_pitch(R) * sizeof(float));
     off_lists = off;
-    off = align256(off + static_cast<size_t>(list_tiles) * kAdapterListPitch * sizeof(int));
+    // a list per row tile, of 64 rows in the variant with more of them
+    off = align256(off + static_cast<size_t>((T + 63) / 64) * kAdapterListPitch * sizeof(int));
     x.plan(&off);
     w.plan(&off);
     up.plan(&off);
     total = off;
-  }
-
-  // the kernel's row tiles (row_tiles in gemm_grouped_kernel.cuh)
-  template <int TM, int STEP>
-  void row_tiles_host(int64_t n) {
-    const int64_t count = (n + TM - 1) / TM;
-    list_tiles = static_cast<int>(count);
-    list_rows = static_cast<int>(((n + count - 1) / count + STEP - 1) / STEP * STEP);
   }
 };
 
@@ -310,15 +332,27 @@ int launch_wgrad(const Operand& a, const Operand& g, const WgradParams& wp, int 
   const int64_t tiles = static_cast<int64_t>(p.E) * p.tiles_m * p.tiles_n;
   const int grid = static_cast<int>(std::min<int64_t>(tiles, sms / 2)) * 2;
   static std::atomic<unsigned long long> configured{0};
-  cudaError_t e = launch(gemm_grouped_wgrad_sm100<kWgradStages>, kWgradThreads, Plan::kDynamicBytes, configured, grid,
-                         2, stream, tmA, tmG, tmD, p);
+  cudaError_t e = opt_in(gemm_grouped_wgrad_sm100<kWgradStages>, Plan::kDynamicBytes, configured);
+  if (e != cudaSuccess) return capi_fail_cuda(e, "grouped weight gradient kernel attribute");
+  e = launch(gemm_grouped_wgrad_sm100<kWgradStages>, kWgradThreads, Plan::kDynamicBytes, grid, 2, stream, tmA, tmG, tmD,
+             p);
   return e == cudaSuccess ? GEMM_OK : capi_fail_cuda(e, "grouped weight gradient kernel launch");
 }
 
-// Few rows per group: the cost is reading the weights, and single CTAs with a
-// deep ring read them best.  More rows: CTA pairs with tiles of up to 256
-// rows, which read every weight once per 256 rows.
-bool small_tiles(int64_t T, int64_t N, int64_t E) { return T <= 64 * E || N <= kGrpCols; }
+// Single CTAs of 128 columns x up to 64 rows, or pairs of 256 x up to 256?
+//  * Up to 16 rows per group: the cost is reading the weights once, and single
+//    CTAs with their deep ring do that best (32 rows over 64 experts 2048 x
+//    1024: 28 us).
+//  * More rows: pairs, which read every weight once per 256 rows (4096 rows
+//    over 64 experts 2048 x 1024: 56 us against 72), unless their tiles would
+//    leave more than half of the machine idle where single CTAs fill it
+//    (64 rows, 4096 x 4096: 32 clusters of 4 against 16 pairs).
+bool small_tiles(int64_t T, int64_t N, int64_t E, int sms) {
+  if (T <= 16 * E || N <= kGrpCols) return true;
+  const int64_t pairs = (T + 255 * E) / 256 * ((N + 255) / 256);
+  const int64_t singles = (T + 63 * E) / 64 * ((N + 127) / 128);
+  return 4 * pairs < sms && singles <= sms;
+}
 
 Operand operand_b(const void* B, int64_t E, int64_t N, int64_t K, int64_t ldb, int64_t stride_b, int trans_b) {
   return Operand(B, E, trans_b ? N : K, trans_b ? K : N, ldb, stride_b);
@@ -403,7 +437,7 @@ int gemm_grouped_launch(const void* A, const void* B, void* C, const void* offse
   p.ldc = ldc;
   p.c_tma = p.c_vec = reinterpret_cast<uintptr_t>(C) % 16u == 0 && ldc % 8 == 0;
   p.zero_rest = zero_rest != 0;
-  if (small_tiles(T, N, E)) return launch_grouped<1, 64, 7, false>(a, b, nullptr, p, sms, stream);
+  if (small_tiles(T, N, E, sms)) return launch_grouped<1, 64, 7, false>(a, b, nullptr, p, sms, stream);
   return launch_grouped<2, 256, 6, false>(a, b, nullptr, p, sms, stream);
 }
 
@@ -561,8 +595,13 @@ int gemm_lora_launch(const void* X, const void* W, const void* down, const void*
   const int vec = trans_down ? 8 : 2 * shrink_rank_tiles(R);   // elements per load
   s.down_vec = reinterpret_cast<uintptr_t>(down) % (2 * vec) == 0 && ld_down % vec == 0 && (L == 1 || stride_down % vec == 0);
   s.lists = reinterpret_cast<int*>(ws + pl.off_lists);
-  s.list_tiles = pl.list_tiles;
-  s.list_rows = pl.list_rows;
+  // the second kernel's row tiles
+  const bool small = small_tiles(T, N, 1, sms);
+  int list_tiles, list_rows;
+  if (small) row_tiles<64, 16>(s.T, list_tiles, list_rows);
+  else row_tiles<256, 32>(s.T, list_tiles, list_rows);
+  s.list_tiles = list_tiles;
+  s.list_rows = list_rows;
   s.err = p.err;
   st = launch_shrink(s, trans_down != 0, dtype == GEMM_DTYPE_BF16, stream);
   if (st != GEMM_OK) return st;
@@ -590,7 +629,7 @@ int gemm_lora_launch(const void* X, const void* W, const void* down, const void*
   p.up = static_cast<const unsigned short*>(pl.up.p);
   p.ld_up = pl.up.ld;
   p.stride_up = L == 1 ? 0 : pl.up.stride;
-  if (T <= kLoraSmallRows) return launch_grouped<1, 64, 6, true>(pl.x, pl.w, &pl.up, p, sms, stream);
+  if (small) return launch_grouped<1, 64, 6, true>(pl.x, pl.w, &pl.up, p, sms, stream);
   return launch_grouped<2, 256, 5, true>(pl.x, pl.w, &pl.up, p, sms, stream);
 }
 

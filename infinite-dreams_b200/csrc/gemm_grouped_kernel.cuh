@@ -119,7 +119,8 @@ constexpr int kLoraRanks = 32;   // ranks per adapter block
 // Two groups of four epilogue warps (one warp per TMEM lane quarter each): they
 // take alternate 32-row chunks, and with adapters one builds hi and one lo.
 constexpr int kGrpEpiWarps = 8;
-constexpr int kGrpThreads = 64 + 32 * kGrpEpiWarps;
+constexpr int kGrpThreads = 64 + 32 * kGrpEpiWarps + 32;
+constexpr int kGrpRowsWarp = 2 + kGrpEpiWarps;   // producer of the rows; warp 0 produces the weights
 
 template <int CG, int TM, int STAGES, bool LORA>
 struct GroupedPlan {
@@ -161,51 +162,54 @@ __device__ __forceinline__ int group_offset(const void* offsets, int off64, int 
 // one may be shorter), rows a multiple of STEP and at most TM.  Equal tiles
 // rather than full ones and a rest: the same count with less padding.
 template <int TM, int STEP>
-__device__ __forceinline__ void row_tiles(int n, int& count, int& rows) {
+__host__ __device__ __forceinline__ void row_tiles(int n, int& count, int& rows) {
   count = (n + TM - 1) / TM;
   rows = (count > 1 ? (n + count - 1) / count + STEP - 1 : n + STEP - 1) / STEP * STEP;
 }
 
 // Few groups: every warp makes the same tables for itself (all write the same
-// values), so no warp waits for another.  False if the offsets are bad.
+// values), so no warp waits for another.  A lane owns up to 8 consecutive
+// groups, its offsets in flight at once.  False if the offsets are bad.
 constexpr int kWarpScanGroups = 256;
 template <class Units>
 __device__ __forceinline__ bool scan_groups_warp(const void* offsets, int off64, int E, int T, int* rows, int* first,
                                                  Units units) {
+  constexpr int kMost = kWarpScanGroups / 32;
   const int lane = static_cast<int>(threadIdx.x & 31);
-  int v[kWarpScanGroups / 32 + 1];
+  const int per = (E + 31) >> 5, g0 = lane * per;
+  int v[kMost + 1];
   bool bad = false;
 #pragma unroll
-  for (int j = 0; j <= kWarpScanGroups / 32; ++j) {   // all loads in flight at once
-    if (j * 32 <= E) v[j] = group_offset(offsets, off64, min(j * 32 + lane, E), T, bad);
+  for (int j = 0; j <= kMost; ++j) {
+    if (j <= per) v[j] = group_offset(offsets, off64, min(g0 + j, E), T, bad);
   }
-  int base = 0;
+  int sum = 0;
 #pragma unroll
-  for (int j = 0; j < kWarpScanGroups / 32; ++j) {
-    if (j * 32 < E) {
-      const int g = j * 32 + lane;
-      // the next offset: the next lane's, or the first of the next 32
-      int next = __shfl_down_sync(0xffffffffu, v[j], 1);
-      const int wrap = __shfl_sync(0xffffffffu, (j + 1) * 32 <= E ? v[j + 1] : v[j], 0);
-      if (lane == 31) next = wrap;
-      const int n = g < E ? next - v[j] : 0;
-      bad |= n < 0;
-      const int mine = g < E ? units(n) : 0;
-      int run = mine;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, run, d);
-        if (lane >= d) run += up;
-      }
-      if (g < E) {
-        rows[g] = v[j];
-        first[g] = base + run - mine;
-        if (g == E - 1) rows[E] = next;
-      }
-      base += __shfl_sync(0xffffffffu, run, 31);
+  for (int j = 0; j < kMost; ++j) {
+    if (j < per) {
+      bad |= v[j + 1] < v[j];
+      sum += units(v[j + 1] - v[j]);   // 0 past the last group
     }
   }
-  if (lane == 0) first[E] = base;
+  int run = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, run, d);
+    if (lane >= d) run += up;
+  }
+  int base = run - sum;
+#pragma unroll
+  for (int j = 0; j < kMost; ++j) {
+    if (j < per && g0 + j < E) {
+      rows[g0 + j] = v[j];
+      first[g0 + j] = base;
+      base += units(v[j + 1] - v[j]);
+      if (g0 + j == E - 1) {
+        rows[E] = v[j + 1];
+        first[E] = base;
+      }
+    }
+  }
   __syncwarp();
   return __all_sync(0xffffffffu, !bad) != 0;
 }
@@ -479,31 +483,31 @@ __device__ __forceinline__ void store_rows(const GroupedParams& p, const uint8_t
   }
 }
 
-// One K block (64) of 128 columns of a stacked weight.  The number of TMA
-// instructions is what counts here: with six per K block (four boxes of 32
-// rows of A, two atoms of B) the issuing thread took 830 cycles per block of
-// a 256 x 256 pair tile whose MMAs take 512; with two it keeps up
-// (8192 x 4096 x 4096 in one group: 244 -> 193 us, B stored N x K).  So the
-// two 64-column atoms of a row-major weight come in one box of a map that
-// sees the columns as (64, N / 64), where N allows it.
+// Where the K blocks of 128 columns of a stacked weight lie in its tensor map.
+//
+// The number of TMA instructions per K block is what bounds a full pair tile
+// if anything but the MMAs does: a thread issues one in 100-150 cycles, and
+// six per block (four boxes of 32 rows of A, two 64-column atoms of B) took
+// 830 cycles where the MMAs take 512.  So each operand comes in one box, the
+// two atoms of a row-major weight through a map that sees the columns as
+// (64, N / 64) where N allows it, and the two operands have a producer each.
+struct WeightBoxes {
+  int x, y, z, e;   // of the first K block
+  int dx, dy;       // per K block
+  bool two;         // a second box for the other atom
+};
+
+__device__ __forceinline__ WeightBoxes weight_boxes(bool kmaj, bool wide, int k0, int col, int e) {
+  if (kmaj) return {k0, col, 0, e, kBK, 0, false};
+  if (wide) return {0, k0, col >> 6, e, 0, kBK, false};
+  return {col, k0, 0, e, 0, kBK, true};
+}
+
 template <bool PAIR>
-__device__ __forceinline__ void load_weights(uint8_t* dst, const CUtensorMap* m, uint64_t* bar, uint32_t bar_cluster,
-                                             bool kmaj, bool wide, int k0, int col, int e) {
-  auto box = [&](uint8_t* to, int x, int y, int z) {
-    if constexpr (PAIR) {
-      tma_load_4d_pair(to, m, bar_cluster, x, y, z, e);
-    } else {
-      tma_load_4d(to, m, bar, x, y, z, e);
-    }
-  };
-  if (kmaj) {
-    box(dst, k0, col, 0);
-  } else if (wide) {
-    box(dst, 0, k0, col >> 6);
-  } else {
-    box(dst, col, k0, 0);
-    box(dst + kBK * 128, col + 64, k0, 0);
-  }
+__device__ __forceinline__ void load_weights(uint32_t dst, const CUtensorMap* m, uint32_t bar, const WeightBoxes& b,
+                                             int step) {
+  tma_load_4d_at<PAIR>(dst, m, bar, b.x + step * b.dx, b.y + step * b.dy, b.z, b.e);
+  if (b.two) tma_load_4d_at<PAIR>(dst + kBK * 128, m, bar, b.x + 64, b.y + step * b.dy, b.z, b.e);
 }
 
 template <int CG, int TM, int STAGES, bool LORA>
@@ -549,7 +553,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
   if (threadIdx.x == 64) {
 #pragma unroll
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full_bar[s], 1);
+      mbar_init(&full_bar[s], 2);   // the two producers of the (even) CTA
       mbar_init(&empty_bar[s], 1);
       mbar_init(&land_bar[s], 1);
     }
@@ -584,6 +588,11 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
   if (csize > 1) cluster_sync();   // the peers' barriers are initialised before any remote use
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  // Parameters are read now, while the previous grid may still run: the
+  // first read of each line of them costs a few hundred cycles.
+  const int kb0 = p.kb_total * part / parts, kb1 = p.kb_total * (part + 1) / parts;
+  asm volatile("" ::"l"(p.offsets), "r"(p.E), "r"(p.T), "r"(p.N), "r"(p.tiles_n), "r"(p.b_kmaj), "l"(p.bias), "l"(p.C),
+               "r"(p.zero_rest), "r"(p.up_kmaj), "r"(kb0), "r"(kb1));
   // With LORA the previous grid is lora_shrink, which lets this one start
   // once everything before it has completed: A and B can be read at once, and
   // only what touches h, the lists or C waits (each thread for itself, below).
@@ -596,11 +605,15 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
     scan_groups<kGrpThreads>(p.offsets, p.off64, p.E, p.T, grp_rows, grp_tiles, scan, p.err, tiles_of);
   }
   const int num_tiles = grp_tiles[p.E];
-  const int kb0 = p.kb_total * part / parts, kb1 = p.kb_total * (part + 1) / parts;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ TMA producer
+  if (warp == 0 || warp == kGrpRowsWarp) {
+    // ------------------------------------------------------------ TMA producers: weights, rows
     if (lane == 0) {
+      const bool weights = warp == 0;
+      const uint32_t slot0 = smem_u32(weights ? sW : sT);
+      const uint32_t slot_bytes = weights ? Plan::kWBytes : Plan::kTBytes;
+      const uint32_t full0 = smem_u32(full_bar);
+      const uint32_t even0 = CG == 2 ? mapa_shared(full0, 0) : full0;   // a pair's bytes complete on the even CTA
       int stage = 0;
       uint32_t phase = 0;
       int issued = 0;
@@ -616,26 +629,19 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
         int box = 0;
         while (box + 1 < box_count(TM) && half <= box_rows(TM, box + 1)) ++box;
         const CUtensorMap* map_a = &maps.a[box];
-        const uint32_t bytes = Plan::kWBytes + static_cast<uint32_t>(box_rows(TM, box)) * 128u;
+        const uint32_t bytes = weights ? Plan::kWBytes : static_cast<uint32_t>(box_rows(TM, box)) * 128u;
+        const WeightBoxes wb = weight_boxes(p.b_kmaj != 0, p.b_wide != 0, kb0 * kBK, bcol, u.e);
         for (int kb = kb0; kb < kb1; ++kb) {
           if (issued >= STAGES && !mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) {
             ok = false;
             break;
           }
-          uint8_t* w_dst = sW + stage * Plan::kWBytes;
-          uint8_t* t_dst = sT + stage * Plan::kTBytes;
-          uint64_t* bar = &full_bar[stage];
-          const int k0 = kb * kBK;
-          if constexpr (CG == 1) {
-            mbar_arrive_expect_tx(bar, bytes);
-            load_weights<false>(w_dst, &maps.b, bar, 0, p.b_kmaj != 0, p.b_wide != 0, k0, bcol, u.e);
-            tma_load_2d(t_dst, map_a, bar, k0, arow);
+          if (leader) mbar_arrive_expect_tx(&full_bar[stage], CG * bytes);
+          const uint32_t dst = slot0 + stage * slot_bytes, bar = even0 + stage * 8;
+          if (weights) {
+            load_weights<CG == 2>(dst, &maps.b, bar, wb, kb - kb0);
           } else {
-            // both CTAs' bytes complete on the even CTA's barrier
-            if (leader) mbar_arrive_expect_tx(bar, 2 * bytes);
-            const uint32_t even = mapa_shared(smem_u32(bar), 0);
-            load_weights<true>(w_dst, &maps.b, bar, even, p.b_kmaj != 0, p.b_wide != 0, k0, bcol, u.e);
-            tma_load_2d_pair(t_dst, map_a, even, k0, arow);
+            tma_load_2d_at<CG == 2>(dst, map_a, bar, kb * kBK, arow);
           }
           full_par ^= 1u << stage;
           on_land &= ~(1u << stage);
@@ -652,16 +658,17 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
           const int adapters = ok ? list[0] : 0;
           const int blocks = rank_blocks * adapters;
           for (int b = blocks * part / parts; b < blocks * (part + 1) / parts; ++b) {
-            const int a = list[1 + b % adapters], r0 = b / adapters * kLoraRanks;
-            if (issued >= STAGES && !mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) {
-              ok = false;
-              break;
+            if (weights) {
+              const int a = list[1 + b % adapters], r0 = b / adapters * kLoraRanks;
+              if (issued >= STAGES && !mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) {
+                ok = false;
+                break;
+              }
+              // on a barrier of this CTA: its epilogue warps look the weights over
+              mbar_arrive_expect_tx(&land_bar[stage], Plan::kWBytes);
+              load_weights<false>(slot0 + stage * slot_bytes, &maps.u, smem_u32(&land_bar[stage]),
+                                  weight_boxes(p.up_kmaj != 0, p.up_wide != 0, r0, bcol, a), 0);
             }
-            uint8_t* w_dst = sW + stage * Plan::kWBytes;
-            // on a barrier of this CTA: its epilogue warps look the weights over
-            uint64_t* bar = &land_bar[stage];
-            mbar_arrive_expect_tx(bar, Plan::kWBytes);
-            load_weights<false>(w_dst, &maps.u, bar, 0, p.up_kmaj != 0, p.up_wide != 0, r0, bcol, a);
             land_par ^= 1u << stage;
             on_land |= 1u << stage;
             ++issued;
@@ -672,7 +679,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
           }
         }
       }
-      griddep_launch_dependents();
+      if (weights) griddep_launch_dependents();
       if (!ok) {
         *abort_flag = 1;
         atomicOr(p.err, kDevErrTimeoutProducer);
@@ -682,7 +689,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
       // teardown)
       for (int s = 0; s < min(issued, STAGES); ++s) {
         const uint32_t bit = 1u << s;
-        if (!(on_land & bit) && !leader) continue;
+        if ((on_land & bit) ? !weights : !leader) continue;
         uint64_t* bar = (on_land & bit) ? &land_bar[s] : &full_bar[s];
         const uint32_t par = (((on_land & bit) ? land_par : full_par) & bit) ? 0u : 1u;   // of the last fill
         const uint64_t t0 = globaltimer_ns();
@@ -1076,7 +1083,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
 //
 // Groups without rows give a zero matrix, written without any MMA.
 constexpr int kWgradThreads = kGrpThreads + 32;
-constexpr int kWgradFixWarp = kGrpThreads / 32;
+constexpr int kWgradFixWarp = kGrpThreads / 32;   // warp 0 produces A, warp kGrpRowsWarp G
 constexpr int kWgradTile = 256;
 
 struct WgradParams {
@@ -1137,23 +1144,12 @@ __device__ __forceinline__ WgradUnit wgrad_unit(const WgradParams& p, const int*
   return u;
 }
 
-// 64 rows x 128 columns of an operand (see load_weights on the box count).
+// 64 rows x 128 columns of an operand (see weight_boxes on the box count).
 template <bool PAIR>
-__device__ __forceinline__ void load_columns(uint8_t* dst, const CUtensorMap* m, uint64_t* bar, uint32_t bar_cluster,
-                                             bool wide, int col, int row) {
-  auto box = [&](uint8_t* to, int x, int z) {
-    if constexpr (PAIR) {
-      tma_load_3d_pair(to, m, bar_cluster, x, row, z);
-    } else {
-      tma_load_3d(to, m, bar, x, row, z);
-    }
-  };
-  if (wide) {
-    box(dst, 0, col >> 6);
-  } else {
-    box(dst, col, 0);
-    box(dst + kBK * 128, col + 64, 0);
-  }
+__device__ __forceinline__ void load_columns(uint32_t dst, const CUtensorMap* m, uint32_t bar, bool wide, int col,
+                                             int row) {
+  tma_load_3d_at<PAIR>(dst, m, bar, wide ? 0 : col, row, wide ? col >> 6 : 0);
+  if (!wide) tma_load_3d_at<PAIR>(dst + kBK * 128, m, bar, col + 64, row, 0);
 }
 
 template <int STAGES>
@@ -1189,9 +1185,9 @@ __global__ void __launch_bounds__(kWgradThreads, 1)
   if (threadIdx.x == 64) {
 #pragma unroll
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full_bar[s], 1);
+      mbar_init(&full_bar[s], 2);   // the two producers of the even CTA
       mbar_init(&empty_bar[s], 1);
-      mbar_init(&land_bar[s], 1);
+      mbar_init(&land_bar[s], 2);
       mbar_init(&fix_bar[s], 2);
     }
     mbar_init(&tfull_bar[0], 1);
@@ -1222,41 +1218,39 @@ __global__ void __launch_bounds__(kWgradThreads, 1)
                              [](int n) { return (n + kBK - 1) / kBK; });
   const int num_tiles = p.E * p.tiles_m * p.tiles_n;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ TMA producer
+  if (warp == 0 || warp == kGrpRowsWarp) {
+    // ------------------------------------------------------------ TMA producers: A, G
     if (lane == 0) {
+      const bool first = warp == 0;
+      const CUtensorMap* map = first ? &tmA : &tmG;
+      const bool wide = first ? p.a_wide != 0 : p.g_wide != 0;
+      const uint32_t slot0 = smem_u32(first ? sA : sG);
+      const uint32_t even0 = mapa_shared(smem_u32(full_bar), 0);
       int stage = 0;
       uint32_t phase = 0;
       int issued = 0;
       // per stage: parity of its last whole / cut fill, and which came last
-      uint32_t full_par = 0, land_par = 0, was_cut = 0, used = 0;
+      uint32_t full_par = 0, land_par = 0, was_cut = 0;
       bool ok = true;
       for (int t = worker; ok && t < num_tiles; t += workers) {
         const WgradUnit u = wgrad_unit(p, grp_rows, t);
-        const int acol = u.tm * kWgradTile + rank * 128;
-        const int gcol = u.tn * kWgradTile + rank * 128;
+        const int col = (first ? u.tm : u.tn) * kWgradTile + rank * 128;
         for (int b = 0; b < u.blocks; ++b) {
           if (issued >= STAGES && !mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) {
             ok = false;
             break;
           }
-          uint8_t* a_dst = sA + stage * Plan::kOpBytes;
-          uint8_t* g_dst = sG + stage * Plan::kOpBytes;
+          const uint32_t dst = slot0 + stage * Plan::kOpBytes;
           const int row = u.row0 + b * kBK;
           const uint32_t bit = 1u << stage;
-          used |= bit;
           if (b == u.blocks - 1 && u.tail) {
-            uint64_t* bar = &land_bar[stage];
-            mbar_arrive_expect_tx(bar, Plan::kStageBytes);
-            load_columns<false>(a_dst, &tmA, bar, 0, p.a_wide != 0, acol, row);
-            load_columns<false>(g_dst, &tmG, bar, 0, p.g_wide != 0, gcol, row);
+            mbar_arrive_expect_tx(&land_bar[stage], Plan::kOpBytes);
+            load_columns<false>(dst, map, smem_u32(&land_bar[stage]), wide, col, row);
             was_cut |= bit;
             land_par ^= bit;
           } else {
-            if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * Plan::kStageBytes);
-            const uint32_t bar = mapa_shared(smem_u32(&full_bar[stage]), 0);
-            load_columns<true>(a_dst, &tmA, nullptr, bar, p.a_wide != 0, acol, row);
-            load_columns<true>(g_dst, &tmG, nullptr, bar, p.g_wide != 0, gcol, row);
+            if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * Plan::kOpBytes);
+            load_columns<true>(dst, map, even0 + stage * 8, wide, col, row);
             was_cut &= ~bit;
             full_par ^= bit;
           }
@@ -1267,7 +1261,7 @@ __global__ void __launch_bounds__(kWgradThreads, 1)
           }
         }
       }
-      griddep_launch_dependents();
+      if (first) griddep_launch_dependents();
       if (!ok) {
         *abort_flag = 1;
         atomicOr(p.err, kDevErrTimeoutProducer);
@@ -1275,9 +1269,9 @@ __global__ void __launch_bounds__(kWgradThreads, 1)
       // every fill must have landed before the CTA exits (whole fills of the
       // odd CTA complete on the even one's barriers and are covered by the
       // cluster barrier at teardown)
-      for (int s = 0; s < STAGES; ++s) {
+      for (int s = 0; s < min(issued, STAGES); ++s) {
         const uint32_t bit = 1u << s;
-        if (!(used & bit) || (!(was_cut & bit) && !leader)) continue;
+        if (!(was_cut & bit) && !leader) continue;
         uint64_t* bar = (was_cut & bit) ? &land_bar[s] : &full_bar[s];
         const uint32_t par = (((was_cut & bit) ? land_par : full_par) & bit) ? 0u : 1u;   // of the last fill
         const uint64_t t0 = globaltimer_ns();
