@@ -46,7 +46,8 @@ def nvcc() -> str:
 
 
 def sources() -> List[Path]:
-    return [CSRC / "gemm_capi.cu", CSRC / "gemm_noalloc.cu", CSRC / "gemm_grouped_capi.cu"] + sorted(GEN.glob("gemm_bank_*.cu"))
+    return [CSRC / "gemm_capi.cu", CSRC / "gemm_noalloc.cu", CSRC / "gemm_grouped_capi.cu",
+            CSRC / "gemm_lora_shrink.cu"] + sorted(GEN.glob("gemm_bank_*.cu"))
 
 
 def headers_digest() -> str:

@@ -234,61 +234,6 @@ int launch_grouped(const Operand& a, const Operand& b, const Operand* up, const 
 }
 
 // ------------------------------------------------------------- low-rank adapters
-// The first kernel's variant: ranks per block (16, 32 or 64, R above 64 in
-// several blocks) and rows of one adapter per MMA chunk (8 or 32).
-using ShrinkFn = void (*)(ShrinkParams);
-
-template <int RT, int NT8>
-ShrinkFn shrink_fn(bool kmaj, bool bf16) {
-  if (kmaj) return bf16 ? lora_shrink<RT, NT8, true, true> : lora_shrink<RT, NT8, true, false>;
-  return bf16 ? lora_shrink<RT, NT8, false, true> : lora_shrink<RT, NT8, false, false>;
-}
-
-int shrink_rank_tiles(int64_t R) { return R <= 16 ? 1 : (R <= 32 ? 2 : 4); }
-int64_t shrink_pitch(int64_t R) { return round_up(R, 16 * shrink_rank_tiles(R)); }
-
-int launch_shrink(const ShrinkParams& sp, bool kmaj, bool bf16, cudaStream_t stream) {
-  ShrinkParams p = sp;
-  const int rt = shrink_rank_tiles(p.R);
-  // Rows per tile: few enough that about 256 CTAs share the work (T = 64: 2
-  // rows x 32 clusters of 8), up to the 32 rows of one MMA chunk.
-  int rows = 1;
-  while (rows < kShrinkMaxRows && rows * 32 < p.T) rows *= 2;
-  p.tile_rows = rows;
-  // CTAs along K: up to about 300 CTAs in all, and no more than give every
-  // warp a slice.
-  const int slices = (p.K + kShrinkSlice - 1) / kShrinkSlice;
-  const int tiles = (p.T + rows - 1) / rows;
-  int cluster = 1;
-  while (cluster < 8 && cluster * kShrinkWarps < slices && cluster * tiles <= 150) cluster *= 2;
-  const bool wide = rows > 8;
-  ShrinkFn fn = rt == 1 ? (wide ? shrink_fn<1, 4>(kmaj, bf16) : shrink_fn<1, 1>(kmaj, bf16))
-                : rt == 2 ? (wide ? shrink_fn<2, 4>(kmaj, bf16) : shrink_fn<2, 1>(kmaj, bf16))
-                          : (wide ? shrink_fn<4, 4>(kmaj, bf16) : shrink_fn<4, 1>(kmaj, bf16));
-  const int bytes = kShrinkWarps * rows * 16 * rt * static_cast<int>(sizeof(float));   // at most 64 KiB
-  static std::atomic<unsigned long long> configured[24];
-  const int which = (((rt == 1 ? 0 : rt == 2 ? 1 : 2) * 2 + wide) * 2 + kmaj) * 2 + bf16;
-  cudaError_t e = opt_in(fn, 64 * 1024, configured[which]);
-  if (e != cudaSuccess) return capi_fail_cuda(e, "adapter kernel attribute");
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((p.T + rows - 1) / rows * cluster),
-                     static_cast<unsigned>((p.R + 16 * rt - 1) / (16 * rt)), 1);
-  cfg.blockDim = dim3(kShrinkThreads, 1, 1);
-  cfg.dynamicSmemBytes = static_cast<size_t>(bytes);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  e = cudaLaunchKernelEx(&cfg, fn, p);
-  return e == cudaSuccess ? GEMM_OK : capi_fail_cuda(e, "adapter kernel launch");
-}
-
 // Workspace of a call with adapters: h, the adapter lists, then repacked operands.
 struct LoraPlan {
   Operand x, w, up;
@@ -591,9 +536,6 @@ int gemm_lora_launch(const void* X, const void* W, const void* down, const void*
   s.K = static_cast<int>(K);
   s.L = static_cast<int>(L);
   s.R = static_cast<int>(R);
-  s.x_vec = 1;   // TMA-addressable, as it came or repacked
-  const int vec = trans_down ? 8 : 2 * shrink_rank_tiles(R);   // elements per load
-  s.down_vec = reinterpret_cast<uintptr_t>(down) % (2 * vec) == 0 && ld_down % vec == 0 && (L == 1 || stride_down % vec == 0);
   s.lists = reinterpret_cast<int*>(ws + pl.off_lists);
   // the second kernel's row tiles
   const bool small = small_tiles(T, N, 1, sms);
@@ -603,7 +545,7 @@ int gemm_lora_launch(const void* X, const void* W, const void* down, const void*
   s.list_tiles = list_tiles;
   s.list_rows = list_rows;
   s.err = p.err;
-  st = launch_shrink(s, trans_down != 0, dtype == GEMM_DTYPE_BF16, stream);
+  st = launch_shrink(s, trans_down != 0, dtype == GEMM_DTYPE_BF16, stream);   // x is TMA-addressable by now
   if (st != GEMM_OK) return st;
 
   p.E = 1;
@@ -630,7 +572,7 @@ int gemm_lora_launch(const void* X, const void* W, const void* down, const void*
   p.ld_up = pl.up.ld;
   p.stride_up = L == 1 ? 0 : pl.up.stride;
   if (small) return launch_grouped<1, 64, 6, true>(pl.x, pl.w, &pl.up, p, sms, stream);
-  return launch_grouped<2, 256, 5, true>(pl.x, pl.w, &pl.up, p, sms, stream);
+  return launch_grouped<2, 256, 6, true>(pl.x, pl.w, &pl.up, p, sms, stream);
 }
 
 }  // extern "C"

@@ -40,13 +40,13 @@
 // (E = 1, no offsets):  C[r, :] = act(A[r, :] * B + h[r, :] * up[a_r] + bias).
 // h (fp32, scaled) comes from lora_shrink (gemm_lora_kernel.cuh), which also
 // lists the adapters of each row tile.  After the K blocks of a tile come its
-// adapter blocks, 32 ranks of one adapter each: the weight slot of a stage
-// holds `up` (64 ranks wide as TMA's swizzle wants it, of which 32 are used)
-// and the row operand is built by the epilogue warps in a buffer of its own:
-// row r holds h[r] when the row picked this adapter and zeros when not, so
-// rows with different adapters share a tile.  h is split into two 16-bit
+// adapter blocks, 32 ranks of one adapter each, which pass through the same
+// ring: the weight slot of a stage holds `up` (64 ranks wide as TMA's swizzle
+// wants it, of which 32 are used), and its row slot is filled by the epilogue
+// warps: row r holds h[r] when the row picked this adapter and zeros when not,
+// so rows with different adapters share a tile.  h is split into two 16-bit
 // numbers, h = hi + lo with |lo| <= half a step of hi, side by side in the 64
-// columns of the buffer, each multiplied with the same `up`: what tensor cores
+// columns of the slot, each multiplied with the same `up`: what tensor cores
 // take is 16-bit, and rounding h to one would cost as much accuracy as the
 // result's own rounding does.
 //
@@ -117,7 +117,7 @@ struct GroupedParams {
 constexpr int kLoraRanks = 32;   // ranks per adapter block
 
 // Two groups of four epilogue warps (one warp per TMEM lane quarter each): they
-// take alternate 32-row chunks, and with adapters one builds hi and one lo.
+// take alternate chunks of rows, and alternate adapter blocks.
 constexpr int kGrpEpiWarps = 8;
 constexpr int kGrpThreads = 64 + 32 * kGrpEpiWarps + 32;
 constexpr int kGrpRowsWarp = 2 + kGrpEpiWarps;   // producer of the rows; warp 0 produces the weights
@@ -134,11 +134,10 @@ struct GroupedPlan {
   static constexpr int kOffW = 0;
   static constexpr int kOffT = kOffW + STAGES * kWBytes;
   static constexpr int kOffOut = kOffT + STAGES * kTBytes;
-  static constexpr int kOffH = kOffOut + 2 * kOutBytes;  // two buffers of adapter rows (hi | lo)
-  static constexpr int kOffRx = kOffH + (LORA ? 2 * kTBytes : 0);   // fp32 sums from the cluster
+  static constexpr int kOffRx = kOffOut + 2 * kOutBytes;  // fp32 sums from the cluster
   static constexpr int kOffBar = kOffRx + (CG == 1 ? TM * kGrpCols * 4 : 0);
-  // full, empty, land, tmem_full[2], tmem_empty[2], h_full[2], h_empty[2], rx_full, rx_empty, done
-  static constexpr int kNumBars = 3 * STAGES + 10 + 1;
+  // full, empty, land, built, tmem_full[2], tmem_empty[2], rx_full, rx_empty, done
+  static constexpr int kNumBars = 4 * STAGES + 6 + 1;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;
   static constexpr int kOffScan = kOffMisc + 32;         // warp totals
   static constexpr int kOffRows = kOffScan + 64;         // group starts [E + 1]
@@ -336,10 +335,10 @@ __device__ __forceinline__ void zero_rows(const GroupedParams& p, int lo, int hi
   }
 }
 
-// The 32 ranks of one row's block as half a row of the swizzled adapter
-// buffer: hi (the first four 16-byte chunks) or lo (the last four).
-__device__ __forceinline__ void split_ranks(const float* h, int valid, bool want_lo, bool bf16, uint4 (&out)[4]) {
-  uint32_t w[16];
+// The 32 ranks of one row's block as a swizzle-ready row: hi in the first four
+// 16-byte chunks, lo in the last four.
+__device__ __forceinline__ void split_ranks(const float* h, int valid, bool bf16, uint4 (&out)[8]) {
+  uint32_t w[32];
 #pragma unroll
   for (int i = 0; i < kLoraRanks; i += 4) {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -347,22 +346,21 @@ __device__ __forceinline__ void split_ranks(const float* h, int valid, bool want
     const float f[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int e = 0; e < 4; e += 2) {
-      uint32_t word = 0;
+      uint32_t hi = 0, lo = 0;
 #pragma unroll
       for (int o = 0; o < 2; ++o) {
-        unsigned short bits = to_16bit(f[e + o], bf16);
-        if (want_lo) {
-          // an h beyond the type's range is infinite in hi; lo must not undo that
-          const float rest = f[e + o] - from_16bit(bits, bf16);
-          bits = to_16bit(isfinite(rest) ? rest : 0.0f, bf16);
-        }
-        word |= static_cast<uint32_t>(bits) << (16 * o);
+        const unsigned short top = to_16bit(f[e + o], bf16);
+        hi |= static_cast<uint32_t>(top) << (16 * o);
+        // an h beyond the type's range is infinite in hi; lo must not undo that
+        const float rest = f[e + o] - from_16bit(top, bf16);
+        lo |= static_cast<uint32_t>(to_16bit(isfinite(rest) ? rest : 0.0f, bf16)) << (16 * o);
       }
-      w[(i + e) / 2] = word;
+      w[(i + e) / 2] = hi;
+      w[16 + (i + e) / 2] = lo;
     }
   }
 #pragma unroll
-  for (int c = 0; c < 4; ++c) out[c] = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+  for (int c = 0; c < 8; ++c) out[c] = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
 }
 
 __device__ __forceinline__ bool nonfinite16(uint32_t h, bool bf16) {
@@ -370,40 +368,32 @@ __device__ __forceinline__ bool nonfinite16(uint32_t h, bool bf16) {
   return (h & exponent) == exponent;
 }
 
-// Replaces the inf and NaN among ranks [16 half, 16 half + 16) of column `col`
-// of a landed `up` tile by zeros; says whether there were any.
-__device__ __forceinline__ bool clear_nonfinite(uint8_t* tile, int col, int half, bool kmaj, bool bf16) {
-  bool any = false;
-  if (kmaj) {   // row `col`, ranks in 16-byte chunks swizzled by the row
+// Replaces the inf and NaN among the first 32 ranks of a landed `up` tile by
+// zeros; says whether this thread found any.  128 threads, four 16-byte chunks
+// each: a tile stored N x R has them in row `thread`, one stored R x N in rows
+// 0..31 of both atoms.  An exponent of all ones plus one in its lowest place
+// carries into the sign bit's place, for both halves of a word at once.
+__device__ __forceinline__ bool clear_nonfinite(uint8_t* tile, int thread, bool kmaj, bool bf16) {
+  const uint32_t exponent = bf16 ? 0x7F807F80u : 0x7C007C00u, one = bf16 ? 0x00800080u : 0x04000400u;
+  uint4* at[4];
+  uint32_t seen = 0;
 #pragma unroll
-    for (int i2 = 0; i2 < 2; ++i2) {
-      const int c = 2 * half + i2;
-      uint32_t* at = reinterpret_cast<uint32_t*>(tile + col * 128 + ((c ^ (col & 7)) << 4));
-      const uint4 v = *reinterpret_cast<const uint4*>(at);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool lo = nonfinite16(w[i], bf16), hi = nonfinite16(w[i] >> 16, bf16);
-        if (lo || hi) {
-          at[i] = w[i] & (lo ? 0xFFFF0000u : 0xFFFFFFFFu) & (hi ? 0x0000FFFFu : 0xFFFFFFFFu);
-          any = true;
-        }
-      }
-    }
-  } else {      // atom col / 64, one rank per row
-    uint8_t* atom = tile + (col >> 6) * (kBK * 128);
-    const int c = col & 63;
-#pragma unroll
-    for (int i = 0; i < kLoraRanks / 2; ++i) {
-      const int r = half * (kLoraRanks / 2) + i;
-      unsigned short* at = reinterpret_cast<unsigned short*>(atom + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
-      if (nonfinite16(*at, bf16)) {
-        *at = 0;
-        any = true;
-      }
+  for (int i = 0; i < 4; ++i) {
+    const int c = i * 128 + thread;
+    at[i] = reinterpret_cast<uint4*>(kmaj ? tile + thread * 128 + ((i ^ (thread & 7)) << 4)
+                                          : tile + (c >> 8) * (kBK * 128) + (c & 255) * 16);
+    const uint4 v = *at[i];
+    seen |= ((v.x & exponent) + one) | ((v.y & exponent) + one) | ((v.z & exponent) + one) | ((v.w & exponent) + one);
+  }
+  if ((seen & 0x80008000u) == 0) return false;
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i) {
+    unsigned short* h = reinterpret_cast<unsigned short*>(at[i]);
+    for (int e = 0; e < 8; ++e) {
+      if (nonfinite16(h[e], bf16)) h[e] = 0;
     }
   }
-  return any;
+  return true;
 }
 
 // What clear_nonfinite took out of row t's value in column n in the adapter
@@ -413,7 +403,7 @@ __device__ __noinline__ float nonfinite_terms(const GroupedParams& p, const int*
   const int a = adapter_of(p.adapter, p.adapter64, t, p.L, bad);
   const int adapters = list[0];
   int ai = 0;
-  while (ai < adapters && list[1 + ai] != a) ++ai;
+  while (ai < adapters && list[kAdapterIds + ai] != a) ++ai;
   float sum = 0.0f;
   if (a < 0 || ai == adapters) return sum;
   for (int r = 0; r < p.R; ++r) {
@@ -522,14 +512,12 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + Plan::kOffBar);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* land_bar = empty_bar + STAGES;   // an adapter's weights, per CTA
-  uint64_t* tfull_bar = land_bar + STAGES;
+  uint64_t* built_bar = land_bar + STAGES;   // ... and its rows of h are in place, on the even CTA
+  uint64_t* tfull_bar = built_bar + STAGES;
   uint64_t* tempty_bar = tfull_bar + 2;
-  uint64_t* hfull_bar = tempty_bar + 2;
-  uint64_t* hempty_bar = hfull_bar + 2;
-  uint64_t* rxfull_bar = hempty_bar + 2;     // the cluster's sums for this CTA have arrived
+  uint64_t* rxfull_bar = tempty_bar + 2;     // the cluster's sums for this CTA have arrived
   uint64_t* rxempty_bar = rxfull_bar + 1;    // ... have been read, in every CTA of the cluster
   uint64_t* done_bar = rxempty_bar + 1;
-  uint8_t* sH = smem + Plan::kOffH;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Plan::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* odd_flags = reinterpret_cast<volatile int*>(tmem_slot + 2);   // three tiles in turn
@@ -556,15 +544,12 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
       mbar_init(&full_bar[s], 2);   // the two producers of the (even) CTA
       mbar_init(&empty_bar[s], 1);
       mbar_init(&land_bar[s], 1);
+      mbar_init(&built_bar[s], kGrpEpiWarps / 2 * CG);   // one epilogue group of every CTA
     }
     mbar_init(&tfull_bar[0], 1);
     mbar_init(&tfull_bar[1], 1);
     mbar_init(&tempty_bar[0], kGrpEpiWarps * CG);
     mbar_init(&tempty_bar[1], kGrpEpiWarps * CG);
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&hfull_bar[b], kGrpEpiWarps * CG);
-      mbar_init(&hempty_bar[b], 1);
-    }
     mbar_init(rxfull_bar, kGrpEpiWarps * parts);
     mbar_init(rxempty_bar, kGrpEpiWarps * parts);
     mbar_init(done_bar, 1);
@@ -657,9 +642,17 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
           const int* list = p.lists + static_cast<long long>(u.rt) * kAdapterListPitch;
           const int adapters = ok ? list[0] : 0;
           const int blocks = rank_blocks * adapters;
-          for (int b = blocks * part / parts; b < blocks * (part + 1) / parts; ++b) {
+          const int b0 = blocks * part / parts, b1 = blocks * (part + 1) / parts;
+          int rb = adapters ? b0 / adapters : 0, ai = b0 - rb * adapters;
+          int next = b0 < b1 ? list[kAdapterIds + ai] : 0;   // one block ahead of its use
+          for (int b = b0; b < b1; ++b) {
+            const int a = next, r0 = rb * kLoraRanks;
+            if (++ai == adapters) {
+              ai = 0;
+              ++rb;
+            }
             if (weights) {
-              const int a = list[1 + b % adapters], r0 = b / adapters * kLoraRanks;
+              if (b + 1 < b1) next = list[kAdapterIds + ai];
               if (issued >= STAGES && !mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) {
                 ok = false;
                 break;
@@ -711,8 +704,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
       int acc = 0;
       uint32_t acc_phase = 0;
       int count = 0;
-      int hb = 0;
-      uint32_t hphase = 0;
+      uint32_t built_par = 0;
       bool ok = true, waited = false;
       for (int t = worker; ok && t < num_tiles; t += workers) {
         if (p.kb_total == 0) break;   // the epilogue writes act(bias) by itself
@@ -751,13 +743,15 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
           const int blocks = rank_blocks * adapters;
           for (int b = blocks * part / parts; b < blocks * (part + 1) / parts; ++b) {
             const int steps = min(kLoraRanks, p.R - b / adapters * kLoraRanks) > kUmmaK ? 2 : 1;
-            if (!mbar_wait_cluster(&hfull_bar[hb], hphase, abort_flag)) {   // `up` has landed, h is built
+            // `up` has landed, h is in place
+            if (!mbar_wait_cluster(&built_bar[stage], (built_par >> stage) & 1u, abort_flag)) {
               ok = false;
               break;
             }
+            built_par ^= 1u << stage;
             tc_fence_after();
             const uint32_t w0 = smem_u32(sW + stage * Plan::kWBytes);
-            const uint32_t h0 = smem_u32(sH + hb * Plan::kTBytes);
+            const uint32_t h0 = smem_u32(sT + stage * Plan::kTBytes);
             for (int j = 0; j < steps; ++j) {
               const uint64_t wd = smem_desc_sw128(w0 + j * u_kstep, u_lbo, 1024);
 #pragma unroll
@@ -766,10 +760,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
               }
             }
             mma_commit<CG>(&empty_bar[stage]);
-            mma_commit<CG>(&hempty_bar[hb]);
             if (++stage == STAGES) stage = 0;
-            hb ^= 1;
-            if (hb == 0) hphase ^= 1u;
           }
         }
         if (!ok) break;
@@ -800,9 +791,9 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
     const uint32_t group_bar = 2u + static_cast<uint32_t>(eg);
     const bool bf16 = p.bf16 != 0;
     const uint32_t tempty_remote0 = (CG == 2) ? mapa_shared(smem_u32(&tempty_bar[0]), 0) : 0u;
-    const uint32_t hfull_remote0 = (CG == 2) ? mapa_shared(smem_u32(&hfull_bar[0]), 0) : 0u;
-    int hb = 0, hcount = 0, stage = 0;
-    uint32_t hphase = 0, land_par = 0;
+    const uint32_t built_remote0 = (CG == 2) ? mapa_shared(smem_u32(&built_bar[0]), 0) : 0u;
+    int stage = 0;
+    uint32_t land_par = 0;
     if constexpr (LORA) griddep_wait();
     if (p.zero_rest) zero_rows(p, grp_rows[0], grp_rows[p.E], et, 32 * kGrpEpiWarps);
     int acc = 0, turn = 0;
@@ -833,12 +824,12 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
       int b0 = 0, b1 = 0;   // this piece's adapter blocks
       if constexpr (LORA) {
         // adapter rows of this CTA's share of the tile: thread gt of a group
-        // builds its half (hi or lo) of row gt
+        // builds row gt of every other block
         list = p.lists + static_cast<long long>(u.rt) * kAdapterListPitch;
         const int adapters = list[0];
         b0 = rank_blocks * adapters * part / parts;
         b1 = rank_blocks * adapters * (part + 1) / parts;
-        const bool mixed = adapters > 1 || list[kAdapterListPitch - 1] > 0;
+        const bool mixed = adapters > 1 || list[1] > 0;
         const int half = u.nmma / CG;
         const int tr = rank * half + gt;   // row of the tile
         bool bad = false;
@@ -846,42 +837,47 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
             (gt < half && tr < u.rows) ? adapter_of(p.adapter, p.adapter64, u.row0 + tr, p.L, bad) : -1;
         const float* hrow = p.h + static_cast<long long>(u.row0 + tr) * p.h_pitch;
         stage = (stage + kb1 - kb0) % STAGES;
-        uint4 own[4];
+        uint4 own[8];
         int have = -1;   // rank block held in `own`
+        int rb = adapters ? b0 / adapters : 0, ai = b0 - rb * adapters;
+        int next = b0 < b1 ? list[kAdapterIds + ai] : 0;   // one block ahead of its use
         for (int b = b0; b < b1; ++b) {
-          const int rb = b / adapters, ai = b - rb * adapters;
-          if (rb != have) {
-            if (mine >= 0) split_ranks(hrow + rb * kLoraRanks, p.h_pitch - rb * kLoraRanks, eg != 0, bf16, own);
-            have = rb;
-          }
-          got = (hcount < 2 || mbar_wait(&hempty_bar[hb], hphase ^ 1u, abort_flag)) &&
-                mbar_wait(&land_bar[stage], (land_par >> stage) & 1u, abort_flag);
-          got = __all_sync(0xffffffffu, got) != 0;
-          if (!got) break;
-          land_par ^= 1u << stage;
-          if (mixed && clear_nonfinite(sW + stage * Plan::kWBytes, col, eg, p.up_kmaj != 0, bf16)) odd_flags[turn] = 1;
-          if (gt < half) {
-            const bool is = mine >= 0 && list[1 + ai] == mine;
-            uint8_t* dst = sH + hb * Plan::kTBytes + gt * 128;
+          const int a = next;
+          if (b + 1 < b1) next = list[kAdapterIds + (ai + 1 == adapters ? 0 : ai + 1)];
+          if (((b - b0) & 1) == eg) {
+            if (rb != have) {
+              if (mine >= 0) split_ranks(hrow + rb * kLoraRanks, p.h_pitch - rb * kLoraRanks, bf16, own);
+              have = rb;
+            }
+            const bool is = mine >= 0 && a == mine;
+            // the producer waited for the slot to be free before it loaded `up`
+            got = mbar_wait(&land_bar[stage], (land_par >> stage) & 1u, abort_flag);
+            got = __all_sync(0xffffffffu, got) != 0;
+            if (!got) break;
+            if (mixed && clear_nonfinite(sW + stage * Plan::kWBytes, gt, p.up_kmaj != 0, bf16)) odd_flags[turn] = 1;
+            if (gt < half) {
+              uint8_t* dst = sT + stage * Plan::kTBytes + gt * 128;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              *reinterpret_cast<uint4*>(dst + (((4 * eg + c) ^ (gt & 7)) << 4)) =
-                  is ? own[c] : make_uint4(0u, 0u, 0u, 0u);
+              for (int c = 0; c < 8; ++c) {
+                *reinterpret_cast<uint4*>(dst + ((c ^ (gt & 7)) << 4)) = is ? own[c] : make_uint4(0u, 0u, 0u, 0u);
+              }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (CG == 1) {
+                mbar_arrive(&built_bar[stage]);
+              } else {
+                mbar_arrive_cluster(built_remote0 + static_cast<uint32_t>(stage * 8));
+              }
             }
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            if constexpr (CG == 1) {
-              mbar_arrive(&hfull_bar[hb]);
-            } else {
-              mbar_arrive_cluster(hfull_remote0 + static_cast<uint32_t>(hb * 8));
-            }
+          if (++ai == adapters) {
+            ai = 0;
+            ++rb;
           }
+          land_par ^= 1u << stage;
           if (++stage == STAGES) stage = 0;
-          ++hcount;
-          hb ^= 1;
-          if (hb == 0) hphase ^= 1u;
         }
         // the next tile's flag; its last readers passed the barrier before this one
         if (et == 0) odd_flags[turn == 2 ? 0 : turn + 1] = 0;

@@ -10,14 +10,14 @@
 // one tile that pick different weights.  Hence mma.sync fragments (16 ranks x
 // 8 rows x 16 K) loaded straight from global memory, with no shared-memory
 // staging and no barrier in the loop: every warp owns 32-wide K slices and
-// runs on its own.  tcgen05 would need 128 TMEM lanes for R = 8..64 ranks and
-// one tile per adapter.
+// runs on its own, the next slice's loads (of the next adapter too) in flight
+// behind the current one's MMAs.  tcgen05 would need 128 TMEM lanes for R =
+// 8..64 ranks and one tile per adapter; the tensor pipe is busy 5% here.
 //
-//  * a cluster of up to 8 CTAs x 8 warps shares the K range of a tile of TT
-//    rows; warp w of CTA c takes the 32-element slices c * 8 + w, + 64, ...
-//  * the rows of the tile are ordered by adapter (a stable rank count in
-//    shared memory); chunks of up to 8 * NT8 rows of one adapter are the MMA
-//    N, the ranks are the MMA M;
+//  * a cluster of up to 8 CTAs x 8 warps shares the K range of a tile of up to
+//    8 rows; warp w of CTA c takes the 32-element slices c * 8 + w, + 64, ...
+//  * the rows of a tile are ordered by adapter; chunks of up to 8 * NT8 rows
+//    of one adapter are the MMA N, the ranks are the MMA M;
 //  * both operands need 8 adjacent K elements per lane.  The order of K inside
 //    an MMA does not matter as long as both agree, so lane q of a quad takes
 //    elements 8q .. 8q + 7 of the slice: one 16-byte load per row of x, and
@@ -28,8 +28,14 @@
 //    warps -> over the cluster through distributed shared memory, always in
 //    the same order.  No workspace, no atomics.
 //
-// The kernel also lists the distinct adapters of each row tile of the second
-// kernel, which needs one pass over `up` per listed adapter.
+// That form is for few rows, where every load is its own latency.  With many
+// rows (lora_shrink_wide) it took 47 us at 4096 x 4096, rank 64 -- one step's
+// loads in flight per warp, and `down` read again for every 32 rows -- so
+// there a CTA takes 256 rows and brings x and `down` through a ring in shared
+// memory by cp.async; see below.
+//
+// Clusters past the last row tile list the distinct adapters of each row tile
+// of the second kernel, which needs one pass over `up` per listed adapter.
 #pragma once
 #include "sm100_ptx.cuh"
 
@@ -39,7 +45,11 @@ constexpr int kShrinkWarps = 8;
 constexpr int kShrinkThreads = 32 * kShrinkWarps;
 constexpr int kShrinkSlice = 32;        // K elements per warp step: two MMAs deep
 constexpr int kShrinkMaxRows = 32;      // rows of a tile
-constexpr int kAdapterListPitch = 260;  // count, up to 256 adapters of a 256-row tile, ..., rows without one
+static_assert(kShrinkMaxRows == 32, "one lane per row of a tile");
+// The adapters of a row tile: their count, the number of rows without one, and
+// from kAdapterIds on up to 256 adapters.
+constexpr int kAdapterIds = 4;
+constexpr int kAdapterListPitch = kAdapterIds + 256;
 
 struct ShrinkParams {
   const unsigned short* x;
@@ -52,12 +62,22 @@ struct ShrinkParams {
   float* h;             // [T, h_pitch]
   int h_pitch;
   int T, K, L, R;
-  int tile_rows;        // TT <= kShrinkMaxRows
-  int x_vec, down_vec;  // rows 16-byte aligned / rank vectors aligned
+  int tile_rows;        // rows of a cluster
+  int tiles;            // clusters that cover the rows
   int* lists;           // [list_tiles, kAdapterListPitch]
   int list_tiles, list_rows;
   int* err;
 };
+
+// 16-rank tiles of a block, and the pitch of h (whole blocks).
+inline int shrink_rank_tiles(int64_t R) { return R <= 16 ? 1 : (R <= 32 ? 2 : 4); }
+inline int64_t shrink_pitch(int64_t R) {
+  const int64_t block = 16 * shrink_rank_tiles(R);
+  return (R + block - 1) / block * block;
+}
+
+// Launches the kernel on rows of x that are 16-byte aligned (gemm_lora_shrink.cu).
+int launch_shrink(const ShrinkParams& p, bool kmaj, bool bf16, cudaStream_t stream);
 
 // adapter[t], or -1 for none.  An index past the last adapter counts as none.
 __device__ __forceinline__ int adapter_of(const void* adapter, int adapter64, long long t, int L, bool& bad) {
@@ -84,75 +104,102 @@ __device__ __forceinline__ void mma_m16n8k16(float (&c)[4], uint32_t a0, uint32_
 }
 
 // 8 adjacent elements src[0..7] as four words; positions at or past `valid`
-// read as zero.
-__device__ __forceinline__ uint4 load8(const unsigned short* src, int valid, bool vec) {
-  if (valid >= 8 && vec) return *reinterpret_cast<const uint4*>(src);
-  uint32_t h[8];
+// read as zero.  VEC: src is 16-byte aligned and `valid` is 8 or more, or 0
+// or less.
+template <bool VEC>
+__device__ __forceinline__ uint4 load8(const unsigned short* src, int valid) {
+  if constexpr (VEC) {
+    return valid > 0 ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
+  } else {
+    uint32_t h[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) h[i] = i < valid ? src[i] : 0u;
-  return make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
+    for (int i = 0; i < 8; ++i) h[i] = i < valid ? src[i] : 0u;
+    return make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
+  }
 }
 
-// The `down` fragments of one slice: a[m][half] holds rank (m, half) of this
-// lane's quad row for its 8 K elements.
-template <int RT, bool KMAJ>
-__device__ __forceinline__ void load_down(const ShrinkParams& p, const unsigned short* d, int r0, int k, int g,
-                                          uint4 (&a)[RT][2]) {
+// The operands of one slice as they were loaded.  KMAJ (`down` stored R x K):
+// d[2 m + half] holds rank (m, half) of this lane's quad row for its 8 K
+// elements.  Else d holds, for each of the 8 K elements, the 2 RT adjacent
+// ranks of this lane, packed.
+template <int RT, int NT8>
+struct Slice {
+  uint4 d[2 * RT];
+  uint4 x[NT8];
+};
+
+template <int RT, int NT8, bool KMAJ, bool VEC>
+__device__ __forceinline__ void load_slice(const ShrinkParams& p, const unsigned short* d, const int (&xrow)[NT8],
+                                           int r0, int k, int g, Slice<RT, NT8>& s) {
   const int kv = p.K - k;   // valid elements from k on (may exceed 8, or be negative)
   if constexpr (KMAJ) {
 #pragma unroll
-    for (int m = 0; m < RT; ++m) {
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int r = r0 + m * 16 + half * 8 + g;
-        a[m][half] = r < p.R ? load8(d + r * p.ld_down + k, kv, p.down_vec != 0) : make_uint4(0u, 0u, 0u, 0u);
-      }
+    for (int i = 0; i < 2 * RT; ++i) {
+      const int r = r0 + i * 8 + g;
+      s.d[i] = load8<VEC>(d + r * p.ld_down + k, r < p.R ? kv : 0);
     }
   } else {
-    constexpr int V = 2 * RT;   // adjacent ranks of this lane: r0 + V g ..
+    constexpr int V = 2 * RT;   // ranks r0 + V g ..
     const int r = r0 + V * g;
-    unsigned short e[8][V];
+    uint32_t w[8 * RT];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const unsigned short* src = d + (k + j) * p.ld_down + r;
-      if (j < kv && p.down_vec && r + V <= p.R) {
-        if constexpr (V == 2) {
-          const ushort2 w = *reinterpret_cast<const ushort2*>(src);
-          e[j][0] = w.x;
-          e[j][1] = w.y;
-        } else if constexpr (V == 4) {
-          const ushort4 w = *reinterpret_cast<const ushort4*>(src);
-          e[j][0] = w.x;
-          e[j][1] = w.y;
-          e[j][2] = w.z;
-          e[j][3] = w.w;
+      if constexpr (VEC) {   // aligned to V elements, R a multiple of V
+        const bool in = j < kv && r < p.R;
+        if constexpr (RT == 1) {
+          w[j] = in ? *reinterpret_cast<const uint32_t*>(src) : 0u;
+        } else if constexpr (RT == 2) {
+          const uint2 v = in ? *reinterpret_cast<const uint2*>(src) : make_uint2(0u, 0u);
+          w[2 * j] = v.x;
+          w[2 * j + 1] = v.y;
         } else {
-          const uint4 w = *reinterpret_cast<const uint4*>(src);
-          const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int i = 0; i < V; ++i) e[j][i] = static_cast<unsigned short>(ww[i / 2] >> (16 * (i & 1)));
+          const uint4 v = in ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
+          w[4 * j] = v.x;
+          w[4 * j + 1] = v.y;
+          w[4 * j + 2] = v.z;
+          w[4 * j + 3] = v.w;
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) e[j][i] = (j < kv && r + i < p.R) ? src[i] : static_cast<unsigned short>(0);
+        for (int i = 0; i < RT; ++i) {
+          const uint32_t lo = (j < kv && r + 2 * i < p.R) ? src[2 * i] : 0u;
+          const uint32_t hi = (j < kv && r + 2 * i + 1 < p.R) ? src[2 * i + 1] : 0u;
+          w[j * RT + i] = lo | (hi << 16);
+        }
       }
     }
 #pragma unroll
-    for (int m = 0; m < RT; ++m) {
+    for (int i = 0; i < 2 * RT; ++i) s.d[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  }
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int i = 2 * m + half;
-        a[m][half] = make_uint4(e[0][i] | (static_cast<uint32_t>(e[1][i]) << 16),
-                                e[2][i] | (static_cast<uint32_t>(e[3][i]) << 16),
-                                e[4][i] | (static_cast<uint32_t>(e[5][i]) << 16),
-                                e[6][i] | (static_cast<uint32_t>(e[7][i]) << 16));
-      }
-    }
+  for (int j = 0; j < NT8; ++j) {
+    s.x[j] = load8<VEC>(p.x + static_cast<long long>(max(xrow[j], 0)) * p.ldx + k, xrow[j] >= 0 ? kv : 0);
+  }
+}
+
+// MMA A fragments (row g, row g + 8) of rank tile m: four K pairs each.
+template <int RT, int NT8, bool KMAJ>
+__device__ __forceinline__ void rank_fragments(const Slice<RT, NT8>& s, int m, uint4& lo, uint4& hi) {
+  if constexpr (KMAJ) {
+    lo = s.d[2 * m];
+    hi = s.d[2 * m + 1];
+  } else {
+    // word m of element j holds ranks (2m, 2m + 1) of the lane: pair elements
+    auto word = [&](int j) {
+      const int at = j * RT + m;
+      const uint4 v = s.d[at / 4];
+      return at % 4 == 0 ? v.x : (at % 4 == 1 ? v.y : (at % 4 == 2 ? v.z : v.w));
+    };
+    lo = make_uint4(__byte_perm(word(0), word(1), 0x5410), __byte_perm(word(2), word(3), 0x5410),
+                    __byte_perm(word(4), word(5), 0x5410), __byte_perm(word(6), word(7), 0x5410));
+    hi = make_uint4(__byte_perm(word(0), word(1), 0x7632), __byte_perm(word(2), word(3), 0x7632),
+                    __byte_perm(word(4), word(5), 0x7632), __byte_perm(word(6), word(7), 0x7632));
   }
 }
 
 // Distinct adapters of rows [row0, row0 + n), n <= 256, in order of their
-// first row: list[0] = count, list[1..].  Called by all threads.
+// first row.  Called by all threads.
 __device__ __forceinline__ void list_adapters(const ShrinkParams& p, int row0, int n, int* list, int* ids,
                                               int* warp_counts) {
   const int tid = static_cast<int>(threadIdx.x);
@@ -162,29 +209,37 @@ __device__ __forceinline__ void list_adapters(const ShrinkParams& p, int row0, i
   if (bad) atomicOr(p.err, kDevErrBadAdapter);
   __syncthreads();
   bool first = a >= 0;
-  for (int i = 0; i < tid && first; ++i) first = ids[i] != a;
+#pragma unroll 1
+  for (int i = 0; i < (tid & ~31) && first; i += 4) {   // earlier warps' rows, four at a time
+    const int4 v = *reinterpret_cast<const int4*>(ids + i);
+    first = v.x != a && v.y != a && v.z != a && v.w != a;
+  }
+  const unsigned same = __match_any_sync(0xffffffffu, a);   // rows of this warp with the same adapter
+  first = first && (same & ((1u << (tid & 31)) - 1u)) == 0u;
   const unsigned vote = __ballot_sync(0xffffffffu, first);
   if ((tid & 31) == 0) warp_counts[tid >> 5] = __popc(vote);
   __syncthreads();
   int at = __popc(vote & ((1u << (tid & 31)) - 1u));
   for (int w = 0; w < (tid >> 5); ++w) at += warp_counts[w];
-  if (first) list[1 + at] = a;
+  if (first) list[kAdapterIds + at] = a;
   if (tid == 0) {
     int total = 0;
     for (int w = 0; w < kShrinkWarps; ++w) total += warp_counts[w];
     list[0] = total;
   }
   const int without = __syncthreads_count(tid < n && a < 0);
-  if (tid == 0) list[kAdapterListPitch - 1] = without;
+  if (tid == 0) list[1] = without;
 }
 
-// grid.x: tiles x cluster size (the cluster is along x); grid.y: blocks of 16 RT ranks.
-template <int RT, int NT8, bool KMAJ, bool BF16>
+// grid.x: (tiles + list tiles) x cluster size (the cluster is along x);
+// grid.y: blocks of 16 RT ranks.
+template <int RT, int NT8, bool KMAJ, bool BF16, bool VEC>
 __global__ void __launch_bounds__(kShrinkThreads) lora_shrink(const __grid_constant__ ShrinkParams p) {
   constexpr int RB = 16 * RT;
   extern __shared__ float red[];   // [kShrinkWarps][tile_rows][RB]
-  __shared__ int ids[kShrinkThreads];
+  __shared__ __align__(16) int ids[kShrinkThreads];
   __shared__ int order[kShrinkMaxRows];
+  __shared__ int order_id[kShrinkMaxRows];
   __shared__ int warp_counts[kShrinkWarps];
   __shared__ int active_s;
   const int tid = static_cast<int>(threadIdx.x);
@@ -193,49 +248,64 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink(const __grid_const
   const int crank = static_cast<int>(cluster_ctarank());
   const int tile = static_cast<int>(blockIdx.x) / cs;
   const int r0 = static_cast<int>(blockIdx.y) * RB;
-  const int row0 = tile * p.tile_rows;
-  const int rows = min(p.tile_rows, p.T - row0);
+  const int slices = (p.K + kShrinkSlice - 1) / kShrinkSlice;
 
   griddep_wait();
   // Everything before this grid is complete now, so the second kernel may
   // start reading x and W; it waits for this grid before it reads h.
   griddep_launch_dependents();
 
-  if (tile < p.list_tiles && crank == 0 && blockIdx.y == 0) {
-    const int first = tile * p.list_rows;
-    list_adapters(p, first, min(p.list_rows, p.T - first), p.lists + static_cast<long long>(tile) * kAdapterListPitch,
-                  ids, warp_counts);
-    __syncthreads();
+  if (tile >= p.tiles) {
+    const int first = (tile - p.tiles) * p.list_rows;
+    if (crank == 0 && blockIdx.y == 0) {
+      list_adapters(p, first, min(p.list_rows, p.T - first),
+                    p.lists + static_cast<long long>(tile - p.tiles) * kAdapterListPitch, ids, warp_counts);
+    }
+    return;
   }
-  // rows of the tile ordered by adapter, those without one left out
-  if (tid < 32) {
+  // rows of the tile ordered by adapter (stable), those without one left out
+  const int row0 = tile * p.tile_rows;
+  if (warp == 0) {
+    const int rows = min(p.tile_rows, p.T - row0);
     bool bad = false;
-    const int a = tid < rows ? adapter_of(p.adapter, p.adapter64, row0 + tid, p.L, bad) : -1;
-    ids[tid] = a;
-    __syncwarp();
+    const int a = lane < rows ? adapter_of(p.adapter, p.adapter64, row0 + lane, p.L, bad) : -1;
     int at = 0;
-    for (int i = 0; i < rows; ++i) at += (ids[i] >= 0) && (ids[i] < a || (ids[i] == a && i < tid));
-    if (a >= 0) order[at] = tid;
+#pragma unroll
+    for (int i = 0; i < kShrinkMaxRows; ++i) {
+      const int o = __shfl_sync(0xffffffffu, a, i);
+      at += (o >= 0 && (o < a || (o == a && i < lane))) ? 1 : 0;
+    }
+    if (a >= 0) {
+      order[at] = lane;
+      order_id[at] = a;
+    }
     const unsigned vote = __ballot_sync(0xffffffffu, a >= 0);
-    if (tid == 0) active_s = __popc(vote);
+    if (lane == 0) active_s = __popc(vote);
   }
   __syncthreads();
   const int active = active_s;
   float* mine = red + static_cast<size_t>(warp) * p.tile_rows * RB;
-  const int slices = (p.K + kShrinkSlice - 1) / kShrinkSlice;
 
-  for (int c0 = 0; c0 < active;) {
-    const int a = ids[order[c0]];
-    int c1 = c0 + 1;
-    while (c1 < active && c1 < c0 + 8 * NT8 && ids[order[c1]] == a) ++c1;
-    const unsigned short* d = p.down + static_cast<long long>(a) * p.stride_down;
-    const unsigned short* xr[NT8];
+  // This warp's steps: every chunk of rows, and in it this warp's slices.
+  const int s_first = crank * kShrinkWarps + warp, s_step = cs * kShrinkWarps;
+  int c0 = 0, c1 = 0;            // rows of the chunk being loaded, in sorted order
+  const unsigned short* d = nullptr;
+  int xrow[NT8];
+  auto open_chunk = [&](int at) {
+    c0 = c1 = at;
+    if (at >= active) return false;
+    const int a = order_id[at];
+    while (c1 < active && c1 < c0 + 8 * NT8 && order_id[c1] == a) ++c1;
+    d = p.down + static_cast<long long>(a) * p.stride_down;
 #pragma unroll
     for (int j = 0; j < NT8; ++j) {
       const int i = c0 + j * 8 + g;
-      xr[j] = i < c1 ? p.x + static_cast<long long>(row0 + order[i]) * p.ldx : nullptr;
+      xrow[j] = i < c1 ? row0 + order[i] : -1;
     }
-    float acc[RT][NT8][4];
+    return true;
+  };
+  float acc[RT][NT8][4];
+  auto clear = [&] {
 #pragma unroll
     for (int m = 0; m < RT; ++m) {
 #pragma unroll
@@ -244,27 +314,9 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink(const __grid_const
         for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.0f;
       }
     }
-#pragma unroll 2
-    for (int s = crank * kShrinkWarps + warp; s < slices; s += cs * kShrinkWarps) {
-      const int k = s * kShrinkSlice + q * 8;
-      uint4 da[RT][2];
-      load_down<RT, KMAJ>(p, d, r0, k, g, da);
-      uint4 xb[NT8];
-#pragma unroll
-      for (int j = 0; j < NT8; ++j) {
-        xb[j] = xr[j] != nullptr ? load8(xr[j] + k, p.K - k, p.x_vec != 0) : make_uint4(0u, 0u, 0u, 0u);
-      }
-#pragma unroll
-      for (int j = 0; j < NT8; ++j) {
-        if (j > 0 && c0 + j * 8 >= c1) break;
-#pragma unroll
-        for (int m = 0; m < RT; ++m) {
-          mma_m16n8k16<BF16>(acc[m][j], da[m][0].x, da[m][1].x, da[m][0].y, da[m][1].y, xb[j].x, xb[j].y);
-          mma_m16n8k16<BF16>(acc[m][j], da[m][0].z, da[m][1].z, da[m][0].w, da[m][1].w, xb[j].z, xb[j].w);
-        }
-      }
-    }
-    // accumulator (rank row g / g + 8, row of x 2q / 2q + 1) -> mine[sorted row][rank]
+  };
+  // accumulator (rank row g / g + 8, row of x 2q / 2q + 1) -> mine[sorted row][rank]
+  auto flush = [&](int f0, int f1) {
 #pragma unroll
     for (int m = 0; m < RT; ++m) {
 #pragma unroll
@@ -272,13 +324,55 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink(const __grid_const
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int half = i >> 1;
-          const int at = c0 + j * 8 + 2 * q + (i & 1);
+          const int at = f0 + j * 8 + 2 * q + (i & 1);
           const int r = KMAJ ? m * 16 + half * 8 + g : 2 * RT * g + 2 * m + half;
-          if (at < c1) mine[at * RB + r] = acc[m][j][i];
+          if (at < f1) mine[at * RB + r] = acc[m][j][i];
         }
       }
     }
-    c0 = c1;
+  };
+  clear();
+  if (s_first < slices) {
+    Slice<RT, NT8> buf[2];
+    bool have = open_chunk(0);
+    int s = s_first;
+    auto load = [&](Slice<RT, NT8>& to) {
+      load_slice<RT, NT8, KMAJ, VEC>(p, d, xrow, r0, s * kShrinkSlice + q * 8, g, to);
+    };
+    // loads the step after `cur` into `next`, then multiplies `cur`
+    auto step = [&](const Slice<RT, NT8>& cur, Slice<RT, NT8>& next) {
+      const int f0 = c0, f1 = c1;
+      s += s_step;
+      const bool last = s >= slices;   // of this chunk
+      if (last) {
+        s = s_first;
+        have = open_chunk(c1);
+      }
+      if (have) load(next);
+#pragma unroll
+      for (int m = 0; m < RT; ++m) {
+        uint4 lo, hi;
+        rank_fragments<RT, NT8, KMAJ>(cur, m, lo, hi);
+#pragma unroll
+        for (int j = 0; j < NT8; ++j) {
+          if (j == 0 || f0 + j * 8 < f1) {
+            mma_m16n8k16<BF16>(acc[m][j], lo.x, hi.x, lo.y, hi.y, cur.x[j].x, cur.x[j].y);
+            mma_m16n8k16<BF16>(acc[m][j], lo.z, hi.z, lo.w, hi.w, cur.x[j].z, cur.x[j].w);
+          }
+        }
+      }
+      if (last) {
+        flush(f0, f1);
+        clear();
+      }
+    };
+    if (have) load(buf[0]);
+    while (have) {   // two buffers in turn: a copy would wait for the loads
+      step(buf[0], buf[1]);
+      if (have) step(buf[1], buf[0]);
+    }
+  } else {
+    for (bool have = open_chunk(0); have; have = open_chunk(c1)) flush(c0, c1);   // no slice: zeros
   }
   __syncthreads();
   // over the warps, in place of the first warp's partial
@@ -289,20 +383,215 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink(const __grid_const
     red[e] = v;
   }
   // over the cluster: CTA c finishes every cs-th element
-  cluster_sync();
+  if (cs > 1) cluster_sync();
+  else __syncthreads();
   const uint32_t base = smem_u32(red);
   for (int e = tid * cs + crank; e < active * RB; e += kShrinkThreads * cs) {
     float v = 0.0f;
-    for (int c = 0; c < cs; ++c) {
-      float o;
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o) : "r"(mapa_shared(base + e * 4, c)));
-      v += o;
-    }
-    const int t = order[e / RB];
-    const float s = p.scale != nullptr ? p.scale[ids[t]] : 1.0f;
-    p.h[static_cast<long long>(row0 + t) * p.h_pitch + r0 + e % RB] = v * s;
+    for (int c = 0; c < cs; ++c) v += ld_dsmem_f32(mapa_shared(base + e * 4, c));
+    const int at = e / RB;
+    const float scale = p.scale != nullptr ? p.scale[order_id[at]] : 1.0f;
+    p.h[static_cast<long long>(row0 + order[at]) * p.h_pitch + r0 + e % RB] = v * scale;
   }
-  cluster_sync();   // no CTA leaves while a peer may still read its partials
+  if (cs > 1) cluster_sync();   // no CTA leaves while a peer may still read its partials
+}
+
+// ------------------------------------------------------------------- many rows
+//
+// A CTA owns 256 rows and 64 ranks, the CTAs of a cluster share K in blocks of
+// 64.  Each distinct adapter of the rows is one pass over this CTA's K blocks:
+// x [256 x 64] and down[a] [64 x 64] arrive by cp.async in a ring of kWideStages
+// (40 KiB each, rows of 128 bytes with their 16-byte chunks swizzled by the
+// row, so that ldmatrix reads them without conflicts), and each of the 8 warps
+// multiplies its 32 rows unless none of them picked the adapter.  The rows
+// that did keep the result.  What it moves: x once per distinct adapter of a
+// tile (once, for long prompts), `down` once per 256 rows.
+constexpr int kWideRows = 256;
+constexpr int kWideRanks = 64;
+constexpr int kWideK = 64;
+constexpr int kWideStages = 3;
+constexpr int kWideXBytes = kWideRows * 128;
+constexpr int kWideStageBytes = kWideXBytes + kWideRanks * 128;
+constexpr int kWideSumBytes = kWideRows * kWideRanks * 4;
+constexpr int kWideBytes = kWideStages * kWideStageBytes + kWideSumBytes;
+
+// 16 bytes of which `valid` bytes (0..16) come from src and the rest is zero.
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, int valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+template <bool TRANS>
+__device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
+  if constexpr (TRANS) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+  } else {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+  }
+}
+
+// Byte offset of 16-byte chunk c of row r in a tile of 128-byte rows.
+__device__ __forceinline__ uint32_t wide_at(int r, int c) { return static_cast<uint32_t>(r * 128 + ((c ^ (r & 7)) << 4)); }
+
+// grid as lora_shrink's, tile_rows = 256; x and `down` rows 16-byte aligned.
+template <bool KMAJ, bool BF16>
+__global__ void __launch_bounds__(kShrinkThreads) lora_shrink_wide(const __grid_constant__ ShrinkParams p) {
+  extern __shared__ __align__(128) uint8_t wide_smem[];
+  __shared__ __align__(16) int ids[kShrinkThreads];
+  __shared__ int list[kAdapterListPitch];
+  __shared__ int warp_counts[kShrinkWarps];
+  const int tid = static_cast<int>(threadIdx.x);
+  const int warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+  const int cs = static_cast<int>(cluster_nctarank());
+  const int crank = static_cast<int>(cluster_ctarank());
+  const int tile = static_cast<int>(blockIdx.x) / cs;
+  const int r0 = static_cast<int>(blockIdx.y) * kWideRanks;
+  const int row0 = tile * kWideRows;
+
+  griddep_wait();
+  griddep_launch_dependents();   // see lora_shrink
+
+  if (tile >= p.tiles) {
+    const int first = (tile - p.tiles) * p.list_rows;
+    if (crank == 0 && blockIdx.y == 0) {
+      list_adapters(p, first, min(p.list_rows, p.T - first),
+                    p.lists + static_cast<long long>(tile - p.tiles) * kAdapterListPitch, ids, warp_counts);
+    }
+    return;
+  }
+  const int rows = min(kWideRows, p.T - row0);
+  list_adapters(p, row0, rows, list, ids, warp_counts);
+  __syncthreads();
+  const int adapters = list[0];
+  const int my_id = ids[tid];   // of row warp * 32 + lane
+  const uint32_t ring = smem_u32(wide_smem);
+  float* sums = reinterpret_cast<float*>(wide_smem + kWideStages * kWideStageBytes);   // [256][64]
+
+  const int blocks = (p.K + kWideK - 1) / kWideK;
+  const int kb0 = blocks * crank / cs, per = blocks * (crank + 1) / cs - kb0;
+  const int steps = adapters * per;
+  auto load = [&](int step) {   // x and down[a] of one step into its stage
+    const int a = list[kAdapterIds + step / per];
+    const int k0 = (kb0 + step % per) * kWideK;
+    const uint32_t sx = ring + static_cast<uint32_t>(step % kWideStages * kWideStageBytes), sd = sx + kWideXBytes;
+    const int c = tid & 7;
+    const int xv = max(0, min(8, p.K - k0 - c * 8)) * 2;   // valid bytes of this thread's chunks of x
+#pragma unroll
+    for (int i = 0; i < kWideRows / 32; ++i) {
+      const int r = i * 32 + (tid >> 3);
+      const bool in = r < rows && xv > 0;
+      const unsigned short* src = in ? p.x + static_cast<long long>(row0 + r) * p.ldx + k0 + c * 8 : p.x;
+      cp_async_16(sx + wide_at(r, c), src, in ? xv : 0);
+    }
+    const unsigned short* d = p.down + static_cast<long long>(a) * p.stride_down;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = i * 32 + (tid >> 3);   // KMAJ: a rank, its K chunks; else a K row, its rank chunks
+      int valid;
+      const unsigned short* src;
+      if constexpr (KMAJ) {
+        valid = r0 + r < p.R ? xv : 0;
+        src = d + static_cast<long long>(r0 + r) * p.ld_down + k0 + c * 8;
+      } else {
+        valid = k0 + r < p.K ? max(0, min(8, p.R - r0 - c * 8)) * 2 : 0;
+        src = d + static_cast<long long>(k0 + r) * p.ld_down + r0 + c * 8;
+      }
+      cp_async_16(sd + wide_at(r, c), valid > 0 ? src : p.x, valid);
+    }
+  };
+  for (int s = 0; s < kWideStages - 1; ++s) {
+    if (s < steps) load(s);
+    cp_async_commit();
+  }
+  float acc[4][4][4];   // [16 ranks][8 rows]
+  bool mine = false;    // a row of this warp picked the adapter
+  for (int step = 0; step < steps; ++step) {
+    cp_async_wait<kWideStages - 2>();
+    __syncthreads();   // every thread's part of this stage is in, and the stage about to be refilled is read
+    if (step + kWideStages - 1 < steps) load(step + kWideStages - 1);
+    cp_async_commit();
+    const int block = step % per;
+    if (block == 0) {
+      mine = __any_sync(0xffffffffu, my_id == list[kAdapterIds + step / per]);
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.0f;
+        }
+      }
+    }
+    if (mine) {
+      const uint32_t sx = ring + static_cast<uint32_t>(step % kWideStages * kWideStageBytes), sd = sx + kWideXBytes;
+#pragma unroll
+      for (int kk = 0; kk < kWideK / 16; ++kk) {
+        // B: 8 rows x 16 K per pair of 8x8 blocks; blocks (rows j, K lo), (j, K hi), (j + 1, K lo), (j + 1, K hi)
+        uint32_t xb[2][4];
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {
+          const int r = warp * 32 + jj * 16 + (lane & 7) + ((lane >> 4) << 3);
+          ldmatrix_x4<false>(sx + wide_at(r, kk * 2 + ((lane >> 3) & 1)), xb[jj]);
+        }
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          // A: blocks (ranks 0-7, K lo), (8-15, K lo), (0-7, K hi), (8-15, K hi)
+          uint32_t da[4];
+          if constexpr (KMAJ) {
+            const int r = m * 16 + (lane & 15);
+            ldmatrix_x4<false>(sd + wide_at(r, kk * 2 + (lane >> 4)), da);
+          } else {
+            const int k = kk * 16 + (lane & 7) + ((lane >> 4) << 3);
+            ldmatrix_x4<true>(sd + wide_at(k, m * 2 + ((lane >> 3) & 1)), da);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            mma_m16n8k16<BF16>(acc[m][j], da[0], da[1], da[2], da[3], xb[j >> 1][(j & 1) * 2], xb[j >> 1][(j & 1) * 2 + 1]);
+          }
+        }
+      }
+      if (block == per - 1) {
+        const int a = list[kAdapterIds + step / per];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int r = warp * 32 + j * 8 + 2 * q + i;
+            if (ids[r] == a) {
+#pragma unroll
+              for (int m = 0; m < 4; ++m) {
+                sums[r * kWideRanks + m * 16 + g] = acc[m][j][i];
+                sums[r * kWideRanks + m * 16 + 8 + g] = acc[m][j][i + 2];
+              }
+            }
+          }
+        }
+      }
+    }
+  }
+  // over the cluster: CTA c finishes every cs-th row
+  if (cs > 1) cluster_sync();
+  else __syncthreads();
+  const uint32_t base = smem_u32(sums);
+  const int e = tid & (kWideRanks - 1);
+  for (int r = (tid / kWideRanks) * cs + crank; r < rows; r += kShrinkThreads / kWideRanks * cs) {
+    const int a = ids[r];
+    if (a < 0 || r0 + e >= p.h_pitch) continue;
+    float v = 0.0f;
+    for (int c = 0; c < cs; ++c) v += ld_dsmem_f32(mapa_shared(base + (r * kWideRanks + e) * 4, c));
+    p.h[static_cast<long long>(row0 + r) * p.h_pitch + r0 + e] = v * (p.scale != nullptr ? p.scale[a] : 1.0f);
+  }
+  if (cs > 1) cluster_sync();   // no CTA leaves while a peer may still read its sums
 }
 
 }  // namespace idb

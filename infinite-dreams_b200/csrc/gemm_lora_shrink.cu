@@ -1,0 +1,95 @@
+// Launcher of lora_shrink (gemm_lora_kernel.cuh): picks the compiled variant
+// and the grid.
+#include <atomic>
+
+#include "../../include/gemm_sm100.h"
+#include "gemm_capi_shared.h"
+#include "gemm_lora_kernel.cuh"
+
+namespace idb {
+namespace {
+
+using ShrinkFn = void (*)(ShrinkParams);
+
+constexpr int kWideFrom = 512;   // more rows than this take lora_shrink_wide
+
+template <int RT, bool VEC>
+ShrinkFn pick(bool kmaj, bool bf16) {
+  if (kmaj) return bf16 ? lora_shrink<RT, 1, true, true, VEC> : lora_shrink<RT, 1, true, false, VEC>;
+  return bf16 ? lora_shrink<RT, 1, false, true, VEC> : lora_shrink<RT, 1, false, false, VEC>;
+}
+
+ShrinkFn pick_wide(bool kmaj, bool bf16) {
+  if (kmaj) return bf16 ? lora_shrink_wide<true, true> : lora_shrink_wide<true, false>;
+  return bf16 ? lora_shrink_wide<false, true> : lora_shrink_wide<false, false>;
+}
+
+}  // namespace
+
+int launch_shrink(const ShrinkParams& sp, bool kmaj, bool bf16, cudaStream_t stream) {
+  ShrinkParams p = sp;
+  const int rt = shrink_rank_tiles(p.R);
+  const int elems = kmaj ? 8 : 2 * rt;   // of `down` per load
+  const bool vec = p.K % 8 == 0 && reinterpret_cast<uintptr_t>(p.down) % (2 * elems) == 0 && p.ld_down % elems == 0 &&
+                   p.stride_down % elems == 0 && (kmaj || p.R % elems == 0);
+  const bool aligned = reinterpret_cast<uintptr_t>(p.down) % 16 == 0 && p.ld_down % 8 == 0 && p.stride_down % 8 == 0;
+  ShrinkFn fn;
+  int cluster = 1, bytes, ranks;
+  if (p.T > kWideFrom && aligned) {
+    // 256 rows to a cluster, as many CTAs along K as keep to one per SM with
+    // at least 4 K blocks each.
+    p.tile_rows = kWideRows;
+    p.tiles = (p.T + kWideRows - 1) / kWideRows;
+    ranks = kWideRanks;
+    const int blocks = (p.K + kWideK - 1) / kWideK, all = p.tiles * ((p.R + ranks - 1) / ranks);
+    while (cluster < 8 && 8 * cluster <= blocks && 2 * cluster * all <= 148) cluster *= 2;
+    fn = pick_wide(kmaj, bf16);
+    bytes = kWideBytes;
+    static std::atomic<unsigned long long> configured[4];   // devices, per variant
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return capi_fail_cuda(e, "cudaGetDevice");
+    std::atomic<unsigned long long>& known = configured[kmaj * 2 + bf16];
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (!(known.load(std::memory_order_acquire) & bit)) {
+      e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+      if (e != cudaSuccess) return capi_fail_cuda(e, "adapter kernel attribute");
+      known.fetch_or(bit, std::memory_order_acq_rel);
+    }
+  } else {
+    // So few rows to a tile that about 256 CTAs share the work (T = 64: 2 rows
+    // x 32 clusters of 8), up to the 8 rows of one MMA; along K no more CTAs
+    // than give every warp a slice.
+    int rows = 1;
+    while (rows < 8 && rows * 32 < p.T) rows *= 2;
+    p.tile_rows = rows;
+    p.tiles = (p.T + rows - 1) / rows;
+    ranks = 16 * rt;
+    const int slices = (p.K + kShrinkSlice - 1) / kShrinkSlice;
+    while (cluster < 8 && cluster * kShrinkWarps < slices && cluster * p.tiles <= 150) cluster *= 2;
+    // operands without vector alignment take the element-wise loads
+    fn = rt == 1   ? (vec ? pick<1, true>(kmaj, bf16) : pick<1, false>(kmaj, bf16))
+         : rt == 2 ? (vec ? pick<2, true>(kmaj, bf16) : pick<2, false>(kmaj, bf16))
+                   : (vec ? pick<4, true>(kmaj, bf16) : pick<4, false>(kmaj, bf16));
+    bytes = kShrinkWarps * rows * ranks * static_cast<int>(sizeof(float));   // at most 16 KiB
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((p.tiles + p.list_tiles) * cluster),
+                     static_cast<unsigned>((p.R + ranks - 1) / ranks), 1);
+  cfg.blockDim = dim3(kShrinkThreads, 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(bytes);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, p);
+  return e == cudaSuccess ? GEMM_OK : capi_fail_cuda(e, "adapter kernel launch");
+}
+
+}  // namespace idb
