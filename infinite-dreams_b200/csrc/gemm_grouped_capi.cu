@@ -194,7 +194,11 @@ int launch_grouped(const Operand& a, const Operand& b, const Operand* up, const 
   std::memset(&maps, 0, sizeof(maps));
   int st = GEMM_OK;
   if (p.K > 0) {
-    for (int i = 0; i < box_count(TM) && st == GEMM_OK; ++i) st = a.encode_rows(&maps.a[i], box_rows(TM, i), "A");
+    const int64_t most = std::min<int64_t>(round_up(p.T, Plan::kStep), TM) / CG;   // rows of a CTA
+    while (p.first_box + 1 < box_count(TM) && most <= box_rows(TM, p.first_box + 1)) ++p.first_box;
+    for (int i = p.first_box; i < box_count(TM) && st == GEMM_OK; ++i) {
+      st = a.encode_rows(&maps.a[i], box_rows(TM, i), "A");
+    }
     if (st == GEMM_OK) st = b.encode_weights(&maps.b, p.b_kmaj != 0, "B");
     p.b_wide = b.wide();
   }
@@ -256,7 +260,7 @@ struct LoraPlan {
   }
 };
 
-constexpr int kWgradStages = 5;
+constexpr int kWgradStages = 4;
 
 int launch_wgrad(const Operand& a, const Operand& g, const WgradParams& wp, int sms, cudaStream_t stream) {
   using Plan = WgradPlan<kWgradStages>;

@@ -90,6 +90,7 @@ struct GroupedParams {
   int T, N, K;
   int kb_total;      // ceil(K / 64)
   int tiles_n;       // ceil(N / (128 * CG))
+  int first_box;     // the largest box of A that T rows can need
   int b_kmaj;        // B[e] stored N x K
   int b_wide;        // stored K x N with N a multiple of 64: both 64-column atoms in one box
   int bf16;
@@ -558,7 +559,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
     fence_mbar_init();
   }
   if (warp == 0 && lane == 0) {
-    for (int i = 0; i < box_count(TM); ++i) prefetch_tmap(&maps.a[i]);
+    for (int i = p.first_box; i < box_count(TM); ++i) prefetch_tmap(&maps.a[i]);
     prefetch_tmap(&maps.b);
     if (LORA) prefetch_tmap(&maps.u);
     if (p.c_tma) prefetch_tmap(&maps.c);
@@ -611,7 +612,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
         const int arow = u.row0 + rank * half;
         const int bcol = (u.tn * CG + rank) * kGrpCols;
         // the smallest box that holds this CTA's rows
-        int box = 0;
+        int box = p.first_box;
         while (box + 1 < box_count(TM) && half <= box_rows(TM, box + 1)) ++box;
         const CUtensorMap* map_a = &maps.a[box];
         const uint32_t bytes = weights ? Plan::kWBytes : static_cast<uint32_t>(box_rows(TM, box)) * 128u;
@@ -806,7 +807,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
         if constexpr (CG == 1) {
           mbar_arrive(&tempty_bar[acc]);
         } else {
-          mbar_arrive_cluster(tempty_remote0 + static_cast<uint32_t>(acc * 8));
+          mbar_arrive_cluster_relaxed(tempty_remote0 + static_cast<uint32_t>(acc * 8));
         }
       }
       acc ^= 1;
@@ -868,7 +869,8 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
               if constexpr (CG == 1) {
                 mbar_arrive(&built_bar[stage]);
               } else {
-                mbar_arrive_cluster(built_remote0 + static_cast<uint32_t>(stage * 8));
+                fence_release_smem_cluster();
+                mbar_arrive_cluster_relaxed(built_remote0 + static_cast<uint32_t>(stage * 8));
               }
             }
           }
@@ -1104,7 +1106,7 @@ struct WgradPlan {
   static constexpr int kOffA = 0;
   static constexpr int kOffG = STAGES * kOpBytes;
   static constexpr int kOffOut = 2 * STAGES * kOpBytes;
-  static constexpr int kOffBar = kOffOut + kGrpEpiWarps * kOutBytes;
+  static constexpr int kOffBar = kOffOut + 2 * kGrpEpiWarps * kOutBytes;
   static constexpr int kNumBars = 4 * STAGES + 4 + 1;    // full, empty, land, fix, tmem_full[2], tmem_empty[2], done
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;
   static constexpr int kOffScan = kOffMisc + 16;
@@ -1372,7 +1374,10 @@ __global__ void __launch_bounds__(kWgradThreads, 1)
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&fix_bar[last]), 0));
+      if (lane == 0) {
+        fence_release_smem_cluster();
+        mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(&fix_bar[last]), 0));
+      }
     }
   } else {
     // ------------------------------------------------------------ epilogue
@@ -1380,17 +1385,16 @@ __global__ void __launch_bounds__(kWgradThreads, 1)
     const bool bf16 = p.bf16 != 0;
     const uint32_t tempty_remote0 = mapa_shared(smem_u32(&tempty_bar[0]), 0);
     const int half = (warp - 2) >> 2;      // column half of this warp: the two warps of a lane quarter share its rows
-    uint8_t* buf = sOut + (warp - 2) * Plan::kOutBytes;
+    uint8_t* bufs = sOut + (warp - 2) * 2 * Plan::kOutBytes;   // two staging boxes in turn
+    int turn = 0;
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
     for (int t = worker; t < num_tiles; t += workers) {
       const WgradUnit u = wgrad_unit(p, grp_rows, t);
       if (u.blocks > 0) {
-        bool got = true;
-        if (lane == 0) got = mbar_wait(&tfull_bar[acc], acc_phase, abort_flag);
-        got = __shfl_sync(0xffffffffu, got ? 1 : 0, 0) != 0;
-        ok = named_bar_and(1, 32 * kGrpEpiWarps, got);
+        // every warp for itself: nothing below waits for another epilogue warp
+        ok = __all_sync(0xffffffffu, mbar_wait(&tfull_bar[acc], acc_phase, abort_flag)) != 0;
         if (!ok) break;
         tc_fence_after();
       }
@@ -1415,28 +1419,30 @@ __global__ void __launch_bounds__(kWgradThreads, 1)
           for (int i = 0; i < 64; ++i) f[i] = 0.0f;
         }
         const bool whole = p.d_tma && (n0 + kStoreCols <= p.N || p.N % 8 == 0);
+        uint8_t* buf = bufs + turn * Plan::kOutBytes;
+        turn ^= 1;
+        // the store issued from this box two chunks ago has read it
         if (p.d_tma) {
-          if (lane == 0) bulk_wait_group_read<0>();
+          if (lane == 0) bulk_wait_group_read<1>();
           __syncwarp();
         }
+        auto stage_row = [&](bool b) {   // one conversion for two values
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          uint32_t w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            w[i] = to_16bit(f[8 * c + 2 * i], bf16) |
-                   (static_cast<uint32_t>(to_16bit(f[8 * c + 2 * i + 1], bf16)) << 16);
+          for (int c = 0; c < 8; ++c) {
+            *reinterpret_cast<uint4*>(buf + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+                make_uint4(pack_16bit(f[8 * c], f[8 * c + 1], b), pack_16bit(f[8 * c + 2], f[8 * c + 3], b),
+                           pack_16bit(f[8 * c + 4], f[8 * c + 5], b), pack_16bit(f[8 * c + 6], f[8 * c + 7], b));
           }
-          *reinterpret_cast<uint4*>(buf + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+        };
+        if (bf16) stage_row(true);
+        else stage_row(false);
         if (whole) fence_proxy_async_smem();
         __syncwarp();
-        if (whole) {
-          if (lane == 0) {
-            tma_store_3d(&tmD, buf, n0, m0, u.e);
-            bulk_commit_group();
-          }
-        } else {
+        if (p.d_tma && lane == 0) {
+          if (whole) tma_store_3d(&tmD, buf, n0, m0, u.e);
+          bulk_commit_group();   // empty when the box is stored below: the count above stays per box
+        }
+        if (!whole) {
           for (int r = 0; r < kStoreRows && m0 + r < p.M; ++r) {
             unsigned short* drow = out + static_cast<long long>(m0 + r) * p.ldd;
 #pragma unroll
@@ -1454,7 +1460,7 @@ __global__ void __launch_bounds__(kWgradThreads, 1)
       if (u.blocks > 0) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(tempty_remote0 + static_cast<uint32_t>(acc * 8));
+        if (lane == 0) mbar_arrive_cluster_relaxed(tempty_remote0 + static_cast<uint32_t>(acc * 8));
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1u;
       }

@@ -190,6 +190,21 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// The same without ordering this thread's memory accesses before it (a release
+// at cluster scope waits for every store in flight, TMA stores to global
+// memory included: 2000-3000 cycles in an epilogue).  For arrivals that hand
+// over what is not memory of the generic proxy, like a TMEM accumulator whose
+// loads have completed; for shared memory, after fence_release_smem_cluster.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// Orders this CTA's shared-memory writes (only those) before a later arrival
+// at cluster scope.
+__device__ __forceinline__ void fence_release_smem_cluster() {
+  asm volatile("fence.release.sync_restrict::shared::cta.cluster;" ::: "memory");
+}
+
 // ----------------------------------------------------------------- TMA
 __device__ __forceinline__ void prefetch_tmap(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
@@ -485,6 +500,16 @@ __device__ __forceinline__ uint32_t idesc_16bit(int m, int n, bool a_mn_major, b
 // fp32 -> the bits of the 16-bit type, rounded to nearest even, and back.
 __device__ __forceinline__ unsigned short to_16bit(float x, bool bf16) {
   return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(x)) : __half_as_ushort(__float2half_rn(x));
+}
+
+// Two of them, `lo` in the low half.
+__device__ __forceinline__ uint32_t pack_16bit(float lo, float hi, bool bf16) {
+  if (bf16) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&b);
+  }
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 __device__ __forceinline__ float from_16bit(unsigned short h, bool bf16) {

@@ -10,6 +10,7 @@
 //   gemm_ex(A, B, cfg_id, alpha, beta, C, bias, act, out) -> out
 //   grouped_gemm(A, B, offsets, bias, act, out) -> out
 //   grouped_gemm_wgrad(A, G, offsets, out) -> out
+//   grouped_linear(x, weight, offsets) -> y, differentiable
 //   lora_gemm(x, W, down, up, adapter, scale, bias, act, out) -> out
 //   reset_workspaces()
 #include <ATen/cuda/CUDAContext.h>
@@ -285,6 +286,43 @@ at::Tensor grouped_gemm_wgrad(const at::Tensor& A, const at::Tensor& G, const at
   return D;
 }
 
+// grouped_gemm as a differentiable function; grouped.py has the same in Python
+// for builds without this module.  In C++ because a small step's cost is the
+// work around its three launches.
+struct GroupedLinear : public torch::autograd::Function<GroupedLinear> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight,
+                            const at::Tensor& offsets) {
+    ctx->save_for_backward({x, weight, offsets});
+    const at::NoGradGuard no_grad;
+    return grouped_gemm(x, weight, offsets, c10::nullopt, GEMM_ACT_NONE, c10::nullopt);
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "grouped_linear can be differentiated once (no create_graph)");
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &x = saved[0], &weight = saved[1], &offsets = saved[2], &dy = grads[0];
+    at::Tensor dx, dw;
+    if (dy.defined()) {
+      if (ctx->needs_input_grad(0)) {
+        dx = grouped_gemm(dy, weight.transpose(1, 2), offsets, c10::nullopt, GEMM_ACT_NONE, c10::nullopt);
+      }
+      if (ctx->needs_input_grad(1)) {
+        c10::optional<at::Tensor> out;
+        if (weight.stride(1) == 1 && weight.stride(2) != 1) {   // stored N x K: so is its gradient
+          out = at::empty({weight.size(0), weight.size(2), weight.size(1)}, dy.options()).transpose(1, 2);
+        }
+        dw = grouped_gemm_wgrad(x, dy, offsets, out);
+      }
+    }
+    return {dx, dw, at::Tensor()};
+  }
+};
+
+at::Tensor grouped_linear(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& offsets) {
+  return GroupedLinear::apply(x, weight, offsets);
+}
+
 at::Tensor lora_gemm(const at::Tensor& x, const at::Tensor& W, const at::Tensor& down, const at::Tensor& up,
                      const at::Tensor& adapter, c10::optional<at::Tensor> scale, c10::optional<at::Tensor> bias,
                      int64_t act, c10::optional<at::Tensor> out) {
@@ -356,6 +394,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("out") = py::none());
   m.def("grouped_gemm_wgrad", &grouped_gemm_wgrad, "out[e] = A[rows of e].T @ G[rows of e]", py::arg("A"),
         py::arg("G"), py::arg("offsets"), py::arg("out") = py::none());
+  m.def("grouped_linear", &grouped_linear, "grouped_gemm, differentiable in x and weight", py::arg("x"),
+        py::arg("weight"), py::arg("offsets"));
   m.def("lora_gemm", &lora_gemm, "out[t] = act(x[t] @ W + scale[a] * (x[t] @ down[a]) @ up[a] + bias), a = adapter[t]",
         py::arg("x"), py::arg("W"), py::arg("down"), py::arg("up"), py::arg("adapter"), py::arg("scale") = py::none(),
         py::arg("bias") = py::none(), py::arg("act") = 0, py::arg("out") = py::none());

@@ -42,7 +42,10 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor)
     transposed view), offsets E + 1 row numbers on the device, as for
     ``infinite_dreams_ext.grouped_gemm``.  Rows outside the groups give zeros
     and receive zero gradients; an empty group's weight gradient is zero.
+    It can be differentiated once.
     """
+    if ext._fast is not None:
+        return ext._fast.grouped_linear(x, weight, offsets)
     return _GroupedLinear.apply(x, weight, offsets)
 
 

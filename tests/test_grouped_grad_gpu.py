@@ -225,3 +225,46 @@ def test_a_step_captured_and_replayed():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(o, w) for o, w in zip(outs, want)), counts
+
+
+def test_linear_in_both_bindings():
+    """The compiled function and the one in Python: the same bits, the same refusal of a second derivative."""
+    from infinite_dreams import infinite_dreams_ext as ext
+    from infinite_dreams.grouped import grouped_linear
+    off = counts_to_offsets([30, 0, 50])
+    x, W = randn((80, 72), torch.bfloat16, 1).requires_grad_(), stacked(3, 72, 88, torch.bfloat16, 2).requires_grad_()
+    dy = randn((80, 88), torch.bfloat16, 3)
+
+    def step():
+        y = grouped_linear(x, W, off)
+        return (y.detach(), *torch.autograd.grad(y, (x, W), dy))
+
+    def twice():
+        dx, = torch.autograd.grad(grouped_linear(x, W, off), x, dy.requires_grad_(), create_graph=True)
+        torch.autograd.grad(dx.sum(), W)
+
+    fast = step()
+    with pytest.raises(RuntimeError):
+        twice()
+    keep, ext._fast = ext._fast, None
+    try:
+        slow = step()
+        with pytest.raises(RuntimeError):
+            twice()
+    finally:
+        ext._fast = keep
+    assert all(torch.equal(f, s) for f, s in zip(fast, slow))
+    with torch.no_grad():
+        assert not grouped_linear(x, W, off).requires_grad
+
+
+def test_weights_as_parameters_of_a_module():
+    """Gradients accumulate into .grad over two backward passes, as an optimizer reads them."""
+    from infinite_dreams.grouped import grouped_linear
+    off = counts_to_offsets([20, 44])
+    W = torch.nn.Parameter(stacked(2, 64, 96, torch.float16, 1))
+    x, dy = randn((64, 64), torch.float16, 2), randn((64, 96), torch.float16, 3)
+    grouped_linear(x, W, off).backward(dy)
+    once = W.grad.clone()
+    grouped_linear(x, W, off).backward(dy)
+    assert torch.equal(W.grad, once + once)
