@@ -71,10 +71,8 @@ constexpr int kGrpRaster = 8;      // row tiles walked before the next column ti
 // L2, which is what the SM's port gives (measured: 60 without the MMAs), so
 // rows that are not needed cost time.
 constexpr int kBoxes = 6;
-__host__ __device__ constexpr int box_rows(int tm, int i) {
-  constexpr int pair[kBoxes] = {128, 112, 96, 80, 64, 32};
-  constexpr int single[kBoxes] = {64, 48, 32, 16, 16, 16};
-  return tm >= 256 ? pair[i] : single[i];
+__host__ __device__ constexpr int box_rows(int tm, int i) {   // 128, 112, 96, 80, 64, 32, or 64, 48, 32, 16
+  return tm >= 256 ? (i < 5 ? 128 - 16 * i : 32) : 64 - 16 * i;
 }
 __host__ __device__ constexpr int box_count(int tm) { return tm >= 256 ? 6 : 4; }
 
@@ -137,8 +135,8 @@ struct GroupedPlan {
   static constexpr int kOffOut = kOffT + STAGES * kTBytes;
   static constexpr int kOffRx = kOffOut + 2 * kOutBytes;  // fp32 sums from the cluster
   static constexpr int kOffBar = kOffRx + (CG == 1 ? TM * kGrpCols * 4 : 0);
-  // full, empty, land, built, tmem_full[2], tmem_empty[2], rx_full, rx_empty, done
-  static constexpr int kNumBars = 4 * STAGES + 6 + 1;
+  // full, empty, land, built, tmem_full[2], tmem_empty[2], rx_full, done
+  static constexpr int kNumBars = 4 * STAGES + 5 + 1;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;
   static constexpr int kOffScan = kOffMisc + 32;         // warp totals
   static constexpr int kOffRows = kOffScan + 64;         // group starts [E + 1]
@@ -502,7 +500,7 @@ __device__ __forceinline__ void load_weights(uint32_t dst, const CUtensorMap* m,
 }
 
 template <int CG, int TM, int STAGES, bool LORA>
-__global__ void __launch_bounds__(kGrpThreads, 1)
+__global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
     gemm_grouped_sm100(const __grid_constant__ GroupedMaps maps, const __grid_constant__ GroupedParams p) {
   using Plan = GroupedPlan<CG, TM, STAGES, LORA>;
   extern __shared__ uint8_t smem_raw[];
@@ -516,9 +514,8 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
   uint64_t* built_bar = land_bar + STAGES;   // ... and its rows of h are in place, on the even CTA
   uint64_t* tfull_bar = built_bar + STAGES;
   uint64_t* tempty_bar = tfull_bar + 2;
-  uint64_t* rxfull_bar = tempty_bar + 2;     // the cluster's sums for this CTA have arrived
-  uint64_t* rxempty_bar = rxfull_bar + 1;    // ... have been read, in every CTA of the cluster
-  uint64_t* done_bar = rxempty_bar + 1;
+  uint64_t* rx_full = tempty_bar + 2;        // the cluster's sums for this CTA have arrived
+  uint64_t* done_bar = rx_full + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Plan::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* odd_flags = reinterpret_cast<volatile int*>(tmem_slot + 2);   // three tiles in turn
@@ -551,8 +548,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
     mbar_init(&tfull_bar[1], 1);
     mbar_init(&tempty_bar[0], kGrpEpiWarps * CG);
     mbar_init(&tempty_bar[1], kGrpEpiWarps * CG);
-    mbar_init(rxfull_bar, kGrpEpiWarps * parts);
-    mbar_init(rxempty_bar, kGrpEpiWarps * parts);
+    mbar_init(rx_full, 1);
     mbar_init(done_bar, 1);
     *abort_flag = 0;
     for (int i = 0; i < 3; ++i) odd_flags[i] = 0;
@@ -813,7 +809,6 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1u;
     };
-    uint32_t rx_phase = 0;
     for (int t = worker; t < num_tiles; t += workers) {
       const GroupedUnit u = grouped_unit<CG, TM>(p, grp_rows, grp_tiles, t);
       const int n0 = (u.tn * CG + rank) * kGrpCols;
@@ -840,6 +835,10 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
         stage = (stage + kb1 - kb0) % STAGES;
         uint4 own[8];
         int have = -1;   // rank block held in `own`
+        if (rank_blocks == 1 && gt < half && tr < u.rows) {   // without waiting for the list or the row's adapter
+          split_ranks(hrow, p.h_pitch, bf16, own);
+          have = 0;
+        }
         int rb = adapters ? b0 / adapters : 0, ai = b0 - rb * adapters;
         int next = b0 < b1 ? list[kAdapterIds + ai] : 0;   // one block ahead of its use
         for (int b = b0; b < b1; ++b) {
@@ -992,51 +991,51 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
           }
           release_acc();
         } else {
-          // every row's partial sums go to the CTA that finishes it
+          // Every row's partial sums go to the CTA that finishes it: the tile
+          // as fp32 rows into the ring, which is idle now (a split launch has
+          // at most one tile per cluster), and from there one bulk copy to
+          // each CTA (stores of single words took 4000 cycles for 64 rows).
           const int per = (u.rows + parts - 1) / parts;   // rows per CTA, at most TM / parts
-          bool got_rx = true;
-          if (t != worker && lane == 0) got_rx = mbar_wait_cluster(rxempty_bar, rx_phase ^ 1u, abort_flag);
-          got_rx = __shfl_sync(0xffffffffu, got_rx ? 1 : 0, 0) != 0;
-          const uint32_t rx = smem_u32(smem + Plan::kOffRx);
-          const uint32_t from = rx + static_cast<uint32_t>(part * per * kGrpCols + col) * 4u;
-#pragma unroll 1
-          for (int r0 = eg * 8; r0 < u.rows && got_rx; r0 += 16) {
-            float f[8];
-            read8(r0, f);
-            int owner = r0 / per, at = r0 - owner * per;
-            const int last = min(8, u.rows - r0);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              if (i < last) {
-                st_dsmem_f32(mapa_shared(from + static_cast<uint32_t>(at * kGrpCols) * 4u, owner), f[i]);
-                if (++at == per) {
-                  at = 0;
-                  ++owner;
-                }
-              }
-            }
-          }
-          release_acc();   // joins the warp: its stores come before the arrivals
-          if (lane < parts) mbar_arrive_cluster(mapa_shared(smem_u32(rxfull_bar), lane));
-          if (lane == 0 && got_rx) got_rx = mbar_wait_cluster(rxfull_bar, rx_phase, abort_flag);
-          got_rx = __shfl_sync(0xffffffffu, got_rx ? 1 : 0, 0) != 0;
-          ok = named_bar_and(1, 32 * kGrpEpiWarps, got_rx);
-          if (!ok) break;
           mine0 = min(part * per, u.rows);
           mine1 = min(mine0 + per, u.rows);
+          const uint32_t rx = smem_u32(smem + Plan::kOffRx), rx_bar = smem_u32(rx_full);
+          constexpr uint32_t kRow = kGrpCols * 4;
+          if (et == 0 && mine0 < mine1) mbar_arrive_expect_tx(rx_full, static_cast<uint32_t>(parts * (mine1 - mine0)) * kRow);
+#pragma unroll 1
+          for (int r0 = eg * 8; r0 < u.rows; r0 += 16) {
+            float f[8];
+            read8(r0, f);
+            float* to = reinterpret_cast<float*>(sW) + r0 * kGrpCols + col;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) to[i * kGrpCols] = f[i];
+          }
+          release_acc();
+          fence_proxy_async_smem();
+          named_bar_sync(1, 32 * kGrpEpiWarps);
+          if (et < parts) {
+            const int rows_to = min(per, u.rows - et * per);
+            if (rows_to > 0) {
+              bulk_copy_dsmem(mapa_shared(rx + static_cast<uint32_t>(part * per) * kRow, et),
+                              smem_u32(sW) + static_cast<uint32_t>(et * per) * kRow,
+                              static_cast<uint32_t>(rows_to) * kRow, mapa_shared(rx_bar, et));
+            }
+          }
+          if (mine0 < mine1) ok = __all_sync(0xffffffffu, mbar_wait(rx_full, 0, abort_flag)) != 0;
+          ok = named_bar_and(1, 32 * kGrpEpiWarps, ok);
+          if (!ok) break;
           const float* sums = reinterpret_cast<const float*>(smem + Plan::kOffRx) + col;
 #pragma unroll 1
-          for (int r = eg; r < mine1 - mine0; r += 2) {
-            float v = 0.0f;
+          for (int r = eg * 4; r < mine1 - mine0; r += 8) {
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+            for (int c = 0; c < parts; ++c) {   // in CTA order
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {   // in CTA order
-              if (c < parts) v += sums[(c * per + r) * kGrpCols];
+              for (int i = 0; i < 4; ++i) v[i] += r + i < per ? sums[(c * per + r + i) * kGrpCols] : 0.0f;
             }
-            st_shared_u16(smem_u32(buf) + static_cast<uint32_t>(r * kGrpCols + col) * 2u, to_16bit(finish(v), bf16));
+            const uint32_t dst = smem_u32(buf) + static_cast<uint32_t>(r * kGrpCols + col) * 2u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) st_shared_u16(dst + i * (kGrpCols * 2), to_16bit(finish(v[i]), bf16));
           }
-          __syncwarp();
-          if (lane < parts) mbar_arrive_cluster(mapa_shared(smem_u32(rxempty_bar), lane));
-          rx_phase ^= 1u;
         }
         // the next tile's staging comes after its accumulator barrier
         named_bar_sync(1, 32 * kGrpEpiWarps);

@@ -44,8 +44,7 @@ namespace idb {
 constexpr int kShrinkWarps = 8;
 constexpr int kShrinkThreads = 32 * kShrinkWarps;
 constexpr int kShrinkSlice = 32;        // K elements per warp step: two MMAs deep
-constexpr int kShrinkMaxRows = 32;      // rows of a tile
-static_assert(kShrinkMaxRows == 32, "one lane per row of a tile");
+constexpr int kShrinkMaxRows = 8;       // rows of a tile
 // The adapters of a row tile: their count, the number of rows without one, and
 // from kAdapterIds on up to 256 adapters.
 constexpr int kAdapterIds = 4;
@@ -237,6 +236,9 @@ template <int RT, int NT8, bool KMAJ, bool BF16, bool VEC>
 __global__ void __launch_bounds__(kShrinkThreads) lora_shrink(const __grid_constant__ ShrinkParams p) {
   constexpr int RB = 16 * RT;
   extern __shared__ float red[];   // [kShrinkWarps][tile_rows][RB]
+  __shared__ float rx[kShrinkMaxRows * RB];   // this CTA's elements from the cluster: [CTA][element / cs]
+  __shared__ uint64_t rx_full;
+  __shared__ int gave_up;
   __shared__ __align__(16) int ids[kShrinkThreads];
   __shared__ int order[kShrinkMaxRows];
   __shared__ int order_id[kShrinkMaxRows];
@@ -250,6 +252,13 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink(const __grid_const
   const int r0 = static_cast<int>(blockIdx.y) * RB;
   const int slices = (p.K + kShrinkSlice - 1) / kShrinkSlice;
 
+  if (tid == 0) {
+    mbar_init(&rx_full, kShrinkWarps * cs);
+    gave_up = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  if (cs > 1) cluster_sync();   // every CTA's barrier is there before any remote arrival
   griddep_wait();
   // Everything before this grid is complete now, so the second kernel may
   // start reading x and W; it waits for this grid before it reads h.
@@ -270,8 +279,8 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink(const __grid_const
     bool bad = false;
     const int a = lane < rows ? adapter_of(p.adapter, p.adapter64, row0 + lane, p.L, bad) : -1;
     int at = 0;
-#pragma unroll
-    for (int i = 0; i < kShrinkMaxRows; ++i) {
+#pragma unroll 8
+    for (int i = 0; i < rows; ++i) {
       const int o = __shfl_sync(0xffffffffu, a, i);
       at += (o >= 0 && (o < a || (o == a && i < lane))) ? 1 : 0;
     }
@@ -382,18 +391,35 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink(const __grid_const
     for (int w = 1; w < kShrinkWarps; ++w) v += red[static_cast<size_t>(w) * p.tile_rows * RB + e];
     red[e] = v;
   }
-  // over the cluster: CTA c finishes every cs-th element
-  if (cs > 1) cluster_sync();
-  else __syncthreads();
-  const uint32_t base = smem_u32(red);
+  if (cs == 1) {
+    for (int e = tid; e < active * RB; e += kShrinkThreads) {   // the elements this thread summed
+      const int at = e / RB;
+      const float scale = p.scale != nullptr ? p.scale[order_id[at]] : 1.0f;
+      p.h[static_cast<long long>(row0 + order[at]) * p.h_pitch + r0 + e % RB] = red[e] * scale;
+    }
+    return;
+  }
+  // Over the cluster: element e is finished by CTA e % cs; every CTA sends it
+  // its partial (a sender may leave; only the receiver waits).
+  const uint32_t rx0 = smem_u32(rx);
+  const int share = (active * RB + cs - 1) / cs;
+  for (int e = tid; e < active * RB; e += kShrinkThreads) {
+    st_dsmem_f32(mapa_shared(rx0 + static_cast<uint32_t>(crank * share + e / cs) * 4u, e % cs), red[e]);
+  }
+  __syncwarp();
+  if (lane < cs) mbar_arrive_cluster(mapa_shared(smem_u32(&rx_full), lane));
+  if (!mbar_wait_cluster(&rx_full, 0, &gave_up)) {
+    gave_up = 1;
+    if (lane == 0) atomicOr(p.err, kDevErrTimeoutEpilogue);
+    return;
+  }
   for (int e = tid * cs + crank; e < active * RB; e += kShrinkThreads * cs) {
     float v = 0.0f;
-    for (int c = 0; c < cs; ++c) v += ld_dsmem_f32(mapa_shared(base + e * 4, c));
+    for (int c = 0; c < cs; ++c) v += rx[c * share + e / cs];   // in CTA order
     const int at = e / RB;
     const float scale = p.scale != nullptr ? p.scale[order_id[at]] : 1.0f;
     p.h[static_cast<long long>(row0 + order[at]) * p.h_pitch + r0 + e % RB] = v * scale;
   }
-  if (cs > 1) cluster_sync();   // no CTA leaves while a peer may still read its partials
 }
 
 // ------------------------------------------------------------------- many rows
