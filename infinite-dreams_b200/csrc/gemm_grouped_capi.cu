@@ -215,23 +215,23 @@ int launch_grouped(const Operand& a, const Operand& b, const Operand* up, const 
   static std::atomic<unsigned long long> configured{0};
   cudaError_t e = opt_in(gemm_grouped_sm100<CG, TM, STAGES, LORA>, Plan::kDynamicBytes, configured);
   if (e != cudaSuccess) return capi_fail_cuda(e, "grouped gemm kernel attribute");
-  // Single CTAs: a cluster splits each tile's K, at least 8 K blocks to a CTA
-  // (joining costs as much as 5), as long as there is a cluster for every
-  // tile.  The number of tiles is an upper bound: only the device knows the
-  // groups.
-  int cluster = CG, clusters = sms / CG;
-  if (CG == 1) {
-    for (int c = 2; c <= 8 && p.kb_total >= 8 * c; c *= 2) {
+  // Single CTAs: the cluster that splits the K of the last tiles, at least 8 K
+  // blocks to a CTA.  Four or eight CTAs while there is a cluster for every
+  // tile; two otherwise.  The number of tiles is an upper bound: only the
+  // device knows the groups.
+  int cluster = CG;
+  if (CG == 1 && p.kb_total >= 16) {
+    cluster = 2;
+    for (int c = 4; c <= 8 && p.kb_total >= 8 * c; c *= 2) {
       int fit = 0;
       st = resident_clusters(gemm_grouped_sm100<CG, TM, STAGES, LORA>, Plan::kDynamicBytes, c, &fit);
       if (st != GEMM_OK) return st;
       if (tiles > fit) break;
       cluster = c;
-      clusters = fit;
     }
   }
-  // persistent: at most one CTA per SM, fewer when there are fewer tiles
-  const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(tiles, clusters))) * cluster;
+  // persistent: at most one CTA per SM
+  const int grid = static_cast<int>(std::min<int64_t>(tiles, sms / cluster)) * cluster;
   e = launch(gemm_grouped_sm100<CG, TM, STAGES, LORA>, kGrpThreads, Plan::kDynamicBytes, grid, cluster,
              stream, maps, p);
   return e == cudaSuccess ? GEMM_OK : capi_fail_cuda(e, "grouped gemm kernel launch");

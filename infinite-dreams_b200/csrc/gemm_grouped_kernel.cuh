@@ -283,6 +283,31 @@ __device__ __forceinline__ int find_group(const int* first, int E, int u) {
   return lo;
 }
 
+// The tiles of one CTA (pair): whole ones, `stride` apart, and then perhaps one
+// that the CTAs of its cluster split along K.  A last wave with no more tiles
+// than clusters is split; it takes half the time with clusters of two (32 rows
+// over 64 experts, 200 tiles on 148 CTAs: the 52 of the second wave).
+struct GroupedWalk {
+  int t, stride;
+  int whole;       // tiles that are walked whole
+  int split_tile;  // at or past `tiles`: none
+  int tiles;
+
+  __device__ __forceinline__ bool next(int& tile, bool& split) {
+    split = t >= whole;
+    tile = split ? split_tile : t;
+    if (split) split_tile = tiles;
+    t += split ? 0 : stride;
+    return tile < tiles;
+  }
+};
+
+__device__ __forceinline__ GroupedWalk grouped_walk(int tiles, int cta, int ctas, int cluster, int clusters) {
+  const int waves = tiles / ctas, rest = tiles - waves * ctas;
+  const int whole = rest <= clusters ? waves * ctas : tiles;
+  return {cta, ctas, whole, whole + cluster, tiles};
+}
+
 struct GroupedUnit {
   int e;      // group
   int rt;     // row tile of the group
@@ -525,13 +550,11 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
 
   const int warp = static_cast<int>(threadIdx.x >> 5);
   const int lane = static_cast<int>(threadIdx.x & 31);
-  // CG = 2: position in the CTA pair.  CG = 1: the tile's K blocks are split
-  // over the `parts` CTAs of a cluster.
+  // CG = 2: position in the CTA pair.  CG = 1: the last tiles' K blocks are
+  // split over the CTAs of a cluster (GroupedWalk).
   const int csize = static_cast<int>(cluster_nctarank());
   const int crank = static_cast<int>(cluster_ctarank());
   const int rank = (CG == 2) ? crank : 0;
-  const int parts = (CG == 1) ? csize : 1;
-  const int part = (CG == 1) ? crank : 0;
   const bool leader = (rank == 0);
   const int worker = static_cast<int>(blockIdx.x) / csize;
   const int workers = static_cast<int>(gridDim.x) / csize;
@@ -572,9 +595,10 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
   const uint32_t tmem_base = *tmem_slot;
   // Parameters are read now, while the previous grid may still run: the
   // first read of each line of them costs a few hundred cycles.
-  const int kb0 = p.kb_total * part / parts, kb1 = p.kb_total * (part + 1) / parts;
+  const int split_kb0 = p.kb_total * crank / csize, split_kb1 = p.kb_total * (crank + 1) / csize;
   asm volatile("" ::"l"(p.offsets), "r"(p.E), "r"(p.T), "r"(p.N), "r"(p.tiles_n), "r"(p.b_kmaj), "l"(p.bias), "l"(p.C),
-               "r"(p.zero_rest), "r"(p.up_kmaj), "r"(kb0), "r"(kb1));
+               "r"(p.zero_rest), "r"(p.up_kmaj), "r"(split_kb0),
+               "r"(split_kb1));
   // With LORA the previous grid is lora_shrink, which lets this one start
   // once everything before it has completed: A and B can be read at once, and
   // only what touches h, the lists or C waits (each thread for itself, below).
@@ -587,6 +611,11 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
     scan_groups<kGrpThreads>(p.offsets, p.off64, p.E, p.T, grp_rows, grp_tiles, scan, p.err, tiles_of);
   }
   const int num_tiles = grp_tiles[p.E];
+  GroupedWalk walk = CG == 2 ? GroupedWalk{worker, workers, num_tiles, num_tiles, num_tiles}
+                             : grouped_walk(num_tiles, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x), worker,
+                                            workers);
+  int t;
+  bool split;
 
   if (warp == 0 || warp == kGrpRowsWarp) {
     // ------------------------------------------------------------ TMA producers: weights, rows
@@ -602,7 +631,9 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
       // per stage: parity of its last fill on full / land, and which came last
       uint32_t full_par = 0, land_par = 0, on_land = 0;
       bool ok = true, waited = false;
-      for (int t = worker; ok && t < num_tiles; t += workers) {
+      while (ok && walk.next(t, split)) {
+        const int parts = split ? csize : 1, part = split ? crank : 0;   // of the tile's K
+        const int kb0 = split ? split_kb0 : 0, kb1 = split ? split_kb1 : p.kb_total;
         const GroupedUnit u = grouped_unit<CG, TM>(p, grp_rows, grp_tiles, t);
         const int half = u.nmma / CG;
         const int arow = u.row0 + rank * half;
@@ -703,7 +734,9 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
       int count = 0;
       uint32_t built_par = 0;
       bool ok = true, waited = false;
-      for (int t = worker; ok && t < num_tiles; t += workers) {
+      while (ok && walk.next(t, split)) {
+        const int parts = split ? csize : 1, part = split ? crank : 0;   // of the tile's K
+        const int kb0 = split ? split_kb0 : 0, kb1 = split ? split_kb1 : p.kb_total;
         if (p.kb_total == 0) break;   // the epilogue writes act(bias) by itself
         const GroupedUnit u = grouped_unit<CG, TM>(p, grp_rows, grp_tiles, t);
         const uint32_t idesc = idesc_16bit(kGrpCols * CG, u.nmma, p.b_kmaj == 0, false, p.bf16 != 0);
@@ -752,8 +785,8 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
             for (int j = 0; j < steps; ++j) {
               const uint64_t wd = smem_desc_sw128(w0 + j * u_kstep, u_lbo, 1024);
 #pragma unroll
-              for (int part = 0; part < 2; ++part) {   // hi, lo
-                mma_f16_ss<CG>(d_tmem, wd, smem_desc_sw128(h0 + part * 64 + j * (kUmmaK * 2), 16, 1024), idesc_up, 1u);
+              for (int lo = 0; lo < 2; ++lo) {
+                mma_f16_ss<CG>(d_tmem, wd, smem_desc_sw128(h0 + lo * 64 + j * (kUmmaK * 2), 16, 1024), idesc_up, 1u);
               }
             }
             mma_commit<CG>(&empty_bar[stage]);
@@ -809,7 +842,9 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1u;
     };
-    for (int t = worker; t < num_tiles; t += workers) {
+    while (walk.next(t, split)) {
+      const int parts = split ? csize : 1, part = split ? crank : 0;   // of the tile's K
+      const int kb0 = split ? split_kb0 : 0, kb1 = split ? split_kb1 : p.kb_total;
       const GroupedUnit u = grouped_unit<CG, TM>(p, grp_rows, grp_tiles, t);
       const int n0 = (u.tn * CG + rank) * kGrpCols;
       const int n = n0 + col;
@@ -992,9 +1027,9 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
           release_acc();
         } else {
           // Every row's partial sums go to the CTA that finishes it: the tile
-          // as fp32 rows into the ring, which is idle now (a split launch has
-          // at most one tile per cluster), and from there one bulk copy to
-          // each CTA (stores of single words took 4000 cycles for 64 rows).
+          // as fp32 rows into the ring, which is idle now (a split tile is its
+          // CTA's last), and from there one bulk copy to each CTA (stores of
+          // single words took 4000 cycles for 64 rows).
           const int per = (u.rows + parts - 1) / parts;   // rows per CTA, at most TM / parts
           mine0 = min(part * per, u.rows);
           mine1 = min(mine0 + per, u.rows);
