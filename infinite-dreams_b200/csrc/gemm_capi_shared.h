@@ -22,8 +22,4 @@ int capi_device(int* sms, int** err_word);
 int capi_encode(CUtensorMap* map, const void* base, int rank, const int64_t* extents, const int64_t* strides,
                 const int* box, bool swizzled, const char* what);
 
-// Copies a rows x cols 16-bit matrix to pitch `ldd` (a multiple of 8
-// elements) with pack_rows_f16.
-int capi_pack(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols, cudaStream_t stream);
-
 }  // namespace idb

@@ -359,46 +359,58 @@ __device__ __forceinline__ void zero_rows(const GroupedParams& p, int lo, int hi
   }
 }
 
-// The 32 ranks of one row's block as a swizzle-ready row: hi in the first four
-// 16-byte chunks, lo in the last four.
-__device__ __forceinline__ void split_ranks(const float* h, int valid, bool bf16, uint4 (&out)[8]) {
-  uint32_t w[32];
-#pragma unroll
-  for (int i = 0; i < kLoraRanks; i += 4) {
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (i < valid) v = __ldcg(reinterpret_cast<const float4*>(h + i));   // the pitch of h is a multiple of 16 ranks
-    const float f[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int e = 0; e < 4; e += 2) {
-      uint32_t hi = 0, lo = 0;
-#pragma unroll
-      for (int o = 0; o < 2; ++o) {
-        const unsigned short top = to_16bit(f[e + o], bf16);
-        hi |= static_cast<uint32_t>(top) << (16 * o);
-        // an h beyond the type's range is infinite in hi; lo must not undo that
-        const float rest = f[e + o] - from_16bit(top, bf16);
-        lo |= static_cast<uint32_t>(to_16bit(isfinite(rest) ? rest : 0.0f, bf16)) << (16 * o);
-      }
-      w[(i + e) / 2] = hi;
-      w[16 + (i + e) / 2] = lo;
-    }
-  }
-#pragma unroll
-  for (int c = 0; c < 8; ++c) out[c] = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
-}
-
 __device__ __forceinline__ bool nonfinite16(uint32_t h, bool bf16) {
   const uint32_t exponent = bf16 ? 0x7F80u : 0x7C00u;
   return (h & exponent) == exponent;
 }
 
+// The same for both halves of a word: bits 15 and 31 say which.  An exponent
+// of all ones plus one in its lowest place carries into the sign bit's place.
+__device__ __forceinline__ uint32_t nonfinite_pair(uint32_t w, bool bf16) {
+  return ((w & (bf16 ? 0x7F807F80u : 0x7C007C00u)) + (bf16 ? 0x00800080u : 0x04000400u)) & 0x80008000u;
+}
+
+// The 32 ranks of one row's block as a swizzle-ready row: hi in the first four
+// 16-byte chunks, lo in the last four.
+__device__ __forceinline__ void split_ranks(const float* h, int valid, bool bf16, uint4 (&out)[8]) {
+  uint32_t hi[16], lo[16];
+  uint32_t seen = 0;
+#pragma unroll
+  for (int i = 0; i < kLoraRanks; i += 4) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (i < valid) v = __ldcg(reinterpret_cast<const float4*>(h + i));   // the pitch of h is a multiple of 16 ranks
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float x = e ? v.z : v.x, y = e ? v.w : v.y;
+      const uint32_t top = pack_16bit(x, y, bf16);
+      hi[i / 2 + e] = top;
+      lo[i / 2 + e] = pack_16bit(x - from_16bit(static_cast<unsigned short>(top), bf16),
+                                 y - from_16bit(static_cast<unsigned short>(top >> 16), bf16), bf16);
+      seen |= nonfinite_pair(top, bf16);
+    }
+  }
+  // An h beyond the type's range is infinite in hi, and lo must not undo that
+  // (inf - inf); a NaN stays in hi too.
+  if (seen) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t bad = nonfinite_pair(hi[i], bf16);
+      if (bad & 0x8000u) lo[i] &= 0xFFFF0000u;
+      if (bad & 0x80000000u) lo[i] &= 0x0000FFFFu;
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    out[c] = make_uint4(hi[4 * c], hi[4 * c + 1], hi[4 * c + 2], hi[4 * c + 3]);
+    out[4 + c] = make_uint4(lo[4 * c], lo[4 * c + 1], lo[4 * c + 2], lo[4 * c + 3]);
+  }
+}
+
 // Replaces the inf and NaN among the first 32 ranks of a landed `up` tile by
 // zeros; says whether this thread found any.  128 threads, four 16-byte chunks
 // each: a tile stored N x R has them in row `thread`, one stored R x N in rows
-// 0..31 of both atoms.  An exponent of all ones plus one in its lowest place
-// carries into the sign bit's place, for both halves of a word at once.
+// 0..31 of both atoms.
 __device__ __forceinline__ bool clear_nonfinite(uint8_t* tile, int thread, bool kmaj, bool bf16) {
-  const uint32_t exponent = bf16 ? 0x7F807F80u : 0x7C007C00u, one = bf16 ? 0x00800080u : 0x04000400u;
   uint4* at[4];
   uint32_t seen = 0;
 #pragma unroll
@@ -407,9 +419,9 @@ __device__ __forceinline__ bool clear_nonfinite(uint8_t* tile, int thread, bool 
     at[i] = reinterpret_cast<uint4*>(kmaj ? tile + thread * 128 + ((i ^ (thread & 7)) << 4)
                                           : tile + (c >> 8) * (kBK * 128) + (c & 255) * 16);
     const uint4 v = *at[i];
-    seen |= ((v.x & exponent) + one) | ((v.y & exponent) + one) | ((v.z & exponent) + one) | ((v.w & exponent) + one);
+    seen |= nonfinite_pair(v.x, bf16) | nonfinite_pair(v.y, bf16) | nonfinite_pair(v.z, bf16) | nonfinite_pair(v.w, bf16);
   }
-  if ((seen & 0x80008000u) == 0) return false;
+  if (seen == 0) return false;
 #pragma unroll 1
   for (int i = 0; i < 4; ++i) {
     unsigned short* h = reinterpret_cast<unsigned short*>(at[i]);
