@@ -15,8 +15,8 @@ namespace idb {
 
 // The operands of a call that TMA cannot address, repacked in one launch: a
 // dependent of the grid before it and the grid after it its dependent, so the
-// launches overlap.  5 x 777 x 1023 weights and 1000 x 777 rows: one launch
-// instead of one per operand took the product from 24.6 to PACK_US us.
+// launches overlap.  1000 rows by 5 x 777 x 1023 weights: 20 us with the
+// repacking, 12 us for 5 x 776 x 1024, which needs none.
 __global__ void pack_stacks(const __grid_constant__ PackJobs jobs) {
   griddep_wait();
   griddep_launch_dependents();
@@ -172,8 +172,8 @@ cudaError_t opt_in(Kernel kernel, int bytes, std::atomic<unsigned long long>& co
 // How many clusters of `cluster` CTAs of this kernel the device holds at once
 // (GPCs whose SMs do not divide leave some out: a B200 holds 33 of 4 and 15
 // of 8 CTAs that fill their SM).  Asked once per kernel, device and size.
-template <class Kernel>
-int resident_clusters(Kernel kernel, int bytes, int cluster, int* out) {
+template <auto kernel>
+int resident_clusters(int bytes, int cluster, int* out) {
   static std::atomic<int> known[64][9];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -263,7 +263,7 @@ int launch_grouped(const Operand& a, const Operand& b, const Operand* up, const 
     cluster = 2;
     for (int c = 4; c <= 8 && p.kb_total >= 8 * c; c *= 2) {
       int fit = 0;
-      st = resident_clusters(gemm_grouped_sm100<CG, TM, STAGES, LORA>, Plan::kDynamicBytes, c, &fit);
+      st = resident_clusters<gemm_grouped_sm100<CG, TM, STAGES, LORA>>(Plan::kDynamicBytes, c, &fit);
       if (st != GEMM_OK) return st;
       if (tiles > fit) break;
       cluster = c;
@@ -277,10 +277,10 @@ int launch_grouped(const Operand& a, const Operand& b, const Operand* up, const 
 }
 
 // ------------------------------------------------------------- low-rank adapters
-// Workspace of a call with adapters: h, the adapter lists, then repacked operands.
+// Workspace of a call with adapters: h, then repacked operands.
 struct LoraPlan {
   Operand x, w, up;
-  size_t off_h = 0, off_lists = 0, total = 0;
+  size_t off_h = 0, total = 0;
 
   LoraPlan(const void* X, const void* W, const void* U, int64_t T, int64_t N, int64_t K, int64_t L, int64_t R,
            int64_t ldx, int64_t ldw, int trans_w, int64_t ld_up, int64_t stride_up, int trans_up)
@@ -289,9 +289,6 @@ struct LoraPlan {
     size_t off = align256(gemm_workspace_counter_bytes());
     off_h = off;
     off = align256(off + static_cast<size_t>(T) * shrink_pitch(R) * sizeof(float));
-    off_lists = off;
-    // a list per row tile, of 64 rows in the variant with more of them
-    off = align256(off + static_cast<size_t>((T + 63) / 64) * kAdapterListPitch * sizeof(int));
     x.plan(&off);
     w.plan(&off);
     up.plan(&off);
@@ -581,14 +578,6 @@ int gemm_lora_launch(const void* X, const void* W, const void* down, const void*
   s.K = static_cast<int>(K);
   s.L = static_cast<int>(L);
   s.R = static_cast<int>(R);
-  s.lists = reinterpret_cast<int*>(ws + pl.off_lists);
-  // the second kernel's row tiles
-  const bool small = small_tiles(T, N, 1, sms);
-  int list_tiles, list_rows;
-  if (small) row_tiles<64, 16>(s.T, list_tiles, list_rows);
-  else row_tiles<256, 32>(s.T, list_tiles, list_rows);
-  s.list_tiles = list_tiles;
-  s.list_rows = list_rows;
   s.err = p.err;
   st = launch_shrink(s, trans_down != 0, dtype == GEMM_DTYPE_BF16, stream);   // x is TMA-addressable by now
   if (st != GEMM_OK) return st;
@@ -611,12 +600,11 @@ int gemm_lora_launch(const void* X, const void* W, const void* down, const void*
   p.R = s.R;
   p.adapter = adapter;
   p.adapter64 = s.adapter64;
-  p.lists = s.lists;
   p.up_kmaj = trans_up;
   p.up = static_cast<const unsigned short*>(pl.up.p);
   p.ld_up = pl.up.ld;
   p.stride_up = L == 1 ? 0 : pl.up.stride;
-  if (small) return launch_grouped<1, 64, 6, true>(pl.x, pl.w, &pl.up, p, sms, stream);
+  if (small_tiles(T, N, 1, sms)) return launch_grouped<1, 64, 6, true>(pl.x, pl.w, &pl.up, p, sms, stream);
   return launch_grouped<2, 256, 6, true>(pl.x, pl.w, &pl.up, p, sms, stream);
 }
 

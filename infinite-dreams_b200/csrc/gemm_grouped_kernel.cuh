@@ -38,8 +38,10 @@
 //
 // LORA = true adds low-rank adapters picked by the row to one shared product
 // (E = 1, no offsets):  C[r, :] = act(A[r, :] * B + h[r, :] * up[a_r] + bias).
-// h (fp32, scaled) comes from lora_shrink (gemm_lora_kernel.cuh), which also
-// lists the adapters of each row tile.  After the K blocks of a tile come its
+// h (fp32, scaled) comes from lora_shrink (gemm_lora_kernel.cuh), which runs
+// beside this kernel's first K blocks: only the rows of h wait for it.  The
+// epilogue warps list the distinct adapters of a tile's rows while its K
+// blocks are multiplied.  After the K blocks of a tile come its
 // adapter blocks, 32 ranks of one adapter each, which pass through the same
 // ring: the weight slot of a stage holds `up` (64 ranks wide as TMA's swizzle
 // wants it, of which 32 are used), and its row slot is filled by the epilogue
@@ -106,7 +108,6 @@ struct GroupedParams {
   int L, R;
   const void* adapter;
   int adapter64;
-  const int* lists;  // [row tiles, kAdapterListPitch]
   int up_kmaj;       // up[a] stored N x R
   int up_wide;
   const unsigned short* up;
@@ -135,11 +136,11 @@ struct GroupedPlan {
   static constexpr int kOffOut = kOffT + STAGES * kTBytes;
   static constexpr int kOffRx = kOffOut + 2 * kOutBytes;  // fp32 sums from the cluster
   static constexpr int kOffBar = kOffRx + (CG == 1 ? TM * kGrpCols * 4 : 0);
-  // full, empty, land, built, tmem_full[2], tmem_empty[2], rx_full, done
-  static constexpr int kNumBars = 4 * STAGES + 5 + 1;
+  // full, empty, land, built, tmem_full[2], tmem_empty[2], rx_full, list, list_read, done
+  static constexpr int kNumBars = 4 * STAGES + 8;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;
   static constexpr int kOffScan = kOffMisc + 32;         // warp totals
-  static constexpr int kOffRows = kOffScan + 64;         // group starts [E + 1]
+  static constexpr int kOffRows = (kOffScan + 64 + 15) / 16 * 16;   // group starts [E + 1]
   static constexpr int kOffTiles = kOffRows + (kMaxGroups + 1) * 4;  // first tile of each group [E + 1]
   static constexpr int kUsed = kOffTiles + (kMaxGroups + 1) * 4;
   static constexpr int kDynamicBytes = kUsed + 1024;
@@ -434,12 +435,12 @@ __device__ __forceinline__ bool clear_nonfinite(uint8_t* tile, int thread, bool 
 
 // What clear_nonfinite took out of row t's value in column n in the adapter
 // blocks [b0, b1) of its tile.
-__device__ __noinline__ float nonfinite_terms(const GroupedParams& p, const int* list, int b0, int b1, int t, int n) {
+__device__ __noinline__ float nonfinite_terms(const GroupedParams& p, const int* list, int adapters, int b0, int b1,
+                                              int t, int n) {
   bool bad = false;
   const int a = adapter_of(p.adapter, p.adapter64, t, p.L, bad);
-  const int adapters = list[0];
   int ai = 0;
-  while (ai < adapters && list[kAdapterIds + ai] != a) ++ai;
+  while (ai < adapters && list[ai] != a) ++ai;
   float sum = 0.0f;
   if (a < 0 || ai == adapters) return sum;
   for (int r = 0; r < p.R; ++r) {
@@ -502,7 +503,7 @@ __device__ __forceinline__ void store_rows(const GroupedParams& p, const uint8_t
   } else {
     const int c = thread & 127;
     if (n0 + c >= p.N) return;
-#pragma unroll 1
+#pragma unroll 4
     for (int r = thread >> 7; r < count; r += threads >> 7) {
       crow[r * p.ldc + c] = reinterpret_cast<const unsigned short*>(buf + r * (kGrpCols * 2))[c];
     }
@@ -552,13 +553,21 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
   uint64_t* tfull_bar = built_bar + STAGES;
   uint64_t* tempty_bar = tfull_bar + 2;
   uint64_t* rx_full = tempty_bar + 2;        // the cluster's sums for this CTA have arrived
-  uint64_t* done_bar = rx_full + 1;
+  uint64_t* list_bar = rx_full + 1;          // the tile's adapters are listed
+  uint64_t* list_read_bar = list_bar + 1;    // both producers and the MMA warp are done with the list
+  uint64_t* done_bar = list_read_bar + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Plan::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* odd_flags = reinterpret_cast<volatile int*>(tmem_slot + 2);   // three tiles in turn
   int* scan = reinterpret_cast<int*>(smem + Plan::kOffScan);
   int* grp_rows = reinterpret_cast<int*>(smem + Plan::kOffRows);
   int* grp_tiles = reinterpret_cast<int*>(smem + Plan::kOffTiles);
+
+  // With adapters there is one group: the rest of the tables holds the
+  // adapter of each row of the tile, the distinct ones, and their counts.
+  int* row_ids = grp_rows + 4;
+  int* list = grp_tiles + 4;
+  volatile int* list_counts = scan;   // adapters, then rows without one; scratch after that
 
   const int warp = static_cast<int>(threadIdx.x >> 5);
   const int lane = static_cast<int>(threadIdx.x & 31);
@@ -584,6 +593,8 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
     mbar_init(&tempty_bar[0], kGrpEpiWarps * CG);
     mbar_init(&tempty_bar[1], kGrpEpiWarps * CG);
     mbar_init(rx_full, 1);
+    mbar_init(list_bar, 1);
+    mbar_init(list_read_bar, leader ? 3 : 2);
     mbar_init(done_bar, 1);
     *abort_flag = 0;
     for (int i = 0; i < 3; ++i) odd_flags[i] = 0;
@@ -612,8 +623,8 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
                "r"(p.zero_rest), "r"(p.up_kmaj), "r"(split_kb0),
                "r"(split_kb1));
   // With LORA the previous grid is lora_shrink, which lets this one start
-  // once everything before it has completed: A and B can be read at once, and
-  // only what touches h, the lists or C waits (each thread for itself, below).
+  // once everything before it has completed: the operands can be read at once,
+  // and only what touches h or C waits (the epilogue warps, below).
   if constexpr (!LORA) griddep_wait();
   const int rank_blocks = LORA ? (p.R + kLoraRanks - 1) / kLoraRanks : 0;
 
@@ -642,7 +653,8 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
       int issued = 0;
       // per stage: parity of its last fill on full / land, and which came last
       uint32_t full_par = 0, land_par = 0, on_land = 0;
-      bool ok = true, waited = false;
+      bool ok = true;
+      uint32_t list_phase = 0;
       while (ok && walk.next(t, split)) {
         const int parts = split ? csize : 1, part = split ? crank : 0;   // of the tile's K
         const int kb0 = split ? split_kb0 : 0, kb1 = split ? split_kb1 : p.kb_total;
@@ -677,22 +689,19 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
           }
         }
         if constexpr (LORA) {
-          if (!waited) griddep_wait();   // the lists are lora_shrink's
-          waited = true;
-          const int* list = p.lists + static_cast<long long>(u.rt) * kAdapterListPitch;
-          const int adapters = ok ? list[0] : 0;
+          ok = ok && mbar_wait(list_bar, list_phase, abort_flag);
+          list_phase ^= 1u;
+          const int adapters = ok ? list_counts[0] : 0;
           const int blocks = rank_blocks * adapters;
           const int b0 = blocks * part / parts, b1 = blocks * (part + 1) / parts;
           int rb = adapters ? b0 / adapters : 0, ai = b0 - rb * adapters;
-          int next = b0 < b1 ? list[kAdapterIds + ai] : 0;   // one block ahead of its use
           for (int b = b0; b < b1; ++b) {
-            const int a = next, r0 = rb * kLoraRanks;
-            if (++ai == adapters) {
-              ai = 0;
-              ++rb;
-            }
             if (weights) {
-              if (b + 1 < b1) next = list[kAdapterIds + ai];
+              const int a = list[ai], r0 = rb * kLoraRanks;
+              if (++ai == adapters) {
+                ai = 0;
+                ++rb;
+              }
               if (issued >= STAGES && !mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) {
                 ok = false;
                 break;
@@ -710,6 +719,7 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
               phase ^= 1u;
             }
           }
+          mbar_arrive(list_read_bar);
         }
       }
       if (weights) griddep_launch_dependents();
@@ -744,8 +754,8 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
       int acc = 0;
       uint32_t acc_phase = 0;
       int count = 0;
-      uint32_t built_par = 0;
-      bool ok = true, waited = false;
+      uint32_t built_par = 0, list_phase = 0;
+      bool ok = true;
       while (ok && walk.next(t, split)) {
         const int parts = split ? csize : 1, part = split ? crank : 0;   // of the tile's K
         const int kb0 = split ? split_kb0 : 0, kb1 = split ? split_kb1 : p.kb_total;
@@ -777,11 +787,12 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
           if (++stage == STAGES) stage = 0;
         }
         if constexpr (LORA) {
-          if (!waited) griddep_wait();
-          waited = true;
+          ok = ok && mbar_wait(list_bar, list_phase, abort_flag);
+          list_phase ^= 1u;
           const uint32_t idesc_up = idesc_16bit(kGrpCols * CG, u.nmma, p.up_kmaj == 0, false, p.bf16 != 0);
           const uint32_t u_lbo = p.up_kmaj ? 16 : kBK * 128, u_kstep = p.up_kmaj ? kUmmaK * 2 : kUmmaK * 128;
-          const int adapters = ok ? p.lists[static_cast<long long>(u.rt) * kAdapterListPitch] : 0;
+          const int adapters = ok ? list_counts[0] : 0;
+          mbar_arrive(list_read_bar);
           const int blocks = rank_blocks * adapters;
           for (int b = blocks * part / parts; b < blocks * (part + 1) / parts; ++b) {
             const int steps = min(kLoraRanks, p.R - b / adapters * kLoraRanks) > kUmmaK ? 2 : 1;
@@ -836,7 +847,8 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
     const uint32_t built_remote0 = (CG == 2) ? mapa_shared(smem_u32(&built_bar[0]), 0) : 0u;
     int stage = 0;
     uint32_t land_par = 0;
-    if constexpr (LORA) griddep_wait();
+    bool waited = !LORA;
+    uint32_t listed = 0;   // tiles whose adapters were listed
     if (p.zero_rest) zero_rows(p, grp_rows[0], grp_rows[p.E], et, 32 * kGrpEpiWarps);
     int acc = 0, turn = 0;
     uint32_t acc_phase = 0;
@@ -863,40 +875,62 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
       const float bias =
           (p.bias != nullptr && n < p.N) ? from_16bit(p.bias[static_cast<long long>(u.e) * p.N + n], bf16) : 0.0f;
       bool got = true;
-      const int* list = nullptr;
-      int b0 = 0, b1 = 0;   // this piece's adapter blocks
+      int adapters = 0, b0 = 0, b1 = 0;   // of the tile; this piece's adapter blocks
       if constexpr (LORA) {
+        // The distinct adapters of the tile's rows, in order of their first
+        // row, while the K blocks are multiplied.
+        bool bad = false;
+        const int id = et < u.rows ? adapter_of(p.adapter, p.adapter64, u.row0 + et, p.L, bad) : -1;
+        if (bad) atomicOr(p.err, kDevErrBadAdapter);
+        row_ids[et] = id;
+        const unsigned same = __match_any_sync(0xffffffffu, id);   // rows of this warp with the same adapter
+        bool first = id >= 0 && (same & ((1u << lane) - 1u)) == 0u;
+        named_bar_sync(1, 32 * kGrpEpiWarps);
+#pragma unroll 1
+        for (int i = 0; i < (et & ~31) && first; i += 4) {   // earlier warps' rows, four at a time
+          const int4 v = *reinterpret_cast<const int4*>(row_ids + i);
+          first = v.x != id && v.y != id && v.z != id && v.w != id;
+        }
+        const unsigned vote = __ballot_sync(0xffffffffu, first);
+        const unsigned none = __ballot_sync(0xffffffffu, et < u.rows && id < 0);
+        if (lane == 0) list_counts[2 + (et >> 5)] = __popc(vote) | (__popc(none) << 16);
+        named_bar_sync(1, 32 * kGrpEpiWarps);
+        int at = __popc(vote & ((1u << lane) - 1u)), all = 0, without = 0;
+        for (int w = 0; w < kGrpEpiWarps; ++w) {
+          const int c = list_counts[2 + w];
+          at += w < (et >> 5) ? c & 0xffff : 0;
+          all += c & 0xffff;
+          without += c >> 16;
+        }
+        if (listed > 0) mbar_wait(list_read_bar, (listed - 1) & 1u, abort_flag);   // the previous tile's
+        ++listed;
+        if (first) list[at] = id;
+        if (et == 0) list_counts[0] = all;
+        named_bar_sync(1, 32 * kGrpEpiWarps);
+        if (et == 0) mbar_arrive(list_bar);
+        adapters = all;
+        if (!waited) griddep_wait();   // from here on h, the workspace and C
+        waited = true;
         // adapter rows of this CTA's share of the tile: thread gt of a group
         // builds row gt of every other block
-        list = p.lists + static_cast<long long>(u.rt) * kAdapterListPitch;
-        const int adapters = list[0];
         b0 = rank_blocks * adapters * part / parts;
         b1 = rank_blocks * adapters * (part + 1) / parts;
-        const bool mixed = adapters > 1 || list[1] > 0;
+        const bool mixed = adapters > 1 || without > 0;
         const int half = u.nmma / CG;
         const int tr = rank * half + gt;   // row of the tile
-        bool bad = false;
-        const int mine =
-            (gt < half && tr < u.rows) ? adapter_of(p.adapter, p.adapter64, u.row0 + tr, p.L, bad) : -1;
+        const int mine = (gt < half && tr < u.rows) ? row_ids[tr] : -1;
         const float* hrow = p.h + static_cast<long long>(u.row0 + tr) * p.h_pitch;
         stage = (stage + kb1 - kb0) % STAGES;
         uint4 own[8];
         int have = -1;   // rank block held in `own`
-        if (rank_blocks == 1 && gt < half && tr < u.rows) {   // without waiting for the list or the row's adapter
-          split_ranks(hrow, p.h_pitch, bf16, own);
-          have = 0;
-        }
         int rb = adapters ? b0 / adapters : 0, ai = b0 - rb * adapters;
-        int next = b0 < b1 ? list[kAdapterIds + ai] : 0;   // one block ahead of its use
         for (int b = b0; b < b1; ++b) {
-          const int a = next;
-          if (b + 1 < b1) next = list[kAdapterIds + (ai + 1 == adapters ? 0 : ai + 1)];
           if (((b - b0) & 1) == eg) {
             if (rb != have) {
               if (mine >= 0) split_ranks(hrow + rb * kLoraRanks, p.h_pitch - rb * kLoraRanks, bf16, own);
               have = rb;
             }
-            const bool is = mine >= 0 && a == mine;
+            const bool is = mine >= 0 && list[ai] == mine;
             // the producer waited for the slot to be free before it loaded `up`
             got = mbar_wait(&land_bar[stage], (land_par >> stage) & 1u, abort_flag);
             got = __all_sync(0xffffffffu, got) != 0;
@@ -966,7 +1000,7 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
           if (LORA && odd && n < p.N) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-              if (r0 + i < u.rows) f[i] += nonfinite_terms(p, list, b0, b1, u.row0 + r0 + i, n);
+              if (r0 + i < u.rows) f[i] += nonfinite_terms(p, list, adapters, b0, b1, u.row0 + r0 + i, n);
             }
           }
           // the store issued from this buffer a chunk ago has read it
@@ -1020,7 +1054,7 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
 #pragma unroll 1
             for (int i = 0; i < 8; ++i) {
               if (r0 + i >= u.rows) break;
-              const float extra = nonfinite_terms(p, list, b0, b1, u.row0 + r0 + i, n);
+              const float extra = nonfinite_terms(p, list, adapters, b0, b1, u.row0 + r0 + i, n);
 #pragma unroll
               for (int q = 0; q < 8; ++q) f[q] += q == i ? extra : 0.0f;
             }

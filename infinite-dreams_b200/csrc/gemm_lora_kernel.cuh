@@ -33,9 +33,6 @@
 // loads in flight per warp, and `down` read again for every 32 rows -- so
 // there a CTA takes 256 rows and brings x and `down` through a ring in shared
 // memory by cp.async; see below.
-//
-// Clusters past the last row tile list the distinct adapters of each row tile
-// of the second kernel, which needs one pass over `up` per listed adapter.
 #pragma once
 #include "sm100_ptx.cuh"
 
@@ -45,10 +42,6 @@ constexpr int kShrinkWarps = 8;
 constexpr int kShrinkThreads = 32 * kShrinkWarps;
 constexpr int kShrinkSlice = 32;        // K elements per warp step: two MMAs deep
 constexpr int kShrinkMaxRows = 8;       // rows of a tile
-// The adapters of a row tile: their count, the number of rows without one, and
-// from kAdapterIds on up to 256 adapters.
-constexpr int kAdapterIds = 4;
-constexpr int kAdapterListPitch = kAdapterIds + 256;
 
 struct ShrinkParams {
   const unsigned short* x;
@@ -63,8 +56,6 @@ struct ShrinkParams {
   int T, K, L, R;
   int tile_rows;        // rows of a cluster
   int tiles;            // clusters that cover the rows
-  int* lists;           // [list_tiles, kAdapterListPitch]
-  int list_tiles, list_rows;
   int* err;
 };
 
@@ -197,41 +188,8 @@ __device__ __forceinline__ void rank_fragments(const Slice<RT, NT8>& s, int m, u
   }
 }
 
-// Distinct adapters of rows [row0, row0 + n), n <= 256, in order of their
-// first row.  Called by all threads.
-__device__ __forceinline__ void list_adapters(const ShrinkParams& p, int row0, int n, int* list, int* ids,
-                                              int* warp_counts) {
-  const int tid = static_cast<int>(threadIdx.x);
-  bool bad = false;
-  const int a = tid < n ? adapter_of(p.adapter, p.adapter64, row0 + tid, p.L, bad) : -1;
-  ids[tid] = a;
-  if (bad) atomicOr(p.err, kDevErrBadAdapter);
-  __syncthreads();
-  bool first = a >= 0;
-#pragma unroll 1
-  for (int i = 0; i < (tid & ~31) && first; i += 4) {   // earlier warps' rows, four at a time
-    const int4 v = *reinterpret_cast<const int4*>(ids + i);
-    first = v.x != a && v.y != a && v.z != a && v.w != a;
-  }
-  const unsigned same = __match_any_sync(0xffffffffu, a);   // rows of this warp with the same adapter
-  first = first && (same & ((1u << (tid & 31)) - 1u)) == 0u;
-  const unsigned vote = __ballot_sync(0xffffffffu, first);
-  if ((tid & 31) == 0) warp_counts[tid >> 5] = __popc(vote);
-  __syncthreads();
-  int at = __popc(vote & ((1u << (tid & 31)) - 1u));
-  for (int w = 0; w < (tid >> 5); ++w) at += warp_counts[w];
-  if (first) list[kAdapterIds + at] = a;
-  if (tid == 0) {
-    int total = 0;
-    for (int w = 0; w < kShrinkWarps; ++w) total += warp_counts[w];
-    list[0] = total;
-  }
-  const int without = __syncthreads_count(tid < n && a < 0);
-  if (tid == 0) list[1] = without;
-}
-
-// grid.x: (tiles + list tiles) x cluster size (the cluster is along x);
-// grid.y: blocks of 16 RT ranks.
+// grid.x: tiles x cluster size (the cluster is along x); grid.y: blocks of 16
+// RT ranks.
 template <int RT, int NT8, bool KMAJ, bool BF16, bool VEC>
 __global__ void __launch_bounds__(kShrinkThreads) lora_shrink(const __grid_constant__ ShrinkParams p) {
   constexpr int RB = 16 * RT;
@@ -239,10 +197,8 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink(const __grid_const
   __shared__ float rx[kShrinkMaxRows * RB];   // this CTA's elements from the cluster: [CTA][element / cs]
   __shared__ uint64_t rx_full;
   __shared__ int gave_up;
-  __shared__ __align__(16) int ids[kShrinkThreads];
   __shared__ int order[kShrinkMaxRows];
   __shared__ int order_id[kShrinkMaxRows];
-  __shared__ int warp_counts[kShrinkWarps];
   __shared__ int active_s;
   const int tid = static_cast<int>(threadIdx.x);
   const int warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
@@ -264,14 +220,6 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink(const __grid_const
   // start reading x and W; it waits for this grid before it reads h.
   griddep_launch_dependents();
 
-  if (tile >= p.tiles) {
-    const int first = (tile - p.tiles) * p.list_rows;
-    if (crank == 0 && blockIdx.y == 0) {
-      list_adapters(p, first, min(p.list_rows, p.T - first),
-                    p.lists + static_cast<long long>(tile - p.tiles) * kAdapterListPitch, ids, warp_counts);
-    }
-    return;
-  }
   // rows of the tile ordered by adapter (stable), those without one left out
   const int row0 = tile * p.tile_rows;
   if (warp == 0) {
@@ -474,7 +422,7 @@ template <bool KMAJ, bool BF16>
 __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_wide(const __grid_constant__ ShrinkParams p) {
   extern __shared__ __align__(128) uint8_t wide_smem[];
   __shared__ __align__(16) int ids[kShrinkThreads];
-  __shared__ int list[kAdapterListPitch];
+  __shared__ int list[kWideRows];
   __shared__ int warp_counts[kShrinkWarps];
   const int tid = static_cast<int>(threadIdx.x);
   const int warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
@@ -487,19 +435,29 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_wide(const __grid_
   griddep_wait();
   griddep_launch_dependents();   // see lora_shrink
 
-  if (tile >= p.tiles) {
-    const int first = (tile - p.tiles) * p.list_rows;
-    if (crank == 0 && blockIdx.y == 0) {
-      list_adapters(p, first, min(p.list_rows, p.T - first),
-                    p.lists + static_cast<long long>(tile - p.tiles) * kAdapterListPitch, ids, warp_counts);
-    }
-    return;
-  }
   const int rows = min(kWideRows, p.T - row0);
-  list_adapters(p, row0, rows, list, ids, warp_counts);
+  // the distinct adapters of the rows, in order of their first row
+  bool bad = false;
+  const int my_id = tid < rows ? adapter_of(p.adapter, p.adapter64, row0 + tid, p.L, bad) : -1;   // row warp * 32 + lane
+  ids[tid] = my_id;
+  const unsigned same = __match_any_sync(0xffffffffu, my_id);
+  bool first = my_id >= 0 && (same & ((1u << lane) - 1u)) == 0u;
   __syncthreads();
-  const int adapters = list[0];
-  const int my_id = ids[tid];   // of row warp * 32 + lane
+#pragma unroll 1
+  for (int i = 0; i < (tid & ~31) && first; i += 4) {   // earlier warps' rows, four at a time
+    const int4 v = *reinterpret_cast<const int4*>(ids + i);
+    first = v.x != my_id && v.y != my_id && v.z != my_id && v.w != my_id;
+  }
+  const unsigned vote = __ballot_sync(0xffffffffu, first);
+  if (lane == 0) warp_counts[warp] = __popc(vote);
+  __syncthreads();
+  int at = __popc(vote & ((1u << lane) - 1u)), adapters = 0;
+  for (int w = 0; w < kShrinkWarps; ++w) {
+    at += w < warp ? warp_counts[w] : 0;
+    adapters += warp_counts[w];
+  }
+  if (first) list[at] = my_id;
+  __syncthreads();
   const uint32_t ring = smem_u32(wide_smem);
   float* sums = reinterpret_cast<float*>(wide_smem + kWideStages * kWideStageBytes);   // [256][64]
 
@@ -507,7 +465,7 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_wide(const __grid_
   const int kb0 = blocks * crank / cs, per = blocks * (crank + 1) / cs - kb0;
   const int steps = adapters * per;
   auto load = [&](int step) {   // x and down[a] of one step into its stage
-    const int a = list[kAdapterIds + step / per];
+    const int a = list[step / per];
     const int k0 = (kb0 + step % per) * kWideK;
     const uint32_t sx = ring + static_cast<uint32_t>(step % kWideStages * kWideStageBytes), sd = sx + kWideXBytes;
     const int c = tid & 7;
@@ -548,7 +506,7 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_wide(const __grid_
     cp_async_commit();
     const int block = step % per;
     if (block == 0) {
-      mine = __any_sync(0xffffffffu, my_id == list[kAdapterIds + step / per]);
+      mine = __any_sync(0xffffffffu, my_id == list[step / per]);
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
 #pragma unroll
@@ -587,7 +545,7 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_wide(const __grid_
         }
       }
       if (block == per - 1) {
-        const int a = list[kAdapterIds + step / per];
+        const int a = list[step / per];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
 #pragma unroll

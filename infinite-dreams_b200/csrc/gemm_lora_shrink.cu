@@ -74,7 +74,7 @@ int launch_shrink(const ShrinkParams& sp, bool kmaj, bool bf16, cudaStream_t str
     bytes = kShrinkWarps * rows * ranks * static_cast<int>(sizeof(float));   // at most 16 KiB
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((p.tiles + p.list_tiles) * cluster),
+  cfg.gridDim = dim3(static_cast<unsigned>(p.tiles * cluster),
                      static_cast<unsigned>((p.R + ranks - 1) / ranks), 1);
   cfg.blockDim = dim3(kShrinkThreads, 1, 1);
   cfg.dynamicSmemBytes = static_cast<size_t>(bytes);
