@@ -538,7 +538,7 @@ __device__ __forceinline__ void load_weights(uint32_t dst, const CUtensorMap* m,
 }
 
 template <int CG, int TM, int STAGES, bool LORA>
-__global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
+__global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
     gemm_grouped_sm100(const __grid_constant__ GroupedMaps maps, const __grid_constant__ GroupedParams p) {
   using Plan = GroupedPlan<CG, TM, STAGES, LORA>;
   extern __shared__ uint8_t smem_raw[];
@@ -639,6 +639,7 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
                                             workers);
   int t;
   bool split;
+  bool arrived = false;   // at the cluster barrier of the teardown
 
   if (warp == 0 || warp == kGrpRowsWarp) {
     // ------------------------------------------------------------ TMA producers: weights, rows
@@ -975,7 +976,7 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
       turn = turn == 2 ? 0 : turn + 1;
       const uint32_t tbase = tmem_base + (static_cast<uint32_t>(ew * 32) << 16) + static_cast<uint32_t>(acc * TM);
 
-      auto finish = [&](float v) {
+      auto finish = [&](float v, float bias) {
         v += bias;
         if (p.act == 1) v = v < 0.0f ? 0.0f : v;   // a NaN stays one
         if (p.act == 2) v = gelu(v);
@@ -1013,7 +1014,7 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
             for (int i = 0; i < 32; ++i) f[i] = gelu(f[i] + bias);
           } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) f[i] = finish(f[i]);
+            for (int i = 0; i < 32; ++i) f[i] = finish(f[i], bias);
           }
           if (bf16) {
 #pragma unroll
@@ -1060,7 +1061,6 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
             }
           }
         };
-        int mine0 = 0, mine1 = u.rows;   // rows that this CTA finishes
         if (parts == 1) {
 #pragma unroll 1
           for (int r0 = eg * 8; r0 < u.rows; r0 += 16) {
@@ -1068,32 +1068,32 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
             read8(r0, f);
             const uint32_t dst = smem_u32(buf) + static_cast<uint32_t>(r0 * kGrpCols + col) * 2u;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) st_shared_u16(dst + i * (kGrpCols * 2), to_16bit(finish(f[i]), bf16));
+            for (int i = 0; i < 8; ++i) st_shared_u16(dst + i * (kGrpCols * 2), to_16bit(finish(f[i], bias), bf16));
           }
           release_acc();
         } else {
           // Every row's partial sums go to the CTA that finishes it: the tile
           // as fp32 rows into the ring, which is idle now (a split tile is its
-          // CTA's last), and from there one bulk copy to each CTA (stores of
-          // single words took 4000 cycles for 64 rows).
+          // CTA's last), and from there one bulk copy to each other CTA
+          // (stores of single words took 4000 cycles for 64 rows).
           const int per = (u.rows + parts - 1) / parts;   // rows per CTA, at most TM / parts
-          mine0 = min(part * per, u.rows);
-          mine1 = min(mine0 + per, u.rows);
+          const int mine0 = min(part * per, u.rows), mine = min(per, u.rows - mine0);   // rows that this CTA finishes
           const uint32_t rx = smem_u32(smem + Plan::kOffRx), rx_bar = smem_u32(rx_full);
           constexpr uint32_t kRow = kGrpCols * 4;
-          if (et == 0 && mine0 < mine1) mbar_arrive_expect_tx(rx_full, static_cast<uint32_t>(parts * (mine1 - mine0)) * kRow);
+          float* own = reinterpret_cast<float*>(sW);
+          float* biases = reinterpret_cast<float*>(sT);
+          if (et == 0 && mine > 0) mbar_arrive_expect_tx(rx_full, static_cast<uint32_t>((parts - 1) * mine) * kRow);
+          if (eg == 0) biases[col] = bias;
 #pragma unroll 1
           for (int r0 = eg * 8; r0 < u.rows; r0 += 16) {
             float f[8];
             read8(r0, f);
-            float* to = reinterpret_cast<float*>(sW) + r0 * kGrpCols + col;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) to[i * kGrpCols] = f[i];
+            for (int i = 0; i < 8; ++i) own[(r0 + i) * kGrpCols + col] = f[i];
           }
-          release_acc();
           fence_proxy_async_smem();
           named_bar_sync(1, 32 * kGrpEpiWarps);
-          if (et < parts) {
+          if (et < parts && et != part) {
             const int rows_to = min(per, u.rows - et * per);
             if (rows_to > 0) {
               bulk_copy_dsmem(mapa_shared(rx + static_cast<uint32_t>(part * per) * kRow, et),
@@ -1101,26 +1101,45 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
                               static_cast<uint32_t>(rows_to) * kRow, mapa_shared(rx_bar, et));
             }
           }
-          if (mine0 < mine1) ok = __all_sync(0xffffffffu, mbar_wait(rx_full, 0, abort_flag)) != 0;
-          ok = named_bar_and(1, 32 * kGrpEpiWarps, ok);
+          if (mine > 0) ok = __all_sync(0xffffffffu, mbar_wait(rx_full, 0, abort_flag)) != 0;
           if (!ok) break;
-          const float* sums = reinterpret_cast<const float*>(smem + Plan::kOffRx) + col;
+          cluster_arrive();   // what peers had for this CTA is here
+          arrived = true;
+          // 8 columns of a row per thread
+          const float* sums = reinterpret_cast<const float*>(smem + Plan::kOffRx);
+          const int seg = (et & 15) * 8;
+          const int valid = min(8, p.N - n0 - seg);   // of them inside C
 #pragma unroll 1
-          for (int r = eg * 4; r < mine1 - mine0; r += 8) {
-            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          for (int r = et >> 4; r < mine; r += 2 * kGrpEpiWarps) {
+            float v[8] = {};
 #pragma unroll 1
             for (int c = 0; c < parts; ++c) {   // in CTA order
-#pragma unroll
-              for (int i = 0; i < 4; ++i) v[i] += r + i < per ? sums[(c * per + r + i) * kGrpCols] : 0.0f;
+              const float4* from = reinterpret_cast<const float4*>(
+                  (c == part ? own + (mine0 + r) * kGrpCols : sums + (c * per + r) * kGrpCols) + seg);
+              const float4 x = from[0], y = from[1];
+              v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+              v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
             }
-            const uint32_t dst = smem_u32(buf) + static_cast<uint32_t>(r * kGrpCols + col) * 2u;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) st_shared_u16(dst + i * (kGrpCols * 2), to_16bit(finish(v[i]), bf16));
+            for (int i = 0; i < 8; ++i) v[i] = finish(v[i], biases[seg + i]);
+            const uint4 packed = make_uint4(pack_16bit(v[0], v[1], bf16), pack_16bit(v[2], v[3], bf16),
+                                            pack_16bit(v[4], v[5], bf16), pack_16bit(v[6], v[7], bf16));
+            unsigned short* out = p.C + static_cast<long long>(u.row0 + mine0 + r) * p.ldc + n0 + seg;
+            if (p.c_vec && valid == 8) {
+              *reinterpret_cast<uint4*>(out) = packed;
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const uint32_t w = i < 2 ? packed.x : i < 4 ? packed.y : i < 6 ? packed.z : packed.w;
+                if (i < valid) out[i] = static_cast<unsigned short>(i & 1 ? w >> 16 : w);
+              }
+            }
           }
+          break;   // a split tile is the CTA's last
         }
         // the next tile's staging comes after its accumulator barrier
         named_bar_sync(1, 32 * kGrpEpiWarps);
-        store_rows(p, buf, u.row0 + mine0, mine1 - mine0, n0, et, 32 * kGrpEpiWarps);
+        store_rows(p, buf, u.row0, u.rows, n0, et, 32 * kGrpEpiWarps);
       }
     }
     if (!ok) {
@@ -1133,7 +1152,10 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 128 : 168)
   // ------------------------------------------------------------ teardown
   tc_fence_before();
   __syncthreads();
-  if (csize > 1) cluster_sync();   // no CTA leaves while a peer may still reach its shared memory
+  if (csize > 1) {   // no CTA leaves while a peer may still reach its shared memory
+    if (!arrived) cluster_arrive();
+    cluster_wait();
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc<CG>(tmem_base, Plan::kTmemCols);

@@ -34,7 +34,7 @@ int launch_shrink(const ShrinkParams& sp, bool kmaj, bool bf16, cudaStream_t str
                    p.stride_down % elems == 0 && (kmaj || p.R % elems == 0);
   const bool aligned = reinterpret_cast<uintptr_t>(p.down) % 16 == 0 && p.ld_down % 8 == 0 && p.stride_down % 8 == 0;
   ShrinkFn fn;
-  int cluster = 1, bytes, ranks;
+  int cluster = 1, bytes, ranks, variant;
   if (p.T > kWideFrom && aligned) {
     // 256 rows to a cluster, as many CTAs along K as keep to one per SM with
     // at least 4 K blocks each.
@@ -45,17 +45,7 @@ int launch_shrink(const ShrinkParams& sp, bool kmaj, bool bf16, cudaStream_t str
     while (cluster < 8 && 8 * cluster <= blocks && 2 * cluster * all <= 148) cluster *= 2;
     fn = pick_wide(kmaj, bf16);
     bytes = kWideBytes;
-    static std::atomic<unsigned long long> configured[4];   // devices, per variant
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return capi_fail_cuda(e, "cudaGetDevice");
-    std::atomic<unsigned long long>& known = configured[kmaj * 2 + bf16];
-    const unsigned long long bit = 1ull << (dev & 63);
-    if (!(known.load(std::memory_order_acquire) & bit)) {
-      e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-      if (e != cudaSuccess) return capi_fail_cuda(e, "adapter kernel attribute");
-      known.fetch_or(bit, std::memory_order_acq_rel);
-    }
+    variant = kmaj * 2 + bf16;
   } else {
     // So few rows to a tile that about 256 CTAs share the work (T = 64: 2 rows
     // x 32 clusters of 8), up to the 8 rows of one MMA; along K no more CTAs
@@ -71,7 +61,25 @@ int launch_shrink(const ShrinkParams& sp, bool kmaj, bool bf16, cudaStream_t str
     fn = rt == 1   ? (vec ? pick<1, true>(kmaj, bf16) : pick<1, false>(kmaj, bf16))
          : rt == 2 ? (vec ? pick<2, true>(kmaj, bf16) : pick<2, false>(kmaj, bf16))
                    : (vec ? pick<4, true>(kmaj, bf16) : pick<4, false>(kmaj, bf16));
+    variant = 4 + (rt == 4 ? 2 : rt - 1) * 8 + vec * 4 + kmaj * 2 + bf16;
     bytes = kShrinkWarps * rows * ranks * static_cast<int>(sizeof(float));   // at most 16 KiB
+  }
+  // Once per kernel and device: the dynamic shared memory above 48 KiB, and the
+  // SM's largest shared-memory split.  The product's CTA needs that split, and
+  // an SM changes it only when it is empty: under a smaller one the product's
+  // CTAs did not start before this grid had ended.
+  static std::atomic<unsigned long long> configured[28];   // devices, per variant
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return capi_fail_cuda(e, "cudaGetDevice");
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (!(configured[variant].load(std::memory_order_acquire) & bit)) {
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess && bytes > 48 * 1024) {
+      e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    }
+    if (e != cudaSuccess) return capi_fail_cuda(e, "adapter kernel attribute");
+    configured[variant].fetch_or(bit, std::memory_order_acq_rel);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.tiles * cluster),
@@ -88,7 +96,7 @@ int launch_shrink(const ShrinkParams& sp, bool kmaj, bool bf16, cudaStream_t str
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, p);
+  e = cudaLaunchKernelEx(&cfg, fn, p);
   return e == cudaSuccess ? GEMM_OK : capi_fail_cuda(e, "adapter kernel launch");
 }
 
