@@ -371,13 +371,14 @@ __device__ __forceinline__ uint32_t nonfinite_pair(uint32_t w, bool bf16) {
   return ((w & (bf16 ? 0x7F807F80u : 0x7C007C00u)) + (bf16 ? 0x00800080u : 0x04000400u)) & 0x80008000u;
 }
 
-// The 32 ranks of one row's block as a swizzle-ready row: hi in the first four
-// 16-byte chunks, lo in the last four.
-__device__ __forceinline__ void split_ranks(const float* h, int valid, bool bf16, uint4 (&out)[8]) {
-  uint32_t hi[16], lo[16];
+// RANKS ranks of one row as 16-byte chunks: hi in the first half of them, lo in
+// the second.
+template <int RANKS>
+__device__ __forceinline__ void split_ranks(const float* h, int valid, bool bf16, uint4 (&out)[RANKS / 4]) {
+  uint32_t hi[RANKS / 2], lo[RANKS / 2];
   uint32_t seen = 0;
 #pragma unroll
-  for (int i = 0; i < kLoraRanks; i += 4) {
+  for (int i = 0; i < RANKS; i += 4) {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (i < valid) v = __ldcg(reinterpret_cast<const float4*>(h + i));   // the pitch of h is a multiple of 16 ranks
 #pragma unroll
@@ -394,38 +395,40 @@ __device__ __forceinline__ void split_ranks(const float* h, int valid, bool bf16
   // (inf - inf); a NaN stays in hi too.
   if (seen) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < RANKS / 2; ++i) {
       const uint32_t bad = nonfinite_pair(hi[i], bf16);
       if (bad & 0x8000u) lo[i] &= 0xFFFF0000u;
       if (bad & 0x80000000u) lo[i] &= 0x0000FFFFu;
     }
   }
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
+  for (int c = 0; c < RANKS / 8; ++c) {
     out[c] = make_uint4(hi[4 * c], hi[4 * c + 1], hi[4 * c + 2], hi[4 * c + 3]);
-    out[4 + c] = make_uint4(lo[4 * c], lo[4 * c + 1], lo[4 * c + 2], lo[4 * c + 3]);
+    out[RANKS / 8 + c] = make_uint4(lo[4 * c], lo[4 * c + 1], lo[4 * c + 2], lo[4 * c + 3]);
   }
 }
 
-// Replaces the inf and NaN among the first 32 ranks of a landed `up` tile by
-// zeros; says whether this thread found any.  128 threads, four 16-byte chunks
-// each: a tile stored N x R has them in row `thread`, one stored R x N in rows
-// 0..31 of both atoms.
-__device__ __forceinline__ bool clear_nonfinite(uint8_t* tile, int thread, bool kmaj, bool bf16) {
+// Replaces the inf and NaN among the first 16 `steps` ranks of a landed `up`
+// tile by zeros; says whether this thread found any.  128 threads, two 16-byte
+// chunks each per 16 ranks: a tile stored N x R has them in row `thread`, one
+// stored R x N in rows 0..15 (16..31) of both atoms.
+__device__ __forceinline__ bool clear_nonfinite(uint8_t* tile, int thread, int steps, bool kmaj, bool bf16) {
   uint4* at[4];
   uint32_t seen = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int c = i * 128 + thread;
+    if (i >= 2 * steps) break;
     at[i] = reinterpret_cast<uint4*>(kmaj ? tile + thread * 128 + ((i ^ (thread & 7)) << 4)
-                                          : tile + (c >> 8) * (kBK * 128) + (c & 255) * 16);
+                                          : tile + (i & 1) * (kBK * 128) + ((i >> 1) * 128 + thread) * 16);
     const uint4 v = *at[i];
     seen |= nonfinite_pair(v.x, bf16) | nonfinite_pair(v.y, bf16) | nonfinite_pair(v.z, bf16) | nonfinite_pair(v.w, bf16);
   }
   if (seen == 0) return false;
-#pragma unroll 1
+#pragma unroll
   for (int i = 0; i < 4; ++i) {
+    if (i >= 2 * steps) break;
     unsigned short* h = reinterpret_cast<unsigned short*>(at[i]);
+#pragma unroll 1
     for (int e = 0; e < 8; ++e) {
       if (nonfinite16(h[e], bf16)) h[e] = 0;
     }
@@ -748,8 +751,12 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0 && leader) {
-      // descriptor strides of the two major orders: see gemm_sm100_kernel.cuh
-      const uint32_t w_lbo = p.b_kmaj ? 16 : kBK * 128, w_kstep = p.b_kmaj ? kUmmaK * 2 : kUmmaK * 128;
+      // Descriptors of stage 0 (strides of the two major orders: see
+      // gemm_sm100_kernel.cuh); an address counts in 16 bytes in their lowest
+      // field.
+      const uint64_t w_desc = smem_desc_sw128(smem_u32(sW), p.b_kmaj ? 16 : kBK * 128, 1024);
+      const uint64_t t_desc = smem_desc_sw128(smem_u32(sT), 16, 1024);
+      const uint32_t w_next = (p.b_kmaj ? kUmmaK * 2 : kUmmaK * 128) >> 4;   // 16 of K on
       int stage = 0;
       uint32_t full_par = 0;   // per stage: parity of its next fill
       int acc = 0;
@@ -777,12 +784,11 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
           }
           full_par ^= 1u << stage;
           tc_fence_after();
-          const uint32_t w0 = smem_u32(sW + stage * Plan::kWBytes);
-          const uint32_t t0 = smem_u32(sT + stage * Plan::kTBytes);
+          const uint64_t wd = w_desc + static_cast<uint32_t>(stage * (Plan::kWBytes >> 4));
+          const uint64_t td = t_desc + static_cast<uint32_t>(stage * (Plan::kTBytes >> 4));
 #pragma unroll
           for (int j = 0; j < kBK / kUmmaK; ++j) {
-            mma_f16_ss<CG>(d_tmem, smem_desc_sw128(w0 + j * w_kstep, w_lbo, 1024),
-                           smem_desc_sw128(t0 + j * (kUmmaK * 2), 16, 1024), idesc, (kb > kb0 || j > 0) ? 1u : 0u);
+            mma_f16_ss<CG>(d_tmem, wd + j * w_next, td + j * (kUmmaK * 2 >> 4), idesc, (kb > kb0 || j > 0) ? 1u : 0u);
           }
           mma_commit<CG>(&empty_bar[stage]);
           if (++stage == STAGES) stage = 0;
@@ -791,30 +797,37 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
           ok = ok && mbar_wait(list_bar, list_phase, abort_flag);
           list_phase ^= 1u;
           const uint32_t idesc_up = idesc_16bit(kGrpCols * CG, u.nmma, p.up_kmaj == 0, false, p.bf16 != 0);
-          const uint32_t u_lbo = p.up_kmaj ? 16 : kBK * 128, u_kstep = p.up_kmaj ? kUmmaK * 2 : kUmmaK * 128;
+          const uint64_t up_desc = smem_desc_sw128(smem_u32(sW), p.up_kmaj ? 16 : kBK * 128, 1024);
+          const uint32_t up_next = (p.up_kmaj ? kUmmaK * 2 : kUmmaK * 128) >> 4;
           const int adapters = ok ? list_counts[0] : 0;
           mbar_arrive(list_read_bar);
           const int blocks = rank_blocks * adapters;
-          for (int b = blocks * part / parts; b < blocks * (part + 1) / parts; ++b) {
-            const int steps = min(kLoraRanks, p.R - b / adapters * kLoraRanks) > kUmmaK ? 2 : 1;
+          const int b0 = blocks * part / parts, b1 = blocks * (part + 1) / parts;
+          int next = adapters ? adapters - b0 % adapters : 0;   // blocks up to the next 32 ranks
+          int ranks = p.R - (adapters ? b0 / adapters * kLoraRanks : 0);
+          for (int b = b0; b < b1; ++b) {
             // `up` has landed, h is in place
-            if (!mbar_wait_cluster(&built_bar[stage], (built_par >> stage) & 1u, abort_flag)) {
+            if (!(CG == 2 ? mbar_wait_cluster(&built_bar[stage], (built_par >> stage) & 1u, abort_flag)
+                          : mbar_wait(&built_bar[stage], (built_par >> stage) & 1u, abort_flag))) {
               ok = false;
               break;
             }
             built_par ^= 1u << stage;
             tc_fence_after();
-            const uint32_t w0 = smem_u32(sW + stage * Plan::kWBytes);
-            const uint32_t h0 = smem_u32(sT + stage * Plan::kTBytes);
-            for (int j = 0; j < steps; ++j) {
-              const uint64_t wd = smem_desc_sw128(w0 + j * u_kstep, u_lbo, 1024);
-#pragma unroll
-              for (int lo = 0; lo < 2; ++lo) {
-                mma_f16_ss<CG>(d_tmem, wd, smem_desc_sw128(h0 + lo * 64 + j * (kUmmaK * 2), 16, 1024), idesc_up, 1u);
-              }
+            const uint64_t ud = up_desc + static_cast<uint32_t>(stage * (Plan::kWBytes >> 4));
+            const uint64_t hd = t_desc + static_cast<uint32_t>(stage * (Plan::kTBytes >> 4));
+            mma_f16_ss<CG>(d_tmem, ud, hd, idesc_up, 1u);
+            mma_f16_ss<CG>(d_tmem, ud, hd + 4, idesc_up, 1u);   // lo: 64 bytes on
+            if (ranks > kUmmaK) {
+              mma_f16_ss<CG>(d_tmem, ud + up_next, hd + 2, idesc_up, 1u);
+              mma_f16_ss<CG>(d_tmem, ud + up_next, hd + 6, idesc_up, 1u);
             }
             mma_commit<CG>(&empty_bar[stage]);
             if (++stage == STAGES) stage = 0;
+            if (--next == 0) {
+              next = adapters;
+              ranks -= kLoraRanks;
+            }
           }
         }
         if (!ok) break;
@@ -912,23 +925,28 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
         adapters = all;
         if (!waited) griddep_wait();   // from here on h, the workspace and C
         waited = true;
-        // adapter rows of this CTA's share of the tile: thread gt of a group
-        // builds row gt of every other block
+        // adapter rows of this CTA's share of the tile: a group builds every
+        // other block, its thread gt row gt, or half the ranks of row gt % 64
+        // where there are no more rows
+        constexpr int kRanks = CG == 1 ? kLoraRanks / 2 : kLoraRanks;
+        constexpr int kChunks = kRanks / 8;
         b0 = rank_blocks * adapters * part / parts;
         b1 = rank_blocks * adapters * (part + 1) / parts;
         const bool mixed = adapters > 1 || without > 0;
         const int half = u.nmma / CG;
-        const int tr = rank * half + gt;   // row of the tile
-        const int mine = (gt < half && tr < u.rows) ? row_ids[tr] : -1;
+        const int row = CG == 1 ? gt & 63 : gt, sub = CG == 1 ? gt >> 6 : 0;
+        const int tr = rank * half + row;   // row of the tile
+        const int mine = (row < half && tr < u.rows) ? row_ids[tr] : -1;
         const float* hrow = p.h + static_cast<long long>(u.row0 + tr) * p.h_pitch;
         stage = (stage + kb1 - kb0) % STAGES;
-        uint4 own[8];
+        uint4 own[2 * kChunks];
         int have = -1;   // rank block held in `own`
         int rb = adapters ? b0 / adapters : 0, ai = b0 - rb * adapters;
         for (int b = b0; b < b1; ++b) {
           if (((b - b0) & 1) == eg) {
             if (rb != have) {
-              if (mine >= 0) split_ranks(hrow + rb * kLoraRanks, p.h_pitch - rb * kLoraRanks, bf16, own);
+              const int r0 = rb * kLoraRanks + sub * kRanks;
+              if (mine >= 0) split_ranks<kRanks>(hrow + r0, p.h_pitch - r0, bf16, own);
               have = rb;
             }
             const bool is = mine >= 0 && list[ai] == mine;
@@ -936,12 +954,14 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
             got = mbar_wait(&land_bar[stage], (land_par >> stage) & 1u, abort_flag);
             got = __all_sync(0xffffffffu, got) != 0;
             if (!got) break;
-            if (mixed && clear_nonfinite(sW + stage * Plan::kWBytes, gt, p.up_kmaj != 0, bf16)) odd_flags[turn] = 1;
-            if (gt < half) {
-              uint8_t* dst = sT + stage * Plan::kTBytes + gt * 128;
+            const int steps = p.R - rb * kLoraRanks > kUmmaK ? 2 : 1;   // of 16 ranks
+            if (mixed && clear_nonfinite(sW + stage * Plan::kWBytes, gt, steps, p.up_kmaj != 0, bf16)) odd_flags[turn] = 1;
+            if (row < half && sub < steps) {
+              uint8_t* dst = sT + stage * Plan::kTBytes + row * 128;
 #pragma unroll
-              for (int c = 0; c < 8; ++c) {
-                *reinterpret_cast<uint4*>(dst + ((c ^ (gt & 7)) << 4)) = is ? own[c] : make_uint4(0u, 0u, 0u, 0u);
+              for (int i = 0; i < 2 * kChunks; ++i) {
+                const int c = (i < kChunks ? 0 : kLoraRanks / 8 - kChunks) + sub * kChunks + i;   // hi, then lo
+                *reinterpret_cast<uint4*>(dst + ((c ^ (row & 7)) << 4)) = is ? own[i] : make_uint4(0u, 0u, 0u, 0u);
               }
             }
             fence_proxy_async_smem();
