@@ -700,15 +700,17 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
           const int b0 = blocks * part / parts, b1 = blocks * (part + 1) / parts;
           int rb = adapters ? b0 / adapters : 0, ai = b0 - rb * adapters;
           for (int b = b0; b < b1; ++b) {
+            // the rows' producer loads nothing here, but has to see every phase
+            // of a slot: two of them on, it would take an old one for its own
+            if (issued >= STAGES && !mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) {
+              ok = false;
+              break;
+            }
             if (weights) {
               const int a = list[ai], r0 = rb * kLoraRanks;
               if (++ai == adapters) {
                 ai = 0;
                 ++rb;
-              }
-              if (issued >= STAGES && !mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) {
-                ok = false;
-                break;
               }
               // on a barrier of this CTA: its epilogue warps look the weights over
               mbar_arrive_expect_tx(&land_bar[stage], Plan::kWBytes);

@@ -84,6 +84,14 @@ def test_every_row_its_own_adapter():
         check(ext.lora_gemm(x, W, down, up, ids), *ref_lora(x, W, down, up, ids))
 
 
+@pytest.mark.parametrize("T,K,N,L,R,pattern", [
+    (20000, 64, 64, 2, 1024, "runs"), (20000, 200, 64, 40, 16, "random"),     # single CTAs
+    (5120, 64, 1024, 40, 16, "random"), (21000, 328, 256, 3, 300, "runs")])   # pairs
+def test_many_tiles_with_many_blocks(T, K, N, L, R, pattern):
+    """CTAs that do several tiles, each with more adapter blocks than twice the ring's stages."""
+    _run(T, K, N, L, R, torch.bfloat16, "nk", pattern, scale=False)
+
+
 @pytest.mark.parametrize("T", [40, 300])
 @pytest.mark.parametrize("stored", ["kn", "nk"])
 @pytest.mark.parametrize("where", ["up", "down", "x"])
