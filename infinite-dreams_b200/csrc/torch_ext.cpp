@@ -139,29 +139,19 @@ at::Tensor gemm_ex(const at::Tensor& A, const at::Tensor& B, int64_t cfg_id, dou
   return C;
 }
 
-// Scratch of one call of the operators below: the cached workspace, or, while
-// the stream is being captured, memory of the graph's own pool with its
-// tickets cleared by the graph.  Two graphs captured on one stream may be
-// replayed on two, so they must not share the cached buffer.
-struct Scratch {
-  at::Tensor owned;
-  void* ptr = nullptr;
-  size_t len = 0;
-};
-
-Scratch scratch(const at::Device& dev, cudaStream_t stream, size_t nbytes) {
-  Scratch s;
-  if (nbytes == 0) return s;
-  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) {
-    s.ptr = workspace(dev, stream, nbytes, &s.len);
-    return s;
-  }
-  s.owned = at::empty({static_cast<int64_t>(nbytes)}, at::TensorOptions().dtype(at::kByte).device(dev));
-  s.ptr = s.owned.data_ptr();
-  s.len = nbytes;
-  C10_CUDA_CHECK(cudaMemsetAsync(s.ptr, 0, std::min(nbytes, gemm_workspace_counter_bytes()), stream));
-  return s;
+// Scratch of one call of the operators below, from torch's allocator and not
+// the cached workspace: their launches come in twos (repacking or the low-rank
+// half, then the product), between which another thread's call on the same
+// stream -- a backward pass has a thread of its own -- would overwrite a shared
+// buffer; and two graphs captured on one stream may be replayed on two.
+at::Tensor scratch(const at::Device& dev, size_t nbytes) {
+  if (nbytes == 0) return {};
+  return at::empty({static_cast<int64_t>(nbytes)}, at::TensorOptions().dtype(at::kByte).device(dev));
 }
+
+void* scratch_ptr(const at::Tensor& ws) { return ws.defined() ? ws.data_ptr() : nullptr; }
+
+size_t scratch_bytes(const at::Tensor& ws) { return ws.defined() ? static_cast<size_t>(ws.numel()) : 0; }
 
 bool is_16bit(const at::Tensor& t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }
 
@@ -177,6 +167,31 @@ void check_index(const at::Tensor& t, const at::Tensor& A, int64_t n, const char
   TORCH_CHECK(t.is_cuda() && t.device() == A.device(), name, " must be on the rows' device");
   TORCH_CHECK(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must be int32 or int64");
   TORCH_CHECK(t.dim() == 1 && t.size(0) == n, name, " must be 1D with ", n, " elements");
+}
+
+// Refuses an `out` that certainly shares elements with an operand: two dense
+// blocks whose ranges meet, or two sets of rows of one pitch whose columns do.
+void check_apart(const at::Tensor& out, std::initializer_list<at::Tensor> ts) {
+  const int64_t es = static_cast<int64_t>(out.element_size());
+  auto extent = [&](const at::Tensor& t) {   // elements from the first to the last
+    int64_t n = 1;
+    for (int64_t d = 0; d < t.dim(); ++d) n += (t.size(d) - 1) * t.stride(d);
+    return n;
+  };
+  if (out.numel() == 0) return;
+  const int64_t o0 = reinterpret_cast<int64_t>(out.data_ptr()), o1 = o0 + extent(out) * es;
+  for (const at::Tensor& t : ts) {
+    if (!t.defined() || t.numel() == 0) continue;
+    const int64_t t0 = reinterpret_cast<int64_t>(t.data_ptr()), t1 = t0 + extent(t) * es;
+    if (t1 <= o0 || o1 <= t0) continue;
+    bool meet = extent(t) == t.numel() && extent(out) == out.numel();
+    if (t.dim() == 2 && out.dim() == 2 && t.stride(1) == 1 && out.stride(1) == 1 && t.size(0) > 1 && out.size(0) > 1 &&
+        t.stride(0) == out.stride(0) && t.stride(0) >= std::max(t.size(1), out.size(1))) {
+      const int64_t row = out.stride(0) * es, c = ((t0 - o0) % row + row) % row;   // where t's columns begin in out's rows
+      meet = c < out.size(1) * es || c + t.size(1) * es > row;
+    }
+    TORCH_CHECK(!meet, "out must not share memory with an operand");
+  }
 }
 
 void check_no_grad(const char* what, std::initializer_list<at::Tensor> ts) {
@@ -237,21 +252,23 @@ at::Tensor grouped_gemm(const at::Tensor& A, const at::Tensor& B, const at::Tens
     bvec = bias->contiguous();
   }
   check_no_grad("grouped_gemm computes no gradients: use grouped.grouped_linear, or call it under torch.no_grad()",
-                {A, B, bvec});
+                {A, B, bvec, out.has_value() ? *out : at::Tensor()});
   const c10::cuda::CUDAGuard guard(A.device());
   at::Tensor As = row_operand(A), off = offsets.contiguous();
   auto [Bs, tb, ldb, sb] = stacked_operand(B);
   at::Tensor C = rows_out(out, T, N, A);
+  if (out.has_value()) check_apart(C, {A, B, bvec});
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(A.device().index()).stream();
   const int64_t lda = pitch(As);
-  Scratch ws = scratch(A.device(), stream, gemm_grouped_workspace_bytes(As.data_ptr(), Bs.data_ptr(), T, N, K, E, lda,
-                                                                        ldb, sb, tb));
+  const at::Tensor ws = scratch(A.device(), gemm_grouped_workspace_bytes(As.data_ptr(), Bs.data_ptr(), T, N, K, E, lda,
+                                                                         ldb, sb, tb));
   check_status(gemm_grouped_launch(As.data_ptr(), Bs.data_ptr(), C.data_ptr(), off.data_ptr(),
                                    off.scalar_type() == at::kLong ? 64 : 32, T, N, K, E, lda, ldb, sb,
                                    std::max<int64_t>(pitch(C), N), tb, bvec.defined() ? bvec.data_ptr() : nullptr,
-                                   static_cast<int>(act), out.has_value() ? 0 : 1, dtype_id(A), ws.ptr, ws.len,
+                                   static_cast<int>(act), out.has_value() ? 0 : 1, dtype_id(A), scratch_ptr(ws), scratch_bytes(ws),
                                    stream),
                "gemm_grouped_launch");
+  if (out.has_value()) torch::autograd::impl::bump_version(C);   // a graph that saved `out` notices
   return C;
 }
 
@@ -265,7 +282,8 @@ at::Tensor grouped_gemm_wgrad(const at::Tensor& A, const at::Tensor& G, const at
   TORCH_CHECK(offsets.dim() == 1 && offsets.size(0) >= 2, "offsets must be 1D with at least 2 elements");
   check_index(offsets, A, offsets.size(0), "offsets");
   const int64_t T = A.size(0), K = A.size(1), N = G.size(1), E = offsets.size(0) - 1;
-  check_no_grad("grouped_gemm_wgrad computes no gradients: call it under torch.no_grad()", {A, G});
+  check_no_grad("grouped_gemm_wgrad computes no gradients: call it under torch.no_grad()",
+                {A, G, out.has_value() ? *out : at::Tensor()});
   const c10::cuda::CUDAGuard guard(A.device());
   at::Tensor D = out.has_value() ? *out : at::empty({E, K, N}, A.options().requires_grad(false));
   TORCH_CHECK(D.is_cuda() && D.device() == A.device() && D.scalar_type() == A.scalar_type() && D.dim() == 3 &&
@@ -274,15 +292,17 @@ at::Tensor grouped_gemm_wgrad(const at::Tensor& A, const at::Tensor& G, const at
   auto [Ds, td, ldd, sd] = stacked_operand(D);
   TORCH_CHECK(Ds.data_ptr() == D.data_ptr(), "out must be row-major or a transposed view, its matrices apart");
   at::Tensor As = row_operand(A), Gs = row_operand(G), off = offsets.contiguous();
+  if (out.has_value()) check_apart(D, {A, G});
   // a gradient stored N x K is the product with the operands exchanged
   const at::Tensor &L = td ? Gs : As, &R = td ? As : Gs;
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(A.device().index()).stream();
-  Scratch ws = scratch(A.device(), stream, gemm_grouped_wgrad_workspace_bytes(L.data_ptr(), R.data_ptr(), T, L.size(1),
-                                                                              R.size(1), pitch(L), pitch(R)));
+  const at::Tensor ws = scratch(A.device(), gemm_grouped_wgrad_workspace_bytes(L.data_ptr(), R.data_ptr(), T, L.size(1),
+                                                                               R.size(1), pitch(L), pitch(R)));
   check_status(gemm_grouped_wgrad_launch(L.data_ptr(), R.data_ptr(), Ds.data_ptr(), off.data_ptr(),
                                          off.scalar_type() == at::kLong ? 64 : 32, T, L.size(1), R.size(1), E,
-                                         pitch(L), pitch(R), ldd, sd, dtype_id(A), ws.ptr, ws.len, stream),
+                                         pitch(L), pitch(R), ldd, sd, dtype_id(A), scratch_ptr(ws), scratch_bytes(ws), stream),
                "gemm_grouped_wgrad_launch");
+  if (out.has_value()) torch::autograd::impl::bump_version(D);
   return D;
 }
 
@@ -353,25 +373,26 @@ at::Tensor lora_gemm(const at::Tensor& x, const at::Tensor& W, const at::Tensor&
     bvec = bias->contiguous();
   }
   check_no_grad("lora_gemm is a serving operator and computes no gradients: call it under torch.no_grad()",
-                {x, W, down, up, svec, bvec});
+                {x, W, down, up, svec, bvec, out.has_value() ? *out : at::Tensor()});
   const c10::cuda::CUDAGuard guard(x.device());
   at::Tensor xs = row_operand(x), ids = adapter.contiguous();
   auto [Ws, tw, ldw] = operand(W);
   auto [Ds, td, ldd, sd] = stacked_operand(down);
   auto [Us, tu, ldu, su] = stacked_operand(up);
   at::Tensor C = rows_out(out, T, N, x);
+  if (out.has_value()) check_apart(C, {x, W, down, up, bvec});
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(x.device().index()).stream();
   const int64_t ldx = pitch(xs);
-  Scratch ws = scratch(x.device(), stream,
-                       gemm_lora_workspace_bytes(xs.data_ptr(), Ws.data_ptr(), Us.data_ptr(), T, N, K, L, R, ldx, ldw,
-                                                 tw, ldu, su, tu));
+  const at::Tensor ws = scratch(x.device(), gemm_lora_workspace_bytes(xs.data_ptr(), Ws.data_ptr(), Us.data_ptr(), T, N,
+                                                                      K, L, R, ldx, ldw, tw, ldu, su, tu));
   check_status(gemm_lora_launch(xs.data_ptr(), Ws.data_ptr(), Ds.data_ptr(), Us.data_ptr(), C.data_ptr(),
                                 ids.data_ptr(), ids.scalar_type() == at::kLong ? 64 : 32, T, N, K, L, R, ldx, ldw, tw,
                                 ldd, sd, td, ldu, su, tu, std::max<int64_t>(pitch(C), N),
                                 svec.defined() ? svec.data_ptr<float>() : nullptr,
-                                bvec.defined() ? bvec.data_ptr() : nullptr, static_cast<int>(act), dtype_id(x), ws.ptr,
-                                ws.len, stream),
+                                bvec.defined() ? bvec.data_ptr() : nullptr, static_cast<int>(act), dtype_id(x), scratch_ptr(ws),
+                                scratch_bytes(ws), stream),
                "gemm_lora_launch");
+  if (out.has_value()) torch::autograd::impl::bump_version(C);
   return C;
 }
 

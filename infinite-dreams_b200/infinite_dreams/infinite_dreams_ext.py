@@ -244,21 +244,18 @@ def gemm_ex(A: torch.Tensor, B: torch.Tensor, *, alpha: float = 1.0, beta: float
     return out
 
 
-def _scratch(device: torch.device, stream: torch.cuda.Stream, nbytes: int):
-    """(keep-alive, pointer, bytes) of one call's workspace.
+def _scratch(device: torch.device, nbytes: int):
+    """(keep-alive, pointer, bytes) of one call's workspace, from torch's allocator and not the cached one.
 
-    While the stream is captured the memory comes from the graph's own pool,
-    its tickets cleared by the graph: two graphs captured on one stream may be
-    replayed on two, so they must not share the cached buffer.
+    These operators' launches come in twos (repacking or the low-rank half,
+    then the product), between which another thread's call on the same stream
+    would overwrite a shared buffer; and two graphs captured on one stream may
+    be replayed on two.
     """
     if nbytes == 0:
         return None, None, 0
-    if torch.cuda.is_current_stream_capturing():
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        ws[:int(lib.gemm_workspace_counter_bytes())].zero_()
-        return ws, ws.data_ptr(), nbytes
-    ptr, size = _workspace(device, stream, nbytes)
-    return None, ptr, size
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr(), nbytes
 
 
 def _is_16bit(t) -> bool:
@@ -284,6 +281,32 @@ def _check_index(t, A: torch.Tensor, n: int, name: str) -> None:
         raise RuntimeError(f"{name} must be int32 or int64")
     if t.dim() != 1 or t.size(0) != n:
         raise RuntimeError(f"{name} must be 1D with {n} elements")
+
+
+def _check_apart(out: torch.Tensor, *tensors) -> None:
+    """Refuses an out that certainly shares elements with an operand: two dense
+    blocks whose ranges meet, or two sets of rows of one pitch whose columns do."""
+    def extent(t):   # elements from the first to the last
+        return 1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+    if out.numel() == 0:
+        return
+    es = out.element_size()
+    o0 = out.data_ptr()
+    o1 = o0 + extent(out) * es
+    for t in tensors:
+        if t is None or t.numel() == 0:
+            continue
+        t0 = t.data_ptr()
+        if t0 + extent(t) * es <= o0 or o1 <= t0:
+            continue
+        meet = extent(t) == t.numel() and extent(out) == out.numel()
+        if (t.dim() == 2 and out.dim() == 2 and t.stride(1) == 1 and out.stride(1) == 1 and t.size(0) > 1
+                and out.size(0) > 1 and t.stride(0) == out.stride(0) and t.stride(0) >= max(t.size(1), out.size(1))):
+            row = out.stride(0) * es
+            c = (t0 - o0) % row   # where t's columns begin in out's rows
+            meet = c < out.size(1) * es or c + t.size(1) * es > row
+        if meet:
+            raise RuntimeError("out must not share memory with an operand")
 
 
 def _check_no_grad(what: str, *tensors) -> None:
@@ -335,7 +358,7 @@ def grouped_gemm(A: torch.Tensor, B: torch.Tensor, offsets: torch.Tensor, *, bia
     synchronises, and offsets that decrease or leave [0, T] are clamped and
     reported by ``check_device_errors``.  Groups may be empty.  Rows outside
     [offsets[0], offsets[E]) are zero in a new ``out`` and left as they are
-    in a given one.  The input gradient of a plain product is
+    in a given one, which must not share memory with an operand.  The input gradient of a plain product is
     ``grouped_gemm(dy, B.transpose(1, 2), offsets)``.  At most 1024 groups.
     """
     if activation not in _capi.ACTIVATIONS:
@@ -365,21 +388,25 @@ def grouped_gemm(A: torch.Tensor, B: torch.Tensor, offsets: torch.Tensor, *, bia
             raise RuntimeError("bias must be (E x N)")
         bias = bias.contiguous()
     _check_no_grad("grouped_gemm computes no gradients: use grouped.grouped_linear, or call it under "
-                   "torch.no_grad()", A, B, bias)
+                   "torch.no_grad()", A, B, bias, out)
     with torch.cuda.device(A.device):
         As, off = _row_operand(A), offsets.contiguous()
         Bs, tb, ldb, sb = _stacked_operand(B)
         C = _rows_out(out, T, N, A)
+        if out is not None:
+            _check_apart(C, A, B, bias)
         stream = torch.cuda.current_stream(A.device)
         lda = _pitch(As)
         need = lib.gemm_grouped_workspace_bytes(As.data_ptr(), Bs.data_ptr(), T, N, K, E, lda, ldb, sb, tb)
-        keep, ws_ptr, ws_len = _scratch(A.device, stream, need)
+        keep, ws_ptr, ws_len = _scratch(A.device, need)
         st = lib.gemm_grouped_launch(As.data_ptr(), Bs.data_ptr(), C.data_ptr(), off.data_ptr(),
                                      64 if off.dtype == torch.int64 else 32, T, N, K, E, lda, ldb, sb,
                                      max(_pitch(C), N), tb, bias.data_ptr() if bias is not None else None, act,
                                      0 if out is not None else 1, _dtype_id(A), ws_ptr, ws_len,
                                      stream.cuda_stream or None)
         _capi.check(st, "gemm_grouped_launch")
+    if out is not None:
+        torch.autograd.graph.increment_version(C)   # a graph that saved out notices
     return C
 
 
@@ -407,7 +434,7 @@ def grouped_gemm_wgrad(A: torch.Tensor, G: torch.Tensor, offsets: torch.Tensor, 
         raise RuntimeError("offsets must be 1D with at least 2 elements")
     _check_index(offsets, A, offsets.size(0), "offsets")
     (T, K), N, E = A.shape, G.size(1), offsets.size(0) - 1
-    _check_no_grad("grouped_gemm_wgrad computes no gradients: call it under torch.no_grad()", A, G)
+    _check_no_grad("grouped_gemm_wgrad computes no gradients: call it under torch.no_grad()", A, G, out)
     with torch.cuda.device(A.device):
         D = torch.empty((E, K, N), dtype=A.dtype, device=A.device) if out is None else out
         if D.device != A.device or D.dtype != A.dtype or tuple(D.shape) != (E, K, N):
@@ -415,17 +442,21 @@ def grouped_gemm_wgrad(A: torch.Tensor, G: torch.Tensor, offsets: torch.Tensor, 
         Ds, td, ldd, sd = _stacked_operand(D)
         if Ds.data_ptr() != D.data_ptr():
             raise RuntimeError("out must be row-major or a transposed view, its matrices apart")
+        if out is not None:
+            _check_apart(D, A, G)
         As, Gs, off = _row_operand(A), _row_operand(G), offsets.contiguous()
         L, R = (Gs, As) if td else (As, Gs)   # a gradient stored N x K: the operands exchanged
         stream = torch.cuda.current_stream(A.device)
         need = lib.gemm_grouped_wgrad_workspace_bytes(L.data_ptr(), R.data_ptr(), T, L.size(1), R.size(1), _pitch(L),
                                                       _pitch(R))
-        keep, ws_ptr, ws_len = _scratch(A.device, stream, need)
+        keep, ws_ptr, ws_len = _scratch(A.device, need)
         st = lib.gemm_grouped_wgrad_launch(L.data_ptr(), R.data_ptr(), Ds.data_ptr(), off.data_ptr(),
                                            64 if off.dtype == torch.int64 else 32, T, L.size(1), R.size(1), E,
                                            _pitch(L), _pitch(R), ldd, sd, _dtype_id(A), ws_ptr, ws_len,
                                            stream.cuda_stream or None)
         _capi.check(st, "gemm_grouped_wgrad_launch")
+    if out is not None:
+        torch.autograd.graph.increment_version(D)   # a graph that saved out notices
     return D
 
 
@@ -480,18 +511,20 @@ def lora_gemm(x: torch.Tensor, W: torch.Tensor, down: torch.Tensor, up: torch.Te
             raise RuntimeError("bias must be (N)")
         bias = bias.contiguous()
     _check_no_grad("lora_gemm is a serving operator and computes no gradients: call it under torch.no_grad()",
-                   x, W, down, up, scale, bias)
+                   x, W, down, up, scale, bias, out)
     with torch.cuda.device(x.device):
         xs, ids = _row_operand(x), adapter.contiguous()
         Ws, tw, ldw = _operand(W)
         Ds, td, ldd, sd = _stacked_operand(down)
         Us, tu, ldu, su = _stacked_operand(up)
         C = _rows_out(out, T, N, x)
+        if out is not None:
+            _check_apart(C, x, W, down, up, bias)
         stream = torch.cuda.current_stream(x.device)
         ldx = _pitch(xs)
         need = lib.gemm_lora_workspace_bytes(xs.data_ptr(), Ws.data_ptr(), Us.data_ptr(), T, N, K, L, R, ldx, ldw, tw,
                                              ldu, su, tu)
-        keep, ws_ptr, ws_len = _scratch(x.device, stream, need)
+        keep, ws_ptr, ws_len = _scratch(x.device, need)
         st = lib.gemm_lora_launch(xs.data_ptr(), Ws.data_ptr(), Ds.data_ptr(), Us.data_ptr(), C.data_ptr(),
                                   ids.data_ptr(), 64 if ids.dtype == torch.int64 else 32, T, N, K, L, R, ldx, ldw, tw,
                                   ldd, sd, td, ldu, su, tu, max(_pitch(C), N),
@@ -499,6 +532,8 @@ def lora_gemm(x: torch.Tensor, W: torch.Tensor, down: torch.Tensor, up: torch.Te
                                   bias.data_ptr() if bias is not None else None, act, _dtype_id(x), ws_ptr, ws_len,
                                   stream.cuda_stream or None)
         _capi.check(st, "gemm_lora_launch")
+    if out is not None:
+        torch.autograd.graph.increment_version(C)   # a graph that saved out notices
     return C
 
 
