@@ -16,7 +16,11 @@
 // 128 (256).  A group's rows are cut into equal tiles of at most TM rows.
 //
 //   CG = 2, TM = 256: a CTA pair owns 256 columns x up to 256 rows; each CTA
-//     loads its 128 columns of B and half of the rows (no multicast).
+//     loads its 128 columns of B and half of the rows (no multicast).  What
+//     bounds it is the way from L2 (10 TB/s over the machine) and the power cap.
+//   CG = 2, TM = 512: two such tiles one below the other share the K blocks of
+//     B: 48 KiB per stage and CTA instead of twice 32.  Each has an accumulator
+//     of its own, so the next tile starts on one while the other is read out.
 //   CG = 1, TM = 64: a cluster of 1, 2, 4 or 8 CTAs owns 128 columns x up to 64
 //     rows, each CTA a share of K; the ring holds over 100 KiB of weights in
 //     flight.  For groups of few rows, whose cost is reading the weights
@@ -125,8 +129,10 @@ constexpr int kGrpRowsWarp = 2 + kGrpEpiWarps;   // producer of the rows; warp 0
 template <int CG, int TM, int STAGES, bool LORA>
 struct GroupedPlan {
   static constexpr int kStep = 16 * CG;                  // granularity of a tile's rows (MMA N)
+  static constexpr int kSubs = TM > 256 ? 2 : 1;         // parts of a tile's rows, each an accumulator of its own
+  static constexpr int kSubRows = TM / kSubs;
   static constexpr int kTokRows = TM / CG;               // rows of A held by this CTA
-  static constexpr int kBoxRows = TM >= 256 ? 128 : 16;  // rows per TMA box of A
+  static constexpr int kSubBytes = kSubRows / CG * kBK * 2;   // rows of one part
   static constexpr int kWBytes = kGrpCols * kBK * 2;     // 16 KiB of B
   static constexpr int kTBytes = kTokRows * kBK * 2;
   static constexpr int kStageBytes = kWBytes + kTBytes;
@@ -144,8 +150,8 @@ struct GroupedPlan {
   static constexpr int kOffTiles = kOffRows + (kMaxGroups + 1) * 4;  // first tile of each group [E + 1]
   static constexpr int kUsed = kOffTiles + (kMaxGroups + 1) * 4;
   static constexpr int kDynamicBytes = kUsed + 1024;
-  static constexpr uint32_t kTmemCols = 2 * TM;          // two accumulators
-  static_assert(TM % (32 * CG) == 0 && TM <= 256, "rows of a tile");
+  static constexpr uint32_t kTmemCols = 2 * kSubRows;    // two accumulators
+  static_assert(TM % (32 * CG) == 0 && kSubRows <= 256 && kSubs * kSubRows == TM, "rows of a tile");
   static_assert(kTBytes % 1024 == 0 && kOffOut % 1024 == 0, "swizzled tiles need 1024-byte alignment");
   static_assert(kDynamicBytes <= 227 * 1024, "shared memory of one CTA");
 };
@@ -284,17 +290,30 @@ __device__ __forceinline__ int find_group(const int* first, int E, int u) {
   return lo;
 }
 
-// The tiles of one CTA (pair): whole ones, `stride` apart, and then perhaps one
-// that the CTAs of its cluster split along K.  A last wave with no more tiles
-// than clusters is split; it takes half the time with clusters of two (32 rows
-// over 64 experts, 200 tiles on 148 CTAs: the 52 of the second wave).
+// The tiles of one CTA (pair): whole ones, `stride` apart, and then perhaps a
+// share of the last, short wave's.
+//  * Single CTAs: a last wave with no more tiles than clusters is split along
+//    K over the CTAs of each cluster; it takes half the time with clusters of
+//    two (32 rows over 64 experts, 200 tiles on 148 CTAs: the 52 of the second
+//    wave).
+//  * Pairs with tiles of two parts: a last wave that half of the pairs could do
+//    is done part by part by all of them.
 struct GroupedWalk {
   int t, stride;
   int whole;       // tiles that are walked whole
-  int split_tile;  // at or past `tiles`: none
+  int split_tile;  // the one to split along K; at or past `tiles`: none
   int tiles;
+  int part;        // the only part of the tile that next() gave, or -1
 
+  template <int SUBS>
   __device__ __forceinline__ bool next(int& tile, bool& split) {
+    if (SUBS == 2) {
+      const int i = t - whole;
+      part = i < 0 ? -1 : i & 1;
+      tile = i < 0 ? t : whole + (i >> 1);
+      t += stride;
+      return tile < tiles;
+    }
     split = t >= whole;
     tile = split ? split_tile : t;
     if (split) split_tile = tiles;
@@ -303,10 +322,15 @@ struct GroupedWalk {
   }
 };
 
-__device__ __forceinline__ GroupedWalk grouped_walk(int tiles, int cta, int ctas, int cluster, int clusters) {
+template <int CG, int SUBS>
+__device__ __forceinline__ GroupedWalk grouped_walk(int tiles, int cta, int ctas, int worker, int workers) {
+  if (CG == 2) {
+    const int waves = tiles / workers, rest = tiles - waves * workers;
+    return {worker, workers, SUBS == 2 && 2 * rest <= workers ? waves * workers : tiles, tiles, tiles, -1};
+  }
   const int waves = tiles / ctas, rest = tiles - waves * ctas;
-  const int whole = rest <= clusters ? waves * ctas : tiles;
-  return {cta, ctas, whole, whole + cluster, tiles};
+  const int whole = rest <= workers ? waves * ctas : tiles;
+  return {cta, ctas, whole, whole + worker, tiles, -1};
 }
 
 struct GroupedUnit {
@@ -316,10 +340,21 @@ struct GroupedUnit {
   int row0;   // first row of A and C
   int rows;   // rows of C to store
   int nmma;   // MMA N: rows rounded up
+  int subs;   // parts of the rows; `rows` and `nmma` are those of the first
+  int rest;   // rows of the second
+
+  // Moves on to the second part.
+  template <int STEP>
+  __device__ __forceinline__ void second() {
+    row0 += rows;
+    rows = rest;
+    nmma = (rest + STEP - 1) / STEP * STEP;
+  }
 };
 
 template <int CG, int TM>
-__device__ __forceinline__ GroupedUnit grouped_unit(const GroupedParams& p, const int* rows, const int* first, int t) {
+__device__ __forceinline__ GroupedUnit grouped_unit(const GroupedParams& p, const int* rows, const int* first, int t,
+                                                    int part) {
   GroupedUnit u;
   u.e = find_group(first, p.E, t);
   int count, tr;
@@ -338,6 +373,19 @@ __device__ __forceinline__ GroupedUnit grouped_unit(const GroupedParams& p, cons
   }
   u.row0 = rows[u.e] + u.rt * tr;
   u.rows = min(tr, rows[u.e + 1] - u.row0);
+  u.subs = 1;
+  u.rest = 0;
+  if (TM > 256 && u.rows > 256) {
+    const int half = ((u.rows + 1) / 2 + 31) / 32 * 32;
+    u.subs = 2;
+    u.rest = u.rows - half;
+    u.rows = half;
+  }
+  if (TM > 256 && part >= 0) {   // one part only, which may have no rows
+    if (part == 1) u.row0 += u.rows, u.rows = u.rest;
+    u.subs = 1;
+    u.rest = 0;
+  }
   u.nmma = (u.rows + 16 * CG - 1) / (16 * CG) * (16 * CG);
   return u;
 }
@@ -637,11 +685,10 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
     scan_groups<kGrpThreads>(p.offsets, p.off64, p.E, p.T, grp_rows, grp_tiles, scan, p.err, tiles_of);
   }
   const int num_tiles = grp_tiles[p.E];
-  GroupedWalk walk = CG == 2 ? GroupedWalk{worker, workers, num_tiles, num_tiles, num_tiles}
-                             : grouped_walk(num_tiles, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x), worker,
-                                            workers);
+  GroupedWalk walk = grouped_walk<CG, Plan::kSubs>(num_tiles, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x),
+                                                   worker, workers);
   int t;
-  bool split;
+  bool split = false;
   bool arrived = false;   // at the cluster barrier of the teardown
 
   if (warp == 0 || warp == kGrpRowsWarp) {
@@ -659,18 +706,32 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
       uint32_t full_par = 0, land_par = 0, on_land = 0;
       bool ok = true;
       uint32_t list_phase = 0;
-      while (ok && walk.next(t, split)) {
+      while (ok && walk.next<Plan::kSubs>(t, split)) {
         const int parts = split ? csize : 1, part = split ? crank : 0;   // of the tile's K
         const int kb0 = split ? split_kb0 : 0, kb1 = split ? split_kb1 : p.kb_total;
-        const GroupedUnit u = grouped_unit<CG, TM>(p, grp_rows, grp_tiles, t);
-        const int half = u.nmma / CG;
-        const int arow = u.row0 + rank * half;
+        const GroupedUnit u = grouped_unit<CG, TM>(p, grp_rows, grp_tiles, t, walk.part);
+        if (Plan::kSubs == 2 && u.rows == 0) continue;
         const int bcol = (u.tn * CG + rank) * kGrpCols;
         // the smallest box that holds this CTA's rows
-        int box = p.first_box;
-        while (box + 1 < box_count(TM) && half <= box_rows(TM, box + 1)) ++box;
+        auto box_of = [&](int half) {
+          int box = p.first_box;
+          while (box + 1 < box_count(TM) && half <= box_rows(TM, box + 1)) ++box;
+          return box;
+        };
+        const int half = u.nmma / CG, box = box_of(half);
+        const int arow = u.row0 + rank * half;
         const CUtensorMap* map_a = &maps.a[box];
-        const uint32_t bytes = weights ? Plan::kWBytes : static_cast<uint32_t>(box_rows(TM, box)) * 128u;
+        uint32_t bytes = weights ? Plan::kWBytes : static_cast<uint32_t>(box_rows(TM, box)) * 128u;
+        int arow2 = 0;
+        const CUtensorMap* map_a2 = nullptr;
+        if (Plan::kSubs == 2 && u.subs == 2) {
+          GroupedUnit v = u;
+          v.template second<Plan::kStep>();
+          const int box2 = box_of(v.nmma / CG);
+          arow2 = v.row0 + rank * (v.nmma / CG);
+          map_a2 = &maps.a[box2];
+          if (!weights) bytes += static_cast<uint32_t>(box_rows(TM, box2)) * 128u;
+        }
         const WeightBoxes wb = weight_boxes(p.b_kmaj != 0, p.b_wide != 0, kb0 * kBK, bcol, u.e);
         for (int kb = kb0; kb < kb1; ++kb) {
           if (issued >= STAGES && !mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) {
@@ -683,6 +744,9 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
             load_weights<CG == 2>(dst, &maps.b, bar, wb, kb - kb0);
           } else {
             tma_load_2d_at<CG == 2>(dst, map_a, bar, kb * kBK, arow);
+            if (Plan::kSubs == 2 && map_a2) {
+              tma_load_2d_at<CG == 2>(dst + Plan::kSubBytes, map_a2, bar, kb * kBK, arow2);
+            }
           }
           full_par ^= 1u << stage;
           on_land &= ~(1u << stage);
@@ -761,24 +825,35 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
       const uint32_t w_next = (p.b_kmaj ? kUmmaK * 2 : kUmmaK * 128) >> 4;   // 16 of K on
       int stage = 0;
       uint32_t full_par = 0;   // per stage: parity of its next fill
-      int acc = 0;
-      uint32_t acc_phase = 0;
-      int count = 0;
+      int acc = 0;                      // the next accumulator
+      uint32_t acc_used = 0, acc_par = 0;   // per accumulator: used before; parity of its next release
       uint32_t built_par = 0, list_phase = 0;
       bool ok = true;
-      while (ok && walk.next(t, split)) {
+      while (ok && walk.next<Plan::kSubs>(t, split)) {
         const int parts = split ? csize : 1, part = split ? crank : 0;   // of the tile's K
         const int kb0 = split ? split_kb0 : 0, kb1 = split ? split_kb1 : p.kb_total;
         if (p.kb_total == 0) break;   // the epilogue writes act(bias) by itself
-        const GroupedUnit u = grouped_unit<CG, TM>(p, grp_rows, grp_tiles, t);
+        const GroupedUnit u = grouped_unit<CG, TM>(p, grp_rows, grp_tiles, t, walk.part);
+        if (Plan::kSubs == 2 && u.rows == 0) continue;
         const uint32_t idesc = idesc_16bit(kGrpCols * CG, u.nmma, p.b_kmaj == 0, false, p.bf16 != 0);
-        if (count >= 2 && !mbar_wait(&tempty_bar[acc], acc_phase ^ 1u, abort_flag)) {
+        const uint32_t idesc2 = Plan::kSubs == 2 ? idesc_16bit(kGrpCols * CG, (u.rest + 31) / 32 * 32, p.b_kmaj == 0,
+                                                              false, p.bf16 != 0)
+                                                 : 0u;
+        // takes accumulator `a` once its last tile has been read out
+        auto take_acc = [&](int a) {
+          const uint32_t bit = 1u << a;
+          if ((acc_used & bit) && !mbar_wait(&tempty_bar[a], (acc_par & bit) ? 1u : 0u, abort_flag)) return false;
+          if (acc_used & bit) acc_par ^= bit;
+          acc_used |= bit;
+          tc_fence_after();
+          return true;
+        };
+        if (!take_acc(acc)) {
           ok = false;
           break;
         }
-        ++count;
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * TM);
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * Plan::kSubRows);
+        const uint32_t d_tmem2 = tmem_base + static_cast<uint32_t>((acc ^ 1) * Plan::kSubRows);
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&full_bar[stage], (full_par >> stage) & 1u, abort_flag)) {
             ok = false;
@@ -791,6 +866,18 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
 #pragma unroll
           for (int j = 0; j < kBK / kUmmaK; ++j) {
             mma_f16_ss<CG>(d_tmem, wd + j * w_next, td + j * (kUmmaK * 2 >> 4), idesc, (kb > kb0 || j > 0) ? 1u : 0u);
+          }
+          if (Plan::kSubs == 2 && u.subs == 2) {
+            if (kb == kb1 - 1) mma_commit<CG>(&tfull_bar[acc]);   // its rows can be read out beside the second part's MMAs
+            if (kb == kb0 && !take_acc(acc ^ 1)) {
+              ok = false;
+              break;
+            }
+#pragma unroll
+            for (int j = 0; j < kBK / kUmmaK; ++j) {
+              mma_f16_ss<CG>(d_tmem2, wd + j * w_next, td + (Plan::kSubBytes >> 4) + j * (kUmmaK * 2 >> 4), idesc2,
+                             (kb > kb0 || j > 0) ? 1u : 0u);
+            }
           }
           mma_commit<CG>(&empty_bar[stage]);
           if (++stage == STAGES) stage = 0;
@@ -833,9 +920,8 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
           }
         }
         if (!ok) break;
-        mma_commit<CG>(&tfull_bar[acc]);
-        acc ^= 1;
-        if (acc == 0) acc_phase ^= 1u;
+        mma_commit<CG>(&tfull_bar[Plan::kSubs == 2 && u.subs == 2 ? acc ^ 1 : acc]);
+        if (u.subs == 1) acc ^= 1;
       }
       if (!ok) {
         *abort_flag = 1;
@@ -867,7 +953,7 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
     uint32_t listed = 0;   // tiles whose adapters were listed
     if (p.zero_rest) zero_rows(p, grp_rows[0], grp_rows[p.E], et, 32 * kGrpEpiWarps);
     int acc = 0, turn = 0;
-    uint32_t acc_phase = 0;
+    uint32_t acc_par = 0;   // per accumulator: parity of its next fill
     bool ok = true;
     auto release_acc = [&] {
       tc_fence_before();
@@ -879,13 +965,24 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
           mbar_arrive_cluster_relaxed(tempty_remote0 + static_cast<uint32_t>(acc * 8));
         }
       }
+      acc_par ^= 1u << acc;
       acc ^= 1;
-      if (acc == 0) acc_phase ^= 1u;
     };
-    while (walk.next(t, split)) {
+    GroupedUnit u;
+    int sub = 1;   // the part of the tile that comes next
+    u.subs = 1;
+    while (true) {
+      if (Plan::kSubs == 1 || sub == u.subs) {
+        if (!walk.next<Plan::kSubs>(t, split)) break;
+        u = grouped_unit<CG, TM>(p, grp_rows, grp_tiles, t, walk.part);
+        sub = 1;
+        if (Plan::kSubs == 2 && u.rows == 0) continue;
+      } else {
+        u.template second<Plan::kStep>();
+        ++sub;
+      }
       const int parts = split ? csize : 1, part = split ? crank : 0;   // of the tile's K
       const int kb0 = split ? split_kb0 : 0, kb1 = split ? split_kb1 : p.kb_total;
-      const GroupedUnit u = grouped_unit<CG, TM>(p, grp_rows, grp_tiles, t);
       const int n0 = (u.tn * CG + rank) * kGrpCols;
       const int n = n0 + col;
       const float bias =
@@ -989,14 +1086,14 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
       }
       // One lane per warp waits for the accumulator; all warps then take the
       // same decision, so none is left at a later barrier.
-      if (got && p.kb_total > 0 && lane == 0) got = mbar_wait(&tfull_bar[acc], acc_phase, abort_flag);
+      if (got && p.kb_total > 0 && lane == 0) got = mbar_wait(&tfull_bar[acc], (acc_par >> acc) & 1u, abort_flag);
       got = __shfl_sync(0xffffffffu, got ? 1 : 0, 0) != 0;
       ok = named_bar_and(1, 32 * kGrpEpiWarps, got);
       if (!ok) break;
       tc_fence_after();
       const bool odd = LORA && odd_flags[turn] != 0;
       turn = turn == 2 ? 0 : turn + 1;
-      const uint32_t tbase = tmem_base + (static_cast<uint32_t>(ew * 32) << 16) + static_cast<uint32_t>(acc * TM);
+      const uint32_t tbase = tmem_base + (static_cast<uint32_t>(ew * 32) << 16) + static_cast<uint32_t>(acc * Plan::kSubRows);
 
       auto finish = [&](float v, float bias) {
         v += bias;

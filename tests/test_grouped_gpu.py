@@ -54,6 +54,25 @@ def test_epilogue(act, counts, dtype):
     _run(counts, 320, 264, dtype, "nk", bias=True, act=act)
 
 
+@pytest.mark.parametrize("counts,N", [
+    ([8192], 4096), ([3001, 0, 257, 4100], 4096), ([5000, 3400], 4096), ([2000, 0, 5600, 500, 1093], 4096),
+    ([1100, 5700, 1400], 4120), ([9000, 257, 30], 4000), ([2560, 5120, 1], 5001)], ids=str)
+@pytest.mark.parametrize("stored,dtype", [("kn", torch.float16), ("nk", torch.bfloat16)])
+def test_tall_tiles(counts, N, stored, dtype):
+    """Large groups: two row parts to a tile, one, and last waves done part by part (or not)."""
+    _run(counts, 136, N, dtype, stored, bias=True, act="gelu", first=3, spare=5)
+    _run(counts, 1000, N, dtype, stored)
+
+
+def test_tall_tiles_without_reduction():
+    from infinite_dreams import infinite_dreams_ext as ext
+    b = randn((2, 4096), torch.float16, 1)
+    out = ext.grouped_gemm(torch.empty(8192, 0, dtype=torch.float16, device="cuda"),
+                           torch.empty(2, 0, 4096, dtype=torch.float16, device="cuda"),
+                           counts_to_offsets([3000, 5192]), bias=b)
+    assert torch.equal(out[:3000], b[:1].expand(3000, -1)) and torch.equal(out[3000:], b[1:].expand(5192, -1))
+
+
 def test_no_reduction():
     """K = 0: act(bias) in the rows of the groups."""
     _run([3, 0, 70], 0, 200, torch.bfloat16, bias=True, act="gelu")
