@@ -533,6 +533,33 @@ __device__ __forceinline__ float gelu(float x) {
   return fmaf(-a, q * t * e, 0.5f * (x + fabsf(x)));
 }
 
+// gelu of two values with packed arithmetic, operation for operation the same.
+__device__ __forceinline__ void gelu2(float& x0, float& x1) {
+  const float a0 = fminf(fabsf(x0), 20.0f), a1 = fminf(fabsf(x1), 20.0f);
+  const uint64_t a = pack_f32x2(a0, a1);
+  const uint64_t d = fma_f32x2(pack_f32x2(0.31f, 0.31f), a, pack_f32x2(1.0f, 1.0f));
+  const uint64_t s = mul_f32x2(mul_f32x2(a, a), pack_f32x2(-0.72134752f, -0.72134752f));
+  float d0, d1, s0, s1, t0, t1, e0, e1;
+  unpack_f32x2(d, d0, d1);
+  unpack_f32x2(s, s0, s1);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t0) : "f"(d0));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t1) : "f"(d1));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(s0));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(s1));
+  const uint64_t t = pack_f32x2(t0, t1);
+  uint64_t q = pack_f32x2(0.035917483f, 0.035917483f);
+  q = fma_f32x2(q, t, pack_f32x2(-0.14193712f, -0.14193712f));
+  q = fma_f32x2(q, t, pack_f32x2(0.15567426f, 0.15567426f));
+  q = fma_f32x2(q, t, pack_f32x2(-0.015496778f, -0.015496778f));
+  q = fma_f32x2(q, t, pack_f32x2(0.11044533f, 0.11044533f));
+  q = fma_f32x2(q, t, pack_f32x2(0.10766225f, 0.10766225f));
+  q = fma_f32x2(q, t, pack_f32x2(0.12407906f, 0.12407906f));
+  q = fma_f32x2(q, t, pack_f32x2(0.1236556f, 0.1236556f));
+  q = mul_f32x2(mul_f32x2(q, t), pack_f32x2(e0, e1));
+  const uint64_t r = mul_f32x2(pack_f32x2(x0 + fabsf(x0), x1 + fabsf(x1)), pack_f32x2(0.5f, 0.5f));
+  unpack_f32x2(fma_f32x2(pack_f32x2(-a0, -a1), q, r), x0, x1);
+}
+
 // `count` staged rows (128 columns of 16 bits each) to C at row `row`, column
 // n0, by `threads` threads.
 __device__ __forceinline__ void store_rows(const GroupedParams& p, const uint8_t* buf, int row, int count, int n0,
@@ -1130,7 +1157,11 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
           const uint32_t dst = smem_u32(buf) + col * 2;
           if (p.act == 2) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) f[i] = gelu(f[i] + bias);
+            for (int i = 0; i < 32; i += 2) {
+              f[i] += bias;
+              f[i + 1] += bias;
+              gelu2(f[i], f[i + 1]);
+            }
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) f[i] = finish(f[i], bias);
