@@ -194,6 +194,12 @@ void check_apart(const at::Tensor& out, std::initializer_list<at::Tensor> ts) {
   }
 }
 
+// A graph that saved `out` notices that it was written; tensors made in
+// inference mode keep no such count.
+void count_write(const at::Tensor& out) {
+  if (!out.is_inference()) torch::autograd::impl::bump_version(out);
+}
+
 void check_no_grad(const char* what, std::initializer_list<at::Tensor> ts) {
   if (!at::GradMode::is_enabled()) return;
   for (const at::Tensor& t : ts) {
@@ -268,7 +274,7 @@ at::Tensor grouped_gemm(const at::Tensor& A, const at::Tensor& B, const at::Tens
                                    static_cast<int>(act), out.has_value() ? 0 : 1, dtype_id(A), scratch_ptr(ws), scratch_bytes(ws),
                                    stream),
                "gemm_grouped_launch");
-  if (out.has_value()) torch::autograd::impl::bump_version(C);   // a graph that saved `out` notices
+  if (out.has_value()) count_write(C);
   return C;
 }
 
@@ -302,7 +308,7 @@ at::Tensor grouped_gemm_wgrad(const at::Tensor& A, const at::Tensor& G, const at
                                          off.scalar_type() == at::kLong ? 64 : 32, T, L.size(1), R.size(1), E,
                                          pitch(L), pitch(R), ldd, sd, dtype_id(A), scratch_ptr(ws), scratch_bytes(ws), stream),
                "gemm_grouped_wgrad_launch");
-  if (out.has_value()) torch::autograd::impl::bump_version(D);
+  if (out.has_value()) count_write(D);
   return D;
 }
 
@@ -392,7 +398,7 @@ at::Tensor lora_gemm(const at::Tensor& x, const at::Tensor& W, const at::Tensor&
                                 bvec.defined() ? bvec.data_ptr() : nullptr, static_cast<int>(act), dtype_id(x), scratch_ptr(ws),
                                 scratch_bytes(ws), stream),
                "gemm_lora_launch");
-  if (out.has_value()) torch::autograd::impl::bump_version(C);
+  if (out.has_value()) count_write(C);
   return C;
 }
 

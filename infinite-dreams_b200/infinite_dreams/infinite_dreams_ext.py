@@ -309,6 +309,12 @@ def _check_apart(out: torch.Tensor, *tensors) -> None:
             raise RuntimeError("out must not share memory with an operand")
 
 
+def _count_write(out: torch.Tensor) -> None:
+    """A graph that saved out notices that it was written; tensors made in inference mode keep no such count."""
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+
+
 def _check_no_grad(what: str, *tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(what)
@@ -406,7 +412,7 @@ def grouped_gemm(A: torch.Tensor, B: torch.Tensor, offsets: torch.Tensor, *, bia
                                      stream.cuda_stream or None)
         _capi.check(st, "gemm_grouped_launch")
     if out is not None:
-        torch.autograd.graph.increment_version(C)   # a graph that saved out notices
+        _count_write(C)
     return C
 
 
@@ -456,7 +462,7 @@ def grouped_gemm_wgrad(A: torch.Tensor, G: torch.Tensor, offsets: torch.Tensor, 
                                            stream.cuda_stream or None)
         _capi.check(st, "gemm_grouped_wgrad_launch")
     if out is not None:
-        torch.autograd.graph.increment_version(D)   # a graph that saved out notices
+        _count_write(D)
     return D
 
 
@@ -533,7 +539,7 @@ def lora_gemm(x: torch.Tensor, W: torch.Tensor, down: torch.Tensor, up: torch.Te
                                   stream.cuda_stream or None)
         _capi.check(st, "gemm_lora_launch")
     if out is not None:
-        torch.autograd.graph.increment_version(C)   # a graph that saved out notices
+        _count_write(C)
     return C
 
 

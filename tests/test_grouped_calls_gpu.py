@@ -67,6 +67,24 @@ def test_out_that_takes_part_in_autograd(ext):
         y.backward()
 
 
+def test_inference_mode(ext):
+    """Weights that ask for gradients and a preallocated out, as a server holds them."""
+    off = counts_to_offsets([10, 20])
+    A, B = randn((30, 64), torch.float16, 1), stacked(2, 64, 64, torch.float16, 2).requires_grad_()
+    W, down, up = (torch.nn.Parameter(w) for w in (randn((64, 64), torch.float16, 3, 0.1),
+                                                   stacked(2, 64, 8, torch.float16, 4),
+                                                   stacked(2, 8, 64, torch.float16, 5)))
+    ids = (torch.arange(30, device="cuda") % 3 - 1).int()
+    plain = torch.empty(30, 64, dtype=torch.float16, device="cuda")
+    with torch.inference_mode():
+        made = torch.empty_like(plain)
+        want = ext.grouped_gemm(A, B, off)
+        for out in (plain, made):
+            assert torch.equal(ext.grouped_gemm(A, B, off, out=out), want)
+            assert torch.equal(ext.lora_gemm(A, W, down, up, ids, out=out), ext.lora_gemm(A, W, down, up, ids))
+        ext.grouped_gemm_wgrad(A, A, off, out=torch.empty(2, 64, 64, dtype=torch.float16, device="cuda"))
+
+
 def test_several_threads(ext):
     """Four threads train and serve on one stream, with operands that are repacked: every pass gives the same bits."""
     from infinite_dreams.grouped import grouped_linear
