@@ -327,11 +327,11 @@ int launch_wgrad(const Operand& a, const Operand& g, const WgradParams& wp, int 
 // Single CTAs of 128 columns x up to 64 rows, or pairs of 256 x up to 256?
 //  * Up to 16 rows per group: the cost is reading the weights once, and single
 //    CTAs with their deep ring do that best (32 rows over 64 experts 2048 x
-//    1024: 28 us).
+//    1024: 25 us against 29).
 //  * More rows: pairs, which read every weight once per 256 rows (4096 rows
-//    over 64 experts 2048 x 1024: 56 us against 72), unless their tiles would
+//    over 64 experts 2048 x 1024: 55 us against 68), unless their tiles would
 //    leave more than half of the machine idle where single CTAs fill it
-//    (64 rows, 4096 x 4096: 32 clusters of 4 against 16 pairs).
+//    (64 rows, 4096 x 4096: 32 clusters of 4 in 13 us against 16 pairs in 26).
 bool small_tiles(int64_t T, int64_t N, int64_t E, int sms) {
   if (T <= 16 * E || N <= kGrpCols) return true;
   const int64_t pairs = (T + 255 * E) / 256 * ((N + 255) / 256);
@@ -345,7 +345,8 @@ bool small_tiles(int64_t T, int64_t N, int64_t E, int sms) {
 // Under the power cap, 8192 rows over 8 experts 4096 x 14336: 769 us against
 // 812 (ragged groups 811 against 852), 4096 x 4096: 223 against 230.  Below:
 // 2048 rows over 2 experts 4096 x 4096 70 us against 57, 4096 rows over 8
-// experts 4096 x 14336 458 us against 427.
+// experts 4096 x 14336 458 us against 427.  (Both columns are medians of calls
+// back to back; the first pair of lines after a second of them.)
 bool tall_tiles(int64_t T, int64_t N, int64_t E, int sms) {
   return T >= 1024 * E && T / 512 * ((N + 255) / 256) >= 3 * (sms / 2);
 }

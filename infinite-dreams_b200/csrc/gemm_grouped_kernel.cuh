@@ -21,18 +21,20 @@
 //   CG = 2, TM = 512: two such tiles one below the other share the K blocks of
 //     B: 48 KiB per stage and CTA instead of twice 32.  Each has an accumulator
 //     of its own, so the next tile starts on one while the other is read out.
-//   CG = 1, TM = 64: a cluster of 1, 2, 4 or 8 CTAs owns 128 columns x up to 64
-//     rows, each CTA a share of K; the ring holds over 100 KiB of weights in
-//     flight.  For groups of few rows, whose cost is reading the weights
-//     (steady state 7.3 TB/s on weights stored K x N, 6.4 stored N x K), and
+//   CG = 1, TM = 64: a CTA owns 128 columns x up to 64 rows; a short last wave
+//     is split along K over the 2, 4 or 8 CTAs of a cluster.  The ring holds
+//     over 100 KiB of weights in flight.  For groups of few rows, whose cost is reading the weights
+//     (steady state 7.3 TB/s on weights stored K x N, 6.2 stored N x K), and
 //     for problems too small to fill the machine with pair tiles.  The
-//     partial sums cross through distributed shared memory: CTA r finishes
-//     every cluster's r-th part of the rows, summing in CTA order.  (Pieces
-//     through global memory with a ticket were measured first: joining two
-//     of them cost 3 us, four times the DSMEM path.)
+//     partial sums cross through distributed shared memory by bulk copies: CTA r
+//     finishes every cluster's r-th part of the rows, summing in CTA order.
+//     (Pieces through global memory with a ticket were measured first: joining
+//     two of them cost 3 us, four times this path.)
 //
-// Roles as in gemm_sm100_kernel.cuh: warp 0 TMA producer, warp 1 TMEM owner
-// and MMA issuer, warps 2..5 epilogue.  The accumulator holds C transposed:
+// Roles: warps 0 and 10 are the TMA producers of the weights and of the rows (one
+// thread issues a load in 100-150 cycles, so two share them), warp 1 owns TMEM
+// and issues the MMAs, warps 2..9 are the epilogue, in two groups that take
+// alternate chunks of rows.  The accumulator holds C transposed:
 // a thread owns one column of C and walks the rows, so bias is one value per
 // thread, and the 32-row chunks go through shared memory to become rows of
 // 256 bytes.  A chunk that lies wholly inside its group is stored by TMA, a
@@ -505,8 +507,8 @@ __device__ __noinline__ float nonfinite_terms(const GroupedParams& p, const int*
   return sum;
 }
 
-// x * Phi(x), Phi the normal distribution, without the branches of erff (whose
-// two paths kept the 32 values of a chunk from overlapping: the epilogue of a
+// x * Phi(x), Phi the normal distribution, without the branches of the math
+// library's error function (whose two paths kept the 32 values of a chunk from overlapping: the epilogue of a
 // 256 x 256 tile took 42000 cycles, more than its mainloop at K = 4096).
 //
 // With a = |x| and q(a) = 1 - Phi(a) = erfc(a / sqrt 2) / 2:
@@ -514,7 +516,7 @@ __device__ __noinline__ float nonfinite_terms(const GroupedParams& p, const int*
 //   q(a) = exp(-a^2 / 2) t Q(t),  t = 1 / (1 + 0.31 a)
 // where Q is the polynomial of degree 7 with the least relative error to
 // exp(a^2 / 2) q(a) / t over 0 <= a <= 20 (an iteratively reweighted
-// least-squares fit to scipy's erfcx), 1.7e-7.  In fp32 the result errs by at most
+// least-squares fit in 64 bits), 1.7e-7.  In fp32 the result errs by at most
 // 4 units of 2^-24 |x| and by 1.5e-6 of its value wherever fp16 is normal.
 // (x + |x|) / 2 rather than max(x, 0), so that a NaN stays one.
 __device__ __forceinline__ float gelu(float x) {
@@ -1332,6 +1334,12 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
 // run ahead, so the fix-up is off the critical path.
 //
 // Groups without rows give a zero matrix, written without any MMA.
+//
+// What bounds it: with few rows to a group, writing D (4096 rows over 64
+// experts 2048 x 1024: 59 us, and 43 with no rows at all, for 268 MB); with
+// many, what bounds the pair tiles above.  Rings of 3, 4 and 5 stages took 244,
+// 220 and 216 us for 8192 rows over 8 experts 4096 x 4096; the fifth stage's
+// shared memory stages the output instead.
 constexpr int kWgradThreads = kGrpThreads + 32;
 constexpr int kWgradFixWarp = kGrpThreads / 32;   // warp 0 produces A, warp kGrpRowsWarp G
 constexpr int kWgradTile = 256;

@@ -12,7 +12,7 @@
 // staging and no barrier in the loop: every warp owns 32-wide K slices and
 // runs on its own, the next slice's loads (of the next adapter too) in flight
 // behind the current one's MMAs.  tcgen05 would need 128 TMEM lanes for R =
-// 8..64 ranks and one tile per adapter; the tensor pipe is busy 5% here.
+// 8..64 ranks and one tile per adapter.
 //
 //  * a cluster of up to 8 CTAs x 8 warps shares the K range of a tile of up to
 //    8 rows; warp w of CTA c takes the 32-element slices c * 8 + w, + 64, ...
@@ -29,10 +29,11 @@
 //    the same order.  No workspace, no atomics.
 //
 // That form is for few rows, where every load is its own latency.  With many
-// rows (lora_shrink_wide) it took 47 us at 4096 x 4096, rank 64 -- one step's
-// loads in flight per warp, and `down` read again for every 32 rows -- so
-// there a CTA takes 256 rows and brings x and `down` through a ring in shared
-// memory by cp.async; see below.
+// rows it reads `down` again for every 8 of them and has one step's loads in
+// flight per warp, so there (lora_shrink_wide) a CTA takes 256 rows and brings
+// x and `down` through a ring in shared memory by cp.async: 4096 rows, 8
+// adapters of rank 64, 4096 x 4096 with the product take 126 us against 145,
+// where the product alone takes 109.
 #pragma once
 #include "sm100_ptx.cuh"
 
