@@ -17,22 +17,63 @@ namespace idb {
 // dependent of the grid before it and the grid after it its dependent, so the
 // launches overlap.  1000 rows by 5 x 777 x 1023 weights: 20 us with the
 // repacking, 12 us for 5 x 776 x 1024, which needs none.
-__global__ void pack_stacks(const __grid_constant__ PackJobs jobs) {
+//
+// A CTA takes slabs of 256 PER chunks of one matrix, all of a thread's loads in
+// flight together; PER = 4 where that leaves every SM two CTAs, else 1 (1879
+// rows by 94 x 4224 x 278 stored N x K: 172 us against 210 with one chunk and
+// its index divisions at a time; 64 rows by 777 x 1024: 11 us).  Matrices whose group is empty are left out: no tile reads
+// them.  (Offsets out of order are clamped upwards by the product, which only
+// empties more groups.)
+constexpr int kPackThreads = 256;
+
+template <int PER, class Index>
+__device__ __forceinline__ void pack_slab(const PackJob& job, int b, Index first) {
+  const Index chunks = static_cast<Index>((job.cols + 7) / 8), total = chunks * static_cast<Index>(job.rows);
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(job.src) + static_cast<uintptr_t>(b * job.stride) * 2u;
+  const uintptr_t end = begin + (static_cast<uintptr_t>(job.rows - 1) * static_cast<uintptr_t>(job.lds) + job.cols) * 2u;
+  unsigned short* dst = static_cast<unsigned short*>(job.dst) + static_cast<long long>(b) * job.rows * job.ldd;
+  uint4 v[PER];
+  long long to[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const Index i = first + k * kPackThreads + threadIdx.x;
+    to[k] = -1;
+    if (i < total) {
+      const Index r = i / chunks;
+      const int c = static_cast<int>(i - r * chunks) * 8;
+      to[k] = static_cast<long long>(r) * job.ldd + c;
+      v[k] = pack_chunk(begin, end, begin + static_cast<uintptr_t>(static_cast<long long>(r) * job.lds + c) * 2u, job.cols - c);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    if (to[k] >= 0) *reinterpret_cast<uint4*>(dst + to[k]) = v[k];
+  }
+}
+
+// Slabs of one matrix of the job.
+__host__ __device__ inline long long pack_slabs(const PackJob& job, int slab) {
+  return (static_cast<long long>(job.rows) * ((job.cols + 7) / 8) + slab - 1) / slab;
+}
+
+template <int PER>
+__global__ void __launch_bounds__(kPackThreads) pack_stacks(const __grid_constant__ PackJobs jobs) {
   griddep_wait();
   griddep_launch_dependents();
+  constexpr int kSlab = kPackThreads * PER;
   for (int j = 0; j < jobs.count; ++j) {
     const PackJob& job = jobs.job[j];
-    const long long chunks = (job.cols + 7) / 8;
-    const long long total = static_cast<long long>(job.batch) * job.rows * chunks;
-    for (long long idx = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; idx < total;
-         idx += static_cast<long long>(gridDim.x) * blockDim.x) {
-      const long long row = idx / chunks;
-      const int c = static_cast<int>(idx - row * chunks) * 8;
-      const long long b = row / job.rows, r = row - b * job.rows;
-      const uintptr_t begin = reinterpret_cast<uintptr_t>(job.src) + static_cast<uintptr_t>(b * job.stride) * 2u;
-      const uintptr_t end = begin + (static_cast<uintptr_t>(job.rows - 1) * static_cast<uintptr_t>(job.lds) + job.cols) * 2u;
-      *reinterpret_cast<uint4*>(static_cast<unsigned short*>(job.dst) + row * job.ldd + c) =
-          pack_chunk(begin, end, begin + static_cast<uintptr_t>(r * job.lds + c) * 2u, job.cols - c);
+    const long long slabs = pack_slabs(job, kSlab);
+    for (long long s = blockIdx.x; s < slabs * job.batch; s += gridDim.x) {
+      const int b = static_cast<int>(s / slabs);
+      if (job.offsets != nullptr) {
+        const bool rows = job.off64 ? static_cast<const long long*>(job.offsets)[b + 1] > static_cast<const long long*>(job.offsets)[b]
+                                    : static_cast<const int*>(job.offsets)[b + 1] > static_cast<const int*>(job.offsets)[b];
+        if (!rows) continue;
+      }
+      const long long first = (s - b * slabs) * kSlab;
+      if (slabs * kSlab < (1ll << 31)) pack_slab<PER, uint32_t>(job, b, static_cast<uint32_t>(first));
+      else pack_slab<PER, unsigned long long>(job, b, static_cast<unsigned long long>(first));
     }
   }
 }
@@ -67,12 +108,13 @@ struct Operand {
     *off = align256(*off + static_cast<size_t>(batch) * rows * round_up(cols, 64) * 2);
   }
 
-  // Adds the copy to `jobs` and describes it from now on.
-  void add(uint8_t* ws, PackJobs* jobs) {
+  // Adds the copy to `jobs` and describes it from now on; with offsets, the
+  // matrices of empty groups are left out.
+  void add(uint8_t* ws, PackJobs* jobs, const void* offsets = nullptr, int off64 = 0) {
     if (!pack) return;
     const int64_t ldp = round_up(cols, 64);
     jobs->job[jobs->count++] = {p, ld, batch == 1 ? 0 : stride, ws + pack_off, ldp, static_cast<int>(batch),
-                                static_cast<int>(rows), static_cast<int>(cols)};
+                                static_cast<int>(rows), static_cast<int>(cols), offsets, off64};
     p = ws + pack_off;
     ld = ldp;
     stride = rows * ldp;
@@ -111,21 +153,23 @@ bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 2u != 0
 
 int launch_pack_stacks(const PackJobs& jobs, cudaStream_t stream) {
   if (jobs.count == 0) return GEMM_OK;
-  int64_t chunks = 0;
-  for (int j = 0; j < jobs.count; ++j) {
-    chunks = std::max<int64_t>(chunks, static_cast<int64_t>(jobs.job[j].batch) * jobs.job[j].rows *
-                                           ((jobs.job[j].cols + 7) / 8));
-  }
+  auto most = [&](int per) {
+    long long n = 0;
+    for (int j = 0; j < jobs.count; ++j) n = std::max(n, pack_slabs(jobs.job[j], kPackThreads * per) * jobs.job[j].batch);
+    return n;
+  };
+  const bool four = most(4) >= 148 * 2;
+  const long long slabs = most(four ? 4 : 1);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>((chunks + 255) / 256, 148 * 8)), 1, 1);
-  cfg.blockDim = dim3(256, 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(slabs, 148 * 8)), 1, 1);
+  cfg.blockDim = dim3(kPackThreads, 1, 1);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, pack_stacks, jobs);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, four ? pack_stacks<4> : pack_stacks<1>, jobs);
   return e == cudaSuccess ? GEMM_OK : capi_fail_cuda(e, "pack_stacks launch");
 }
 
@@ -417,7 +461,7 @@ int gemm_grouped_launch(const void* A, const void* B, void* C, const void* offse
   if (st != GEMM_OK) return st;
   PackJobs jobs = {};
   a.add(static_cast<uint8_t*>(workspace), &jobs);
-  b.add(static_cast<uint8_t*>(workspace), &jobs);
+  b.add(static_cast<uint8_t*>(workspace), &jobs, offsets, offsets_bits == 64);
   st = launch_pack_stacks(jobs, stream);
   if (st != GEMM_OK) return st;
   p.offsets = offsets;

@@ -27,15 +27,20 @@ __device__ __forceinline__ uint4 shift_chunks(uint4 c0, uint4 c1, int o) {
 // belong to the row (the others read as zero), out of a matrix in [begin,
 // end).  The one or two aligned 16-byte chunks that cover them are read with
 // vector loads (neighbouring threads read the same chunks, which the cache
-// serves).  Where such a chunk would reach outside the matrix, or the row
-// ends, the elements are read one by one, so no load leaves the caller's
-// memory.
+// serves); what they hold of the next row is masked.  Where such a chunk would
+// reach outside the matrix the elements are read one by one, so no load leaves
+// the caller's memory.
 __device__ __forceinline__ uint4 pack_chunk(uintptr_t begin, uintptr_t end, uintptr_t a, int left) {
   const uintptr_t lo = a & ~static_cast<uintptr_t>(15);
   const int o = static_cast<int>(a - lo);
-  if (left >= 8 && lo >= begin && lo + (o ? 32u : 16u) <= end) {
-    const uint4 c0 = __ldg(reinterpret_cast<const uint4*>(lo));
-    return o ? shift_chunks(c0, __ldg(reinterpret_cast<const uint4*>(lo + 16)), o) : c0;
+  if (lo >= begin && lo + (o ? 32u : 16u) <= end) {
+    uint4 v = __ldg(reinterpret_cast<const uint4*>(lo));
+    if (o) v = shift_chunks(v, __ldg(reinterpret_cast<const uint4*>(lo + 16)), o);
+    if (left < 8) {
+      auto keep = [&](uint32_t w, int i) { return left > i + 1 ? w : (left > i ? w & 0xFFFFu : 0u); };
+      v = make_uint4(keep(v.x, 0), keep(v.y, 2), keep(v.z, 4), keep(v.w, 6));
+    }
+    return v;
   }
   const unsigned short* sp = reinterpret_cast<const unsigned short*>(a);
   unsigned short v[8];
@@ -52,6 +57,8 @@ struct PackJob {
   void* dst;             // one matrix after the other, pitch ldd
   long long ldd;
   int batch, rows, cols;
+  const void* offsets;   // not null: matrix b is skipped unless offsets[b] < offsets[b + 1]
+  int off64;
 };
 constexpr int kMaxPackJobs = 3;
 struct PackJobs {
