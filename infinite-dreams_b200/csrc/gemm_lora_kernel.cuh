@@ -30,10 +30,10 @@
 //
 // That form is for few rows, where every load is its own latency.  With many
 // rows it reads `down` again for every 8 of them and has one step's loads in
-// flight per warp, so there (lora_shrink_wide) a CTA takes 256 rows and brings
-// x and `down` through a ring in shared memory by cp.async: 4096 rows, 8
-// adapters of rank 64, 4096 x 4096 with the product take 126 us against 145,
-// where the product alone takes 109.
+// flight per warp, so there (lora_shrink_wide) a CTA takes 64 or 256 rows and
+// brings x and `down` through a ring in shared memory by cp.async: 4096 rows, 4
+// adapters of rank 64, 4096 x 4096 take 125 us with the product, which alone
+// takes 107.
 #pragma once
 #include "sm100_ptx.cuh"
 
@@ -373,22 +373,27 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink(const __grid_const
 
 // ------------------------------------------------------------------- many rows
 //
-// A CTA owns 256 rows and 64 ranks, the CTAs of a cluster share K in blocks of
-// 64.  Each distinct adapter of the rows is one pass over this CTA's K blocks:
-// x [256 x 64] and down[a] [64 x 64] arrive by cp.async in a ring of kWideStages
-// (40 KiB each, rows of 128 bytes with their 16-byte chunks swizzled by the
-// row, so that ldmatrix reads them without conflicts), and each of the 8 warps
-// multiplies its 32 rows unless none of them picked the adapter.  The rows
-// that did keep the result.  What it moves: x once per distinct adapter of a
-// tile (once, for long prompts), `down` once per 256 rows.
-constexpr int kWideRows = 256;
+// A CTA owns ROWS rows (256, or 64 while that leaves SMs idle) and 64 ranks, the
+// CTAs of a cluster share K in blocks of 64.  Each distinct adapter of the rows is
+// one pass over this CTA's K blocks: x [ROWS x 64] and down[a] [64 x 64] arrive by
+// cp.async in a ring (rows of 128 bytes with their 16-byte chunks
+// swizzled by the row, so that ldmatrix reads them without conflicts).  With 256
+// rows each of the 8 warps multiplies 32 of them by all ranks, with 64 rows 32 of
+// them by 16 ranks, unless none of them picked the adapter.  The rows that did
+// keep the result.  What it moves: x once per distinct adapter of a tile (once,
+// for long prompts), `down` once per tile.  What bounds it is the latency of a
+// step (barrier, ldmatrix, mma.sync, 1 to 2 us), so few rows are spread thin.
 constexpr int kWideRanks = 64;
 constexpr int kWideK = 64;
-constexpr int kWideStages = 3;
-constexpr int kWideXBytes = kWideRows * 128;
-constexpr int kWideStageBytes = kWideXBytes + kWideRanks * 128;
-constexpr int kWideSumBytes = kWideRows * kWideRanks * 4;
-constexpr int kWideBytes = kWideStages * kWideStageBytes + kWideSumBytes;
+template <int ROWS>
+struct WidePlan {
+  static constexpr int kStages = 4;
+  static constexpr int kXBytes = ROWS * 128;
+  static constexpr int kStageBytes = kXBytes + kWideRanks * 128;
+  static constexpr int kBytes = kStages * kStageBytes + ROWS * kWideRanks * 4;   // and the sums
+  static constexpr int kRowWarps = ROWS / 32;               // warps side by side in the rows
+  static constexpr int kRankTiles = 4 * kRowWarps / kShrinkWarps;   // 16-rank tiles of a warp
+};
 
 // 16 bytes of which `valid` bytes (0..16) come from src and the rest is zero.
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, int valid) {
@@ -418,12 +423,13 @@ __device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
 // Byte offset of 16-byte chunk c of row r in a tile of 128-byte rows.
 __device__ __forceinline__ uint32_t wide_at(int r, int c) { return static_cast<uint32_t>(r * 128 + ((c ^ (r & 7)) << 4)); }
 
-// grid as lora_shrink's, tile_rows = 256; x and `down` rows 16-byte aligned.
-template <bool KMAJ, bool BF16>
+// grid as lora_shrink's, tile_rows = ROWS; x and `down` rows 16-byte aligned.
+template <int ROWS, bool KMAJ, bool BF16>
 __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_wide(const __grid_constant__ ShrinkParams p) {
+  using Plan = WidePlan<ROWS>;
   extern __shared__ __align__(128) uint8_t wide_smem[];
   __shared__ __align__(16) int ids[kShrinkThreads];
-  __shared__ int list[kWideRows];
+  __shared__ int list[ROWS];
   __shared__ int warp_counts[kShrinkWarps];
   const int tid = static_cast<int>(threadIdx.x);
   const int warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
@@ -431,23 +437,25 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_wide(const __grid_
   const int crank = static_cast<int>(cluster_ctarank());
   const int tile = static_cast<int>(blockIdx.x) / cs;
   const int r0 = static_cast<int>(blockIdx.y) * kWideRanks;
-  const int row0 = tile * kWideRows;
+  const int row0 = tile * ROWS;
+  const int rw = warp % Plan::kRowWarps;                         // which 32 rows,
+  const int mw = warp / Plan::kRowWarps * Plan::kRankTiles;      // and from which 16 ranks on
 
   griddep_wait();
   griddep_launch_dependents();   // see lora_shrink
 
-  const int rows = min(kWideRows, p.T - row0);
+  const int rows = min(ROWS, p.T - row0);
   // the distinct adapters of the rows, in order of their first row
   bool bad = false;
-  const int my_id = tid < rows ? adapter_of(p.adapter, p.adapter64, row0 + tid, p.L, bad) : -1;   // row warp * 32 + lane
-  ids[tid] = my_id;
-  const unsigned same = __match_any_sync(0xffffffffu, my_id);
-  bool first = my_id >= 0 && (same & ((1u << lane) - 1u)) == 0u;
+  const int id = tid < rows ? adapter_of(p.adapter, p.adapter64, row0 + tid, p.L, bad) : -1;
+  ids[tid] = id;
+  const unsigned same = __match_any_sync(0xffffffffu, id);
+  bool first = id >= 0 && (same & ((1u << lane) - 1u)) == 0u;
   __syncthreads();
 #pragma unroll 1
   for (int i = 0; i < (tid & ~31) && first; i += 4) {   // earlier warps' rows, four at a time
     const int4 v = *reinterpret_cast<const int4*>(ids + i);
-    first = v.x != my_id && v.y != my_id && v.z != my_id && v.w != my_id;
+    first = v.x != id && v.y != id && v.z != id && v.w != id;
   }
   const unsigned vote = __ballot_sync(0xffffffffu, first);
   if (lane == 0) warp_counts[warp] = __popc(vote);
@@ -457,31 +465,35 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_wide(const __grid_
     at += w < warp ? warp_counts[w] : 0;
     adapters += warp_counts[w];
   }
-  if (first) list[at] = my_id;
+  if (first) list[at] = id;
   __syncthreads();
+  const int my_id = ids[rw * 32 + lane];   // of the warp's rows
   const uint32_t ring = smem_u32(wide_smem);
-  float* sums = reinterpret_cast<float*>(wide_smem + kWideStages * kWideStageBytes);   // [256][64]
+  float* sums = reinterpret_cast<float*>(wide_smem + Plan::kStages * Plan::kStageBytes);   // [ROWS][64]
 
   const int blocks = (p.K + kWideK - 1) / kWideK;
   const int kb0 = blocks * crank / cs, per = blocks * (crank + 1) / cs - kb0;
   const int steps = adapters * per;
-  auto load = [&](int step) {   // x and down[a] of one step into its stage
-    const int a = list[step / per];
-    const int k0 = (kb0 + step % per) * kWideK;
-    const uint32_t sx = ring + static_cast<uint32_t>(step % kWideStages * kWideStageBytes), sd = sx + kWideXBytes;
-    const int c = tid & 7;
+  // What a thread copies of a step: chunk c of the rows (tid / 8) + 32 i of x and
+  // of `down`.  Everything that repeats is counted on, not divided out: the loop
+  // below has a barrier per step and nothing to hide a chain of divisions behind.
+  const int c = tid & 7, r8 = tid >> 3;
+  const uint32_t at0 = wide_at(r8, c);
+  const unsigned short* xr = p.x + static_cast<long long>(row0 + r8) * p.ldx + c * 8;
+  int l_block = 0, l_adapter = 0, l_stage = 0;
+  auto load = [&] {   // x and down[a] of the next step into the next stage
+    const int k0 = (kb0 + l_block) * kWideK;
+    const uint32_t sx = ring + static_cast<uint32_t>(l_stage * Plan::kStageBytes), sd = sx + Plan::kXBytes;
     const int xv = max(0, min(8, p.K - k0 - c * 8)) * 2;   // valid bytes of this thread's chunks of x
 #pragma unroll
-    for (int i = 0; i < kWideRows / 32; ++i) {
-      const int r = i * 32 + (tid >> 3);
-      const bool in = r < rows && xv > 0;
-      const unsigned short* src = in ? p.x + static_cast<long long>(row0 + r) * p.ldx + k0 + c * 8 : p.x;
-      cp_async_16(sx + wide_at(r, c), src, in ? xv : 0);
+    for (int i = 0; i < ROWS / 32; ++i) {
+      const bool in = i * 32 + r8 < rows && xv > 0;
+      cp_async_16(sx + at0 + i * 4096, in ? xr + static_cast<long long>(i * 32) * p.ldx + k0 : p.x, in ? xv : 0);
     }
-    const unsigned short* d = p.down + static_cast<long long>(a) * p.stride_down;
+    const unsigned short* d = p.down + static_cast<long long>(list[l_adapter]) * p.stride_down;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int r = i * 32 + (tid >> 3);   // KMAJ: a rank, its K chunks; else a K row, its rank chunks
+      const int r = i * 32 + r8;   // KMAJ: a rank, its K chunks; else a K row, its rank chunks
       int valid;
       const unsigned short* src;
       if constexpr (KMAJ) {
@@ -491,25 +503,31 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_wide(const __grid_
         valid = k0 + r < p.K ? max(0, min(8, p.R - r0 - c * 8)) * 2 : 0;
         src = d + static_cast<long long>(k0 + r) * p.ld_down + r0 + c * 8;
       }
-      cp_async_16(sd + wide_at(r, c), valid > 0 ? src : p.x, valid);
+      cp_async_16(sd + at0 + i * 4096, valid > 0 ? src : p.x, valid);
     }
+    if (++l_block == per) {
+      l_block = 0;
+      ++l_adapter;
+    }
+    if (++l_stage == Plan::kStages) l_stage = 0;
   };
-  for (int s = 0; s < kWideStages - 1; ++s) {
-    if (s < steps) load(s);
+  for (int s = 0; s < Plan::kStages - 1; ++s) {
+    if (s < steps) load();
     cp_async_commit();
   }
-  float acc[4][4][4];   // [16 ranks][8 rows]
+  float acc[Plan::kRankTiles][4][4];   // [16 ranks][8 rows]
+  const int rank_tiles = (p.R - r0 + 15) / 16 - mw;   // that exist, from the warp's first on; the others stay zero
   bool mine = false;    // a row of this warp picked the adapter
+  int block = 0, adapter = 0, stage = 0;
   for (int step = 0; step < steps; ++step) {
-    cp_async_wait<kWideStages - 2>();
+    cp_async_wait<Plan::kStages - 2>();
     __syncthreads();   // every thread's part of this stage is in, and the stage about to be refilled is read
-    if (step + kWideStages - 1 < steps) load(step + kWideStages - 1);
+    if (step + Plan::kStages - 1 < steps) load();
     cp_async_commit();
-    const int block = step % per;
     if (block == 0) {
-      mine = __any_sync(0xffffffffu, my_id == list[step / per]);
+      mine = __any_sync(0xffffffffu, my_id == list[adapter]);
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
+      for (int m = 0; m < Plan::kRankTiles; ++m) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
 #pragma unroll
@@ -518,26 +536,27 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_wide(const __grid_
       }
     }
     if (mine) {
-      const uint32_t sx = ring + static_cast<uint32_t>(step % kWideStages * kWideStageBytes), sd = sx + kWideXBytes;
+      const uint32_t sx = ring + static_cast<uint32_t>(stage * Plan::kStageBytes), sd = sx + Plan::kXBytes;
 #pragma unroll
       for (int kk = 0; kk < kWideK / 16; ++kk) {
         // B: 8 rows x 16 K per pair of 8x8 blocks; blocks (rows j, K lo), (j, K hi), (j + 1, K lo), (j + 1, K hi)
         uint32_t xb[2][4];
 #pragma unroll
         for (int jj = 0; jj < 2; ++jj) {
-          const int r = warp * 32 + jj * 16 + (lane & 7) + ((lane >> 4) << 3);
+          const int r = rw * 32 + jj * 16 + (lane & 7) + ((lane >> 4) << 3);
           ldmatrix_x4<false>(sx + wide_at(r, kk * 2 + ((lane >> 3) & 1)), xb[jj]);
         }
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
+        for (int m = 0; m < Plan::kRankTiles; ++m) {
+          if (m >= rank_tiles) break;
           // A: blocks (ranks 0-7, K lo), (8-15, K lo), (0-7, K hi), (8-15, K hi)
           uint32_t da[4];
           if constexpr (KMAJ) {
-            const int r = m * 16 + (lane & 15);
+            const int r = (mw + m) * 16 + (lane & 15);
             ldmatrix_x4<false>(sd + wide_at(r, kk * 2 + (lane >> 4)), da);
           } else {
             const int k = kk * 16 + (lane & 7) + ((lane >> 4) << 3);
-            ldmatrix_x4<true>(sd + wide_at(k, m * 2 + ((lane >> 3) & 1)), da);
+            ldmatrix_x4<true>(sd + wide_at(k, (mw + m) * 2 + ((lane >> 3) & 1)), da);
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -546,35 +565,64 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_wide(const __grid_
         }
       }
       if (block == per - 1) {
-        const int a = list[step / per];
+        const int a = list[adapter];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const int r = warp * 32 + j * 8 + 2 * q + i;
+            const int r = rw * 32 + j * 8 + 2 * q + i;
             if (ids[r] == a) {
 #pragma unroll
-              for (int m = 0; m < 4; ++m) {
-                sums[r * kWideRanks + m * 16 + g] = acc[m][j][i];
-                sums[r * kWideRanks + m * 16 + 8 + g] = acc[m][j][i + 2];
+              for (int m = 0; m < Plan::kRankTiles; ++m) {
+                sums[r * kWideRanks + (mw + m) * 16 + g] = acc[m][j][i];
+                sums[r * kWideRanks + (mw + m) * 16 + 8 + g] = acc[m][j][i + 2];
               }
             }
           }
         }
       }
     }
+    if (++block == per) {
+      block = 0;
+      ++adapter;
+    }
+    if (++stage == Plan::kStages) stage = 0;
   }
-  // over the cluster: CTA c finishes every cs-th row
+  // over the cluster, in CTA order: CTA c finishes every cs-th row, a thread four
+  // ranks of it
   if (cs > 1) cluster_sync();
   else __syncthreads();
   const uint32_t base = smem_u32(sums);
-  const int e = tid & (kWideRanks - 1);
-  for (int r = (tid / kWideRanks) * cs + crank; r < rows; r += kShrinkThreads / kWideRanks * cs) {
-    const int a = ids[r];
-    if (a < 0 || r0 + e >= p.h_pitch) continue;
-    float v = 0.0f;
-    for (int c = 0; c < cs; ++c) v += ld_dsmem_f32(mapa_shared(base + (r * kWideRanks + e) * 4, c));
-    p.h[static_cast<long long>(row0 + r) * p.h_pitch + r0 + e] = v * (p.scale != nullptr ? p.scale[a] : 1.0f);
+  const int e = (tid & 15) * 4;
+  if (r0 + e < p.h_pitch) {   // the pitch is whole blocks of 16
+    auto store = [&](int r, float4 v) {
+      const int a = ids[r];
+      if (a < 0) return;
+      const float scale = p.scale != nullptr ? p.scale[a] : 1.0f;
+      *reinterpret_cast<float4*>(p.h + static_cast<long long>(row0 + r) * p.h_pitch + r0 + e) =
+          make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale);
+    };
+    if (cs == 1) {
+#pragma unroll 4
+      for (int r = tid >> 4; r < rows; r += kShrinkThreads / 16) {
+        store(r, *reinterpret_cast<const float4*>(sums + r * kWideRanks + e));
+      }
+    } else {
+#pragma unroll 1
+      for (int r = (tid >> 4) * cs + crank; r < rows; r += kShrinkThreads / 16 * cs) {
+        float4 part[8];   // in flight together
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          if (c < cs) part[c] = ld_dsmem_f32x4(mapa_shared(base + (r * kWideRanks + e) * 4, c));
+        }
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          if (c < cs) v = make_float4(v.x + part[c].x, v.y + part[c].y, v.z + part[c].z, v.w + part[c].w);
+        }
+        store(r, v);
+      }
+    }
   }
   if (cs > 1) cluster_sync();   // no CTA leaves while a peer may still read its sums
 }

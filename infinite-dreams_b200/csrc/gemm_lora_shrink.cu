@@ -19,9 +19,10 @@ ShrinkFn pick(bool kmaj, bool bf16) {
   return bf16 ? lora_shrink<RT, 1, false, true, VEC> : lora_shrink<RT, 1, false, false, VEC>;
 }
 
+template <int ROWS>
 ShrinkFn pick_wide(bool kmaj, bool bf16) {
-  if (kmaj) return bf16 ? lora_shrink_wide<true, true> : lora_shrink_wide<true, false>;
-  return bf16 ? lora_shrink_wide<false, true> : lora_shrink_wide<false, false>;
+  if (kmaj) return bf16 ? lora_shrink_wide<ROWS, true, true> : lora_shrink_wide<ROWS, true, false>;
+  return bf16 ? lora_shrink_wide<ROWS, false, true> : lora_shrink_wide<ROWS, false, false>;
 }
 
 }  // namespace
@@ -36,16 +37,27 @@ int launch_shrink(const ShrinkParams& sp, bool kmaj, bool bf16, cudaStream_t str
   ShrinkFn fn;
   int cluster = 1, bytes, ranks, variant;
   if (p.T > kWideFrom && aligned) {
-    // 256 rows to a cluster, as many CTAs along K as keep to one per SM with
-    // at least 4 K blocks each.
-    p.tile_rows = kWideRows;
-    p.tiles = (p.T + kWideRows - 1) / kWideRows;
+    // 256 rows to a cluster if that gives at least half of the SMs a CTA, else
+    // 64; as many CTAs along K as keep to one (two) per SM with at least 4 K
+    // blocks each.  With the product, rank 64: 8192 rows in long runs, 4096 x
+    // 4096, 245 us against 254 with 64 rows; 4096 rows, 1024 x 1024, 33 against
+    // 44 with 256.
     ranks = kWideRanks;
-    const int blocks = (p.K + kWideK - 1) / kWideK, all = p.tiles * ((p.R + ranks - 1) / ranks);
-    while (cluster < 8 && 8 * cluster <= blocks && 2 * cluster * all <= 148) cluster *= 2;
-    fn = pick_wide(kmaj, bf16);
-    bytes = kWideBytes;
-    variant = kmaj * 2 + bf16;
+    const int blocks = (p.K + kWideK - 1) / kWideK, rank_blocks = (p.R + ranks - 1) / ranks;
+    auto tiles_of = [&](int rows) { return (p.T + rows - 1) / rows; };
+    auto cluster_of = [&](int64_t ctas, int most) {
+      int c = 1;
+      while (c < 8 && 8 * c <= blocks && 2 * c * ctas <= most) c *= 2;
+      return c;
+    };
+    const int64_t tall_ctas = static_cast<int64_t>(tiles_of(256)) * rank_blocks;
+    const bool tall = 2 * tall_ctas * cluster_of(tall_ctas, 148) >= 148;
+    p.tile_rows = tall ? 256 : 64;
+    p.tiles = tiles_of(p.tile_rows);
+    cluster = cluster_of(static_cast<int64_t>(p.tiles) * rank_blocks, tall ? 148 : 296);
+    fn = tall ? pick_wide<256>(kmaj, bf16) : pick_wide<64>(kmaj, bf16);
+    bytes = tall ? WidePlan<256>::kBytes : WidePlan<64>::kBytes;
+    variant = tall * 4 + kmaj * 2 + bf16;
   } else {
     // So few rows to a tile that about 256 CTAs share the work (T = 64: 2 rows
     // x 32 clusters of 8), up to the 8 rows of one MMA; along K no more CTAs
@@ -61,14 +73,14 @@ int launch_shrink(const ShrinkParams& sp, bool kmaj, bool bf16, cudaStream_t str
     fn = rt == 1   ? (vec ? pick<1, true>(kmaj, bf16) : pick<1, false>(kmaj, bf16))
          : rt == 2 ? (vec ? pick<2, true>(kmaj, bf16) : pick<2, false>(kmaj, bf16))
                    : (vec ? pick<4, true>(kmaj, bf16) : pick<4, false>(kmaj, bf16));
-    variant = 4 + (rt == 4 ? 2 : rt - 1) * 8 + vec * 4 + kmaj * 2 + bf16;
+    variant = 8 + (rt == 4 ? 2 : rt - 1) * 8 + vec * 4 + kmaj * 2 + bf16;
     bytes = kShrinkWarps * rows * ranks * static_cast<int>(sizeof(float));   // at most 16 KiB
   }
   // Once per kernel and device: the dynamic shared memory above 48 KiB, and the
   // SM's largest shared-memory split.  The product's CTA needs that split, and
   // an SM changes it only when it is empty: under a smaller one the product's
   // CTAs did not start before this grid had ended.
-  static std::atomic<unsigned long long> configured[28];   // devices, per variant
+  static std::atomic<unsigned long long> configured[32];   // devices, per variant
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return capi_fail_cuda(e, "cudaGetDevice");

@@ -84,6 +84,16 @@ def test_every_row_its_own_adapter():
         check(ext.lora_gemm(x, W, down, up, ids), *ref_lora(x, W, down, up, ids))
 
 
+@pytest.mark.parametrize("T,K,N,L,R", [(513, 64, 64, 3, 8), (700, 4096, 72, 5, 64), (1999, 320, 136, 4, 24),
+                                       (2100, 2000, 64, 9, 130), (4700, 1032, 64, 3, 48), (5000, 4096, 128, 6, 16),
+                                       (9000, 520, 64, 4, 200)])
+@pytest.mark.parametrize("stored", ["kn", "nk"])
+@pytest.mark.parametrize("pattern", ["random", "runs"])
+def test_many_rows(T, K, N, L, R, stored, pattern):
+    """The low-rank half's two tiles, with K split over clusters and without."""
+    _run(T, K, N, L, R, torch.float16 if T % 2 else torch.bfloat16, stored, pattern)
+
+
 @pytest.mark.parametrize("T,K,N,L,R,pattern", [
     (20000, 64, 64, 2, 1024, "runs"), (20000, 200, 64, 40, 16, "random"),     # single CTAs
     (5120, 64, 1024, 40, 16, "random"), (21000, 328, 256, 3, 300, "runs")])   # pairs
