@@ -11,7 +11,11 @@ namespace {
 
 using ShrinkFn = void (*)(ShrinkParams);
 
-constexpr int kWideFrom = 512;   // more rows than this take lora_shrink_wide
+// More rows than this take lora_shrink_wide.  It passes over x once per adapter of
+// a tile, so it wins where neighbours share one (2048 rows of rank 64 in long
+// runs, 4096 x 4096 with the product: 70 us against 78) and loses where they do
+// not (rank 16, every row another adapter: 137 against 96).
+constexpr int kWideFrom = 2048;
 
 template <int RT, bool VEC>
 ShrinkFn pick(bool kmaj, bool bf16) {
