@@ -25,20 +25,12 @@ MOST_MADS = 8192 * 4096 * 14336
 MOST_WEIGHTS = 8 * 4096 * 14336
 
 
-_modules = None
-
-
 def _ext():
-    """The framework's modules, imported once as a program does."""
-    global _modules
-    if _modules is not None:
-        return _modules
     root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "infinite-dreams_b200")
     if root not in sys.path:
         sys.path.insert(0, root)
     from infinite_dreams import grouped, infinite_dreams_ext
-    _modules = infinite_dreams_ext, grouped
-    return _modules
+    return infinite_dreams_ext, grouped
 
 
 def listed():
