@@ -59,10 +59,12 @@
 // result's own rounding does.
 //
 // A row that did not pick the adapter multiplies `up` with zeros, and 0 * inf
-// is not 0.  So where a tile mixes adapters the thread that owns a column
-// looks its ranks over once they have landed, replaces an inf or NaN by 0 in
-// shared memory, and adds what it replaced to the rows of that adapter in the
-// epilogue: one request's weights cannot reach another's rows.
+// is not 0; nor is hi * inf + lo * inf the h * inf of a row that did (lo may be
+// 0 or have the other sign).  So the thread that owns a column looks its ranks
+// over once they have landed, replaces an inf or NaN by 0 in shared memory, and
+// adds what it replaced to the rows of that adapter in the epilogue: one
+// request's weights cannot reach another's rows, and what its own rows get does
+// not depend on its neighbours.
 #pragma once
 #include "gemm_lora_kernel.cuh"
 #include "gemm_sm100_kernel.cuh"
@@ -651,7 +653,7 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
   // adapter of each row of the tile, the distinct ones, and their counts.
   int* row_ids = grp_rows + 4;
   int* list = grp_tiles + 4;
-  volatile int* list_counts = scan;   // adapters, then rows without one; scratch after that
+  volatile int* list_counts = scan;   // adapters; scratch after that
 
   const int warp = static_cast<int>(threadIdx.x >> 5);
   const int lane = static_cast<int>(threadIdx.x & 31);
@@ -1038,15 +1040,13 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
           first = v.x != id && v.y != id && v.z != id && v.w != id;
         }
         const unsigned vote = __ballot_sync(0xffffffffu, first);
-        const unsigned none = __ballot_sync(0xffffffffu, et < u.rows && id < 0);
-        if (lane == 0) list_counts[2 + (et >> 5)] = __popc(vote) | (__popc(none) << 16);
+        if (lane == 0) list_counts[2 + (et >> 5)] = __popc(vote);
         named_bar_sync(1, 32 * kGrpEpiWarps);
-        int at = __popc(vote & ((1u << lane) - 1u)), all = 0, without = 0;
+        int at = __popc(vote & ((1u << lane) - 1u)), all = 0;
         for (int w = 0; w < kGrpEpiWarps; ++w) {
           const int c = list_counts[2 + w];
-          at += w < (et >> 5) ? c & 0xffff : 0;
-          all += c & 0xffff;
-          without += c >> 16;
+          at += w < (et >> 5) ? c : 0;
+          all += c;
         }
         if (listed > 0) mbar_wait(list_read_bar, (listed - 1) & 1u, abort_flag);   // the previous tile's
         ++listed;
@@ -1064,7 +1064,6 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
         constexpr int kChunks = kRanks / 8;
         b0 = rank_blocks * adapters * part / parts;
         b1 = rank_blocks * adapters * (part + 1) / parts;
-        const bool mixed = adapters > 1 || without > 0;
         const int half = u.nmma / CG;
         const int row = CG == 1 ? gt & 63 : gt, sub = CG == 1 ? gt >> 6 : 0;
         const int tr = rank * half + row;   // row of the tile
@@ -1087,7 +1086,7 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
             got = __all_sync(0xffffffffu, got) != 0;
             if (!got) break;
             const int steps = p.R - rb * kLoraRanks > kUmmaK ? 2 : 1;   // of 16 ranks
-            if (mixed && clear_nonfinite(sW + stage * Plan::kWBytes, gt, steps, p.up_kmaj != 0, bf16)) odd_flags[turn] = 1;
+            if (clear_nonfinite(sW + stage * Plan::kWBytes, gt, steps, p.up_kmaj != 0, bf16)) odd_flags[turn] = 1;
             if (row < half && sub < steps) {
               uint8_t* dst = sT + stage * Plan::kTBytes + row * 128;
 #pragma unroll
