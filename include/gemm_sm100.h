@@ -184,9 +184,10 @@ size_t gemm_grouped_wgrad_workspace_bytes(const void* A, const void* G, int64_t 
  *  scale   = fp32 [L] or NULL (1); bias = [N] or NULL; activation = GEMM_ACT_*.
  * Every operand is read in place; X, W and up are repacked into the workspace
  * when TMA cannot address them (16-byte base, pitches and strides multiples
- * of 8 elements).  x * down is kept in fp32 and enters the second product as
- * two 16-bit numbers (their sum is exact to 16 or more bits; in fp16 a
- * value past 65504 is infinite); fp32 accumulation, one rounding.  Two launches.  R <= GEMM_LORA_MAX_RANK.  The
+ * of 8 elements).  scale * x * down is kept in fp32 and enters the second
+ * product as two bf16 numbers, whatever the type of the operands: their sum is
+ * within 2^-16 of it, over the whole range of fp32.  fp32 accumulation, one
+ * rounding.  Two launches.  R <= GEMM_LORA_MAX_RANK.  The
  * workspace (never 0 bytes) comes from gemm_lora_workspace_bytes under the
  * contract of gemm_launch.  No counterpart in the reference. */
 #define GEMM_LORA_MAX_RANK 1024

@@ -477,8 +477,8 @@ def lora_gemm(x: torch.Tensor, W: torch.Tensor, down: torch.Tensor, up: torch.Te
     alike.  adapter: T int32 or int64 numbers on the device, in any order;
     negative means none, a number past the last adapter counts as none and
     is reported by ``check_device_errors``.  scale is float32 [L], bias [N].
-    Adapters of smaller ranks are padded with zeros; R is at most 1024.  x @
-    down is kept to 16 bits or more (beyond fp16's range it is infinite).
+    Adapters of smaller ranks are padded with zeros; R is at most 1024.
+    scale * (x @ down) is kept to 2^-16 of it, over the range of float32.
     One request's inf or NaN does not reach the rows of others.  A serving
     operator: it computes no gradients and refuses inputs that ask for them.
     """
