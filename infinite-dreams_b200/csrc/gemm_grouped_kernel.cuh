@@ -562,7 +562,8 @@ __device__ __noinline__ float nonfinite_terms(const GroupedParams& p, const int*
 // exp(a^2 / 2) q(a) / t over 0 <= a <= 20 (an iteratively reweighted
 // least-squares fit in 64 bits), 1.7e-7.  In fp32 the result errs by at most
 // 4 units of 2^-24 |x| and by 1.5e-6 of its value wherever fp16 is normal.
-// (x + |x|) / 2 rather than max(x, 0), so that a NaN stays one.
+// x / 2 + |x| / 2 rather than max(x, 0), so that a NaN stays one (halves first:
+// x + |x| overflows where bf16 does not).
 __device__ __forceinline__ float gelu(float x) {
   const float a = fminf(fabsf(x), 20.0f);
   float t, e;
@@ -576,7 +577,7 @@ __device__ __forceinline__ float gelu(float x) {
   q = fmaf(q, t, 0.10766225f);
   q = fmaf(q, t, 0.12407906f);
   q = fmaf(q, t, 0.1236556f);
-  return fmaf(-a, q * t * e, 0.5f * (x + fabsf(x)));
+  return fmaf(-a, q * t * e, fmaf(0.5f, fabsf(x), 0.5f * x));
 }
 
 // gelu of two values with packed arithmetic, operation for operation the same.
@@ -602,7 +603,8 @@ __device__ __forceinline__ void gelu2(float& x0, float& x1) {
   q = fma_f32x2(q, t, pack_f32x2(0.12407906f, 0.12407906f));
   q = fma_f32x2(q, t, pack_f32x2(0.1236556f, 0.1236556f));
   q = mul_f32x2(mul_f32x2(q, t), pack_f32x2(e0, e1));
-  const uint64_t r = mul_f32x2(pack_f32x2(x0 + fabsf(x0), x1 + fabsf(x1)), pack_f32x2(0.5f, 0.5f));
+  const uint64_t half = pack_f32x2(0.5f, 0.5f);
+  const uint64_t r = fma_f32x2(half, pack_f32x2(fabsf(x0), fabsf(x1)), mul_f32x2(half, pack_f32x2(x0, x1)));
   unpack_f32x2(fma_f32x2(pack_f32x2(-a0, -a1), q, r), x0, x1);
 }
 
