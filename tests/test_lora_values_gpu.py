@@ -3,7 +3,7 @@ with `down` far from 1."""
 import pytest
 import torch
 
-from grouped_helpers import DTYPES, check, half_step, randn, rounded, stacked, sum_error
+from grouped_helpers import DTYPES, check, half_step, randn, ref_lora, rounded, stacked, sum_error
 
 pytestmark = pytest.mark.gpu
 
@@ -119,3 +119,40 @@ def test_products_with_down_at_the_ends_of_the_ranges(T, dtype):
         scale = torch.tensor([h], device="cuda")
         got = ext.lora_gemm(x, W, down, up, ids, scale=scale)
         _infinite_alike(got, *_bound(x, W, down, up, ids, scale), dtype)
+
+
+def _padded(shape, dtype, seed, scale=1.0):
+    """A tensor of this shape cut out of one with more rows and columns, all of them NaN, whose pitch is aligned."""
+    full = torch.full((*shape[:-2], shape[-2] + 2, -(-shape[-1] // 8) * 8 + 8), float("nan"), dtype=dtype, device="cuda")
+    part = full[..., :shape[-2], :shape[-1]]
+    part.copy_(randn(shape, dtype, seed, scale))
+    return part
+
+
+@pytest.mark.parametrize("R", [3, 16, 21, 40, 65])
+@pytest.mark.parametrize("T", [1, 40, 300, 2101])
+@pytest.mark.parametrize("K,N", [(133, 141), (1029, 265)])
+@pytest.mark.parametrize("stored", ["kn", "nk"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_padding_does_not_enter(R, T, K, N, stored, dtype):
+    """NaN beside and below every operand whose pitch is aligned while its width is not."""
+    from infinite_dreams import infinite_dreams_ext as ext
+    L = 4
+    x = _padded((T, K), dtype, 1)
+    W, down, up = (_padded(s, dtype, i, f) if stored == "kn" else
+                   _padded((*s[:-2], s[-1], s[-2]), dtype, i, f).transpose(-1, -2)
+                   for s, i, f in (((K, N), 2, K ** -0.5), ((L, K, R), 3, K ** -0.5), ((L, R, N), 4, R ** -0.5)))
+    ids = torch.arange(T, device="cuda") % (L + 1) - 1
+    check(ext.lora_gemm(x, W, down, up, ids), *ref_lora(x, W, down, up, ids))
+
+
+@pytest.mark.parametrize("K", [1024, 2048, 4096, 8200])
+@pytest.mark.parametrize("N", [129, 1500])
+@pytest.mark.parametrize("T", [1, 7, 64])
+@pytest.mark.parametrize("act", ["none", "gelu"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_few_rows_with_the_sum_split_over_a_cluster(K, N, T, act, dtype):
+    from infinite_dreams import infinite_dreams_ext as ext
+    W, down, up = stacked(1, K, N, dtype, 1)[0], stacked(3, K, 24, dtype, 2), stacked(3, 24, N, dtype, 3)
+    x, b, ids = randn((T, K), dtype, 4), randn((N,), dtype, 5), torch.arange(T, device="cuda") % 4 - 1
+    check(ext.lora_gemm(x, W, down, up, ids, bias=b, activation=act), *ref_lora(x, W, down, up, ids, None, b, act))
