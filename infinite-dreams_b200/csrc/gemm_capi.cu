@@ -192,6 +192,13 @@ bool tma_addressable(const void* p, int64_t pitch_elems) {
   return (reinterpret_cast<uintptr_t>(p) % 16u) == 0 && (pitch_elems % 8) == 0;
 }
 
+// C as the target of TMA stores: a box is clipped at the last column in units of
+// 16 bytes, so rows that end inside one (a C cut out of a wider matrix) take the
+// other stores; by TMA they would write up to 7 elements past the row.
+bool tma_storable(const void* p, int64_t pitch_elems, int64_t cols) {
+  return tma_addressable(p, pitch_elems) && cols % 8 == 0;
+}
+
 int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
 struct Plan {
@@ -576,7 +583,7 @@ int launch_impl(const void* A, const void* B, void* C, int64_t M, int64_t N, int
     p.split_k = pl.split_k;
     p.partials = nullptr;
     p.counters = nullptr;
-    const bool c_tma = tma_addressable(C, ldc);
+    const bool c_tma = tma_storable(C, ldc, N);
     if (c_tma) {
       st = encode_2d_cached(&tmC, C, N, M, ldc, skinny_c_box(pl.tile_n / pl.split_k), pl.tile_m, "C", false);
       if (st != GEMM_OK) return st;
@@ -602,7 +609,7 @@ int launch_impl(const void* A, const void* B, void* C, int64_t M, int64_t N, int
   }
   if (st != GEMM_OK) return st;
   // With a multicast C every box leaves through multimem stores instead.
-  const bool c_tma = !op.mc_C && tma_addressable(C, ldc);
+  const bool c_tma = !op.mc_C && tma_storable(C, ldc, N);
   if (c_tma) {
     st = encode_2d_cached(&tmC, C, N, M, ldc, kStoreCols, kStoreRows, "C");
     if (st != GEMM_OK) return st;
