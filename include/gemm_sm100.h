@@ -145,7 +145,8 @@ size_t gemm_workspace_bytes_ex(const void* A, const void* B, int64_t M, int64_t 
  *  rows outside [offsets[0], offsets[E]) are written as zeros when zero_rest
  *            != 0 and left as they are otherwise;
  *  bias    = E x N (contiguous) or NULL; activation = GEMM_ACT_*.
- * fp32 accumulation, one rounding.  E <= 1024.  K = 0 gives act(bias).
+ * fp32 accumulation, one rounding.  E <= 1024; T, N and K at most 2^31 - 1024
+ * each (here and in the two entry points below).  K = 0 gives act(bias).
  * The workspace comes from gemm_grouped_workspace_bytes under the contract of
  * gemm_launch.  No counterpart in the reference. */
 int gemm_grouped_launch(const void* A, const void* B, void* C, const void* offsets, int offsets_bits, int64_t T,

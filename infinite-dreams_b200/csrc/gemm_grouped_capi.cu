@@ -82,6 +82,10 @@ namespace {
 
 constexpr int64_t kInt32Max = (1ll << 31) - 1;
 
+// Largest extent of a call: the kernels round rows and columns up to whole tiles
+// (at most 512) and step by the grid, in 32 bits.
+constexpr int64_t kMaxExtent = (1ll << 31) - 1024;
+
 int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
@@ -187,8 +191,8 @@ int check_workspace(size_t need, const void* ws, size_t ws_bytes) {
 
 int check_common(int64_t T, int64_t N, int64_t K, int64_t E, int offsets_bits, int dtype, const char* groups) {
   if (T < 0 || N < 0 || K < 0) return capi_fail(GEMM_ERR_INVALID_ARG, "T, N, K must be >= 0");
-  if (T > kInt32Max || N > kInt32Max || K > kInt32Max) {
-    return capi_fail(GEMM_ERR_UNSUPPORTED, "T, N, K must each be < 2^31");
+  if (T > kMaxExtent || N > kMaxExtent || K > kMaxExtent) {
+    return capi_fail(GEMM_ERR_UNSUPPORTED, "T, N, K must each be at most 2^31 - 1024");
   }
   if (E < 1) return capi_fail(GEMM_ERR_INVALID_ARG, std::string(groups) + " must be >= 1");
   if (offsets_bits != 32 && offsets_bits != 64) {
