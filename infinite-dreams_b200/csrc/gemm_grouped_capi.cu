@@ -665,6 +665,7 @@ int gemm_lora_launch(const void* X, const void* W, const void* down, const void*
   p.up = static_cast<const unsigned short*>(pl.up.p);
   p.ld_up = pl.up.ld;
   p.stride_up = L == 1 ? 0 : pl.up.stride;
+  p.packed = jobs.count > 0;
   if (small_tiles(T, N, 1, sms)) return launch_grouped<1, 64, 6, true>(pl.x, pl.w, &pl.up, p, sms, stream);
   return launch_grouped<2, 256, 6, true>(pl.x, pl.w, &pl.up, p, sms, stream);
 }

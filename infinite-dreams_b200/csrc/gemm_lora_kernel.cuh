@@ -71,9 +71,10 @@ inline int64_t shrink_pitch(int64_t R) {
 int launch_shrink(const ShrinkParams& p, bool kmaj, bool bf16, cudaStream_t stream);
 
 // adapter[t], or -1 for none.  An index past the last adapter counts as none.
+// Read past L1: the product's grid does so before it waits for the one before it.
 __device__ __forceinline__ int adapter_of(const void* adapter, int adapter64, long long t, int L, bool& bad) {
   const long long v =
-      adapter64 ? static_cast<const long long*>(adapter)[t] : static_cast<const int*>(adapter)[t];
+      adapter64 ? __ldcg(static_cast<const long long*>(adapter) + t) : __ldcg(static_cast<const int*>(adapter) + t);
   bad |= v >= L;
   return (v < 0 || v >= L) ? -1 : static_cast<int>(v);
 }
