@@ -788,7 +788,17 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
       uint32_t full_par = 0, land_par = 0, on_land = 0;
       bool ok = true;
       uint32_t list_phase = 0;
+      // With LORA, what follows the first tile's K blocks waits for h in the end.
+      // The bounded waits are for the work of this grid: the time that
+      // lora_shrink takes is not theirs, so it is waited out first.
+      bool first = true, waited = !LORA;
+      auto wait_for_h = [&] {
+        if (!waited) griddep_wait();
+        waited = true;
+      };
       while (ok && walk.next<Plan::kSubs>(t, split)) {
+        if (!first) wait_for_h();
+        first = false;
         const int parts = split ? csize : 1, part = split ? crank : 0;   // of the tile's K
         const int kb0 = split ? split_kb0 : 0, kb1 = split ? split_kb1 : p.kb_total;
         const GroupedUnit u = grouped_unit<CG, TM>(p, grp_rows, grp_tiles, t, walk.part);
@@ -848,6 +858,7 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
           for (int b = b0; b < b1; ++b) {
             // the rows' producer loads nothing here, but has to see every phase
             // of a slot: two of them on, it would take an old one for its own
+            if ((on_land >> stage) & 1u) wait_for_h();   // the slot's last block is multiplied with h
             if (issued >= STAGES && !mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) {
               ok = false;
               break;
@@ -910,7 +921,7 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
       int acc = 0;                      // the next accumulator
       uint32_t acc_used = 0, acc_par = 0;   // per accumulator: used before; parity of its next release
       uint32_t built_par = 0, list_phase = 0;
-      bool ok = true;
+      bool ok = true, waited = !LORA;
       while (ok && walk.next<Plan::kSubs>(t, split)) {
         const int parts = split ? csize : 1, part = split ? crank : 0;   // of the tile's K
         const int kb0 = split ? split_kb0 : 0, kb1 = split ? split_kb1 : p.kb_total;
@@ -966,6 +977,8 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
         }
         if constexpr (LORA) {
           ok = ok && mbar_wait(list_bar, list_phase, abort_flag);
+          if (!waited) griddep_wait();   // see the producers
+          waited = true;
           list_phase ^= 1u;
           const uint32_t idesc_up = idesc_16bit(kGrpCols * CG, u.nmma, p.up_kmaj == 0, false, true);   // bf16 parts
           const uint64_t up_desc = smem_desc_sw128(smem_u32(sW), p.up_kmaj ? 16 : kBK * 128, 1024);

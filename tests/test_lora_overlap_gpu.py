@@ -44,3 +44,26 @@ def test_operands_written_right_before_the_call(T, cut):
         assert all(torch.equal(a, b) for a, b in zip(calls(False), want))
     x, W, down, up, bias, ids = made[0]
     check(want[0], *ref_lora(x[:, :K], W[:, :N], down[..., :R], up[..., :N], ids, None, bias))
+
+
+def test_a_low_rank_half_longer_than_the_bounded_waits():
+    """The product's waits give up after two seconds of its own, not of the kernel that it waits for (2.8 s here)."""
+    from infinite_dreams import infinite_dreams_ext as ext
+    T, K, N, L, R, dt = 320000, 8192, 64, 8, 1024, torch.bfloat16
+    W = randn((K, N), dt, 1, K ** -0.5)
+    # rows of 1025 elements: read one element at a time
+    down, up = randn((L, K, R + 1), dt, 2, K ** -0.5)[..., :R], randn((L, R, N), dt, 3, R ** -0.5)
+    x = torch.empty(T, K, dtype=dt, device="cuda")
+    part = randn((T // 32, K), dt, 4)
+    for i in range(32):
+        x[i * (T // 32):(i + 1) * (T // 32)] = part
+    ids = (torch.arange(T, device="cuda") % L).int()
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    out = ext.lora_gemm(x, W, down, up, ids)
+    end.record()
+    torch.cuda.synchronize()
+    ext.check_device_errors()
+    assert start.elapsed_time(end) > 2000   # else this shows nothing: give it more rows
+    for at in (slice(0, 300), slice(T // 2, T // 2 + 300), slice(T - 300, T)):
+        check(out[at], *ref_lora(x[at], W, down, up, ids[at]))
