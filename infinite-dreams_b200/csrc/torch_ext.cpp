@@ -201,9 +201,10 @@ void count_write(const at::Tensor& out) {
 }
 
 void check_no_grad(const char* what, std::initializer_list<at::Tensor> ts) {
-  if (!at::GradMode::is_enabled()) return;
   for (const at::Tensor& t : ts) {
-    TORCH_CHECK(!t.defined() || !t.requires_grad(), what);
+    if (!t.defined()) continue;
+    TORCH_CHECK(!at::GradMode::is_enabled() || !t.requires_grad(), what);
+    TORCH_CHECK(!t._fw_grad(0).defined(), "the operator has no forward-mode derivative: an input's tangent would be lost");
   }
 }
 

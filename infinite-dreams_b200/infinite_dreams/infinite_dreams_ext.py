@@ -318,6 +318,8 @@ def _count_write(out: torch.Tensor) -> None:
 def _check_no_grad(what: str, *tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(what)
+    if any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("the operator has no forward-mode derivative: an input's tangent would be lost")
 
 
 def _stacked_operand(X: torch.Tensor) -> Tuple[torch.Tensor, int, int, int]:
