@@ -169,28 +169,70 @@ void check_index(const at::Tensor& t, const at::Tensor& A, int64_t n, const char
   TORCH_CHECK(t.dim() == 1 && t.size(0) == n, name, " must be 1D with ", n, " elements");
 }
 
-// Refuses an `out` that certainly shares elements with an operand: two dense
-// blocks whose ranges meet, or two sets of rows of one pitch whose columns do.
-void check_apart(const at::Tensor& out, std::initializer_list<at::Tensor> ts) {
-  const int64_t es = static_cast<int64_t>(out.element_size());
-  auto extent = [&](const at::Tensor& t) {   // elements from the first to the last
+int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b < 0 ? 1 : 0); }
+
+// Whether a tensor shares bytes with `out`, which is rows of adjacent elements (2D),
+// or a stack of them (3D, row-major or transposed, its matrices apart).
+bool shares_memory(const at::Tensor& out, const at::Tensor& t) {
+  auto extent = [](const at::Tensor& x) {   // bytes from the first to the last element
     int64_t n = 1;
-    for (int64_t d = 0; d < t.dim(); ++d) n += (t.size(d) - 1) * t.stride(d);
-    return n;
+    for (int64_t d = 0; d < x.dim(); ++d) n += (x.size(d) - 1) * x.stride(d);
+    return n * static_cast<int64_t>(x.element_size());
   };
-  if (out.numel() == 0) return;
-  const int64_t o0 = reinterpret_cast<int64_t>(out.data_ptr()), o1 = o0 + extent(out) * es;
-  for (const at::Tensor& t : ts) {
-    if (!t.defined() || t.numel() == 0) continue;
-    const int64_t t0 = reinterpret_cast<int64_t>(t.data_ptr()), t1 = t0 + extent(t) * es;
-    if (t1 <= o0 || o1 <= t0) continue;
-    bool meet = extent(t) == t.numel() && extent(out) == out.numel();
-    if (t.dim() == 2 && out.dim() == 2 && t.stride(1) == 1 && out.stride(1) == 1 && t.size(0) > 1 && out.size(0) > 1 &&
-        t.stride(0) == out.stride(0) && t.stride(0) >= std::max(t.size(1), out.size(1))) {
-      const int64_t row = out.stride(0) * es, c = ((t0 - o0) % row + row) % row;   // where t's columns begin in out's rows
-      meet = c < out.size(1) * es || c + t.size(1) * es > row;
+  const int64_t es = static_cast<int64_t>(out.element_size()), ts = static_cast<int64_t>(t.element_size());
+  const int64_t o0 = reinterpret_cast<int64_t>(out.data_ptr()), t0 = reinterpret_cast<int64_t>(t.data_ptr());
+  if (t0 + extent(t) <= o0 || o0 + extent(out) <= t0) return false;
+  if (extent(t) == t.numel() * ts && extent(out) == out.numel() * es) return true;   // two dense blocks
+  if (t.dim() == 2 && out.dim() == 2 && es == ts && t.stride(1) == 1 && out.stride(1) == 1 && t.size(0) > 1 &&
+      out.size(0) > 1 && t.stride(0) == out.stride(0) && t.stride(0) >= std::max(t.size(1), out.size(1))) {
+    // columns of one buffer: where t's begin in out's rows
+    const int64_t row = out.stride(0) * es, c = floor_div(t0 - o0, row) * -row + t0 - o0;
+    return c < out.size(1) * es || c + t.size(1) * es > row;
+  }
+  // out: E matrices, se bytes apart, of R rows, sr apart, of `width` bytes
+  const int64_t d = out.dim();
+  const bool trans = d == 3 && out.stride(2) != 1 && out.size(2) > 1;
+  const int64_t row_dim = d - (trans ? 1 : 2), col_dim = d - (trans ? 2 : 1);
+  const int64_t far = extent(out) + 1;   // the pitch of one thing
+  const int64_t R = out.size(row_dim), width = out.size(col_dim) * es, E = d == 3 ? out.size(0) : 1;
+  const int64_t sr = R > 1 ? out.stride(row_dim) * es : far, se = E > 1 ? out.stride(0) * es : far;
+  auto meets = [&](int64_t a, int64_t b) {   // the bytes [a, b)
+    a -= o0;
+    b -= o0;
+    const int64_t e = floor_div(a, se), next_e = std::max<int64_t>(e + 1, 0);
+    if (next_e < E && next_e * se < b) return true;   // the next matrix begins before b
+    if (e < 0 || e >= E) return false;
+    const int64_t r = floor_div(a - e * se, sr), next_r = r + 1;
+    return (r < R && a - e * se - r * sr < width) || (next_r < R && e * se + next_r * sr < b);
+  };
+  // t: runs of adjacent elements
+  int64_t run_dim = -1;
+  for (int64_t i = 0; i < t.dim(); ++i) {
+    if (t.stride(i) == 1 && t.size(i) > 1) run_dim = i;
+  }
+  const int64_t run = (run_dim >= 0 ? t.size(run_dim) : 1) * ts;
+  int64_t size[3] = {1, 1, 1}, stride[3] = {0, 0, 0};
+  for (int64_t i = 0; i < t.dim(); ++i) {
+    if (i == run_dim || t.stride(i) == 0) continue;
+    size[i] = t.size(i);
+    stride[i] = t.stride(i) * ts;
+  }
+  for (int64_t i = 0; i < size[0]; ++i) {
+    for (int64_t j = 0; j < size[1]; ++j) {
+      for (int64_t k = 0; k < size[2]; ++k) {
+        const int64_t at = t0 + i * stride[0] + j * stride[1] + k * stride[2];
+        if (meets(at, at + run)) return true;
+      }
     }
-    TORCH_CHECK(!meet, "out must not share memory with an operand");
+  }
+  return false;
+}
+
+// The kernels read operands while they write `out`.
+void check_apart(const at::Tensor& out, std::initializer_list<at::Tensor> ts) {
+  if (out.numel() == 0) return;
+  for (const at::Tensor& t : ts) {
+    TORCH_CHECK(!t.defined() || t.numel() == 0 || !shares_memory(out, t), "out must not share memory with an operand");
   }
 }
 
@@ -264,7 +306,7 @@ at::Tensor grouped_gemm(const at::Tensor& A, const at::Tensor& B, const at::Tens
   at::Tensor As = row_operand(A), off = offsets.contiguous();
   auto [Bs, tb, ldb, sb] = stacked_operand(B);
   at::Tensor C = rows_out(out, T, N, A);
-  if (out.has_value()) check_apart(C, {A, B, bvec});
+  if (out.has_value()) check_apart(C, {A, B, offsets, bias.value_or(at::Tensor())});
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(A.device().index()).stream();
   const int64_t lda = pitch(As);
   const at::Tensor ws = scratch(A.device(), gemm_grouped_workspace_bytes(As.data_ptr(), Bs.data_ptr(), T, N, K, E, lda,
@@ -299,7 +341,7 @@ at::Tensor grouped_gemm_wgrad(const at::Tensor& A, const at::Tensor& G, const at
   auto [Ds, td, ldd, sd] = stacked_operand(D);
   TORCH_CHECK(Ds.data_ptr() == D.data_ptr(), "out must be row-major or a transposed view, its matrices apart");
   at::Tensor As = row_operand(A), Gs = row_operand(G), off = offsets.contiguous();
-  if (out.has_value()) check_apart(D, {A, G});
+  if (out.has_value()) check_apart(D, {A, G, offsets});
   // a gradient stored N x K is the product with the operands exchanged
   const at::Tensor &L = td ? Gs : As, &R = td ? As : Gs;
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(A.device().index()).stream();
@@ -387,7 +429,7 @@ at::Tensor lora_gemm(const at::Tensor& x, const at::Tensor& W, const at::Tensor&
   auto [Ds, td, ldd, sd] = stacked_operand(down);
   auto [Us, tu, ldu, su] = stacked_operand(up);
   at::Tensor C = rows_out(out, T, N, x);
-  if (out.has_value()) check_apart(C, {x, W, down, up, bvec});
+  if (out.has_value()) check_apart(C, {x, W, down, up, adapter, scale.value_or(at::Tensor()), bias.value_or(at::Tensor())});
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(x.device().index()).stream();
   const int64_t ldx = pitch(xs);
   const at::Tensor ws = scratch(x.device(), gemm_lora_workspace_bytes(xs.data_ptr(), Ws.data_ptr(), Us.data_ptr(), T, N,

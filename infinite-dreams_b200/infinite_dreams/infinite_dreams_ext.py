@@ -283,29 +283,53 @@ def _check_index(t, A: torch.Tensor, n: int, name: str) -> None:
         raise RuntimeError(f"{name} must be 1D with {n} elements")
 
 
+def _shares_memory(out: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether t shares bytes with out, which is rows of adjacent elements (2D), or a stack of them (3D, row-major
+    or transposed, its matrices apart)."""
+    def extent(x):   # bytes from the first to the last element
+        return (1 + sum((n - 1) * st for n, st in zip(x.shape, x.stride()))) * x.element_size()
+    es, ts = out.element_size(), t.element_size()
+    o0, t0 = out.data_ptr(), t.data_ptr()
+    if t0 + extent(t) <= o0 or o0 + extent(out) <= t0:
+        return False
+    if extent(t) == t.numel() * ts and extent(out) == out.numel() * es:   # two dense blocks
+        return True
+    if (t.dim() == 2 and out.dim() == 2 and es == ts and t.stride(1) == 1 and out.stride(1) == 1 and t.size(0) > 1
+            and out.size(0) > 1 and t.stride(0) == out.stride(0) and t.stride(0) >= max(t.size(1), out.size(1))):
+        row = out.stride(0) * es
+        c = (t0 - o0) % row   # columns of one buffer: where t's begin in out's rows
+        return c < out.size(1) * es or c + t.size(1) * es > row
+    # out: E matrices, se bytes apart, of R rows, sr apart, of `width` bytes
+    d = out.dim()
+    trans = d == 3 and out.stride(2) != 1 and out.size(2) > 1
+    row_dim, col_dim = d - (1 if trans else 2), d - (2 if trans else 1)
+    far = extent(out) + 1   # the pitch of one thing
+    R, width, E = out.size(row_dim), out.size(col_dim) * es, out.size(0) if d == 3 else 1
+    sr = out.stride(row_dim) * es if R > 1 else far
+    se = out.stride(0) * es if E > 1 else far
+    # t: runs of adjacent elements, the bytes [a, b) from out's first
+    run_dims = [i for i in range(t.dim()) if t.stride(i) == 1 and t.size(i) > 1]
+    run = (t.size(run_dims[-1]) if run_dims else 1) * ts
+    a = torch.tensor([t0 - o0])
+    for i in range(t.dim()):
+        if i not in run_dims[-1:] and t.stride(i) != 0:
+            a = (a[:, None] + torch.arange(t.size(i))[None, :] * (t.stride(i) * ts)).flatten()
+    b = a + run
+    e = torch.div(a, se, rounding_mode="floor")
+    next_e = (e + 1).clamp_min(0)
+    meet = (next_e < E) & (next_e * se < b)          # the next matrix begins before b
+    left = a - e * se
+    r = torch.div(left, sr, rounding_mode="floor")
+    inside = ((r < R) & (left - r * sr < width)) | ((r + 1 < R) & (e * se + (r + 1) * sr < b))
+    return bool((meet | ((e >= 0) & (e < E) & inside)).any())
+
+
 def _check_apart(out: torch.Tensor, *tensors) -> None:
-    """Refuses an out that certainly shares elements with an operand: two dense
-    blocks whose ranges meet, or two sets of rows of one pitch whose columns do."""
-    def extent(t):   # elements from the first to the last
-        return 1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+    """The kernels read operands while they write out."""
     if out.numel() == 0:
         return
-    es = out.element_size()
-    o0 = out.data_ptr()
-    o1 = o0 + extent(out) * es
     for t in tensors:
-        if t is None or t.numel() == 0:
-            continue
-        t0 = t.data_ptr()
-        if t0 + extent(t) * es <= o0 or o1 <= t0:
-            continue
-        meet = extent(t) == t.numel() and extent(out) == out.numel()
-        if (t.dim() == 2 and out.dim() == 2 and t.stride(1) == 1 and out.stride(1) == 1 and t.size(0) > 1
-                and out.size(0) > 1 and t.stride(0) == out.stride(0) and t.stride(0) >= max(t.size(1), out.size(1))):
-            row = out.stride(0) * es
-            c = (t0 - o0) % row   # where t's columns begin in out's rows
-            meet = c < out.size(1) * es or c + t.size(1) * es > row
-        if meet:
+        if t is not None and t.numel() > 0 and _shares_memory(out, t):
             raise RuntimeError("out must not share memory with an operand")
 
 
@@ -394,7 +418,6 @@ def grouped_gemm(A: torch.Tensor, B: torch.Tensor, offsets: torch.Tensor, *, bia
         _check_like(bias, A, "bias")
         if tuple(bias.shape) != (E, N):
             raise RuntimeError("bias must be (E x N)")
-        bias = bias.contiguous()
     _check_no_grad("grouped_gemm computes no gradients: use grouped.grouped_linear, or call it under "
                    "torch.no_grad()", A, B, bias, out)
     with torch.cuda.device(A.device):
@@ -402,7 +425,8 @@ def grouped_gemm(A: torch.Tensor, B: torch.Tensor, offsets: torch.Tensor, *, bia
         Bs, tb, ldb, sb = _stacked_operand(B)
         C = _rows_out(out, T, N, A)
         if out is not None:
-            _check_apart(C, A, B, bias)
+            _check_apart(C, A, B, offsets, bias)
+        bias = None if bias is None else bias.contiguous()
         stream = torch.cuda.current_stream(A.device)
         lda = _pitch(As)
         need = lib.gemm_grouped_workspace_bytes(As.data_ptr(), Bs.data_ptr(), T, N, K, E, lda, ldb, sb, tb)
@@ -450,9 +474,9 @@ def grouped_gemm_wgrad(A: torch.Tensor, G: torch.Tensor, offsets: torch.Tensor, 
         Ds, td, ldd, sd = _stacked_operand(D)
         if Ds.data_ptr() != D.data_ptr():
             raise RuntimeError("out must be row-major or a transposed view, its matrices apart")
-        if out is not None:
-            _check_apart(D, A, G)
         As, Gs, off = _row_operand(A), _row_operand(G), offsets.contiguous()
+        if out is not None:
+            _check_apart(D, A, G, offsets)
         L, R = (Gs, As) if td else (As, Gs)   # a gradient stored N x K: the operands exchanged
         stream = torch.cuda.current_stream(A.device)
         need = lib.gemm_grouped_wgrad_workspace_bytes(L.data_ptr(), R.data_ptr(), T, L.size(1), R.size(1), _pitch(L),
@@ -512,12 +536,10 @@ def lora_gemm(x: torch.Tensor, W: torch.Tensor, down: torch.Tensor, up: torch.Te
     if scale is not None:
         if scale.device != x.device or scale.dtype != torch.float32 or tuple(scale.shape) != (L,):
             raise RuntimeError("scale must be a float32 tensor of L elements on x's device")
-        scale = scale.contiguous()
     if bias is not None:
         _check_like(bias, x, "bias")
         if tuple(bias.shape) != (N,):
             raise RuntimeError("bias must be (N)")
-        bias = bias.contiguous()
     _check_no_grad("lora_gemm is a serving operator and computes no gradients: call it under torch.no_grad()",
                    x, W, down, up, scale, bias, out)
     with torch.cuda.device(x.device):
@@ -527,7 +549,8 @@ def lora_gemm(x: torch.Tensor, W: torch.Tensor, down: torch.Tensor, up: torch.Te
         Us, tu, ldu, su = _stacked_operand(up)
         C = _rows_out(out, T, N, x)
         if out is not None:
-            _check_apart(C, x, W, down, up, bias)
+            _check_apart(C, x, W, down, up, adapter, scale, bias)
+        scale, bias = (None if t is None else t.contiguous() for t in (scale, bias))
         stream = torch.cuda.current_stream(x.device)
         ldx = _pitch(xs)
         need = lib.gemm_lora_workspace_bytes(xs.data_ptr(), Ws.data_ptr(), Us.data_ptr(), T, N, K, L, R, ldx, ldw, tw,
