@@ -16,8 +16,8 @@
 //
 //  * a cluster of up to 8 CTAs x 8 warps shares the K range of a tile of up to
 //    8 rows; warp w of CTA c takes the 32-element slices c * 8 + w, + 64, ...
-//  * the rows of a tile are ordered by adapter; chunks of up to 8 * NT8 rows
-//    of one adapter are the MMA N, the ranks are the MMA M;
+//  * the rows of a tile are ordered by adapter; the rows of one adapter are the
+//    MMA N, the ranks are the MMA M;
 //  * both operands need 8 adjacent K elements per lane.  The order of K inside
 //    an MMA does not matter as long as both agree, so lane q of a quad takes
 //    elements 8q .. 8q + 7 of the slice: one 16-byte load per row of x, and
@@ -114,15 +114,15 @@ __device__ __forceinline__ uint4 load8(const unsigned short* src, int valid) {
 // d[2 m + half] holds rank (m, half) of this lane's quad row for its 8 K
 // elements.  Else d holds, for each of the 8 K elements, the 2 RT adjacent
 // ranks of this lane, packed.
-template <int RT, int NT8>
+template <int RT>
 struct Slice {
   uint4 d[2 * RT];
-  uint4 x[NT8];
+  uint4 x;
 };
 
-template <int RT, int NT8, bool KMAJ, bool VEC>
-__device__ __forceinline__ void load_slice(const ShrinkParams& p, const unsigned short* d, const int (&xrow)[NT8],
-                                           int r0, int k, int g, Slice<RT, NT8>& s) {
+template <int RT, bool KMAJ, bool VEC>
+__device__ __forceinline__ void load_slice(const ShrinkParams& p, const unsigned short* d, int xrow, int r0, int k,
+                                           int g, Slice<RT>& s) {
   const int kv = p.K - k;   // valid elements from k on (may exceed 8, or be negative)
   if constexpr (KMAJ) {
 #pragma unroll
@@ -164,15 +164,12 @@ __device__ __forceinline__ void load_slice(const ShrinkParams& p, const unsigned
 #pragma unroll
     for (int i = 0; i < 2 * RT; ++i) s.d[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
   }
-#pragma unroll
-  for (int j = 0; j < NT8; ++j) {
-    s.x[j] = load8<VEC>(p.x + static_cast<long long>(max(xrow[j], 0)) * p.ldx + k, xrow[j] >= 0 ? kv : 0);
-  }
+  s.x = load8<VEC>(p.x + static_cast<long long>(max(xrow, 0)) * p.ldx + k, xrow >= 0 ? kv : 0);
 }
 
 // MMA A fragments (row g, row g + 8) of rank tile m: four K pairs each.
-template <int RT, int NT8, bool KMAJ>
-__device__ __forceinline__ void rank_fragments(const Slice<RT, NT8>& s, int m, uint4& lo, uint4& hi) {
+template <int RT, bool KMAJ>
+__device__ __forceinline__ void rank_fragments(const Slice<RT>& s, int m, uint4& lo, uint4& hi) {
   if constexpr (KMAJ) {
     lo = s.d[2 * m];
     hi = s.d[2 * m + 1];
@@ -191,9 +188,11 @@ __device__ __forceinline__ void rank_fragments(const Slice<RT, NT8>& s, int m, u
 }
 
 // grid.x: tiles x cluster size (the cluster is along x); grid.y: blocks of 16
-// RT ranks.
-template <int RT, int NT8, bool KMAJ, bool BF16, bool VEC>
-__global__ void __launch_bounds__(kShrinkThreads) lora_shrink(const __grid_constant__ ShrinkParams p) {
+// RT ranks.  56 registers for 16 ranks: two CTAs leave an SM room for one of the
+// product's (64 rows, 32 adapters of rank 16, 4096 x 4096: 18.1 us, 20.2 with 59,
+// which count as 64).
+template <int RT, bool KMAJ, bool BF16, bool VEC>
+__global__ void __maxnreg__(RT == 1 ? 56 : RT == 2 ? 80 : 128) lora_shrink(const __grid_constant__ ShrinkParams p) {
   constexpr int RB = 16 * RT;
   extern __shared__ float red[];   // [kShrinkWarps][tile_rows][RB]
   __shared__ float rx[kShrinkMaxRows * RB];   // this CTA's elements from the cluster: [CTA][element / cs]
@@ -249,29 +248,22 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink(const __grid_const
   const int s_first = crank * kShrinkWarps + warp, s_step = cs * kShrinkWarps;
   int c0 = 0, c1 = 0;            // rows of the chunk being loaded, in sorted order
   const unsigned short* d = nullptr;
-  int xrow[NT8];
+  int xrow = -1;
   auto open_chunk = [&](int at) {
     c0 = c1 = at;
     if (at >= active) return false;
     const int a = order_id[at];
-    while (c1 < active && c1 < c0 + 8 * NT8 && order_id[c1] == a) ++c1;
+    while (c1 < active && order_id[c1] == a) ++c1;
     d = p.down + static_cast<long long>(a) * p.stride_down;
-#pragma unroll
-    for (int j = 0; j < NT8; ++j) {
-      const int i = c0 + j * 8 + g;
-      xrow[j] = i < c1 ? row0 + order[i] : -1;
-    }
+    xrow = c0 + g < c1 ? row0 + order[c0 + g] : -1;
     return true;
   };
-  float acc[RT][NT8][4];
+  float acc[RT][4];
   auto clear = [&] {
 #pragma unroll
     for (int m = 0; m < RT; ++m) {
 #pragma unroll
-      for (int j = 0; j < NT8; ++j) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.0f;
-      }
+      for (int i = 0; i < 4; ++i) acc[m][i] = 0.0f;
     }
   };
   // accumulator (rank row g / g + 8, row of x 2q / 2q + 1) -> mine[sorted row][rank]
@@ -279,27 +271,24 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink(const __grid_const
 #pragma unroll
     for (int m = 0; m < RT; ++m) {
 #pragma unroll
-      for (int j = 0; j < NT8; ++j) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int half = i >> 1;
-          const int at = f0 + j * 8 + 2 * q + (i & 1);
-          const int r = KMAJ ? m * 16 + half * 8 + g : 2 * RT * g + 2 * m + half;
-          if (at < f1) mine[at * RB + r] = acc[m][j][i];
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int half = i >> 1;
+        const int at = f0 + 2 * q + (i & 1);
+        const int r = KMAJ ? m * 16 + half * 8 + g : 2 * RT * g + 2 * m + half;
+        if (at < f1) mine[at * RB + r] = acc[m][i];
       }
     }
   };
   clear();
   if (s_first < slices) {
-    Slice<RT, NT8> buf[2];
+    Slice<RT> buf[2];
     bool have = open_chunk(0);
     int s = s_first;
-    auto load = [&](Slice<RT, NT8>& to) {
-      load_slice<RT, NT8, KMAJ, VEC>(p, d, xrow, r0, s * kShrinkSlice + q * 8, g, to);
+    auto load = [&](Slice<RT>& to) {
+      load_slice<RT, KMAJ, VEC>(p, d, xrow, r0, s * kShrinkSlice + q * 8, g, to);
     };
     // loads the step after `cur` into `next`, then multiplies `cur`
-    auto step = [&](const Slice<RT, NT8>& cur, Slice<RT, NT8>& next) {
+    auto step = [&](const Slice<RT>& cur, Slice<RT>& next) {
       const int f0 = c0, f1 = c1;
       s += s_step;
       const bool last = s >= slices;   // of this chunk
@@ -311,14 +300,9 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink(const __grid_const
 #pragma unroll
       for (int m = 0; m < RT; ++m) {
         uint4 lo, hi;
-        rank_fragments<RT, NT8, KMAJ>(cur, m, lo, hi);
-#pragma unroll
-        for (int j = 0; j < NT8; ++j) {
-          if (j == 0 || f0 + j * 8 < f1) {
-            mma_m16n8k16<BF16>(acc[m][j], lo.x, hi.x, lo.y, hi.y, cur.x[j].x, cur.x[j].y);
-            mma_m16n8k16<BF16>(acc[m][j], lo.z, hi.z, lo.w, hi.w, cur.x[j].z, cur.x[j].w);
-          }
-        }
+        rank_fragments<RT, KMAJ>(cur, m, lo, hi);
+        mma_m16n8k16<BF16>(acc[m], lo.x, hi.x, lo.y, hi.y, cur.x.x, cur.x.y);
+        mma_m16n8k16<BF16>(acc[m], lo.z, hi.z, lo.w, hi.w, cur.x.z, cur.x.w);
       }
       if (last) {
         flush(f0, f1);

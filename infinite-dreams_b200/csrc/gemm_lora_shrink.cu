@@ -19,8 +19,8 @@ constexpr int kWideFrom = 2048;
 
 template <int RT, bool VEC>
 ShrinkFn pick(bool kmaj, bool bf16) {
-  if (kmaj) return bf16 ? lora_shrink<RT, 1, true, true, VEC> : lora_shrink<RT, 1, true, false, VEC>;
-  return bf16 ? lora_shrink<RT, 1, false, true, VEC> : lora_shrink<RT, 1, false, false, VEC>;
+  if (kmaj) return bf16 ? lora_shrink<RT, true, true, VEC> : lora_shrink<RT, true, false, VEC>;
+  return bf16 ? lora_shrink<RT, false, true, VEC> : lora_shrink<RT, false, false, VEC>;
 }
 
 template <int ROWS>
