@@ -155,17 +155,17 @@ struct Operand {
 
 bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 2u != 0; }
 
-int launch_pack_stacks(const PackJobs& jobs, cudaStream_t stream) {
+int launch_pack_stacks(const PackJobs& jobs, int sms, cudaStream_t stream) {
   if (jobs.count == 0) return GEMM_OK;
   auto most = [&](int per) {
     long long n = 0;
     for (int j = 0; j < jobs.count; ++j) n = std::max(n, pack_slabs(jobs.job[j], kPackThreads * per) * jobs.job[j].batch);
     return n;
   };
-  const bool four = most(4) >= 148 * 2;
+  const bool four = most(4) >= 2 * sms;
   const long long slabs = most(four ? 4 : 1);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(slabs, 148 * 8)), 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(slabs, 8 * sms)), 1, 1);
   cfg.blockDim = dim3(kPackThreads, 1, 1);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -466,7 +466,7 @@ int gemm_grouped_launch(const void* A, const void* B, void* C, const void* offse
   PackJobs jobs = {};
   a.add(static_cast<uint8_t*>(workspace), &jobs);
   b.add(static_cast<uint8_t*>(workspace), &jobs, offsets, offsets_bits == 64);
-  st = launch_pack_stacks(jobs, stream);
+  st = launch_pack_stacks(jobs, sms, stream);
   if (st != GEMM_OK) return st;
   p.offsets = offsets;
   p.off64 = offsets_bits == 64;
@@ -547,7 +547,7 @@ int gemm_grouped_wgrad_launch(const void* A, const void* G, void* D, const void*
   PackJobs jobs = {};
   a.add(static_cast<uint8_t*>(workspace), &jobs);
   g.add(static_cast<uint8_t*>(workspace), &jobs);
-  st = launch_pack_stacks(jobs, stream);
+  st = launch_pack_stacks(jobs, sms, stream);
   if (st != GEMM_OK) return st;
   p.offsets = offsets;
   p.off64 = offsets_bits == 64;
@@ -621,7 +621,7 @@ int gemm_lora_launch(const void* X, const void* W, const void* down, const void*
   pl.x.add(ws, &jobs);
   pl.w.add(ws, &jobs);
   pl.up.add(ws, &jobs);
-  st = launch_pack_stacks(jobs, stream);
+  st = launch_pack_stacks(jobs, sms, stream);
   if (st != GEMM_OK) return st;
 
   ShrinkParams s = {};
@@ -640,7 +640,7 @@ int gemm_lora_launch(const void* X, const void* W, const void* down, const void*
   s.L = static_cast<int>(L);
   s.R = static_cast<int>(R);
   s.err = p.err;
-  st = launch_shrink(s, trans_down != 0, dtype == GEMM_DTYPE_BF16, stream);   // x is TMA-addressable by now
+  st = launch_shrink(s, trans_down != 0, dtype == GEMM_DTYPE_BF16, sms, stream);   // x is TMA-addressable by now
   if (st != GEMM_OK) return st;
 
   p.E = 1;

@@ -68,7 +68,7 @@ inline int64_t shrink_pitch(int64_t R) {
 }
 
 // Launches the kernel on rows of x that are 16-byte aligned (gemm_lora_shrink.cu).
-int launch_shrink(const ShrinkParams& p, bool kmaj, bool bf16, cudaStream_t stream);
+int launch_shrink(const ShrinkParams& p, bool kmaj, bool bf16, int sms, cudaStream_t stream);
 
 // adapter[t], or -1 for none.  An index past the last adapter counts as none.
 // Read past L1: the product's grid does so before it waits for the one before it.

@@ -31,7 +31,7 @@ ShrinkFn pick_wide(bool kmaj, bool bf16) {
 
 }  // namespace
 
-int launch_shrink(const ShrinkParams& sp, bool kmaj, bool bf16, cudaStream_t stream) {
+int launch_shrink(const ShrinkParams& sp, bool kmaj, bool bf16, int sms, cudaStream_t stream) {
   ShrinkParams p = sp;
   const int rt = shrink_rank_tiles(p.R);
   const int elems = kmaj ? 8 : 2 * rt;   // of `down` per load
@@ -55,15 +55,15 @@ int launch_shrink(const ShrinkParams& sp, bool kmaj, bool bf16, cudaStream_t str
       return c;
     };
     const int64_t tall_ctas = static_cast<int64_t>(tiles_of(256)) * rank_blocks;
-    const bool tall = 2 * tall_ctas * cluster_of(tall_ctas, 148) >= 148;
+    const bool tall = 2 * tall_ctas * cluster_of(tall_ctas, sms) >= sms;
     p.tile_rows = tall ? 256 : 64;
     p.tiles = tiles_of(p.tile_rows);
-    cluster = cluster_of(static_cast<int64_t>(p.tiles) * rank_blocks, tall ? 148 : 296);
+    cluster = cluster_of(static_cast<int64_t>(p.tiles) * rank_blocks, tall ? sms : 2 * sms);
     fn = tall ? pick_wide<256>(kmaj, bf16) : pick_wide<64>(kmaj, bf16);
     bytes = tall ? WidePlan<256>::kBytes : WidePlan<64>::kBytes;
     variant = tall * 4 + kmaj * 2 + bf16;
   } else {
-    // So few rows to a tile that about 256 CTAs share the work (T = 64: 2 rows
+    // So few rows to a tile that two CTAs per SM share the work (T = 64: 2 rows
     // x 32 clusters of 8), up to the 8 rows of one MMA; along K no more CTAs
     // than give every warp a slice.
     int rows = 1;
@@ -72,7 +72,7 @@ int launch_shrink(const ShrinkParams& sp, bool kmaj, bool bf16, cudaStream_t str
     p.tiles = (p.T + rows - 1) / rows;
     ranks = 16 * rt;
     const int slices = (p.K + kShrinkSlice - 1) / kShrinkSlice;
-    while (cluster < 8 && cluster * kShrinkWarps < slices && cluster * p.tiles <= 150) cluster *= 2;
+    while (cluster < 8 && cluster * kShrinkWarps < slices && cluster * p.tiles <= sms) cluster *= 2;
     // operands without vector alignment take the element-wise loads
     fn = rt == 1   ? (vec ? pick<1, true>(kmaj, bf16) : pick<1, false>(kmaj, bf16))
          : rt == 2 ? (vec ? pick<2, true>(kmaj, bf16) : pick<2, false>(kmaj, bf16))
