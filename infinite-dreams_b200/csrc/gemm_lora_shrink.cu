@@ -11,11 +11,21 @@ namespace {
 
 using ShrinkFn = void (*)(ShrinkParams);
 
-// More rows than this take lora_shrink_wide.  It passes over x once per adapter of
-// a tile, so it wins where neighbours share one (2048 rows of rank 64 in long
-// runs, 4096 x 4096 with the product: 70 us against 78) and loses where they do
-// not (rank 16, every row another adapter: 137 against 96).
+// More rows than kWideFrom take lora_shrink_wide, if there are few adapters.  It
+// passes over x once per distinct adapter of a tile, 64 ranks at a time, which only
+// the device knows the number of; the number of adapters bounds it.  So up to 4
+// adapters per 16 ranks of the other form's block.  Both forms, wide first, K =
+// 4096 with a product of 128 columns, rows in long runs and every row another
+// adapter, us:
+//   8192 rows, rank 64:   16 adapters   53, 360     115, 514
+//                         64            71, 1248    119, 624
+//   8192 rows, rank 16:    4 adapters   46,  86      56, 122
+//                         16            46, 249      55, 200
+//                         64            59, 842      56, 232
+//   32768 rows, rank 64:  16 adapters  167, 1369    405, 1854
+//                        256           234, 12545   411, 2476
 constexpr int kWideFrom = 2048;
+constexpr int kWideAdapters = 4;
 
 template <int RT, bool VEC>
 ShrinkFn pick(bool kmaj, bool bf16) {
@@ -40,7 +50,7 @@ int launch_shrink(const ShrinkParams& sp, bool kmaj, bool bf16, int sms, cudaStr
   const bool aligned = reinterpret_cast<uintptr_t>(p.down) % 16 == 0 && p.ld_down % 8 == 0 && p.stride_down % 8 == 0;
   ShrinkFn fn;
   int cluster = 1, bytes, ranks, variant;
-  if (p.T > kWideFrom && aligned) {
+  if (p.T > kWideFrom && p.L <= kWideAdapters * rt && aligned) {
     // 256 rows to a cluster if that gives at least half of the SMs a CTA, else
     // 64; as many CTAs along K as keep to one (two) per SM with at least 4 K
     // blocks each.  With the product, rank 64: 8192 rows in long runs, 4096 x

@@ -67,3 +67,39 @@ def test_a_low_rank_half_longer_than_the_bounded_waits():
     assert start.elapsed_time(end) > 2000   # else this shows nothing: give it more rows
     for at in (slice(0, 300), slice(T // 2, T // 2 + 300), slice(T - 300, T)):
         check(out[at], *ref_lora(x[at], W, down, up, ids[at]))
+
+
+@pytest.mark.parametrize("T,K,L,R", [(5000, 1024, 3, 16), (2100, 520, 4, 8), (4100, 264, 8, 32), (4100, 264, 9, 32),
+                                     (5000, 512, 40, 64), (9000, 200, 300, 16), (3000, 328, 17, 100)])
+@pytest.mark.parametrize("stored", ["kn", "nk"])
+def test_many_rows_of_few_and_of_many_adapters(T, K, L, R, stored):
+    """Both forms of the low-rank half past 2048 rows, on either side of the rule that picks one."""
+    from infinite_dreams import infinite_dreams_ext as ext
+    dt = torch.bfloat16
+    x, W, down, up = (randn((T, K), dt, 1), stacked(1, K, 72, dt, 2, stored)[0], stacked(L, K, R, dt, 3, stored),
+                      stacked(L, R, 72, dt, 4, stored))
+    for ids in (torch.arange(T, device="cuda") * 7 % (L + 1) - 1, torch.arange(T, device="cuda") * L // T):
+        check(ext.lora_gemm(x, W, down, up, ids), *ref_lora(x, W, down, up, ids))
+
+
+def test_rows_that_each_pick_another_adapter_cost_no_pass_over_x_each():
+    """8192 rows of 64 adapters of rank 16: about four times as long one by one as in runs (fourteen times where the
+    low-rank half passed over a tile's rows once per adapter)."""
+    from infinite_dreams import infinite_dreams_ext as ext
+    T, K, N, L, R, dt = 8192, 4096, 128, 64, 16, torch.bfloat16
+    x, W, down, up = (randn((T, K), dt, 1), randn((K, N), dt, 2), stacked(L, K, R, dt, 3), stacked(L, R, N, dt, 4))
+    rows = torch.arange(T, device="cuda")
+
+    def best(ids):
+        times = []
+        for _ in range(10):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            for _ in range(5):
+                ext.lora_gemm(x, W, down, up, ids)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(start.elapsed_time(end))
+        return min(times)
+
+    assert best(rows * 7 % L) < 8 * best(rows * L // T)
