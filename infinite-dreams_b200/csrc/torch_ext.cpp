@@ -63,8 +63,8 @@ at::Tensor output(const c10::optional<at::Tensor>& out, int64_t M, int64_t N, co
   if (!out.has_value()) return at::empty({M, N}, A.options());
   const at::Tensor& C = *out;
   TORCH_CHECK(C.scalar_type() == at::kHalf && C.dim() == 2 && C.size(0) == M && C.size(1) == N &&
-                  C.device() == A.device() && (C.stride(1) == 1 || N <= 1),
-              "out must be a float16 (M x N) tensor with unit column stride on A's device");
+                  C.device() == A.device() && (C.stride(1) == 1 || N <= 1) && (M <= 1 || C.stride(0) >= N),
+              "out must be a float16 (M x N) tensor with unit column stride on A's device, its rows apart");
   return C;
 }
 
@@ -112,7 +112,7 @@ at::Tensor gemm_ex(const at::Tensor& A, const at::Tensor& B, int64_t cfg_id, dou
     TORCH_CHECK(D.scalar_type() == at::kHalf && D.dim() == 2 && D.size(0) == M && D.size(1) == N &&
                     D.device() == A.device(),
                 "C must be a float16 (M x N) tensor on A's device");
-    if (D.stride(1) != 1 && N > 1) D = D.contiguous();
+    if ((D.stride(1) != 1 && N > 1) || (M > 1 && D.stride(0) < N)) D = D.contiguous();   // expanded rows too
   }
   at::Tensor bvec;
   if (bias.has_value()) {

@@ -211,7 +211,7 @@ def gemm_ex(A: torch.Tensor, B: torch.Tensor, *, alpha: float = 1.0, beta: float
             raise RuntimeError("beta != 0 needs C")
         if C.dtype != torch.float16 or tuple(C.shape) != (M, N) or C.device != dev:
             raise RuntimeError("C must be a float16 (M x N) tensor on A's device")
-        if C.stride(1) != 1 and N > 1:
+        if (C.stride(1) != 1 and N > 1) or (M > 1 and C.stride(0) < N):   # expanded rows too
             C = C.contiguous()
     if bias is not None:
         if bias.dtype != torch.float16 or bias.numel() != N or bias.device != dev:
@@ -228,8 +228,9 @@ def gemm_ex(A: torch.Tensor, B: torch.Tensor, *, alpha: float = 1.0, beta: float
         if out is None:
             out = torch.empty((M, N), dtype=torch.float16, device=dev)
         elif (out.dtype != torch.float16 or tuple(out.shape) != (M, N) or out.device != dev
-              or (out.stride(1) != 1 and N > 1)):
-            raise RuntimeError("out must be a float16 (M x N) tensor with unit column stride on A's device")
+              or (out.stride(1) != 1 and N > 1) or (M > 1 and out.stride(0) < N)):
+            raise RuntimeError("out must be a float16 (M x N) tensor with unit column stride on A's device, its rows "
+                               "apart")
         stream = torch.cuda.current_stream(dev)
         a_ptr, b_ptr = A_s.data_ptr(), B_s.data_ptr()
         need = lib.gemm_workspace_bytes_ex(a_ptr, b_ptr, M, N, K, lda, ldb, ta, tb, int(cfg_id))

@@ -25,3 +25,23 @@ def test_columns_beside_the_output_stay(cuda_device, M, N, K):
         assert bool((wide == 7).all()), cfg
     torch.cuda.synchronize()
     ext.check_device_errors()
+
+
+@pytest.mark.parametrize("binding", ["compiled", "ctypes"])
+@pytest.mark.parametrize("M,N", [(300, 136), (16, 256), (5, 1)])
+def test_rows_that_lie_on_one_another(cuda_device, binding, M, N):
+    """One row given as C for all of them is read as such, and an out whose rows are not apart is refused."""
+    from infinite_dreams import infinite_dreams_ext as ext
+    g = torch.Generator(device="cuda").manual_seed(M)
+    A = torch.randn(M, 64, generator=g, device="cuda").half()
+    B = torch.randn(64, N, generator=g, device="cuda").half()
+    row = torch.randn(1, N, generator=g, device="cuda").half()
+    keep, ext._fast = ext._fast, ext._fast if binding == "compiled" else None
+    try:
+        want = ext.gemm_ex(A, B, beta=1.0, C=row.expand(M, N).contiguous())
+        assert torch.equal(ext.gemm_ex(A, B, beta=1.0, C=row.expand(M, N)), want)
+        for out in (row.expand(M, N), torch.empty(M + N, dtype=torch.float16, device="cuda").as_strided((M, N), (0, 1))):
+            with pytest.raises(RuntimeError, match="rows apart"):
+                ext.gemm_ex(A, B, out=out)
+    finally:
+        ext._fast = keep
