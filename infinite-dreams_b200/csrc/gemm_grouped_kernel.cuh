@@ -728,8 +728,10 @@ __global__ void __maxnreg__(CG == 1 && LORA ? 96 : 168)
     fence_mbar_init();
   }
   if (warp == 0 && lane == 0) {
-    for (int i = p.first_box; i < box_count(TM); ++i) prefetch_tmap(&maps.a[i]);
-    prefetch_tmap(&maps.b);
+    if (p.kb_total > 0) {   // K = 0: no maps
+      for (int i = p.first_box; i < box_count(TM); ++i) prefetch_tmap(&maps.a[i]);
+      prefetch_tmap(&maps.b);
+    }
     if (LORA) prefetch_tmap(&maps.u);
     if (p.c_tma) prefetch_tmap(&maps.c);
   }

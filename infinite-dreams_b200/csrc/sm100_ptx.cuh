@@ -129,8 +129,9 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
 // A grid launched with programmatic stream serialization may start while the
 // previous grid in the stream is still running; griddep_wait() returns once
 // that grid has completed and its memory is visible, so everything that reads
-// or writes global memory comes after it.  griddep_launch_dependents() lets
-// the next such grid begin its own set-up early.
+// or writes global memory comes after it (but for the adapters' product, which
+// says in gemm_grouped_kernel.cuh what it reads before and why).
+// griddep_launch_dependents() lets the next such grid begin its own set-up early.
 __device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ void griddep_launch_dependents() {
