@@ -188,11 +188,13 @@ __device__ __forceinline__ void rank_fragments(const Slice<RT>& s, int m, uint4&
 }
 
 // grid.x: tiles x cluster size (the cluster is along x); grid.y: blocks of 16
-// RT ranks.  56 registers for 16 ranks: two CTAs leave an SM room for one of the
-// product's (64 rows, 32 adapters of rank 16, 4096 x 4096: 18.1 us, 20.2 with 59,
-// which count as 64).
+// RT ranks.  Registers: 56 for 16 ranks stored R x K, so that two CTAs leave an SM
+// room for one of the product's (64 rows, 32 adapters of rank 16, 4096 x 4096:
+// 18.1 us, 20.2 with 59, which count as 64); stored K x R that costs more than it
+// brings (2000 rows of 64 adapters, K = 4096: 144 us, 126 with 64).  Up to 96 for 32
+// ranks (2000 rows, 64 adapters: 108 us, 140 with 80).
 template <int RT, bool KMAJ, bool BF16, bool VEC>
-__global__ void __maxnreg__(RT == 1 ? 56 : RT == 2 ? 80 : 128) lora_shrink(const __grid_constant__ ShrinkParams p) {
+__global__ void __maxnreg__(RT == 1 ? (KMAJ ? 56 : 64) : RT == 2 ? 96 : 128) lora_shrink(const __grid_constant__ ShrinkParams p) {
   constexpr int RB = 16 * RT;
   extern __shared__ float red[];   // [kShrinkWarps][tile_rows][RB]
   __shared__ float rx[kShrinkMaxRows * RB];   // this CTA's elements from the cluster: [CTA][element / cs]

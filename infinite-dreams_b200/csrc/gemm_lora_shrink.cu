@@ -17,13 +17,13 @@ using ShrinkFn = void (*)(ShrinkParams);
 // adapters per 16 ranks of the other form's block.  Both forms, wide first, K =
 // 4096 with a product of 128 columns, rows in long runs and every row another
 // adapter, us:
-//   8192 rows, rank 64:   16 adapters   53, 360     115, 514
-//                         64            71, 1248    119, 624
-//   8192 rows, rank 16:    4 adapters   46,  86      56, 122
-//                         16            46, 249      55, 200
-//                         64            59, 842      56, 232
-//   32768 rows, rank 64:  16 adapters  167, 1369    405, 1854
-//                        256           234, 12545   411, 2476
+//   8192 rows, rank 64:   16 adapters   54, 359     116, 518
+//                         64            72, 1249    119, 625
+//   8192 rows, rank 16:    4 adapters   46,  87      55, 120
+//                         16            46, 249      55, 195
+//                         64            58, 842      56, 226
+//   32768 rows, rank 64:  16 adapters  167, 1370    406, 1860
+//                        256           234, 12479   411, 2480
 constexpr int kWideFrom = 2048;
 constexpr int kWideAdapters = 4;
 
