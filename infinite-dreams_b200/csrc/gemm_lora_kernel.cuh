@@ -347,6 +347,10 @@ __global__ void __maxnreg__(RT == 1 ? (KMAJ ? 56 : 64) : RT == 2 ? 96 : 128) lor
   if (!mbar_wait_cluster(&rx_full, 0, &gave_up)) {
     gave_up = 1;
     if (lane == 0) atomicOr(p.err, kDevErrTimeoutEpilogue);
+    // stays until every peer has left or is here too: none may write into the
+    // shared memory of a CTA that is gone
+    cluster_arrive();
+    cluster_wait();
     return;
   }
   for (int e = tid * cs + crank; e < active * RB; e += kShrinkThreads * cs) {
