@@ -47,9 +47,9 @@ def test_operands_written_right_before_the_call(T, cut):
 
 
 def test_a_low_rank_half_longer_than_the_bounded_waits():
-    """The product's waits give up after two seconds of its own, not of the kernel that it waits for (2.8 s here)."""
+    """The product's waits give up after two seconds of its own, not of the kernel that it waits for (3.2 s here)."""
     from infinite_dreams import infinite_dreams_ext as ext
-    T, K, N, L, R, dt = 320000, 8192, 64, 8, 1024, torch.bfloat16
+    T, K, N, L, R, dt = 400000, 8192, 64, 8, 1024, torch.bfloat16
     W = randn((K, N), dt, 1, K ** -0.5)
     # rows of 1025 elements: read one element at a time
     down, up = randn((L, K, R + 1), dt, 2, K ** -0.5)[..., :R], randn((L, R, N), dt, 3, R ** -0.5)
